@@ -39,6 +39,10 @@ extern "C" {
 #define RNB_B200_TYPE_Q8_0 8u
 #define RNB_B200_TYPE_Q4_K 12u
 #define RNB_B200_TYPE_Q6_K 14u
+/* GGML type ids of activations and cache rows in the paged-cache operators */
+#define RNB_B200_TYPE_F32 0u
+#define RNB_B200_TYPE_F16 1u
+#define RNB_B200_TYPE_BF16 30u
 
 /* Message of the last failing call on this thread (never NULL). */
 const char *rnb_b200_last_error(void);
@@ -752,6 +756,109 @@ int rnb_b200_attention_decode_hd128_noalloc(const float *q_dev, const uint16_t *
  * last read completed; non-zero = a bounded wait inside a kernel gave up and the outputs written
  * since then are not to be trusted (the codes are those of rnb_b200_dev_error_flag). */
 int rnb_b200_attention_decode_hd128_noalloc_status(int *status_out, void *stream);
+/* ---- paged key-value cache -----------------------------------------------------------------------
+ * For programs that keep many sequences: the cache of a layer is a pool of pages of `page_size`
+ * positions, and a table per sequence names the page of every `page_size` positions.  The reference keeps
+ * one contiguous cache per sequence (crates/rnb-llm/src/kv_cache.rs); nothing here has a counterpart in it.
+ *
+ * Device-pointer tier: all pointers but the host structs themselves and the lists of
+ * rnb_b200_dev_paged_kv_copy are device addresses on the library's device (RNB_CUDA_DEVICE); calls may
+ * come with another device current, allocate nothing, do not synchronise and can be captured into graphs.
+ * Tables, lengths and starts are read on the device when the work runs.  What they hold is checked there:
+ * a page outside the pool, a length outside the table or a start out of order raises
+ * RNB_B200_DEVICE_BAD_PAGE in the device error word (rnb_b200_dev_error_flag) instead of touching memory
+ * outside the pool; what the call writes for such a sequence is then not to be used.  Entries of pages
+ * that no query sees are not read and may hold anything. */
+#define RNB_B200_DEVICE_BAD_PAGE 5
+typedef struct {
+    uint32_t type;      /* RNB_B200_TYPE_F16 or _BF16 */
+    int32_t head_dim;   /* a multiple of 8 up to 512; attention: 64 or 128 */
+    int32_t kv_heads;
+    int32_t page_size;  /* positions per page: a power of two from 8 to 256 */
+    int32_t n_pages;
+    /* elements from one page, position and head to the next: multiples of 8, at least head_dim.  Rows of
+     * head_dim elements are contiguous and must not overlap; any order of the three is taken */
+    uint64_t page_stride, pos_stride, head_stride;
+    void *k, *v;        /* 16-byte aligned */
+} rnb_b200_paged_cache;
+typedef struct {
+    const int32_t *table;   /* [n_seq] rows of max_pages entries, table_stride entries apart */
+    int32_t table_stride, max_pages;
+    int32_t n_seq;
+    int32_t n_tokens;       /* rows of the call's token matrices */
+    const int32_t *kv_len;  /* [n_seq] positions in the cache, the call's own tokens included; 0: none */
+    /* [n_seq + 1] first row of every sequence's tokens, from 0 and not descending; null: row i is the one token of
+     * sequence i.  The last tokens of a sequence's kv_len positions are the call's; rows from
+     * q_start[n_seq] on are padding: not read, and left as they are in outputs */
+    const int32_t *q_start;
+} rnb_b200_paged_batch;
+/* K and V rows of the call's tokens to their places in the pages, rounded to the cache's type (to nearest,
+ * ties to even).  src_type: F32, or the cache's type.  k_new, v_new [n_tokens][kv_heads][head_dim], 16-byte
+ * aligned, src_stride elements from one token to the next (a multiple of 8).  Pages that several sequences
+ * share are the caller's to part first (rnb_b200_kv_pages_extend says which). */
+int rnb_b200_dev_paged_kv_append(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t src_type,
+                                 const void *k_new, const void *v_new, size_t src_stride, void *stream);
+/* Copies pages within the pool: for every i the first rows[i] positions (null: all) of all heads of page
+ * src[i] to page dst[i], keys and values, in n_layers layers that lie layer_stride elements (a multiple of
+ * 8) apart.  The lists are host memory, read before the call returns.  Copies happen as if at the same time:
+ * a page may be copied to several places, but be written once only, and a page that is written must not be
+ * read (RNB_B200_VALIDATION_FAILED). */
+int rnb_b200_dev_paged_kv_copy(const rnb_b200_paged_cache *cache, size_t n_layers, uint64_t layer_stride, const int32_t *src,
+                               const int32_t *dst, const int32_t *rows, size_t n_pages, void *stream);
+/* softmax(scale q.K^T) V over the pages.  A query at position p sees positions j <= p with window = 0, else
+ * those with j > p - window or j < sinks.  A query that sees nothing (kv_len 0) gets zeros.  q_type: F32 with an
+ * F16 cache, or the cache's type; `out` has the same type.  Sums, maxima and the softmax are f32, and f32 queries
+ * keep f32 accuracy (queries and probabilities enter the products as two f16 terms).  q, out
+ * [n_tokens][heads][head_dim], 16-byte aligned, q_stride / out_stride elements from one token to the next
+ * (multiples of 8); heads a multiple of kv_heads.  lse (may be null): f32 [n_tokens][heads], the logarithm of
+ * the sum of exponentials, -inf for a query that sees nothing.
+ * `workspace`: rnb_b200_paged_workspace_bytes() bytes, 256-byte aligned, initialised once by
+ * rnb_b200_paged_workspace_init; one workspace serves any number of calls one after another (of any sizes, of both
+ * calls, of captured graphs), but calls that may overlap on the GPU need one each.
+ * _decode: one new token per sequence (q_start null), the work split over the lengths so that few sequences
+ * use the whole GPU too.  _prefill: the tokens of every sequence, causal. */
+size_t rnb_b200_paged_workspace_bytes(void);
+int rnb_b200_paged_workspace_init(void *workspace, size_t workspace_bytes, void *stream);
+int rnb_b200_dev_attention_decode_paged(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type,
+                                        const void *q, size_t q_stride, size_t num_heads, float scale, int32_t window, int32_t sinks,
+                                        void *workspace, size_t workspace_bytes, void *out, size_t out_stride, float *lse,
+                                        void *stream);
+int rnb_b200_dev_attention_prefill_paged(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type,
+                                         const void *q, size_t q_stride, size_t num_heads, float scale, int32_t window, int32_t sinks,
+                                         void *workspace, size_t workspace_bytes, void *out, size_t out_stride, float *lse,
+                                         void *stream);
+/* Book-keeping of the pages, on the host only: which page holds what, how many sequences share it, which are
+ * free.  Calls on one handle from several threads take turns.  A call that fails changes nothing.
+ * Pages are handed out lowest number first. */
+typedef struct rnb_b200_kv_pages rnb_b200_kv_pages;
+typedef struct {
+    int32_t n_pages, page_size, free_pages, n_seqs;
+} rnb_b200_kv_pages_info;
+int rnb_b200_kv_pages_create(int32_t n_pages, int32_t page_size, rnb_b200_kv_pages **out);
+void rnb_b200_kv_pages_destroy(rnb_b200_kv_pages *p);
+int rnb_b200_kv_pages_get_info(const rnb_b200_kv_pages *p, rnb_b200_kv_pages_info *out);
+/* a new, empty sequence */
+int rnb_b200_kv_pages_new(rnb_b200_kv_pages *p, int32_t *seq_out);
+/* Room for n_new more positions.  Where the last page is shared and partly filled, the sequence gets a page of
+ * its own in its place, and *n_copies = 1 asks for the copy of `rows` positions of page `src` to page `dst`
+ * (rnb_b200_dev_paged_kv_copy) before anything is appended.  Too few free pages: RNB_B200_OUT_OF_MEMORY. */
+int rnb_b200_kv_pages_extend(rnb_b200_kv_pages *p, int32_t seq, int32_t n_new, int32_t *n_copies, int32_t *src, int32_t *dst, int32_t *rows);
+/* a sequence with the same positions, sharing all pages */
+int rnb_b200_kv_pages_fork(rnb_b200_kv_pages *p, int32_t seq, int32_t *seq_out);
+/* keeps the first `len` positions */
+int rnb_b200_kv_pages_truncate(rnb_b200_kv_pages *p, int32_t seq, int32_t len);
+/* Frees pages that the next token, at position len, and later ones do not see: those whose positions all lie in
+ * sinks .. len - window.  Their entries become -1. */
+int rnb_b200_kv_pages_release(rnb_b200_kv_pages *p, int32_t seq, int32_t window, int32_t sinks);
+int rnb_b200_kv_pages_free(rnb_b200_kv_pages *p, int32_t seq);
+/* Moves the used pages to the front of the pool: tables change at once, and src[i] -> dst[i], i < *n_copies, are
+ * the copies (of whole pages) to make before the next append or attention.  cap: room in src and dst; too
+ * little (n_pages / 2 is always enough): RNB_B200_VALIDATION_FAILED with *n_copies = what is needed. */
+int rnb_b200_kv_pages_compact(rnb_b200_kv_pages *p, int32_t *src, int32_t *dst, size_t cap, size_t *n_copies);
+/* Tables and lengths of n sequences for rnb_b200_paged_batch: rows of `stride` entries, unused ones -1 (too short a
+ * row: RNB_B200_VALIDATION_FAILED).  Either of the two may be null. */
+int rnb_b200_kv_pages_tables(const rnb_b200_kv_pages *p, const int32_t *seqs, size_t n, int32_t *table, size_t stride, int32_t *kv_len);
+
 /* Reads and clears the device error word set by kernels whose bounded waits gave up. */
 int rnb_b200_dev_error_flag(int *flag_out);
 

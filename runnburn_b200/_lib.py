@@ -57,7 +57,7 @@ BLOCK_SANDWICH, BLOCK_PARALLEL = 0, 1
 NORM_RMS, NORM_LAYER = 0, 1
 ACT_GELU_TANH, ACT_SILU = 0, 1
 ROTATION_YARN, ROTATION_LINEAR = 1, 2
-TYPE_F32, TYPE_BF16 = 0, 30
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30
 
 
 class Rotation(C.Structure):
@@ -83,6 +83,20 @@ class LayerWeights(C.Structure):
                [(n, QWeight) for n in ("wq", "wk", "wv", "wo", "gate", "up", "down")] + \
                [("router", C.c_void_p)] + \
                [(n, QWeight) for n in ("gate_exps", "up_exps", "down_exps")]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [("type", C.c_uint32)] + [(n, C.c_int32) for n in ("head_dim", "kv_heads", "page_size", "n_pages")] + \
+               [(n, C.c_uint64) for n in ("page_stride", "pos_stride", "head_stride")] + [("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [("table", C.c_void_p)] + [(n, C.c_int32) for n in ("table_stride", "max_pages", "n_seq", "n_tokens")] + \
+               [("kv_len", C.c_void_p), ("q_start", C.c_void_p)]
+
+
+class KvPagesInfo(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_pages", "page_size", "free_pages", "n_seqs")]
 
 
 _lib = None
@@ -229,6 +243,21 @@ def load() -> C.CDLL:
         "rnb_b200_gguf_model_config": [vp, i32, vp],
         "rnb_b200_decoder_load_gguf": [vp, vp, i32],
         "rnb_b200_inject_resident_alloc_ooms_for_test": [sz],
+        "rnb_b200_dev_paged_kv_append": [vp, vp, u32, vp, vp, sz, vp],
+        "rnb_b200_dev_paged_kv_copy": [vp, sz, u64, vp, vp, vp, sz, vp],
+        "rnb_b200_paged_workspace_init": [vp, sz, vp],
+        "rnb_b200_dev_attention_decode_paged": [vp, vp, u32, vp, sz, sz, f32, i32, i32, vp, sz, vp, sz, vp, vp],
+        "rnb_b200_dev_attention_prefill_paged": [vp, vp, u32, vp, sz, sz, f32, i32, i32, vp, sz, vp, sz, vp, vp],
+        "rnb_b200_kv_pages_create": [i32, i32, vp],
+        "rnb_b200_kv_pages_get_info": [vp, vp],
+        "rnb_b200_kv_pages_new": [vp, vp],
+        "rnb_b200_kv_pages_extend": [vp, i32, i32, vp, vp, vp, vp],
+        "rnb_b200_kv_pages_fork": [vp, i32, vp],
+        "rnb_b200_kv_pages_truncate": [vp, i32, i32],
+        "rnb_b200_kv_pages_release": [vp, i32, i32, i32],
+        "rnb_b200_kv_pages_free": [vp, i32],
+        "rnb_b200_kv_pages_compact": [vp, vp, vp, sz, vp],
+        "rnb_b200_kv_pages_tables": [vp, vp, sz, vp, sz, vp],
     }
     for name, args in sig.items():
         fn = getattr(L, name)
@@ -242,6 +271,10 @@ def load() -> C.CDLL:
     L.rnb_b200_resident_limit_for.restype = u64
     L.rnb_b200_dev_q8k_bytes.argtypes = [sz]
     L.rnb_b200_dev_q8k_bytes.restype = sz
+    L.rnb_b200_paged_workspace_bytes.argtypes = []
+    L.rnb_b200_paged_workspace_bytes.restype = sz
+    L.rnb_b200_kv_pages_destroy.argtypes = [vp]
+    L.rnb_b200_kv_pages_destroy.restype = None
     L.rnb_b200_flash_decode_scratch_bytes.argtypes = [sz, i32]
     L.rnb_b200_flash_decode_scratch_bytes.restype = sz
     _lib = L

@@ -1,0 +1,252 @@
+// Operators of a paged key-value cache (declarations: include/rnb_b200.h): checks of arguments and launches.
+#include <algorithm>
+
+#include "launch_k.hpp"
+#include "paged.cuh"
+#include "paged_attention_plain.cuh"
+
+namespace rnb {
+
+// The library's device for the length of a call, whatever device the caller has current.
+struct PkCall {
+    std::lock_guard<std::mutex> g;
+    State &st;
+    int before = -1, rc;
+    PkCall() : g(state_mutex()), st(state()) { rc = enter(); }
+    ~PkCall() {
+        if (before >= 0 && before != st.device) cudaSetDevice(before);
+    }
+    int enter() {
+        RNB_CU(cudaGetDevice(&before));
+        RNB_TRY(st.open());
+        if (before != st.device) RNB_CU(cudaSetDevice(st.device));
+        return RNB_B200_OK;
+    }
+};
+
+static int pk_bad(const char *what) { return fail(RNB_B200_VALIDATION_FAILED, "paged cache: %s", what); }
+
+static int pk_check_cache(const rnb_b200_paged_cache *c, PkCache *out) {
+    if (!c || !c->k || !c->v) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
+    if (c->type != RNB_B200_TYPE_F16 && c->type != RNB_B200_TYPE_BF16) return fail(RNB_B200_UNSUPPORTED, "paged cache: type must be F16 or BF16, got %u", c->type);
+    if (c->head_dim < 8 || c->head_dim > 512 || c->head_dim % 8) return fail(RNB_B200_VALIDATION_FAILED, "paged cache: head_dim must be a multiple of 8 up to 512, got %d", c->head_dim);
+    if (c->kv_heads < 1 || c->kv_heads > 65535) return fail(RNB_B200_VALIDATION_FAILED, "paged cache: kv_heads must be in 1..65535, got %d", c->kv_heads);
+    if (c->page_size < 8 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
+        return fail(RNB_B200_VALIDATION_FAILED, "paged cache: page_size must be a power of two from 8 to 256, got %d", c->page_size);
+    if (c->n_pages < 1) return fail(RNB_B200_VALIDATION_FAILED, "paged cache: n_pages must be at least 1, got %d", c->n_pages);
+    // Strides from the smallest to the largest: each at least what the ones below it span, so that no two rows overlap.  A stride that is
+    // never stepped (one head) may be anything.
+    const uint64_t dim = (uint64_t)c->head_dim;
+    struct Step {
+        uint64_t stride, n;
+    } steps[3] = {{c->page_stride, (uint64_t)c->n_pages}, {c->pos_stride, (uint64_t)c->page_size}, {c->head_stride, (uint64_t)c->kv_heads}};
+    std::sort(steps, steps + 3, [](const Step &a, const Step &b) { return a.stride < b.stride; });
+    uint64_t span = dim;
+    for (const Step &s : steps) {
+        if (s.stride % 8 || s.stride > (uint64_t)1 << 38) return pk_bad("strides must be multiples of 8 elements below 2^38");
+        if (s.n == 1) continue;
+        if (s.stride < span) return pk_bad("rows overlap: a stride is smaller than what lies below it");
+        span = s.stride * (s.n - 1) + span;
+    }
+    if (((uintptr_t)c->k | (uintptr_t)c->v) & 15u) return pk_bad("k and v must be 16-byte aligned");
+    int shift = 0;
+    while ((1 << shift) < c->page_size) shift++;
+    *out = {(uint16_t *)c->k, (uint16_t *)c->v, c->page_stride, c->pos_stride, c->head_stride, c->n_pages, shift, c->kv_heads, c->head_dim};
+    return RNB_B200_OK;
+}
+static int pk_check_batch(const rnb_b200_paged_batch *b, PkBatch *out) {
+    if (!b) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
+    if (b->n_seq < 0 || b->n_tokens < 0) return pk_bad("n_seq and n_tokens must not be negative");
+    if (!b->q_start && b->n_tokens != b->n_seq) return fail(RNB_B200_VALIDATION_FAILED, "paged cache: one token per sequence without q_start, got %d tokens of %d sequences", b->n_tokens, b->n_seq);
+    if (b->n_seq > 0 && (!b->table || !b->kv_len)) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
+    if (b->max_pages < 1 || b->table_stride < b->max_pages) return pk_bad("max_pages must be at least 1 and table_stride at least max_pages");
+    if (((uintptr_t)b->table | (uintptr_t)b->kv_len | (uintptr_t)b->q_start) & 3u) return pk_bad("table, kv_len and q_start must be 4-byte aligned");
+    *out = {b->table, b->kv_len, b->q_start, b->table_stride, b->max_pages, b->n_seq, b->n_tokens};
+    return RNB_B200_OK;
+}
+
+// ---- append and copy ----------------------------------------------------------------------------------
+static int pk_append(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t src_type, const void *k_new, const void *v_new, size_t src_stride,
+                     cudaStream_t s) {
+    PkCache c{};
+    PkBatch b{};
+    RNB_TRY(pk_check_cache(cache, &c));
+    RNB_TRY(pk_check_batch(batch, &b));
+    if (src_type != RNB_B200_TYPE_F32 && src_type != cache->type) return fail(RNB_B200_UNSUPPORTED, "paged cache: rows must be F32 or of the cache's type, got type %u", src_type);
+    if (b.n_tokens == 0 || b.n_seq == 0) return RNB_B200_OK;
+    if (!k_new || !v_new) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
+    if (((uintptr_t)k_new | (uintptr_t)v_new) & 15u || src_stride % 8) return pk_bad("rows must be 16-byte aligned and src_stride a multiple of 8");
+    if (b.n_tokens > 1 && src_stride < (size_t)c.kv_heads * c.head_dim) return pk_bad("src_stride is smaller than a token's rows");
+    PkCall call;
+    RNB_TRY(call.rc);
+    const dim3 grid((unsigned)b.n_tokens), block((unsigned)std::min(256, (c.kv_heads * c.head_dim / 8 + 31) / 32 * 32));
+    int *err = call.st.dev_error;
+    if (cache->type == RNB_B200_TYPE_F16) {
+        if (src_type == RNB_B200_TYPE_F32) RNB_CU(launch_k(paged_append_kernel<float, F16>, grid, block, 0, s, c, b, (const float *)k_new, (const float *)v_new, src_stride, err));
+        else RNB_CU(launch_k(paged_append_kernel<F16, F16>, grid, block, 0, s, c, b, (const F16 *)k_new, (const F16 *)v_new, src_stride, err));
+    } else {
+        if (src_type == RNB_B200_TYPE_F32) RNB_CU(launch_k(paged_append_kernel<float, Bf16>, grid, block, 0, s, c, b, (const float *)k_new, (const float *)v_new, src_stride, err));
+        else RNB_CU(launch_k(paged_append_kernel<Bf16, Bf16>, grid, block, 0, s, c, b, (const Bf16 *)k_new, (const Bf16 *)v_new, src_stride, err));
+    }
+    return RNB_B200_OK;
+}
+
+template <int N>
+static int pk_copy_some(const PkCache &c, size_t n_layers, uint64_t layer_stride, const int32_t *src, const int32_t *dst, const int32_t *rows, size_t n, cudaStream_t s) {
+    PkPairs<N> pairs;
+    pairs.n = (int)n;
+    for (size_t i = 0; i < n; i++) {
+        pairs.src[i] = src[i];
+        pairs.dst[i] = dst[i];
+        pairs.rows[i] = rows ? rows[i] : 1 << c.page_shift;
+    }
+    const int chunks = (c.kv_heads * c.head_dim / 8) << c.page_shift;
+    const dim3 grid((unsigned)n, (unsigned)std::min(64, (chunks + 1023) / 1024), (unsigned)(2 * n_layers));
+    RNB_CU(launch_k(paged_copy_kernel<N>, grid, dim3(256), 0, s, c, layer_stride, pairs));
+    return RNB_B200_OK;
+}
+static int pk_copy(const rnb_b200_paged_cache *cache, size_t n_layers, uint64_t layer_stride, const int32_t *src, const int32_t *dst, const int32_t *rows, size_t n,
+                   cudaStream_t s) {
+    PkCache c{};
+    RNB_TRY(pk_check_cache(cache, &c));
+    if (n_layers < 1 || n_layers > 32767) return fail(RNB_B200_VALIDATION_FAILED, "paged cache: n_layers must be in 1..32767, got %zu", n_layers);
+    if (layer_stride % 8 || (n_layers > 1 && layer_stride < (uint64_t)c.head_dim)) return pk_bad("layer_stride must be a multiple of 8 and at least head_dim");
+    if (n == 0) return RNB_B200_OK;
+    if (!src || !dst) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
+    if (n > (size_t)c.n_pages) return pk_bad("more copies than pages");
+    std::vector<uint8_t> role(c.n_pages, 0);   // 1: read, 2: written
+    for (size_t i = 0; i < n; i++) {
+        if (src[i] < 0 || src[i] >= c.n_pages || dst[i] < 0 || dst[i] >= c.n_pages)
+            return fail(RNB_B200_VALIDATION_FAILED, "paged cache: copy %zu is of page %d to page %d, the pool has %d", i, src[i], dst[i], c.n_pages);
+        if (rows && (rows[i] < 0 || rows[i] > 1 << c.page_shift))
+            return fail(RNB_B200_VALIDATION_FAILED, "paged cache: copy %zu is of %d positions, a page has %d", i, rows[i], 1 << c.page_shift);
+        if (role[src[i]] & 2 || role[dst[i]] || src[i] == dst[i])
+            return fail(RNB_B200_VALIDATION_FAILED, "paged cache: copy %zu (page %d to page %d): a page is written twice, or read and written", i, src[i], dst[i]);
+        role[src[i]] = 1;
+        role[dst[i]] = 2;
+    }
+    PkCall call;
+    RNB_TRY(call.rc);
+    for (size_t at = 0; at < n;) {
+        const size_t left = n - at, m = left > 64 ? std::min<size_t>(left, 2048) : left;
+        if (m > 64) RNB_TRY(pk_copy_some<2048>(c, n_layers, layer_stride, src + at, dst + at, rows ? rows + at : nullptr, m, s));
+        else RNB_TRY(pk_copy_some<64>(c, n_layers, layer_stride, src + at, dst + at, rows ? rows + at : nullptr, m, s));
+        at += m;
+    }
+    return RNB_B200_OK;
+}
+
+// ---- attention ------------------------------------------------------------------------------------------
+struct PkAttention {   // a checked call
+    PkCache c{};
+    PkBatch b{};
+    uint32_t q_type, c_type;
+    const void *q;
+    size_t q_stride, out_stride;
+    int heads, window, sinks;
+    float scale;
+    void *out, *workspace;
+    float *lse;
+};
+constexpr size_t PK_WORKSPACE_BYTES = 256;
+
+static int pk_check_attention(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type, const void *q, size_t q_stride, size_t num_heads,
+                              float scale, int32_t window, int32_t sinks, void *workspace, size_t workspace_bytes, void *out, size_t out_stride, float *lse, PkAttention *a) {
+    RNB_TRY(pk_check_cache(cache, &a->c));
+    RNB_TRY(pk_check_batch(batch, &a->b));
+    if (cache->head_dim != 64 && cache->head_dim != 128) return fail(RNB_B200_UNSUPPORTED, "paged attention: head_dim must be 64 or 128, got %d", cache->head_dim);
+    if (num_heads == 0 || num_heads > 65535 || num_heads % (size_t)cache->kv_heads != 0)
+        return fail(RNB_B200_VALIDATION_FAILED, "attention: num_heads(%zu) must be a multiple of num_kv_heads(%d)", num_heads, cache->kv_heads);
+    if (!(q_type == cache->type || (q_type == RNB_B200_TYPE_F32 && cache->type == RNB_B200_TYPE_F16)))
+        return fail(RNB_B200_UNSUPPORTED, "paged attention: queries must be F32 on an F16 cache or of the cache's type, got type %u on %u", q_type, cache->type);
+    if (window < 0 || sinks < 0) return fail(RNB_B200_VALIDATION_FAILED, "paged attention: window and sinks must not be negative, got %d and %d", window, sinks);
+    if (!(scale - scale == 0.f)) return fail(RNB_B200_VALIDATION_FAILED, "paged attention: scale must be finite");
+    if (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < PK_WORKSPACE_BYTES)
+        return fail(RNB_B200_VALIDATION_FAILED, "paged attention: the workspace must be 256-byte aligned and hold %zu bytes, got %zu", PK_WORKSPACE_BYTES, workspace_bytes);
+    if (a->b.n_tokens > 0 && (!q || !out)) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
+    if (((uintptr_t)q | (uintptr_t)out) & 15u || q_stride % 8 || out_stride % 8 || ((uintptr_t)lse & 3u))
+        return fail(RNB_B200_VALIDATION_FAILED, "paged attention: q and out must be 16-byte aligned with strides that are multiples of 8, lse 4-byte aligned");
+    if (a->b.n_tokens > 1 && (q_stride < num_heads * cache->head_dim || out_stride < num_heads * cache->head_dim))
+        return fail(RNB_B200_VALIDATION_FAILED, "paged attention: q_stride and out_stride must be at least num_heads * head_dim");
+    a->q_type = q_type;
+    a->c_type = cache->type;
+    a->q = q;
+    a->q_stride = q_stride;
+    a->out_stride = out_stride;
+    a->heads = (int)num_heads;
+    a->window = window;
+    a->sinks = window ? sinks : 0;
+    a->scale = scale;
+    a->out = out;
+    a->workspace = workspace;
+    a->lse = lse;
+    return RNB_B200_OK;
+}
+
+template <class Q, class C>
+static int pk_attention_plain(const PkAttention &a, cudaStream_t s, int *err) {
+    const size_t items = (size_t)a.b.n_tokens * a.heads;
+    const dim3 grid((unsigned)((items + 3) / 4));
+    auto kernel = a.c.head_dim == 64 ? paged_attention_plain_kernel<Q, C, 64> : paged_attention_plain_kernel<Q, C, 128>;
+    RNB_CU(launch_k(kernel, grid, dim3(128), 0, s, a.c, a.b, (const Q *)a.q, a.q_stride, a.heads, a.scale, a.window, a.sinks, (Q *)a.out, a.out_stride, a.lse, err));
+    return RNB_B200_OK;
+}
+static int pk_attention(const PkAttention &a, cudaStream_t s) {
+    if (a.b.n_tokens == 0 || a.b.n_seq == 0) return RNB_B200_OK;
+    PkCall call;
+    RNB_TRY(call.rc);
+    int *err = call.st.dev_error;
+    if (a.q_type == RNB_B200_TYPE_F32) return pk_attention_plain<float, F16>(a, s, err);
+    return a.q_type == RNB_B200_TYPE_F16 ? pk_attention_plain<F16, F16>(a, s, err) : pk_attention_plain<Bf16, Bf16>(a, s, err);
+}
+
+// Nothing is thrown through the C entries.
+template <class F>
+static int pk_guarded(F &&f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc &) {
+        return fail(RNB_B200_OUT_OF_MEMORY, "paged cache: out of host memory");
+    }
+}
+
+}  // namespace rnb
+
+using namespace rnb;
+
+extern "C" {
+
+int rnb_b200_dev_paged_kv_append(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t src_type, const void *k_new, const void *v_new,
+                                 size_t src_stride, void *stream) {
+    return pk_append(cache, batch, src_type, k_new, v_new, src_stride, (cudaStream_t)stream);
+}
+int rnb_b200_dev_paged_kv_copy(const rnb_b200_paged_cache *cache, size_t n_layers, uint64_t layer_stride, const int32_t *src, const int32_t *dst, const int32_t *rows,
+                               size_t n_pages, void *stream) {
+    return pk_guarded([&] { return pk_copy(cache, n_layers, layer_stride, src, dst, rows, n_pages, (cudaStream_t)stream); });
+}
+size_t rnb_b200_paged_workspace_bytes(void) { return PK_WORKSPACE_BYTES; }
+int rnb_b200_paged_workspace_init(void *workspace, size_t workspace_bytes, void *stream) {
+    if (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < PK_WORKSPACE_BYTES)
+        return fail(RNB_B200_VALIDATION_FAILED, "paged attention: the workspace must be 256-byte aligned and hold %zu bytes, got %zu", PK_WORKSPACE_BYTES, workspace_bytes);
+    PkCall call;
+    RNB_TRY(call.rc);
+    RNB_CU(cudaMemsetAsync(workspace, 0, PK_WORKSPACE_BYTES, (cudaStream_t)stream));
+    return RNB_B200_OK;
+}
+int rnb_b200_dev_attention_decode_paged(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type, const void *q, size_t q_stride,
+                                        size_t num_heads, float scale, int32_t window, int32_t sinks, void *workspace, size_t workspace_bytes, void *out,
+                                        size_t out_stride, float *lse, void *stream) {
+    PkAttention a{};
+    RNB_TRY(pk_check_attention(cache, batch, q_type, q, q_stride, num_heads, scale, window, sinks, workspace, workspace_bytes, out, out_stride, lse, &a));
+    if (a.b.q_start) return fail(RNB_B200_VALIDATION_FAILED, "paged decode attention takes one token per sequence: q_start must be null");
+    return pk_attention(a, (cudaStream_t)stream);
+}
+int rnb_b200_dev_attention_prefill_paged(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type, const void *q, size_t q_stride,
+                                         size_t num_heads, float scale, int32_t window, int32_t sinks, void *workspace, size_t workspace_bytes, void *out,
+                                         size_t out_stride, float *lse, void *stream) {
+    PkAttention a{};
+    RNB_TRY(pk_check_attention(cache, batch, q_type, q, q_stride, num_heads, scale, window, sinks, workspace, workspace_bytes, out, out_stride, lse, &a));
+    return pk_attention(a, (cudaStream_t)stream);
+}
+
+}  // extern "C"

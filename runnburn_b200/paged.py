@@ -1,0 +1,252 @@
+"""A key-value cache in pages: attention over it, its writes and copies, and the book-keeping of its pages.
+
+The functions take device tensors of PyTorch (anything with `data_ptr`, `shape`, `stride`, `dtype` and `device` will do) and run on
+the given stream, else on PyTorch's current one; they do not synchronise and allocate nothing but a missing `out`, so calls with `out`
+can be captured into graphs.  Tables, lengths and starts are read when the work runs.  What they hold is checked on the
+device: a page outside the pool, a length that the table cannot hold or a start out of order sets the device error word
+(`ops.dev_error_flag()` returns 5) instead of touching memory outside.  The C ABI behind it is declared in include/rnb_b200.h.
+
+    pages = KvPages(n_pages, page_size)                    # host: who holds which page
+    cache = PagedCache(k, v)                               # [n_pages, page_size, kv_heads, head_dim] each, any strides
+    seq = pages.new()
+    pages.extend(seq, n)                                   # room for n tokens (and a copy, where a fork shares the last page)
+    table, kv_len = pages.tables([seq])                    # -> device
+    batch = PagedBatch(table, kv_len, q_start)
+    paged_kv_append(cache, batch, k_new, v_new)
+    attention_prefill_paged(cache, batch, q, scale, out=out, workspace=workspace)
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import _lib
+from ._lib import TYPE_BF16, TYPE_F16, TYPE_F32, check, load
+
+DEVICE_BAD_PAGE = 5
+
+_types: dict = {}
+
+
+def _type(t) -> int:
+    """GGML type id of a tensor's element type."""
+    if not _types:
+        import torch
+        _types.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16})
+    try:
+        return _types[t.dtype]
+    except KeyError:
+        raise TypeError(f"expected float32, float16 or bfloat16, got {t.dtype}") from None
+
+
+def _on_device(*tensors):
+    device = tensors[0].device
+    for t in tensors:
+        if t.device != device or device.type != "cuda":
+            raise ValueError(f"tensors have to be on one CUDA device, got {t.device} and {device}")
+    return device
+
+
+def _stream(device, stream):
+    if stream is not None:
+        return stream
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _ints(t, what: str, ndim: int):
+    if str(t.dtype) != "torch.int32" or t.dim() != ndim or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{what} has to be an int32 tensor of {ndim} dimension(s), its last one contiguous")
+    return t
+
+
+class PagedCache:
+    """The pools of a layer's keys and values, [n_pages, page_size, kv_heads, head_dim], or of several layers, [n_layers, ...]; strides are
+    the tensors' own (the same for both), so views of one buffer and other orders of the dimensions are taken as they are."""
+
+    def __init__(self, k, v):
+        if k.dim() not in (4, 5) or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
+            raise ValueError("k and v have to be alike, [n_pages, page_size, kv_heads, head_dim] or with a dimension of layers before these")
+        if k.shape[-1] > 1 and k.stride(-1) != 1:
+            raise ValueError("the elements of a head's row have to be contiguous")
+        self.device = _on_device(k, v)
+        self.k, self.v = k, v
+        self.n_layers, self.layer_stride = (k.shape[0], k.stride(0)) if k.dim() == 5 else (1, 0)
+        self.n_pages, self.page_size, self.kv_heads, self.head_dim = k.shape[-4:]
+        page, pos, head = k.stride()[-4:-1]
+        self._c = _lib.PagedCache(_type(k), self.head_dim, self.kv_heads, self.page_size, self.n_pages, page, pos, head, k.data_ptr(), v.data_ptr())
+        self._ref = C.byref(self._c)
+
+    def layer(self, i: int) -> "PagedCache":
+        """The cache of one layer, for the calls that take one."""
+        return PagedCache(self.k[i], self.v[i])
+
+
+class PagedBatch:
+    """Sequences of a call: their page tables [n_seq, max_pages], positions in the cache [n_seq] (the call's own tokens included) and, unless
+    every sequence has one token, where their tokens start in the token matrices, [n_seq + 1]; all int32 on the device.  n_tokens: rows of
+    the token matrices (needed with q_start; more rows than q_start[n_seq] are padding).  The tensors may change in place between calls."""
+
+    def __init__(self, table, kv_len, q_start=None, n_tokens: int | None = None):
+        _ints(table, "table", 2), _ints(kv_len, "kv_len", 1)
+        n_seq = table.shape[0]
+        if kv_len.shape[0] != n_seq:
+            raise ValueError(f"table has {n_seq} sequences, kv_len {kv_len.shape[0]}")
+        self.device = _on_device(table, kv_len, *(() if q_start is None else (q_start,)))
+        if q_start is not None:
+            if _ints(q_start, "q_start", 1).shape[0] != n_seq + 1:
+                raise ValueError(f"q_start has to have {n_seq + 1} entries, got {q_start.shape[0]}")
+            if n_tokens is None:
+                raise ValueError("n_tokens is needed with q_start")
+        elif n_tokens is None:
+            n_tokens = n_seq
+        self.table, self.kv_len, self.q_start, self.n_tokens = table, kv_len, q_start, n_tokens
+        self._c = _lib.PagedBatch(table.data_ptr(), max(table.stride(0), table.shape[1]) if n_seq < 2 else table.stride(0), table.shape[1], n_seq, n_tokens, kv_len.data_ptr(),
+                                  None if q_start is None else q_start.data_ptr())
+        self._ref = C.byref(self._c)
+
+
+class Workspace:
+    """Scratch of the attention calls.  Calls that may overlap on the GPU (other streams) need one each."""
+
+    def __init__(self, device=None, stream=None):
+        import torch
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        n = load().rnb_b200_paged_workspace_bytes()
+        self.buffer = torch.empty(n, dtype=torch.uint8, device=device)
+        self.device, self.ptr, self.bytes = self.buffer.device, self.buffer.data_ptr(), n
+        check(load().rnb_b200_paged_workspace_init(self.ptr, n, _stream(self.device, stream)))
+
+
+def _rows(t, what: str, tokens: int, heads: int | None, dim: int):
+    """[tokens, heads, dim] with contiguous heads; the stride from one token to the next."""
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what} has to be [{tokens}, {heads or 'heads'}, {dim}], got {tuple(shape)}")
+    a, b, c = t.stride()
+    if c != 1 or (b != dim and shape[1] > 1):
+        raise ValueError(f"{what}: the heads of a token have to be contiguous")
+    return a if tokens > 1 else shape[1] * dim
+
+
+def _attention(fn, cache, batch, q, scale, out, window, sinks, lse, workspace, stream):
+    n, dim = batch.n_tokens, cache.head_dim
+    q_stride = _rows(q, "q", n, None, dim)
+    heads = q.shape[1]
+    if out is None:
+        out = q.new_empty(q.shape)
+    out_stride = _rows(out, "out", n, heads, dim)
+    if out.dtype != q.dtype:
+        raise ValueError(f"out has to have the queries' type {q.dtype}, got {out.dtype}")
+    device = _on_device(q, out, cache, batch, workspace)
+    if lse is not None:
+        _on_device(q, lse)
+        if str(lse.dtype) != "torch.float32" or tuple(lse.shape) != (n, heads) or not lse.is_contiguous():
+            raise ValueError(f"lse has to be a contiguous float32 tensor [{n}, {heads}]")
+        lse = lse.data_ptr()
+    check(fn(cache._ref, batch._ref, _type(q), q.data_ptr(), q_stride, heads, scale, window, sinks, workspace.ptr, workspace.bytes, out.data_ptr(), out_stride, lse,
+             _stream(device, stream)))
+    return out
+
+
+def attention_decode_paged(cache: PagedCache, batch: PagedBatch, q, scale: float, *, workspace: Workspace, out=None, window: int = 0, sinks: int = 0, lse=None, stream=None):
+    """Attention of one new token per sequence, q [n_seq, heads, head_dim]: softmax(scale q.K^T) V over the sequence's positions, with a
+    window over its last `window` positions and its first `sinks`.  Returns `out` (as q); lse, float32 [n_seq, heads], receives the logarithms
+    of the sums.  A sequence of length 0 gets zeros and -inf."""
+    return _attention(load().rnb_b200_dev_attention_decode_paged, cache, batch, q, scale, out, window, sinks, lse, workspace, stream)
+
+
+def attention_prefill_paged(cache: PagedCache, batch: PagedBatch, q, scale: float, *, workspace: Workspace, out=None, window: int = 0, sinks: int = 0, lse=None, stream=None):
+    """Causal attention of the batch's tokens, q [n_tokens, heads, head_dim]: the last tokens of every sequence's positions are the call's, and
+    a token at position p sees positions up to p (with a window, those after p - window and the first `sinks`)."""
+    return _attention(load().rnb_b200_dev_attention_prefill_paged, cache, batch, q, scale, out, window, sinks, lse, workspace, stream)
+
+
+def paged_kv_append(cache: PagedCache, batch: PagedBatch, k_new, v_new, *, stream=None) -> None:
+    """Writes the rows of the batch's tokens, [n_tokens, kv_heads, head_dim], to their places in the pages, rounded to the cache's type."""
+    stride = _rows(k_new, "k_new", batch.n_tokens, cache.kv_heads, cache.head_dim)
+    if _rows(v_new, "v_new", batch.n_tokens, cache.kv_heads, cache.head_dim) != stride or k_new.dtype != v_new.dtype:
+        raise ValueError("k_new and v_new have to be alike")
+    device = _on_device(k_new, v_new, cache, batch)
+    check(load().rnb_b200_dev_paged_kv_append(cache._ref, batch._ref, _type(k_new), k_new.data_ptr(), v_new.data_ptr(), stride, _stream(device, stream)))
+
+
+def _host(a) -> np.ndarray:
+    return np.ascontiguousarray(a, dtype=np.int32).ravel()
+
+
+def paged_kv_copy(cache: PagedCache, src, dst, rows=None, *, stream=None) -> None:
+    """Copies page src[i] to page dst[i] in all layers, its first rows[i] positions (None: all).  The lists are host integers.  A page may
+    be copied to several places; one that is written must be written once and not read."""
+    src, dst, rows = _host(src), _host(dst), None if rows is None else _host(rows)
+    if src.size != dst.size or (rows is not None and rows.size != src.size):
+        raise ValueError("src, dst and rows have to be equally long")
+    check(load().rnb_b200_dev_paged_kv_copy(cache._ref, cache.n_layers, cache.layer_stride, src.ctypes.data, dst.ctypes.data, None if rows is None else rows.ctypes.data,
+                                            src.size, _stream(cache.device, stream)))
+
+
+class KvPages:
+    """Who holds which page, on the host.  Sequences are numbers; `extend` and `compact` return the copies, as (src, dst, rows) for
+    `paged_kv_copy`, to make before the cache is used again."""
+
+    def __init__(self, n_pages: int, page_size: int):
+        h = C.c_void_p()
+        check(load().rnb_b200_kv_pages_create(n_pages, page_size, C.byref(h)))
+        self._h, self.n_pages, self.page_size = h, n_pages, page_size
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            load().rnb_b200_kv_pages_destroy(self._h)
+            self._h = None
+
+    __del__ = close
+
+    def info(self) -> dict:
+        i = _lib.KvPagesInfo()
+        check(load().rnb_b200_kv_pages_get_info(self._h, C.byref(i)))
+        return {n: getattr(i, n) for n, _ in i._fields_}
+
+    def new(self) -> int:
+        s = C.c_int32()
+        check(load().rnb_b200_kv_pages_new(self._h, C.byref(s)))
+        return s.value
+
+    def extend(self, seq: int, n_new: int):
+        """Room for n_new more positions; ([], [], []) or the one copy that parts a shared last page."""
+        n, src, dst, rows = (C.c_int32() for _ in range(4))
+        check(load().rnb_b200_kv_pages_extend(self._h, seq, n_new, C.byref(n), C.byref(src), C.byref(dst), C.byref(rows)))
+        return ([src.value], [dst.value], [rows.value]) if n.value else ([], [], [])
+
+    def fork(self, seq: int) -> int:
+        s = C.c_int32()
+        check(load().rnb_b200_kv_pages_fork(self._h, seq, C.byref(s)))
+        return s.value
+
+    def truncate(self, seq: int, length: int) -> None:
+        check(load().rnb_b200_kv_pages_truncate(self._h, seq, length))
+
+    def release(self, seq: int, window: int, sinks: int = 0) -> None:
+        """Frees the pages that neither the window of the next token nor the sinks reach."""
+        check(load().rnb_b200_kv_pages_release(self._h, seq, window, sinks))
+
+    def free(self, seq: int) -> None:
+        check(load().rnb_b200_kv_pages_free(self._h, seq))
+
+    def compact(self):
+        """Moves the used pages to the front of the pool; (src, dst, None)."""
+        src, dst = (np.empty(max(1, self.n_pages // 2), np.int32) for _ in range(2))
+        n = C.c_size_t()
+        check(load().rnb_b200_kv_pages_compact(self._h, src.ctypes.data, dst.ctypes.data, self.n_pages // 2, C.byref(n)))
+        return src[:n.value], dst[:n.value], None
+
+    def tables(self, seqs, max_pages: int | None = None):
+        """(int32 [n, max_pages], int32 [n]): page tables and lengths on the host, unused entries -1."""
+        seqs = _host(seqs)
+        lens = np.empty(seqs.size, np.int32)
+        check(load().rnb_b200_kv_pages_tables(self._h, seqs.ctypes.data, seqs.size, None, 0, lens.ctypes.data))
+        if max_pages is None:
+            max_pages = max(1, -(-int(lens.max(initial=0)) // self.page_size))
+        table = np.empty((seqs.size, max_pages), np.int32)
+        check(load().rnb_b200_kv_pages_tables(self._h, seqs.ctypes.data, seqs.size, table.ctypes.data, max_pages, None))
+        return table, lens

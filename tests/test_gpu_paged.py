@@ -1,0 +1,450 @@
+"""The paged cache on the GPU against its definition in 64 bits (tests/paged_util.py): sizes at the edges of pages and tiles, sequences of
+length zero, windows and sinks, layouts, and not-a-numbers in every place that no query sees."""
+import math
+
+import pytest
+
+import paged_util as pu
+from paged_util import LSE_OFF, TYPES, tolerance, worst
+
+pytestmark = pytest.mark.gpu
+
+PAIRS = [("f32", "f16"), ("f16", "f16"), ("bf16", "bf16")]
+EDGES = [0, 1, 7, 8, 9, 63, 64, 65, 127, 128, 129, 191, 0]
+
+
+@pytest.fixture(scope="module")
+def P():
+    import torch  # noqa: F401
+
+    from runnburn_b200 import build
+    build.build_library()
+    from runnburn_b200 import ops, paged
+    ops.open()
+    ops.dev_error_flag()
+    return paged
+
+
+@pytest.fixture(scope="module")
+def ws(P):
+    return P.Workspace()
+
+
+@pytest.fixture(autouse=True)
+def no_flag(P):
+    from runnburn_b200 import ops
+    yield
+    assert ops.dev_error_flag() == 0
+
+
+class Case:
+    def __init__(self, P, kv_len, new=None, heads=4, kv_heads=2, dim=128, page=16, q="f32", cache="f16", window=0, sinks=0, order="page pos head", seed=0, nan=True, padding=0,
+                 gain=1.0):
+        import torch
+        g, h = torch.Generator("cuda").manual_seed(seed + 1), torch.Generator().manual_seed(seed)
+        self.P, self.kv, self.new, self.page = P, kv_len, new or [1] * len(kv_len), page
+        n_pages = sum(-(-n // page) for n in kv_len) + 3
+        self.table = pu.tables(kv_len, page, n_pages, h)
+        self.k, self.v = pu.pools(n_pages, page, kv_heads, dim, TYPES[cache], g, order)
+        if nan:
+            for t in (self.k, self.v):
+                pu.poison(t, self.table, page, kv_len, self.new, window, sinks)
+        self.starts = [0]
+        for n in self.new:
+            self.starts.append(self.starts[-1] + n)
+        self.tokens = self.starts[-1] + padding
+        self.q = (torch.randn(self.tokens, heads, dim, device="cuda", generator=g) * gain).to(TYPES[q])
+        self.scale, self.window, self.sinks = dim ** -0.5, window, sinks
+        self.cache = P.PagedCache(self.k, self.v)
+        i32 = dict(dtype=torch.int32, device="cuda")
+        self.batch = P.PagedBatch(self.table.cuda(), torch.tensor(kv_len, **i32), None if new is None else torch.tensor(self.starts, **i32), self.tokens)
+        self.call = P.attention_decode_paged if new is None else P.attention_prefill_paged
+        self.lse = torch.full((self.tokens, heads), 7.0, device="cuda")
+
+    def run(self, ws, **kw):
+        return self.call(self.cache, self.batch, self.q, self.scale, window=self.window, sinks=self.sinks, workspace=ws, **({"lse": self.lse} | kw))
+
+    def want(self):
+        return pu.attention(self.q, self.k, self.v, self.table, self.page, self.kv, self.starts, self.scale, self.window, self.sinks)
+
+    def check(self, got, more=1.0):
+        import torch
+        out, lse, mass = self.want()
+        n = self.starts[-1]
+        assert not torch.isnan(got[:n]).any()
+        tol = tolerance(out, mass, got.dtype) * more
+        assert (off := worst(got[:n], out[:n], tol[:n])) <= 1, off
+        empty = lse[:n] == -math.inf
+        assert torch.equal(self.lse[:n] == -math.inf, empty) and not got[:n][empty].any()
+        d = (self.lse[:n].double() - lse[:n])[~empty].abs()
+        assert bool((d <= more * LSE_OFF + lse[:n][~empty].abs() * 2.0 ** -22).all()), float(d.max())
+
+
+# ---- one token per sequence ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q,cache", PAIRS)
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (1, 1), (8, 1), (7, 1), (9, 1), (32, 2), (40, 1), (15, 3), (64, 1), (130, 2)])
+def test_decode_heads(P, ws, heads, kv_heads, dim, q, cache):
+    c = Case(P, EDGES, heads=heads, kv_heads=kv_heads, dim=dim, q=q, cache=cache, seed=heads)
+    c.check(c.run(ws))
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("q,cache,dim", [("f32", "f16", 128), ("bf16", "bf16", 64)])
+@pytest.mark.parametrize("order", ["page pos head", "page head pos", "head page pos", "pos head page"])
+def test_decode_pages_and_layouts(P, ws, page, q, cache, dim, order):
+    c = Case(P, EDGES + [255, 256, 257, 700], page=page, q=q, cache=cache, dim=dim, order=order, seed=page)
+    c.check(c.run(ws))
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (64, 0), (100, 4), (63, 65), (128, 64), (500, 1), (1, 1000), (2000, 3)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_decode_windows(P, ws, window, sinks, dim):
+    c = Case(P, EDGES + [500, 501, 640, 777, 1500], window=window, sinks=sinks, dim=dim, page=32, seed=window)
+    c.check(c.run(ws))
+
+
+@pytest.mark.parametrize("kv_len,heads,kv_heads", [([1], 8, 8), ([0], 8, 8), ([37], 2, 2), ([9000], 8, 1), ([20011], 16, 2), ([9000, 3, 0, 12345], 8, 2), ([5000] * 9, 4, 4),
+                                                   ([70001], 1, 1), (list(range(300)), 4, 1), ([1] * 700, 2, 2), ([4000, 0, 0, 0, 1], 32, 8)])
+@pytest.mark.parametrize("q,cache,dim", [("f32", "f16", 128), ("f16", "f16", 64), ("bf16", "bf16", 128)])
+def test_decode_split_and_joined(P, ws, kv_len, heads, kv_heads, q, cache, dim):
+    c = Case(P, kv_len, heads=heads, kv_heads=kv_heads, page=64, q=q, cache=cache, dim=dim, seed=len(kv_len))
+    first = c.run(ws)
+    c.check(first)
+    assert (c.run(ws) == first).all()   # the sums' order does not depend on who comes first
+
+
+# ---- prompts ------------------------------------------------------------------------------------------------------------
+PROMPTS = [
+    ([1], [1]), ([5], [5]), ([64], [64]), ([129], [65]), ([300, 0, 77], [33, 0, 77]), ([1000, 130, 7, 64], [1, 130, 2, 63]), ([257], [256]), ([513, 700], [513, 31]),
+    ([2100], [16]), ([6000, 0, 40], [3, 0, 40]), ([40, 8], [41, 9]), ([5, 600], [70, 1]),
+]
+
+
+@pytest.mark.parametrize("kv,new", PROMPTS)
+@pytest.mark.parametrize("q,cache,dim", [("f32", "f16", 128), ("f32", "f16", 64), ("f16", "f16", 128), ("bf16", "bf16", 64), ("bf16", "bf16", 128)])
+def test_prompts(P, ws, kv, new, q, cache, dim):
+    """Among them tokens before position 0 (more tokens than positions), which see nothing."""
+    c = Case(P, kv, new, q=q, cache=cache, dim=dim, seed=sum(kv))
+    c.check(c.run(ws))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (8, 1), (7, 1), (5, 5), (12, 4), (32, 1), (48, 1), (130, 2), (160, 1)])
+@pytest.mark.parametrize("q,cache", [("f32", "f16"), ("bf16", "bf16")])
+def test_prompt_heads(P, ws, heads, kv_heads, q, cache):
+    c = Case(P, [200, 0, 333, 64], [70, 0, 1, 64], heads=heads, kv_heads=kv_heads, q=q, cache=cache, seed=heads)
+    c.check(c.run(ws))
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("order", ["page pos head", "page head pos", "head page pos", "pos head page"])
+@pytest.mark.parametrize("q,cache,dim", [("f32", "f16", 128), ("f16", "f16", 64)])
+def test_prompt_pages_and_layouts(P, ws, page, order, q, cache, dim):
+    c = Case(P, [300, 77, 640], [129, 77, 5], page=page, order=order, q=q, cache=cache, dim=dim, seed=page)
+    c.check(c.run(ws))
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (64, 0), (100, 4), (63, 65), (128, 64), (300, 1), (1, 1000), (2000, 3), (37, 130)])
+@pytest.mark.parametrize("q,cache,dim", [("f32", "f16", 128), ("bf16", "bf16", 64)])
+def test_prompt_windows(P, ws, window, sinks, q, cache, dim):
+    c = Case(P, [700, 129, 1500, 64], [700, 1, 140, 64], page=32, window=window, sinks=sinks, q=q, cache=cache, dim=dim, seed=window)
+    c.check(c.run(ws))
+
+
+@pytest.mark.parametrize("q,cache", PAIRS)
+def test_long_prompt(P, ws, q, cache):
+    """Sums over many tiles."""
+    c = Case(P, [9001], [300], heads=2, kv_heads=1, page=64, q=q, cache=cache)
+    c.check(c.run(ws))
+
+
+# ---- both ---------------------------------------------------------------------------------------------------------------
+BOTH = [(None, [300, 0, 77, 2000]), ([33, 0, 77, 200], [300, 0, 77, 2000])]
+
+
+@pytest.mark.parametrize("new,kv", BOTH)
+@pytest.mark.parametrize("q,cache", PAIRS)
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-3])
+def test_any_scale(P, ws, new, kv, q, cache, scale):
+    c = Case(P, kv, new, q=q, cache=cache)
+    c.scale = scale
+    c.check(c.run(ws), more=3)   # |scores| of 0.2 * 81 instead of 7
+
+
+@pytest.mark.parametrize("new,kv", BOTH)
+@pytest.mark.parametrize("gain", [1e6, 1e-6, 3e30])
+def test_f32_queries_of_any_size(P, ws, new, kv, gain):
+    """Queries far outside of f16: what counts is the score."""
+    c = Case(P, kv, new, gain=gain)
+    c.scale = 128 ** -0.5 / gain
+    c.check(c.run(ws))
+
+
+@pytest.mark.parametrize("new,kv", BOTH)
+@pytest.mark.parametrize("q,cache", PAIRS)
+@pytest.mark.parametrize("way", ["growing", "falling", "sharp"])
+def test_maxima_that_move(P, ws, new, kv, q, cache, way):
+    """Scores that grow or fall by some 60 over the sequence, and single keys that take everything.  A score of size 60 has errors nine times
+    those of the bound's 7."""
+    import torch
+    c = Case(P, kv, new, q=q, cache=cache, nan=False)
+    c.q += 1.0
+    for s, n in enumerate(kv):
+        j = torch.arange(n)
+        page, row = c.table[s, j // c.page].long().cuda(), (j % c.page).cuda()
+        ramp = torch.linspace(0, 5, max(n, 2), device="cuda")[:n]
+        ramp = ramp.flip(0) if way == "falling" else ramp
+        if way == "sharp":
+            ramp = torch.where(torch.arange(n, device="cuda") % 50 == 17, 5.0, 0.0)
+        c.k[page, row] = (c.k[page, row].float() + ramp[:, None, None]).to(c.k.dtype)
+    c.check(c.run(ws), more=9)
+
+
+@pytest.mark.parametrize("new,kv", BOTH)
+@pytest.mark.parametrize("q", ["f32", "bf16"])
+def test_views_and_padding(P, ws, new, kv, q):
+    """Queries and outputs as slices of wider rows; what lies beside and behind the batch's tokens stays."""
+    import torch
+    c = Case(P, kv, new, q=q, cache="f16" if q == "f32" else "bf16", padding=5 if new else 0)
+    n = c.starts[-1]
+    wide_q, wide_o = torch.full((c.tokens, 16, 128), math.nan, device="cuda", dtype=c.q.dtype), torch.full((c.tokens, 9, 128), 3.0, device="cuda", dtype=c.q.dtype)
+    wide_q[:n, 2:6] = c.q[:n]
+    c.q = wide_q[:, 2:6]
+    got = c.run(ws, out=wide_o[:, 3:7])
+    c.check(got)
+    assert (wide_o[:, :3] == 3).all() and (wide_o[:, 7:] == 3).all() and (wide_o[n:] == 3).all() and (c.lse[n:] == 7).all()
+    assert torch.equal(c.run(ws, lse=None)[:n], got[:n])
+
+
+@pytest.mark.parametrize("new,kv", BOTH)
+def test_values_that_are_not_finite_where_seen(P, ws, new, kv):
+    """An infinite or undefined value reaches the queries that see it, in its own dimension, and no other."""
+    import torch
+    c = Case(P, kv, new, heads=4, kv_heads=2)
+    spots = [(0, 290, 1, 5, math.inf), (0, 280, 0, 9, math.nan), (3, 1990, 1, 77, -math.inf), (3, 1855, 0, 64, math.nan), (2, 60, 0, 0, math.inf)]
+    clean = c.v.clone()
+    for s, j, h, d, x in spots:
+        c.v[c.table[s, j // c.page], j % c.page, h, d] = x
+        clean[c.table[s, j // c.page], j % c.page, h, d] = 0
+    got = c.run(ws)
+    out, _, mass = pu.attention(c.q, c.k, clean, c.table, c.page, c.kv, c.starts, c.scale)
+    strange = torch.zeros_like(got, dtype=torch.bool)
+    for s, j, h, d, x in spots:
+        n = c.new[s]
+        for i in range(n):
+            if c.kv[s] - n + i >= j:
+                row = got[c.starts[s] + i, 2 * h:2 * h + 2, d]
+                assert (torch.isnan(row).all() if x != x else (row == x).all()), (s, j, i, row)
+                strange[c.starts[s] + i, 2 * h:2 * h + 2, d] = True
+    ok = torch.where(strange, 0.0, got.double())
+    assert worst(ok, torch.where(strange, 0.0, out), tolerance(out, mass, got.dtype)) <= 1
+
+
+@pytest.mark.parametrize("new,kv", BOTH)
+def test_graphs_streams_and_one_workspace(P, new, kv):
+    """A captured call follows what its buffers hold when it is replayed; two graphs take turns on a workspace, with eager calls between."""
+    import torch
+    cases = [Case(P, kv, new, seed=1), Case(P, kv[::-1], new[::-1] if new else None, heads=16, kv_heads=1, q="bf16", cache="bf16", dim=64, seed=2)]
+    ws, graphs, outs = P.Workspace(), [], []
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for c in cases:
+            out = torch.empty_like(c.q)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                c.run(ws, out=out)
+            graphs.append(g), outs.append(out)
+        for _ in range(2):
+            for c, g, out in zip(cases, graphs, outs):
+                out.zero_()
+                g.replay()
+                eager = c.run(ws)
+                g.replay()
+                assert torch.equal(out, eager)
+    stream.synchronize()
+    for c, out in zip(cases, outs):
+        c.check(out)
+    # other lengths, pages and queries in the same buffers
+    c = cases[0]
+    c.kv = [max(0, n - 7) for n in kv]
+    c.batch.kv_len.copy_(torch.tensor(c.kv, dtype=torch.int32))
+    c.table = c.table.flip(1).contiguous() if new is None else c.table
+    if new is None:   # every entry is used by now
+        c.table = torch.randint(0, c.k.shape[0], c.table.shape, dtype=torch.int32, generator=torch.Generator().manual_seed(3))
+        c.k.normal_(), c.v.normal_()
+        c.batch.table.copy_(c.table)
+    c.q.normal_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        graphs[0].replay()
+    stream.synchronize()
+    c.check(outs[0])
+
+
+@pytest.mark.parametrize("new,kv", BOTH)
+def test_what_points_outside_is_flagged(P, ws, new, kv):
+    """Entries out of range, lengths beyond the table and starts out of order are reported, and the other sequences come out right."""
+    import torch
+    from runnburn_b200 import ops
+    for spoil in ("entry", "negative entry", "length", "negative length") + (("start", "too many tokens") if new else ()):
+        c = Case(P, kv, new, nan=False)
+        if "entry" in spoil:
+            c.batch.table[3, 1] = -1 if "negative" in spoil else c.k.shape[0]
+        elif "length" in spoil:
+            c.batch.kv_len[3] = -5 if "negative" in spoil else c.table.shape[1] * c.page + 1
+        elif spoil == "start":
+            c.batch.q_start[3] = c.batch.q_start[4] + 3
+        else:
+            c.batch.q_start[4] = c.tokens + 40
+        got = c.run(ws)
+        torch.cuda.synchronize()
+        assert ops.dev_error_flag() == P.DEVICE_BAD_PAGE, spoil
+        out, _, mass = c.want()
+        m = c.starts[2]
+        assert worst(got[:m], out[:m], tolerance(out, mass, got.dtype)[:m]) <= 1
+
+
+def test_offsets_past_32_bits(P, ws):
+    """Pages 2^31 elements and more apart."""
+    import torch
+    stride, page, dim = 2 ** 31 + 64, 16, 64
+    big = torch.empty(3 * stride, dtype=torch.float16, device="cuda")
+    for new in (None, [9]):
+        c = Case(P, [40], new, kv_heads=1, heads=2, dim=dim, page=page, nan=False)
+        k, v = (big[o:].as_strided((3, page, 1, dim), (stride, 2 * dim, dim, 1)) for o in (0, dim))
+        c.table = torch.tensor([[2, 0, 1]], dtype=torch.int32)
+        c.batch.table.copy_(c.table)
+        k.copy_(torch.randn(k.shape)), v.copy_(torch.randn(v.shape))
+        c.k, c.v, c.cache = k, v, P.PagedCache(k, v)
+        c.check(c.run(ws))
+    k_new = torch.randn(1, 1, dim, device="cuda")
+    one = P.PagedBatch(c.batch.table[:, :2], torch.tensor([16], dtype=torch.int32, device="cuda"))
+    P.paged_kv_append(c.cache, one, k_new, -k_new)
+    assert torch.equal(k[2, 15], k_new[0].half()) and torch.equal(v[2, 15], -k_new[0].half())
+    P.paged_kv_copy(c.cache, [2], [1])
+    assert torch.equal(k[1], k[2]) and torch.equal(v[1], v[2])
+
+
+# ---- append and copy ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("src,cache", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("page,kv_heads,dim,order", [(16, 8, 128, "page pos head"), (8, 1, 64, "page head pos"), (64, 3, 8, "head page pos"), (256, 5, 200, "pos head page"),
+                                                     (32, 40, 128, "page pos head")])
+def test_append(P, src, cache, page, kv_heads, dim, order):
+    """Every row to its place, to the bit, and nothing else is touched."""
+    import torch
+    g, h = torch.Generator("cuda").manual_seed(5), torch.Generator().manual_seed(5)
+    for new, kv in (([1, 1, 1, 1], [1, 17, 400, 256]), ([3, 0, 150, 40], [3, 0, 300, 41])):
+        n_pages = sum(-(-n // page) for n in kv) + 2
+        table = pu.tables(kv, page, n_pages, h)
+        k, v = pu.pools(n_pages, page, kv_heads, dim, TYPES[cache], g, order)
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        wide = torch.randn(starts[-1] + 3, 2 * kv_heads + 1, dim, device="cuda", generator=g) * 300
+        wide[0, 0, :8] = torch.tensor([math.inf, -math.inf, 1e9, 65519.0, 65520.0, 1e-8, 2.0 ** -25, 6e-8])
+        wide = wide.to(TYPES[src])
+        k_new, v_new = wide[:, :kv_heads], wide[:, kv_heads + 1:]
+        want_k, want_v = k.clone(), v.clone()
+        for s, (m, n) in enumerate(zip(new, kv)):
+            for i in range(m):
+                j = n - m + i
+                want_k[table[s, j // page], j % page] = k_new[starts[s] + i].to(k.dtype)
+                want_v[table[s, j // page], j % page] = v_new[starts[s] + i].to(v.dtype)
+        i32 = dict(dtype=torch.int32, device="cuda")
+        decode = new == [1] * 4
+        batch = P.PagedBatch(table.cuda(), torch.tensor(kv, **i32), None if decode else torch.tensor(starts, **i32), starts[-1] + (0 if decode else 3))
+        m = batch.n_tokens
+        P.paged_kv_append(P.PagedCache(k, v), batch, k_new[:m], v_new[:m])
+        assert torch.equal(k, want_k) and torch.equal(v, want_v)
+
+
+def test_append_flags_what_has_no_place(P):
+    import torch
+    from runnburn_b200 import ops
+    for kv, table, new in (([40], [[0, 1]], None), ([0], [[0, 1]], None), ([20], [[0, 9]], None), ([20], [[0, -1]], None), ([2], [[0, 1]], [0, 3])):
+        k, v = torch.zeros(4, 16, 1, 64, device="cuda", dtype=torch.float16), torch.zeros(4, 16, 1, 64, device="cuda", dtype=torch.float16)
+        i32 = dict(dtype=torch.int32, device="cuda")
+        n = 1 if new is None else 3
+        batch = P.PagedBatch(torch.tensor(table, **i32), torch.tensor(kv, **i32), None if new is None else torch.tensor(new, **i32), n)
+        P.paged_kv_append(P.PagedCache(k, v), batch, torch.ones(n, 1, 64, device="cuda"), torch.ones(n, 1, 64, device="cuda"))
+        torch.cuda.synchronize()
+        assert ops.dev_error_flag() == P.DEVICE_BAD_PAGE
+        assert int(k.sum()) == (2 * 64 if new else 64 if kv == [40] else 0)
+
+
+@pytest.mark.parametrize("layers,order", [(1, "page pos head"), (3, "page pos head"), (2, "page head pos"), (2, "pos head page")])
+@pytest.mark.parametrize("page,kv_heads,dim,pages,n", [(16, 8, 128, 40, 17), (8, 1, 8, 300, 140), (256, 3, 72, 9, 4), (64, 2, 64, 5000, 2500)])
+def test_copy(P, layers, order, page, kv_heads, dim, pages, n):
+    import torch
+    g = torch.Generator().manual_seed(n)
+    both = [pu.pools(pages, page, kv_heads, dim, torch.bfloat16, torch.Generator("cuda").manual_seed(i), order) for i in range(layers)]
+    k, v = (torch.stack([b[i] for b in both]) if order == "page pos head" else torch.stack([b[i].permute(2, 0, 1, 3) for b in both]).permute(0, 2, 3, 1, 4) for i in range(2))
+    if layers == 1:
+        k, v = k[0], v[0]
+    perm = torch.randperm(pages, generator=g)
+    src, dst, rows = perm[:n].clone(), perm[n:2 * n], torch.randint(0, page + 1, (n,), generator=g)
+    src[-1] = src[0]   # one page to two places
+    for use in (None, rows):
+        want_k, want_v = k.clone(), v.clone()
+        for w, t in ((want_k, k), (want_v, v)):
+            a = w if layers > 1 else w[None]
+            b = t if layers > 1 else t[None]
+            keep = torch.ones(n, page, dtype=torch.bool) if use is None else torch.arange(page) < use[:, None]
+            a[:, dst.cuda()] = torch.where(keep.cuda()[None, :, :, None, None], b[:, src.cuda()], b[:, dst.cuda()])
+        P.paged_kv_copy(P.PagedCache(k, v), src, dst, use)
+        assert torch.equal(k, want_k) and torch.equal(v, want_v)
+
+
+# ---- together -----------------------------------------------------------------------------------------------------------
+def test_a_server_s_steps(P, ws):
+    """Two prompts with a common beginning, then steps with window attention: append, attention, fork, copy on write, release, free and
+    compaction, against sequences that are kept whole."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(9)
+    L, page, kvh, H, D, window, sinks, n_pages = 2, 16, 2, 8, 64, 40, 3, 30
+    pool = torch.full((2, L, n_pages, page, kvh, D), math.nan, device="cuda", dtype=torch.bfloat16)
+    cache, pages = P.PagedCache(pool[0], pool[1]), P.KvPages(n_pages, page)
+    whole = {}   # seq -> rows [L][2][n][kvh][D]
+    i32 = dict(dtype=torch.int32, device="cuda")
+
+    def step(seqs, new):
+        for s, n in zip(seqs, new):
+            P.paged_kv_copy(cache, *pages.extend(s, n))
+        table, lens = pages.tables(seqs)
+        start = torch.tensor([0] + new).cumsum(0).to(torch.int32)
+        batch = P.PagedBatch(torch.tensor(table, **i32), torch.tensor(lens, **i32), None if new == [1] * len(new) else start.cuda(), sum(new))
+        for layer in range(L):
+            q, k, v = (torch.randn(sum(new), h, D, device="cuda", generator=g).bfloat16() for h in (H, kvh, kvh))
+            one = cache.layer(layer)
+            P.paged_kv_append(one, batch, k, v)
+            out = (P.attention_decode_paged if batch.q_start is None else P.attention_prefill_paged)(one, batch, q, D ** -0.5, window=window, sinks=sinks, workspace=ws)
+            for i, s in enumerate(seqs):
+                lo, hi = int(start[i]), int(start[i + 1])
+                rows = whole.setdefault(s, [[torch.empty(0, kvh, D, device="cuda", dtype=torch.bfloat16)] * 2 for _ in range(L)])
+                rows[layer] = [torch.cat([rows[layer][0], k[lo:hi]]), torch.cat([rows[layer][1], v[lo:hi]])]
+                n = rows[layer][0].shape[0]
+                one_page = -(-n // 8) * 8
+                kk, vv = (torch.cat([t, torch.zeros(one_page - n, kvh, D, device="cuda", dtype=t.dtype)])[None] for t in rows[layer])
+                want, _, mass = pu.attention(q[lo:hi], kk, vv, torch.zeros(1, 1, dtype=torch.int32), one_page, [n], [0, hi - lo], D ** -0.5, window, sinks)
+                assert worst(out[lo:hi], want, tolerance(want, mass, out.dtype)) <= 1
+
+    a, b = pages.new(), pages.new()
+    step([a, b], [70, 21])
+    c = pages.fork(a)
+    whole[c] = [list(x) for x in whole[a]]
+    step([a, b, c], [1, 1, 1])
+    step([c], [19])
+    for s in (a, b, c):
+        pages.release(s, window, sinks)
+    step([c, a, b], [1, 1, 1])
+    pages.free(a)
+    before = pages.info()["free_pages"]
+    P.paged_kv_copy(cache, *pages.compact())
+    assert pages.info()["free_pages"] == before
+    for _ in range(3):
+        step([b, c], [1, 1])
+    d = pages.fork(c)
+    whole[d] = [list(x) for x in whole[c]]
+    step([d, b], [33, 7])
+    step([c, d, b], [1, 1, 1])

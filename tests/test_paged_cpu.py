@@ -1,0 +1,278 @@
+"""The paged cache without a GPU: book-keeping of the pages against a model of it, and calls that are refused before anything runs."""
+import ctypes as C
+import random
+
+import numpy as np
+import pytest
+
+
+@pytest.fixture(scope="module")
+def r():
+    from runnburn_b200 import build
+    build.build_library()
+    import runnburn_b200
+    return runnburn_b200
+
+
+class Model:
+    """What the pages hold, position by position: the cache is a dict (page, row) -> value."""
+
+    def __init__(self, pages, r):
+        self.p, self.r, self.cache, self.want = pages, r, {}, {}
+
+    def copy(self, src, dst, rows):
+        rows = [self.p.page_size] * len(src) if rows is None else rows
+        assert not set(src) & set(dst) and len(set(dst)) == len(dst)
+        for a, b, n in zip(src, dst, rows):
+            for i in range(n):
+                self.cache[b, i] = self.cache.get((a, i))
+
+    def extend(self, seq, values):
+        self.copy(*self.p.extend(seq, len(values)))
+        table, lens = self.p.tables([seq])
+        at = len(self.want[seq])
+        assert lens[0] == at + len(values)
+        for i, v in enumerate(values, at):
+            page = table[0, i // self.p.page_size]
+            assert 0 <= page < self.p.n_pages
+            self.cache[page, i % self.p.page_size] = v
+        self.want[seq] = self.want[seq] + list(values)
+
+    def check(self):
+        used = set()
+        for s, want in self.want.items():
+            table, lens = self.p.tables([s])
+            assert lens[0] == len(want)
+            for i, v in enumerate(want):
+                page = int(table[0, i // self.p.page_size])
+                if page < 0:
+                    assert v is None or self.released.get(s, 0) > i
+                    continue
+                used.add(page)
+                assert self.cache[page, i % self.p.page_size] == v
+        info = self.p.info()
+        assert info["free_pages"] == self.p.n_pages - len(used) and info["n_seqs"] == len(self.want)
+        return used
+
+    released: dict = {}
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("page", [8, 16])
+def test_sequences_keep_what_they_hold(r, seed, page):
+    rng, m = random.Random(seed * 31 + page), Model(r.paged.KvPages(60, page), r)
+    stamp = iter(range(10 ** 9))
+    for _ in range(400):
+        seqs = list(m.want)
+        act = rng.choice(["new", "extend", "extend", "extend", "fork", "truncate", "free", "compact"])
+        if act == "new" and len(seqs) < 8:
+            m.want[m.p.new()] = []
+        elif act == "extend" and seqs:
+            s = rng.choice(seqs)
+            before = m.p.info()
+            try:
+                m.extend(s, [next(stamp) for _ in range(rng.choice([0, 1, 2, page, 3 * page + 1]))])
+            except r.RnbError as e:
+                assert e.status == 3 and "pages needed" in str(e) and m.p.info() == before
+        elif act == "fork" and seqs and len(seqs) < 8:
+            s = rng.choice(seqs)
+            m.want[m.p.fork(s)] = list(m.want[s])
+        elif act == "truncate" and seqs:
+            s = rng.choice(seqs)
+            n = rng.randint(0, len(m.want[s]))
+            m.p.truncate(s, n)
+            m.want[s] = m.want[s][:n]
+        elif act == "free" and seqs and rng.random() < 0.5:
+            s = rng.choice(seqs)
+            m.p.free(s)
+            del m.want[s]
+        elif act == "compact":
+            m.copy(*m.p.compact())
+            used = m.check()
+            assert used == set(range(len(used)))
+        m.check()
+
+
+@pytest.mark.parametrize("window,sinks,n", [(1, 0, 40), (5, 0, 40), (16, 3, 100), (30, 8, 100), (200, 4, 100), (100, 0, 100), (8, 99, 100), (8, 17, 64)])
+def test_release_keeps_what_later_tokens_see(r, window, sinks, n):
+    p = r.paged.KvPages(20, 8)
+    s = p.new()
+    p.extend(s, n)
+    p.release(s, window, sinks)
+    table, _ = p.tables([s])
+    for i in range(-(-n // 8)):
+        needed = any(j > n - window or j < sinks for j in range(8 * i, 8 * i + 8))   # seen from position n on, or still to be written
+        assert (table[0, i] >= 0) == needed
+    free = p.info()["free_pages"]
+    p.release(s, window, sinks)
+    assert p.info()["free_pages"] == free
+    # the sequence goes on; its table is longer than what it holds
+    p.extend(s, 24)
+    assert p.tables([s])[1][0] == n + 24
+    if table[0, 0] >= 0 and (table[0] < 0).any():
+        first = int(np.argmax(table[0] < 0))
+        with pytest.raises(r.RnbError, match="released page"):
+            p.truncate(s, 8 * first + 3)
+        p.truncate(s, 8 * first)
+    p.free(s)
+    assert p.info()["free_pages"] == 20
+
+
+def test_shared_pages_are_freed_once(r):
+    p = r.paged.KvPages(4, 8)
+    a = p.new()
+    p.extend(a, 12)
+    b = p.fork(a)
+    c = p.fork(b)
+    assert p.info() == dict(n_pages=4, page_size=8, free_pages=2, n_seqs=3)
+    assert p.extend(a, 1) == ([1], [2], [4])          # the others keep the page
+    assert p.extend(b, 1) == ([1], [3], [4])
+    assert p.extend(c, 1) == ([], [], [])             # nobody else is left on it
+    with pytest.raises(r.RnbError) as e:
+        p.extend(c, 9)
+    assert e.value.status == 3
+    p.free(a)
+    p.free(a2 := p.fork(b))
+    assert a2 == a and p.info()["free_pages"] == 1
+    p.free(b), p.free(c)
+    assert p.info()["free_pages"] == 4
+    for call in (lambda: p.free(b), lambda: p.fork(7), lambda: p.extend(-1, 1), lambda: p.truncate(9, 0), lambda: p.release(b, 4), lambda: p.tables([b])):
+        with pytest.raises(r.RnbError, match="no sequence"):
+            call()
+
+
+def test_book_keeping_refuses(r):
+    L = r.load()
+    for pages, size in ((0, 16), (-1, 16), (4, 0), (4, 4), (4, 24), (4, 512)):
+        with pytest.raises(r.RnbError) as e:
+            r.paged.KvPages(pages, size)
+        assert e.value.status == 2
+    p = r.paged.KvPages(8, 8)
+    s = p.new()
+    p.extend(s, 20)
+    for call, what in ((lambda: p.truncate(s, 21), "cannot keep"), (lambda: p.truncate(s, -1), "cannot keep"), (lambda: p.release(s, 0), "window"),
+                       (lambda: p.release(s, 4, -1), "sinks"), (lambda: p.extend(s, -1), "cannot add"), (lambda: p.extend(s, 2 ** 31 - 1), "cannot add"),
+                       (lambda: p.tables([s], 2), "3 pages")):
+        with pytest.raises(r.RnbError, match=what) as e:
+            call()
+        assert e.value.status == 2
+    t = p.new()
+    p.extend(t, 16)
+    p.free(s)
+    n = C.c_size_t()
+    assert L.rnb_b200_kv_pages_compact(p._h, None, None, 0, C.byref(n)) == 2 and n.value == 2   # nothing moved for want of room
+    assert p.tables([t])[0].tolist() == [[3, 4]]
+    src, dst, _ = p.compact()
+    assert (src.tolist(), dst.tolist()) == ([3, 4], [0, 1]) and p.tables([t])[0].tolist() == [[0, 1]]
+    assert L.rnb_b200_kv_pages_create(4, 8, None) == 2 and L.rnb_b200_kv_pages_new(None, C.byref(n)) == 2
+
+
+# ---- calls that are refused on the host: nothing here is read, the addresses are made up --------------------------------
+ADDRESS = 0x10000
+
+
+def cache(r, **kw):
+    f = dict(type=1, head_dim=128, kv_heads=2, page_size=16, n_pages=10, page_stride=4096, pos_stride=256, head_stride=128, k=ADDRESS, v=ADDRESS) | kw
+    return r._lib.PagedCache(*[f[n] for n, _ in r._lib.PagedCache._fields_])
+
+
+def batch(r, **kw):
+    f = dict(table=ADDRESS, table_stride=4, max_pages=4, n_seq=2, n_tokens=2, kv_len=ADDRESS, q_start=None) | kw
+    return r._lib.PagedBatch(*[f[n] for n, _ in r._lib.PagedBatch._fields_])
+
+
+BAD_CACHE = [
+    (dict(type=0), 1, "F16 or BF16"), (dict(type=8), 1, "F16 or BF16"), (dict(head_dim=4), 2, "head_dim"), (dict(head_dim=132), 2, "head_dim"),
+    (dict(head_dim=520), 2, "head_dim"), (dict(kv_heads=0), 2, "kv_heads"), (dict(page_size=4), 2, "page_size"), (dict(page_size=24), 2, "page_size"),
+    (dict(page_size=512), 2, "page_size"), (dict(n_pages=0), 2, "n_pages"), (dict(k=None), 2, "null"), (dict(v=None), 2, "null"), (dict(k=ADDRESS + 8), 2, "16-byte"),
+    (dict(v=ADDRESS + 2), 2, "16-byte"), (dict(pos_stride=260), 2, "strides"), (dict(page_stride=2 ** 40), 2, "strides"), (dict(head_stride=64), 2, "overlap"),
+    (dict(pos_stride=128), 2, "overlap"), (dict(page_stride=4088), 2, "overlap"), (dict(pos_stride=0), 2, "overlap"),
+]
+BAD_BATCH = [
+    (dict(n_seq=-1), 2, "negative"), (dict(n_tokens=-1), 2, "negative"), (dict(n_tokens=3), 2, "one token per sequence"), (dict(table=None), 2, "null"),
+    (dict(kv_len=None), 2, "null"), (dict(max_pages=0), 2, "max_pages"), (dict(table_stride=3), 2, "table_stride"), (dict(table=ADDRESS + 2), 2, "4-byte"),
+    (dict(kv_len=ADDRESS + 1), 2, "4-byte"), (dict(q_start=ADDRESS + 2, n_tokens=9), 2, "4-byte"),
+]
+
+
+def attend(L, c, b, q_type=0, q=ADDRESS, q_stride=512, heads=4, scale=0.1, window=0, sinks=0, ws=ADDRESS, ws_bytes=None, out=ADDRESS, out_stride=512, lse=None, prefill=False):
+    fn = L.rnb_b200_dev_attention_prefill_paged if prefill else L.rnb_b200_dev_attention_decode_paged
+    n = L.rnb_b200_paged_workspace_bytes() if ws_bytes is None else ws_bytes
+    return fn(C.byref(c) if c else None, C.byref(b) if b else None, q_type, q, q_stride, heads, scale, window, sinks, ws, n, out, out_stride, lse, None)
+
+
+def refused(L, rc, status, what):
+    assert rc == status and what in L.rnb_b200_last_error().decode(), (rc, L.rnb_b200_last_error())
+
+
+@pytest.mark.parametrize("kw,status,what", BAD_CACHE)
+def test_a_bad_cache_is_refused(r, kw, status, what):
+    L, c, b, one = r.load(), cache(r, **kw), batch(r), np.zeros(1, np.int32)
+    refused(L, attend(L, c, b), status, what)
+    refused(L, attend(L, c, b, prefill=True), status, what)
+    refused(L, L.rnb_b200_dev_paged_kv_append(C.byref(c), C.byref(b), 0, ADDRESS, ADDRESS, 256, None), status, what)
+    refused(L, L.rnb_b200_dev_paged_kv_copy(C.byref(c), 1, 0, one.ctypes.data, one.ctypes.data, None, 1, None), status, what)
+
+
+@pytest.mark.parametrize("kw,status,what", BAD_BATCH)
+def test_a_bad_batch_is_refused(r, kw, status, what):
+    L, c, b = r.load(), cache(r), batch(r, **kw)
+    refused(L, attend(L, c, b, prefill=b.q_start is not None), status, what)
+    refused(L, L.rnb_b200_dev_paged_kv_append(C.byref(c), C.byref(b), 0, ADDRESS, ADDRESS, 256, None), status, what)
+
+
+@pytest.mark.parametrize("kw,status,what", [
+    (dict(q_type=30), 1, "queries"), (dict(q_type=12), 1, "queries"), (dict(q=None), 2, "null"), (dict(out=None), 2, "null"), (dict(heads=0), 2, "multiple of num_kv_heads"),
+    (dict(heads=3), 2, "multiple of num_kv_heads"), (dict(heads=65536), 2, "num_heads"), (dict(q=ADDRESS + 8), 2, "16-byte"), (dict(out=ADDRESS + 4), 2, "16-byte"),
+    (dict(q_stride=516), 2, "multiples of 8"), (dict(out_stride=516), 2, "multiples of 8"), (dict(q_stride=504), 2, "at least"), (dict(out_stride=256), 2, "at least"),
+    (dict(lse=ADDRESS + 2), 2, "lse"), (dict(window=-1), 2, "window"), (dict(sinks=-1), 2, "sinks"), (dict(scale=float("nan")), 2, "scale"),
+    (dict(scale=float("inf")), 2, "scale"), (dict(ws=None), 2, "workspace"), (dict(ws=ADDRESS + 64), 2, "workspace"), (dict(ws_bytes=100), 2, "workspace"),
+])
+def test_attention_refuses(r, kw, status, what):
+    L = r.load()
+    for prefill in (False, True):
+        refused(L, attend(L, cache(r), batch(r), prefill=prefill, **kw), status, what)
+
+
+def test_calls_refuse_what_only_they_can_see(r):
+    L = r.load()
+    refused(L, attend(L, None, batch(r)), 2, "null")
+    refused(L, attend(L, cache(r), None), 2, "null")
+    refused(L, attend(L, cache(r, head_dim=96, head_stride=96, pos_stride=192, page_stride=192 * 16), batch(r)), 1, "head_dim must be 64 or 128")
+    refused(L, attend(L, cache(r, type=30), batch(r), q_type=0), 1, "queries")
+    refused(L, attend(L, cache(r), batch(r, q_start=ADDRESS)), 2, "q_start must be null")
+    append = lambda *a: L.rnb_b200_dev_paged_kv_append(C.byref(cache(r)), C.byref(batch(r)), *a, None)  # noqa: E731
+    refused(L, append(30, ADDRESS, ADDRESS, 256), 1, "F32 or of the cache's type")
+    refused(L, append(0, None, ADDRESS, 256), 2, "null")
+    refused(L, append(0, ADDRESS, None, 256), 2, "null")
+    refused(L, append(0, ADDRESS + 4, ADDRESS, 256), 2, "16-byte")
+    refused(L, append(0, ADDRESS, ADDRESS, 252), 2, "multiple of 8")
+    refused(L, append(0, ADDRESS, ADDRESS, 128), 2, "smaller than a token")
+    refused(L, L.rnb_b200_paged_workspace_init(None, 1 << 30, None), 2, "workspace")
+    refused(L, L.rnb_b200_paged_workspace_init(ADDRESS, 8, None), 2, "workspace")
+
+
+@pytest.mark.parametrize("src,dst,rows,what", [
+    ([0], [10], None, "the pool has 10"), ([-1], [2], None, "the pool has 10"), ([0], [0], None, "read and written"), ([0, 1], [2, 2], None, "written twice"),
+    ([0, 1], [1, 2], None, "read and written"), ([1, 0], [2, 1], None, "read and written"), ([0], [1], [17], "17 positions"), ([0], [1], [-1], "-1 positions"),
+    ([0] * 11, list(range(11)), None, "more copies than pages"),
+])
+def test_copies_refuse(r, src, dst, rows, what):
+    L = r.load()
+    a = [np.asarray(x, np.int32) if x is not None else None for x in (src, dst, rows)]
+    refused(L, L.rnb_b200_dev_paged_kv_copy(C.byref(cache(r)), 1, 0, a[0].ctypes.data, a[1].ctypes.data, a[2].ctypes.data if rows else None, len(src), None), 2, what)
+
+
+def test_copies_refuse_bad_layers(r):
+    L, z = r.load(), np.array([0, 1], np.int32)
+    for layers, stride in ((0, 0), (40000, 1 << 20), (2, 0), (2, 12)):
+        refused(L, L.rnb_b200_dev_paged_kv_copy(C.byref(cache(r)), layers, stride, z[:1].ctypes.data, z[1:].ctypes.data, None, 1, None), 2, "layer")
+
+
+def test_nothing_to_do_is_no_call(r):
+    """No tokens, no sequences, no copies: fine without a GPU."""
+    L = r.load()
+    assert attend(L, cache(r), batch(r, n_seq=0, n_tokens=0, table=None, kv_len=None), q=None, out=None) == 0
+    assert attend(L, cache(r), batch(r, n_tokens=0, q_start=ADDRESS), prefill=True) == 0
+    assert L.rnb_b200_dev_paged_kv_append(C.byref(cache(r)), C.byref(batch(r, n_seq=0, n_tokens=0)), 0, None, None, 0, None) == 0
+    assert L.rnb_b200_dev_paged_kv_copy(C.byref(cache(r)), 1, 0, None, None, None, 0, None) == 0
