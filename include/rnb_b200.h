@@ -770,6 +770,7 @@ int rnb_b200_attention_decode_hd128_noalloc_status(int *status_out, void *stream
  * outside the pool; what the call writes for such a sequence is then not to be used.  Entries of pages
  * that no query sees are not read and may hold anything. */
 #define RNB_B200_DEVICE_BAD_PAGE 5
+#define RNB_B200_DEVICE_BAD_WORKSPACE 6 /* attention with a workspace that was not initialised: nothing is written */
 typedef struct {
     uint32_t type;      /* RNB_B200_TYPE_F16 or _BF16 */
     int32_t head_dim;   /* a multiple of 8 up to 512; attention: 64 or 128 */

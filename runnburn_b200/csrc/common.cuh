@@ -31,6 +31,7 @@ constexpr int DEV_ERR_BAD_JOB = 2;        // job table inconsistent with the lau
 constexpr int DEV_ERR_GEMM_TIMEOUT = 3;   // tensor-core matmul: a pipeline wait gave up
 constexpr int DEV_ERR_PEER_TIMEOUT = 4;   // multi-GPU exchange: a peer's slice did not arrive in time
 constexpr int DEV_ERR_BAD_PAGE = 5;       // paged cache: a table entry, length or start that points outside
+constexpr int DEV_ERR_BAD_WORKSPACE = 6;  // paged attention: a workspace that was not initialised
 
 __host__ __device__ inline size_t row_bytes_of(int type, size_t cols) {
     switch (type) {

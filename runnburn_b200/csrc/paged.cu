@@ -4,6 +4,7 @@
 #include "launch_k.hpp"
 #include "paged.cuh"
 #include "paged_attention_plain.cuh"
+#include "paged_decode.cuh"
 
 namespace rnb {
 
@@ -148,7 +149,9 @@ struct PkAttention {   // a checked call
     void *out, *workspace;
     float *lse;
 };
-constexpr size_t PK_WORKSPACE_BYTES = 256;
+// the mark, the counters, and two records for every CTA of the decode kernel (16 heads of 128 dims are the largest)
+constexpr size_t PK_WORKSPACE_BYTES = PD_WS_RECORDS + 2 * PD_MAX_GRID * PdShape<128, 1>::RECORD;
+static_assert(PD_WS_RECORDS % 256 == 0, "records are read by 16 bytes");
 
 static int pk_check_attention(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type, const void *q, size_t q_stride, size_t num_heads,
                               float scale, int32_t window, int32_t sinks, void *workspace, size_t workspace_bytes, void *out, size_t out_stride, float *lse, PkAttention *a) {
@@ -191,10 +194,46 @@ static int pk_attention_plain(const PkAttention &a, cudaStream_t s, int *err) {
     RNB_CU(launch_k(kernel, grid, dim3(128), 0, s, a.c, a.b, (const Q *)a.q, a.q_stride, a.heads, a.scale, a.window, a.sinks, (Q *)a.out, a.out_stride, a.lse, err));
     return RNB_B200_OK;
 }
+template <class Q, class C, int D, int HT>
+static int pk_decode_launch(const PkAttention &a, cudaStream_t s, State &st) {
+    using S = PdShape<D, HT>;
+    static bool ready = false;   // under the library's lock; one device
+    if (!ready) RNB_CU(cudaFuncSetAttribute(paged_decode_kernel<Q, C, D, HT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
+    ready = true;
+    PdParams P{};
+    P.q = a.q;
+    P.q_stride = a.q_stride;
+    P.out_stride = a.out_stride;
+    P.heads = a.heads;
+    P.group = a.heads / a.c.kv_heads;
+    P.splits = (P.group + 8 * HT - 1) / (8 * HT);
+    P.window = a.window;
+    P.sinks = a.sinks;
+    P.scale_log2 = a.scale * 1.4426950408889634f;
+    P.out = a.out;
+    P.lse = a.lse;
+    P.workspace = (uint8_t *)a.workspace;
+    P.err = st.dev_error;
+    const int grid = std::min(std::min(st.sm_count, 148) * S::PER_SM, PD_MAX_GRID);
+    static_assert(148 * S::PER_SM * 2 * S::RECORD <= PK_WORKSPACE_BYTES - PD_WS_RECORDS, "records");
+    RNB_CU(launch_k(paged_decode_kernel<Q, C, D, HT>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s, a.c, a.b, P));
+    return RNB_B200_OK;
+}
+// Up to eight query heads per key head: four warps; more: eight warps, 16 heads at a time.
+template <class Q, class C>
+static int pk_decode(const PkAttention &a, cudaStream_t s, State &st) {
+    const bool many = a.heads / a.c.kv_heads > 8;
+    if (a.c.head_dim == 64) return many ? pk_decode_launch<Q, C, 64, 2>(a, s, st) : pk_decode_launch<Q, C, 64, 1>(a, s, st);
+    return many ? pk_decode_launch<Q, C, 128, 2>(a, s, st) : pk_decode_launch<Q, C, 128, 1>(a, s, st);
+}
 static int pk_attention(const PkAttention &a, cudaStream_t s) {
     if (a.b.n_tokens == 0 || a.b.n_seq == 0) return RNB_B200_OK;
     PkCall call;
     RNB_TRY(call.rc);
+    if (!a.b.q_start) {
+        if (a.q_type == RNB_B200_TYPE_F32) return pk_decode<float, F16>(a, s, call.st);
+        return a.q_type == RNB_B200_TYPE_F16 ? pk_decode<F16, F16>(a, s, call.st) : pk_decode<Bf16, Bf16>(a, s, call.st);
+    }
     int *err = call.st.dev_error;
     if (a.q_type == RNB_B200_TYPE_F32) return pk_attention_plain<float, F16>(a, s, err);
     return a.q_type == RNB_B200_TYPE_F16 ? pk_attention_plain<F16, F16>(a, s, err) : pk_attention_plain<Bf16, Bf16>(a, s, err);
@@ -230,7 +269,8 @@ int rnb_b200_paged_workspace_init(void *workspace, size_t workspace_bytes, void 
         return fail(RNB_B200_VALIDATION_FAILED, "paged attention: the workspace must be 256-byte aligned and hold %zu bytes, got %zu", PK_WORKSPACE_BYTES, workspace_bytes);
     PkCall call;
     RNB_TRY(call.rc);
-    RNB_CU(cudaMemsetAsync(workspace, 0, PK_WORKSPACE_BYTES, (cudaStream_t)stream));
+    RNB_CU(cudaMemsetAsync((uint8_t *)workspace + PD_WS_HEAD, 0, PD_WS_RECORDS - PD_WS_HEAD, (cudaStream_t)stream));
+    RNB_CU(cudaMemsetAsync(workspace, (int)(PD_WS_MARK & 0xffu), PD_WS_HEAD, (cudaStream_t)stream));
     return RNB_B200_OK;
 }
 int rnb_b200_dev_attention_decode_paged(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type, const void *q, size_t q_stride,

@@ -1,0 +1,417 @@
+// Attention of one new token per sequence over a paged cache: one pass over the visible positions with a running maximum and sum.
+//
+// The work is a list of tiles of 64 positions, (sequence, key head, tile) with the tiles fastest, that the launch cuts into equal
+// runs, one per CTA: lengths may differ as they like, and one long sequence uses the whole chip.  Every CTA finds its run by a scan over the lengths.
+// A (sequence, key head) that lies within one run is finished there; of one that is cut, each CTA leaves (maximum, sum, output) in the
+// workspace, and the CTA that arrives last joins them in the order of the runs, so the result does not depend on who was last.
+//
+// In a CTA four warps share a tile, 16 positions each, with a softmax of their own that is joined at the end of a segment; eight query heads
+// are the rows of the products (HT = 2: eight warps for up to 16 heads).  Rows 0-7 hold the queries rounded to the cache's type and rows 8-15 what the
+// rounding left, so one product gives both and their sum keeps f32 queries at 22 bits; the same with the probabilities.  Queries are scaled
+// by a power of two per head into the range of f16, probabilities by 2^BIAS, so that small ones keep their bits.  Products start from zero and are
+// added to the f32 sums in registers: long sums in the tensor cores' accumulators would be cut off at each step.
+//
+// K and V tiles come in by 16-byte asynchronous copies, each thread following the page of its rows: any page size and stride, and rows that
+// are not visible are filled with zeros, so what lies there never enters a product.
+#pragma once
+#include "paged.cuh"
+
+namespace rnb {
+
+constexpr int PD_TILE = 64;
+constexpr float PD_BIAS = 12.f;
+constexpr int PD_MIN_TILES = 4;   // of a run: a cut costs a join
+constexpr size_t PD_WS_HEAD = 256;                      // a mark that the workspace has been initialised
+constexpr int PD_MAX_GRID = 1024;                       // runs of a launch
+constexpr size_t PD_WS_RECORDS = PD_WS_HEAD + PD_MAX_GRID * sizeof(unsigned);
+constexpr unsigned PD_WS_MARK = 0x5a5a5a5au;
+
+template <int D, int HT>
+struct PdShape {
+    static constexpr int THREADS = 128 * HT;
+    static constexpr int STAGES = D == 128 ? 3 : 4;
+    static constexpr int PER_SM = HT == 1 ? (D == 128 ? 2 : 3) : (D == 128 ? 1 : 2);
+    static constexpr int ROW = D + 8;                                                    // floats between the heads of a partial output: no bank conflicts
+    static constexpr uint32_t TILE_BYTES = PD_TILE * D * 2;
+    static constexpr size_t MERGE = sizeof(float) * HT * 4 * 8 * ROW;                    // outputs of the warps; weights of the parts in a join
+    static constexpr size_t JOIN = sizeof(float) * HT * 8 * 148 * PER_SM;
+    static constexpr size_t SMEM = STAGES * 2 * TILE_BYTES + (MERGE > JOIN ? MERGE : JOIN) + sizeof(float) * HT * 8 * 10 + 64;
+    static constexpr size_t RECORD = sizeof(float) * HT * 8 * (D + 4);                   // per head: maximum, sum, two unused, output
+};
+
+struct PdParams {
+    const void *q;
+    size_t q_stride, out_stride;
+    int heads, group, splits, window, sinks;   // splits: CTAs' worth of heads per key head
+    float scale_log2;
+    void *out;
+    float *lse;
+    uint8_t *workspace;
+    int *err;
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void pd_copy16(uint32_t dst, const void *src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void pd_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void pd_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float pd_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The tiles of a query that sees positions 0 .. sink - 1 and from .. len - 1.
+struct PdSeen {
+    int len, from, sink, lead, skip;   // tile i starts at position 64 (i < lead ? i : i + skip)
+    int tiles;
+};
+__device__ __forceinline__ PdSeen pd_seen(int len, int window, int sinks) {
+    PdSeen s;
+    s.len = len;
+    s.from = window && len > window ? len - window : 0;
+    s.sink = min(sinks, s.from);
+    s.lead = min((s.sink + PD_TILE - 1) / PD_TILE, s.from / PD_TILE);
+    s.skip = s.from / PD_TILE - s.lead;
+    s.tiles = max(1, (len + PD_TILE - 1) / PD_TILE - s.skip);   // an empty one too: its output is written
+    return s;
+}
+
+template <class Q, class C, int D, int HT>
+RNB_GLOBAL void __launch_bounds__(PdShape<D, HT>::THREADS, PdShape<D, HT>::PER_SM)
+paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
+    using S = PdShape<D, HT>;
+    constexpr int KS = D / 16, CH = D / 8, PASS_ROWS = S::THREADS / CH, PASSES = PD_TILE / PASS_ROWS;
+    extern __shared__ __align__(128) uint8_t pd_smem[];
+    float *const merge = reinterpret_cast<float *>(pd_smem + S::STAGES * 2 * S::TILE_BYTES);
+    float *const ml = reinterpret_cast<float *>(pd_smem + S::SMEM - 64 - sizeof(float) * HT * 8 * 10);   // [head][m of 4 warps, l of 4 warps, M, L]
+    volatile int *const note = reinterpret_cast<volatile int *>(pd_smem + S::SMEM - 64);
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, w4 = warp & 3, ht = warp >> 2;
+    const int VH = c.kv_heads * P.splits;
+
+    // ---- this CTA's run: units [begin, end) of VH * (tiles of all sequences) ----
+    if (warp == 0) {
+        long long sum = 0;
+        for (int r = lane; r < b.n_seq; r += 32) sum += pd_seen(pk_length(b, c.page_shift, r, P.err), P.window, P.sinks).tiles;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const long long units = sum * VH, per = max((units + gridDim.x - 1) / gridDim.x, (long long)PD_MIN_TILES), begin = per * blockIdx.x;
+        // the sequence that unit `begin` lies in
+        long long before = 0;
+        int row = 0;
+        for (int r0 = 0; r0 < b.n_seq && begin < units; r0 += 32) {
+            const int n = r0 + lane < b.n_seq ? pd_seen(pk_length(b, c.page_shift, r0 + lane, P.err), P.window, P.sinks).tiles : 0;
+            long long up = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, up, o);
+                if (lane >= o) up += x;
+            }
+            const unsigned behind = __ballot_sync(0xffffffffu, (before + up) * VH > begin);
+            if (behind) {
+                const int l = __ffs(behind) - 1;
+                row = r0 + l;
+                before += __shfl_sync(0xffffffffu, up - n, l);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, up, 31);
+        }
+        if (lane == 0) {
+            const bool ready = *reinterpret_cast<volatile unsigned *>(P.workspace) == PD_WS_MARK;
+            if (!ready) atomicExch(P.err, DEV_ERR_BAD_WORKSPACE);
+            long long *const w = reinterpret_cast<long long *>(pd_smem);
+            w[0] = ready && begin < units ? min(per, units - begin) : 0;
+            w[1] = begin;
+            w[2] = begin - before * VH;   // unit within the sequence
+            w[3] = per;
+            w[4] = row;
+        }
+    }
+    __syncthreads();
+    const long long *const found = reinterpret_cast<const long long *>(pd_smem);
+    const long long n_units = found[0], begin = found[1], per = found[3];
+    struct Walk {
+        int row, vh, i;
+        PdSeen s;
+    } at;
+    at.row = (int)found[4];
+    at.s = pd_seen(0, 0, 0);
+    if (n_units > 0) {
+        at.s = pd_seen(pk_length(b, c.page_shift, at.row, P.err), P.window, P.sinks);
+        at.vh = (int)(found[2] / at.s.tiles);
+        at.i = (int)(found[2] % at.s.tiles);
+    }
+    __syncthreads();
+    if (n_units == 0) return;
+    auto advance = [&](Walk &w) {
+        if (++w.i < w.s.tiles) return;
+        w.i = 0;
+        if (++w.vh < VH) return;
+        w.vh = 0;
+        if (++w.row < b.n_seq) w.s = pd_seen(pk_length(b, c.page_shift, w.row, P.err), P.window, P.sinks);
+    };
+    auto start = [](const Walk &w) { return PD_TILE * (w.i < w.s.lead ? w.i : w.i + w.s.skip); };
+
+    // ---- copies: a thread has the same 16 bytes of PASSES rows; their pages are looked up one tile ahead ----
+    const int c_row = tid / CH, c_at = tid % CH;
+    const uint32_t c_dst = smem_u32(pd_smem) + c_row * (D * 2) + ((c_at ^ (c_row & 7)) << 4);   // PASS_ROWS is a multiple of 8
+    Walk next = at;
+    long long left = n_units;
+    int pages[PASSES];
+    auto visible = [](const PdSeen &s, int pos) { return pos < s.len && (pos >= s.from || pos < s.sink); };
+    auto look_up = [&]() {
+        const int p0 = start(next) + c_row;
+#pragma unroll
+        for (int p = 0; p < PASSES; p++) {
+            const int pos = p0 + p * PASS_ROWS;
+            pages[p] = left > 0 && visible(next.s, pos) ? b.table[(size_t)next.row * b.table_stride + (pos >> c.page_shift)] : -1;
+        }
+    };
+    auto issue = [&](int stage) {
+        if (left > 0) {
+            const uint32_t dst = c_dst + stage * 2 * S::TILE_BYTES;
+            const int p0 = start(next) + c_row;
+            const size_t head = (size_t)(next.vh / P.splits) * c.head_stride + c_at * 8;
+#pragma unroll
+            for (int p = 0; p < PASSES; p++) {
+                const int pos = p0 + p * PASS_ROWS;
+                bool live = visible(next.s, pos);
+                if (live && (unsigned)pages[p] >= (unsigned)c.n_pages) {
+                    atomicExch(P.err, DEV_ERR_BAD_PAGE);
+                    live = false;
+                }
+                const size_t from = live ? (size_t)pages[p] * c.page_stride + (size_t)(pos & ((1 << c.page_shift) - 1)) * c.pos_stride + head : 0;
+                pd_copy16(dst + p * PASS_ROWS * (D * 2), c.k + from, live);
+                pd_copy16(dst + S::TILE_BYTES + p * PASS_ROWS * (D * 2), c.v + from, live);
+            }
+            left--;
+            advance(next);
+            look_up();
+        }
+        pd_commit();
+    };
+    look_up();
+    for (int s = 0; s < S::STAGES - 1; s++) issue(s);
+
+    // ---- products ----
+    const int head = lane >> 2, quad = lane & 3;   // of the rows and columns that this thread holds
+    uint32_t qa[KS][4];
+    float o[KS * 2][2], m = -INFINITY, l = 0.f, to_log2 = 0.f;
+    const uint32_t k_row = 16 * w4 + (lane & 7) + ((lane >> 4) << 3), v_row = 16 * w4 + (lane & 7) + (((lane >> 3) & 1) << 3);
+    const uint32_t k_base = smem_u32(pd_smem) + k_row * (D * 2), v_base = smem_u32(pd_smem) + S::TILE_BYTES + v_row * (D * 2);
+    const uint32_t k_x = k_row & 7, v_x = v_row & 7, k_c = (lane >> 3) & 1, v_c = lane >> 4;
+    bool fresh = true;   // a segment begins
+    long long unit = begin;
+    int first_tile = at.i;
+    int stage = 0;
+    for (long long u = 0; u < n_units; u++, unit++, stage = stage + 1 < S::STAGES ? stage + 1 : 0) {
+        pd_wait<S::STAGES - 2>();
+        __syncthreads();
+        issue(stage > 0 ? stage - 1 : S::STAGES - 1);   // the one that the tile before has left
+        const int group0 = (at.vh % P.splits) * (8 * HT) + ht * 8, mine = group0 + head, q_head = (at.vh / P.splits) * P.group + mine;
+        if (fresh) {
+            fresh = false;
+            first_tile = at.i;
+            float2 x[KS][2];
+            float most = 0.f;
+            const Q *const q = reinterpret_cast<const Q *>(P.q) + (size_t)at.row * P.q_stride + (size_t)q_head * D + quad * 2;
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    x[k][h] = make_float2(0.f, 0.f);
+                    if (mine < P.group) {
+                        if constexpr (sizeof(Q) == 4) {
+                            x[k][h] = *reinterpret_cast<const float2 *>(q + k * 16 + h * 8);
+                            most = fmaxf(most, fmaxf(fabsf(x[k][h].x), fabsf(x[k][h].y)));
+                        } else {
+                            qa[k][2 * h] = *reinterpret_cast<const uint32_t *>(q + k * 16 + h * 8);
+                        }
+                    } else {
+                        qa[k][2 * h] = 0;
+                    }
+                    qa[k][2 * h + 1] = 0;
+                }
+            to_log2 = P.scale_log2;
+            if constexpr (sizeof(Q) == 4) {
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                // 2^e with largest * 2^-e in 1 .. 2; f32's own extremes stay in range
+                int e = (int)((__float_as_uint(most) >> 23) & 255u) - 127;
+                e = most == 0.f ? 0 : max(-126, min(126, e));
+                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                to_log2 = P.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) pk_split<C>(x[k][h].x * down, x[k][h].y * down, qa[k][2 * h], qa[k][2 * h + 1]);
+            }
+#pragma unroll
+            for (int n = 0; n < KS * 2; n++) o[n][0] = o[n][1] = 0.f;
+            m = -INFINITY;
+            l = 0.f;
+        }
+        const int p0 = start(at) + 16 * w4;
+        if (p0 < at.s.len && (p0 + 15 >= at.s.from || p0 < at.s.sink)) {
+            float s0[4] = {}, s1[4] = {};
+            const uint32_t kt = k_base + stage * 2 * S::TILE_BYTES, vt = v_base + stage * 2 * S::TILE_BYTES;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                uint32_t r[4];
+                pk_ldmatrix(r, kt + (((2 * k + k_c) ^ k_x) << 4));
+                pk_mma<C>(s0, qa[k], r[0], r[1]);
+                pk_mma<C>(s1, qa[k], r[2], r[3]);
+            }
+            float t[4] = {s0[0] + s0[2], s0[1] + s0[3], s1[0] + s1[2], s1[1] + s1[3]};
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                t[i] = visible(at.s, p0 + quad * 2 + (i & 1) + (i >> 1) * 8) ? t[i] * to_log2 : -INFINITY;
+                mx = fmaxf(mx, t[i]);
+            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float m_new = fmaxf(m, mx), ref = m_new == -INFINITY ? 0.f : m_new, corr = pd_exp2(m - ref);
+            m = m_new;
+#pragma unroll
+            for (int i = 0; i < 4; i++) t[i] = pd_exp2(t[i] - ref + PD_BIAS);
+            l = l * corr + ((t[0] + t[1]) + (t[2] + t[3]));
+            uint32_t pa[4];
+            pk_split<C>(t[0], t[1], pa[0], pa[1]);
+            pk_split<C>(t[2], t[3], pa[2], pa[3]);
+#pragma unroll
+            for (int d = 0; d < KS; d++) {
+                uint32_t r[4];
+                pk_ldmatrix_trans(r, vt + (((2 * d + v_c) ^ v_x) << 4));
+                float x0[4] = {}, x1[4] = {};
+                pk_mma<C>(x0, pa, r[0], r[1]);
+                pk_mma<C>(x1, pa, r[2], r[3]);
+                // an infinite value is one already in the first term; its product with the remainder says nothing
+                auto both = [](float hi, float lo) { return fabsf(hi) < INFINITY ? hi + lo : hi; };
+                o[2 * d][0] = fmaf(o[2 * d][0], corr, both(x0[0], x0[2]));
+                o[2 * d][1] = fmaf(o[2 * d][1], corr, both(x0[1], x0[3]));
+                o[2 * d + 1][0] = fmaf(o[2 * d + 1][0], corr, both(x1[0], x1[2]));
+                o[2 * d + 1][1] = fmaf(o[2 * d + 1][1], corr, both(x1[1], x1[3]));
+            }
+        }
+        const bool ends = at.i == at.s.tiles - 1;
+        if (ends || u == n_units - 1) {
+            // ---- the segment's end: the four warps' parts of each head ----
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            float *const of_head = ml + (ht * 8 + head) * 10;
+            if (quad == 0) {
+                of_head[w4] = m;
+                of_head[4 + w4] = l;
+            }
+            __syncthreads();
+            const float M = fmaxf(fmaxf(of_head[0], of_head[1]), fmaxf(of_head[2], of_head[3])), ref = M == -INFINITY ? 0.f : M;
+            const float weight = pd_exp2(m - ref);
+            float *const mine_o = merge + ((ht * 4 + w4) * 8 + head) * S::ROW + quad * 2;
+#pragma unroll
+            for (int n = 0; n < KS * 2; n++) *reinterpret_cast<float2 *>(mine_o + n * 8) = make_float2(o[n][0] * weight, o[n][1] * weight);
+            if (w4 == 0 && quad == 0) {
+                float L = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; w++) L += of_head[4 + w] * pd_exp2(of_head[w] - ref);
+                of_head[8] = M;
+                of_head[9] = L;
+            }
+            __syncthreads();
+            const int heads_here = min(8 * HT, P.group - (at.vh % P.splits) * (8 * HT)), head0 = (at.vh / P.splits) * P.group + (at.vh % P.splits) * (8 * HT);
+            const bool whole = ends && first_tile == 0;
+            // the CTAs that share the segment, and this one's record: the first of its two where the segment began before it
+            const long long seg = unit - at.i;
+            const int cta0 = (int)(seg / per), parts = (int)((seg + at.s.tiles - 1) / per) - cta0 + 1;
+            float *const record = reinterpret_cast<float *>(P.workspace + PD_WS_RECORDS + (size_t)(2 * blockIdx.x + (first_tile == 0 ? 1 : 0)) * S::RECORD);
+            auto put = [&](int h, int d, float4 v, float M, float L) {   // four dims of an output
+                const float inv = L > 0.f ? 1.f / L : L != L ? L : 0.f;
+                Q *const out = reinterpret_cast<Q *>(P.out) + (size_t)at.row * P.out_stride + (size_t)(head0 + h) * D + d;
+                if constexpr (sizeof(Q) == 4) *reinterpret_cast<float4 *>(out) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                else *reinterpret_cast<uint2 *>(out) = make_uint2(pk_pack<Q>(v.x * inv, v.y * inv), pk_pack<Q>(v.z * inv, v.w * inv));
+                if (d == 0 && P.lse) P.lse[(size_t)at.row * P.heads + head0 + h] = L > 0.f ? (M - PD_BIAS + log2f(L)) * 0.6931471805599453f : L != L ? L : -INFINITY;
+            };
+            for (int e = tid; e < heads_here * (D / 4); e += S::THREADS) {
+                const int h = e / (D / 4), d = e % (D / 4) * 4;
+                const float *const from = merge + ((h >> 3) * 32 + (h & 7)) * S::ROW + d;
+                float4 v = *reinterpret_cast<const float4 *>(from);
+#pragma unroll
+                for (int w = 1; w < 4; w++) {
+                    const float4 x = *reinterpret_cast<const float4 *>(from + w * 8 * S::ROW);
+                    v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+                }
+                const float M_h = ml[h * 10 + 8], L_h = ml[h * 10 + 9];
+                if (whole) {
+                    put(h, d, v, M_h, L_h);
+                } else {
+                    float *const r = record + h * (D + 4);
+                    if (d == 0) *reinterpret_cast<float2 *>(r) = make_float2(M_h, L_h);
+                    *reinterpret_cast<float4 *>(r + 4 + d) = v;
+                }
+            }
+            if (!whole) {
+                __threadfence();
+                __syncthreads();
+                if (tid == 0) {
+                    unsigned *const count = reinterpret_cast<unsigned *>(P.workspace + PD_WS_HEAD) + cta0;
+                    const bool last = atomicAdd(count, 1u) == (unsigned)parts - 1;
+                    if (last) *count = 0;   // for the next launch
+                    *note = last;
+                    __threadfence();
+                }
+                __syncthreads();
+                if (*note) {
+                    // ---- join: part p is of CTA cta0 + p, its second record for p = 0 and its first one after that ----
+                    const float *const base = reinterpret_cast<const float *>(P.workspace + PD_WS_RECORDS);
+                    auto part = [&](int p, int h) { return base + ((size_t)2 * (cta0 + p) + (p == 0 ? 1 : 0)) * (S::RECORD / 4) + h * (D + 4); };
+                    for (int h = warp; h < heads_here; h += S::THREADS / 32) {
+                        float M_h = -INFINITY, L_h = 0.f;
+                        for (int p = lane; p < parts; p += 32) M_h = fmaxf(M_h, ld_l2(part(p, h)));
+                        M_h = warp_max(M_h);
+                        const float ref_h = M_h == -INFINITY ? 0.f : M_h;
+                        for (int p = lane; p < parts; p += 32) {
+                            const float2 x = ld_l2(reinterpret_cast<const float2 *>(part(p, h)));
+                            const float w = pd_exp2(x.x - ref_h);
+                            merge[p * (8 * HT) + h] = w;
+                            L_h += w * x.y;
+                        }
+                        L_h = warp_sum(L_h);
+                        if (lane == 0) {
+                            ml[h * 10 + 8] = M_h;
+                            ml[h * 10 + 9] = L_h;
+                        }
+                    }
+                    __syncthreads();
+                    for (int e = tid; e < heads_here * (D / 4); e += S::THREADS) {
+                        const int h = e / (D / 4), d = e % (D / 4) * 4;
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (int p0 = 0; p0 < parts; p0 += 8) {
+                            float4 x[8];
+#pragma unroll
+                            for (int i = 0; i < 8; i++) x[i] = p0 + i < parts ? ld_l2(reinterpret_cast<const float4 *>(part(p0 + i, h) + 4 + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                            for (int i = 0; i < 8; i++)
+                                if (p0 + i < parts) {
+                                    const float w = merge[(p0 + i) * (8 * HT) + h];
+                                    v = make_float4(fmaf(w, x[i].x, v.x), fmaf(w, x[i].y, v.y), fmaf(w, x[i].z, v.z), fmaf(w, x[i].w, v.w));
+                                }
+                        }
+                        put(h, d, v, ml[h * 10 + 8], ml[h * 10 + 9]);
+                    }
+                }
+            }
+            fresh = true;
+        }
+        advance(at);
+    }
+    pd_wait<0>();
+}
+#endif  // __CUDACC__
+
+}  // namespace rnb
