@@ -1,4 +1,6 @@
 // Operators of a paged key-value cache (declarations: include/rnb_b200.h): checks of arguments and launches.
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "launch_k.hpp"
@@ -194,6 +196,31 @@ static int pk_attention_plain(const PkAttention &a, cudaStream_t s, int *err) {
     RNB_CU(launch_k(kernel, grid, dim3(128), 0, s, a.c, a.b, (const Q *)a.q, a.q_stride, a.heads, a.scale, a.window, a.sinks, (Q *)a.out, a.out_stride, a.lse, err));
     return RNB_B200_OK;
 }
+static int pk_encode(PkTensorMap *out, void *base, const PkAttention &a) {
+    static_assert(sizeof(PkTensorMap) == sizeof(CUtensorMap) && alignof(PkTensorMap) >= alignof(CUtensorMap), "descriptor size");
+    typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                    const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static EncodeTiled encode = nullptr;
+    if (!encode) {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        RNB_CU(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+        if (q != cudaDriverEntryPointSuccess || !fn) return fail(RNB_B200_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
+        encode = reinterpret_cast<EncodeTiled>(fn);
+    }
+    const PkCache &c = a.c;
+    auto step = [](uint64_t stride, uint64_t n) { return (cuuint64_t)(n > 1 ? stride * 2 : 128); };   // of one entry only: never stepped
+    const cuuint64_t page = (cuuint64_t)1 << c.page_shift;
+    const cuuint64_t dims[5] = {64, page, (cuuint64_t)c.head_dim / 64, (cuuint64_t)c.kv_heads, (cuuint64_t)c.n_pages};
+    const cuuint64_t strides[4] = {step(c.pos_stride, page), 128, step(c.head_stride, c.kv_heads), step(c.page_stride, c.n_pages)};
+    const cuuint32_t box[5] = {64, (cuuint32_t)std::min<cuuint64_t>(page, PD_TILE), (cuuint32_t)c.head_dim / 64, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+    const CUresult r = encode(reinterpret_cast<CUtensorMap *>(out), a.c_type == RNB_B200_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+                              base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(RNB_B200_CUDA_ERROR, "cuTensorMapEncodeTiled(pages) failed with driver code %d", (int)r);
+    return RNB_B200_OK;
+}
+
 template <class Q, class C, int D, int HT>
 static int pk_decode_launch(const PkAttention &a, cudaStream_t s, State &st) {
     using S = PdShape<D, HT>;
@@ -216,7 +243,10 @@ static int pk_decode_launch(const PkAttention &a, cudaStream_t s, State &st) {
     P.err = st.dev_error;
     const int grid = std::min(std::min(st.sm_count, 148) * S::PER_SM, PD_MAX_GRID);
     static_assert(148 * S::PER_SM * 2 * S::RECORD <= PK_WORKSPACE_BYTES - PD_WS_RECORDS, "records");
-    RNB_CU(launch_k(paged_decode_kernel<Q, C, D, HT>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s, a.c, a.b, P));
+    PkMaps maps;
+    RNB_TRY(pk_encode(&maps.k, a.c.k, a));
+    RNB_TRY(pk_encode(&maps.v, a.c.v, a));
+    RNB_CU(launch_k(paged_decode_kernel<Q, C, D, HT>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s, a.c, a.b, P, maps));
     return RNB_B200_OK;
 }
 // Up to eight query heads per key head: four warps; more: eight warps, 16 heads at a time.

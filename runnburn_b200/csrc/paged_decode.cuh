@@ -11,8 +11,9 @@
 // by a power of two per head into the range of f16, probabilities by 2^BIAS, so that small ones keep their bits.  Products start from zero and are
 // added to the f32 sums in registers: long sums in the tensor cores' accumulators would be cut off at each step.
 //
-// K and V tiles come in by 16-byte asynchronous copies, each thread following the page of its rows: any page size and stride, and rows that
-// are not visible are filled with zeros, so what lies there never enters a product.
+// A warp of its own brings K and V tiles in by tiled copies, a box per page (or 64 positions of a larger one), its lanes following the table
+// one tile ahead; a ring of barriers lets every warp go at its own pace.  Boxes that hold nothing visible are not fetched.  Where a tile
+// has rows that are not visible, their scores are left out and their values set to zero, so what lies there never enters a product.
 #pragma once
 #include "paged.cuh"
 
@@ -28,14 +29,14 @@ constexpr unsigned PD_WS_MARK = 0x5a5a5a5au;
 
 template <int D, int HT>
 struct PdShape {
-    static constexpr int THREADS = 128 * HT;
-    static constexpr int STAGES = D == 128 ? 3 : 4;
+    static constexpr int WORKERS = 128 * HT, THREADS = WORKERS + 32;
+    static constexpr int STAGES = D == 128 ? (HT == 1 ? 3 : 5) : 4;
     static constexpr int PER_SM = HT == 1 ? (D == 128 ? 2 : 3) : (D == 128 ? 1 : 2);
-    static constexpr int ROW = D + 8;                                                    // floats between the heads of a partial output: no bank conflicts
+    static constexpr int ROW = D + 4;                                                    // floats between the heads of a partial output
     static constexpr uint32_t TILE_BYTES = PD_TILE * D * 2;
     static constexpr size_t MERGE = sizeof(float) * HT * 4 * 8 * ROW;                    // outputs of the warps; weights of the parts in a join
     static constexpr size_t JOIN = sizeof(float) * HT * 8 * 148 * PER_SM;
-    static constexpr size_t SMEM = STAGES * 2 * TILE_BYTES + (MERGE > JOIN ? MERGE : JOIN) + sizeof(float) * HT * 8 * 10 + 64;
+    static constexpr size_t SMEM = STAGES * 2 * TILE_BYTES + (MERGE > JOIN ? MERGE : JOIN) + sizeof(float) * HT * 8 * 10 + 128;
     static constexpr size_t RECORD = sizeof(float) * HT * 8 * (D + 4);                   // per head: maximum, sum, two unused, output
 };
 
@@ -50,14 +51,25 @@ struct PdParams {
     int *err;
 };
 
+// Pools as tensors of [page][head][64-element part of a row][position][64]: a box is up to 64 positions of a page with all parts of their rows, each part
+// in the 128-byte swizzle.
+struct alignas(64) PkTensorMap {
+    unsigned long long opaque[16];
+};
+struct PkMaps {
+    PkTensorMap k, v;
+};
+
 #ifdef __CUDACC__
-__device__ __forceinline__ void pd_copy16(uint32_t dst, const void *src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+__device__ __forceinline__ void pk_tma_5d(uint32_t dst, const PkTensorMap *map, int pos, int head, int page, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+                 ::"r"(dst), "l"(map), "r"(0), "r"(pos), "r"(0), "r"(head), "r"(page), "r"(smem_u32(bar))
+                 : "memory");
 }
-__device__ __forceinline__ void pd_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// the workers of a CTA, without its copying warp
 template <int N>
-__device__ __forceinline__ void pd_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void pk_sync_some() {
+    asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ float pd_exp2(float x) {
     float y;
@@ -83,14 +95,23 @@ __device__ __forceinline__ PdSeen pd_seen(int len, int window, int sinks) {
 
 template <class Q, class C, int D, int HT>
 RNB_GLOBAL void __launch_bounds__(PdShape<D, HT>::THREADS, PdShape<D, HT>::PER_SM)
-paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
+paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ PkMaps maps) {
     using S = PdShape<D, HT>;
-    constexpr int KS = D / 16, CH = D / 8, PASS_ROWS = S::THREADS / CH, PASSES = PD_TILE / PASS_ROWS;
-    extern __shared__ __align__(128) uint8_t pd_smem[];
+    constexpr int KS = D / 16;
+    extern __shared__ __align__(1024) uint8_t pd_smem[];
     float *const merge = reinterpret_cast<float *>(pd_smem + S::STAGES * 2 * S::TILE_BYTES);
-    float *const ml = reinterpret_cast<float *>(pd_smem + S::SMEM - 64 - sizeof(float) * HT * 8 * 10);   // [head][m of 4 warps, l of 4 warps, M, L]
-    volatile int *const note = reinterpret_cast<volatile int *>(pd_smem + S::SMEM - 64);
+    float *const ml = reinterpret_cast<float *>(pd_smem + S::SMEM - 128 - sizeof(float) * HT * 8 * 10);   // [head][m of 4 warps, l of 4 warps, M, L]
+    uint64_t *const full = reinterpret_cast<uint64_t *>(pd_smem + S::SMEM - 128), *const empty = full + S::STAGES;
+    volatile int *const note = reinterpret_cast<volatile int *>(full + 2 * S::STAGES);
     pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::STAGES; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 4 * HT);
+        }
+        mbar_fence_init();
+        note[1] = (smem_u32(pd_smem) & 1023u) != 0;   // a wait gave up (or the swizzle would not hold): no more waits, the results are void
+    }
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, w4 = warp & 3, ht = warp >> 2;
     const int VH = c.kv_heads * P.splits;
@@ -158,62 +179,75 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
     };
     auto start = [](const Walk &w) { return PD_TILE * (w.i < w.s.lead ? w.i : w.i + w.s.skip); };
 
-    // ---- copies: a thread has the same 16 bytes of PASSES rows; their pages are looked up one tile ahead ----
-    const int c_row = tid / CH, c_at = tid % CH;
-    const uint32_t c_dst = smem_u32(pd_smem) + c_row * (D * 2) + ((c_at ^ (c_row & 7)) << 4);   // PASS_ROWS is a multiple of 8
-    Walk next = at;
-    long long left = n_units;
-    int pages[PASSES];
     auto visible = [](const PdSeen &s, int pos) { return pos < s.len && (pos >= s.from || pos < s.sink); };
-    auto look_up = [&]() {
-        const int p0 = start(next) + c_row;
-#pragma unroll
-        for (int p = 0; p < PASSES; p++) {
-            const int pos = p0 + p * PASS_ROWS;
-            pages[p] = left > 0 && visible(next.s, pos) ? b.table[(size_t)next.row * b.table_stride + (pos >> c.page_shift)] : -1;
-        }
-    };
-    auto issue = [&](int stage) {
-        if (left > 0) {
-            const uint32_t dst = c_dst + stage * 2 * S::TILE_BYTES;
-            const int p0 = start(next) + c_row;
-            const size_t head = (size_t)(next.vh / P.splits) * c.head_stride + c_at * 8;
-#pragma unroll
-            for (int p = 0; p < PASSES; p++) {
-                const int pos = p0 + p * PASS_ROWS;
-                bool live = visible(next.s, pos);
-                if (live && (unsigned)pages[p] >= (unsigned)c.n_pages) {
-                    atomicExch(P.err, DEV_ERR_BAD_PAGE);
-                    live = false;
-                }
-                const size_t from = live ? (size_t)pages[p] * c.page_stride + (size_t)(pos & ((1 << c.page_shift) - 1)) * c.pos_stride + head : 0;
-                pd_copy16(dst + p * PASS_ROWS * (D * 2), c.k + from, live);
-                pd_copy16(dst + S::TILE_BYTES + p * PASS_ROWS * (D * 2), c.v + from, live);
+    const int box = min(1 << c.page_shift, PD_TILE);   // positions of a box
+
+    if (warp == 4 * HT) {
+        // ---- copies: lane i has box i / 2 of a tile, keys or values ----
+        const int mine = (lane >> 1) * box;
+        const PkTensorMap *const map = lane & 1 ? &maps.v : &maps.k;
+        const uint32_t dst = smem_u32(pd_smem) + (lane & 1) * S::TILE_BYTES + mine * (D * 2);
+        bool ok = note[1] == 0;
+        long long u = 0;
+        int stage = 0;
+        uint32_t phase = 1;   // of the empty barriers: a fresh one counts as passed
+        auto look_up = [&](int &pos, bool &live) {   // the page of this lane's box of tile `at`
+            pos = start(at) + mine;
+            live = mine < PD_TILE && pos < at.s.len && (pos + box > at.s.from || pos < at.s.sink);
+            return live ? b.table[(size_t)at.row * b.table_stride + (pos >> c.page_shift)] : 0;
+        };
+        int pos, vh = at.vh;
+        bool live;
+        int page = look_up(pos, live);
+        for (; u < n_units && ok; u++) {
+            if (live && (unsigned)page >= (unsigned)c.n_pages) {
+                atomicExch(P.err, DEV_ERR_BAD_PAGE);
+                live = false;
             }
-            left--;
-            advance(next);
-            look_up();
+            const bool now = live;
+            const int at_pos = pos & ((1 << c.page_shift) - 1), at_page = page, at_head = vh / P.splits;
+            if (u + 1 < n_units) {
+                advance(at);
+                vh = at.vh;
+                page = look_up(pos, live);
+            }
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[stage], phase));
+            if (!ok) break;
+            const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, now)) * (uint32_t)box * (D * 2);
+            if (lane == 0) mbar_arrive_expect_tx(&full[stage], bytes);
+            __syncwarp();
+            if (now) pk_tma_5d(dst + stage * 2 * S::TILE_BYTES, map, at_pos, at_head, at_page, &full[stage]);
+            if (++stage == S::STAGES) stage = 0, phase ^= 1;
         }
-        pd_commit();
-    };
-    look_up();
-    for (int s = 0; s < S::STAGES - 1; s++) issue(s);
+        if (!ok && lane == 0) {
+            note[1] = 1;
+            atomicExch(P.err, DEV_ERR_MBAR_TIMEOUT);
+        }
+        // no copy is under way when the CTA ends: the last STAGES tiles have been waited for by the workers, or are here
+        for (int i = 0; i < S::STAGES && u > 0; i++, u--) {
+            if (--stage < 0) stage = S::STAGES - 1, phase ^= 1;
+            mbar_wait_bounded(&full[stage], phase ^ 1);
+        }
+        return;
+    }
 
     // ---- products ----
     const int head = lane >> 2, quad = lane & 3;   // of the rows and columns that this thread holds
     uint32_t qa[KS][4];
     float o[KS * 2][2], m = -INFINITY, l = 0.f, to_log2 = 0.f;
+    // a row's place in a tile: boxes one after the other, in a box the parts of 64 elements, rows of 128 bytes
+    auto place = [&](uint32_t r) { return (r & ~(uint32_t)(box - 1)) * (D * 2) + (r & (uint32_t)(box - 1)) * 128u; };
+    const uint32_t part = (uint32_t)box * 128u;
     const uint32_t k_row = 16 * w4 + (lane & 7) + ((lane >> 4) << 3), v_row = 16 * w4 + (lane & 7) + (((lane >> 3) & 1) << 3);
-    const uint32_t k_base = smem_u32(pd_smem) + k_row * (D * 2), v_base = smem_u32(pd_smem) + S::TILE_BYTES + v_row * (D * 2);
+    const uint32_t k_base = smem_u32(pd_smem) + place(k_row), v_base = smem_u32(pd_smem) + S::TILE_BYTES + place(v_row);
     const uint32_t k_x = k_row & 7, v_x = v_row & 7, k_c = (lane >> 3) & 1, v_c = lane >> 4;
+    uint32_t phase = 0;
+    bool ok = note[1] == 0;
     bool fresh = true;   // a segment begins
     long long unit = begin;
     int first_tile = at.i;
     int stage = 0;
-    for (long long u = 0; u < n_units; u++, unit++, stage = stage + 1 < S::STAGES ? stage + 1 : 0) {
-        pd_wait<S::STAGES - 2>();
-        __syncthreads();
-        issue(stage > 0 ? stage - 1 : S::STAGES - 1);   // the one that the tile before has left
+    for (long long u = 0; u < n_units; u++, unit++) {
         const int group0 = (at.vh % P.splits) * (8 * HT) + ht * 8, mine = group0 + head, q_head = (at.vh / P.splits) * P.group + mine;
         if (fresh) {
             fresh = false;
@@ -258,13 +292,18 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
             l = 0.f;
         }
         const int p0 = start(at) + 16 * w4;
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[stage], phase));
+        if (!ok && lane == 0) {
+            note[1] = 1;
+            atomicExch(P.err, DEV_ERR_MBAR_TIMEOUT);
+        }
         if (p0 < at.s.len && (p0 + 15 >= at.s.from || p0 < at.s.sink)) {
             float s0[4] = {}, s1[4] = {};
             const uint32_t kt = k_base + stage * 2 * S::TILE_BYTES, vt = v_base + stage * 2 * S::TILE_BYTES;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 uint32_t r[4];
-                pk_ldmatrix(r, kt + (((2 * k + k_c) ^ k_x) << 4));
+                pk_ldmatrix(r, kt + (k >> 2) * part + (((2 * (k & 3) + k_c) ^ k_x) << 4));
                 pk_mma<C>(s0, qa[k], r[0], r[1]);
                 pk_mma<C>(s1, qa[k], r[2], r[3]);
             }
@@ -282,13 +321,24 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
 #pragma unroll
             for (int i = 0; i < 4; i++) t[i] = pd_exp2(t[i] - ref + PD_BIAS);
             l = l * corr + ((t[0] + t[1]) + (t[2] + t[3]));
+            if (p0 + 15 >= at.s.len || (p0 < at.s.from && p0 + 15 >= at.s.sink)) {
+                // values that are not visible become zeros: whatever they were, zero times it has to be zero
+                const uint4 zero = make_uint4(0, 0, 0, 0);
+                for (int e = lane; e < 16 * (D / 8); e += 32) {
+                    const uint32_t r = 16 * w4 + e / (D / 8), ch = e % (D / 8);
+                    if (!visible(at.s, start(at) + (int)r))
+                        *reinterpret_cast<uint4 *>(pd_smem + stage * 2 * S::TILE_BYTES + S::TILE_BYTES + place(r) + (ch >> 3) * part + (ch & 7) * 16) = zero;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the next copy to the same place
+                __syncwarp();
+            }
             uint32_t pa[4];
             pk_split<C>(t[0], t[1], pa[0], pa[1]);
             pk_split<C>(t[2], t[3], pa[2], pa[3]);
 #pragma unroll
             for (int d = 0; d < KS; d++) {
                 uint32_t r[4];
-                pk_ldmatrix_trans(r, vt + (((2 * d + v_c) ^ v_x) << 4));
+                pk_ldmatrix_trans(r, vt + (d >> 2) * part + (((2 * (d & 3) + v_c) ^ v_x) << 4));
                 float x0[4] = {}, x1[4] = {};
                 pk_mma<C>(x0, pa, r[0], r[1]);
                 pk_mma<C>(x1, pa, r[2], r[3]);
@@ -300,6 +350,9 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
                 o[2 * d + 1][1] = fmaf(o[2 * d + 1][1], corr, both(x1[1], x1[3]));
             }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[stage]);
+        if (++stage == S::STAGES) stage = 0, phase ^= 1;
         const bool ends = at.i == at.s.tiles - 1;
         if (ends || u == n_units - 1) {
             // ---- the segment's end: the four warps' parts of each head ----
@@ -310,7 +363,7 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
                 of_head[w4] = m;
                 of_head[4 + w4] = l;
             }
-            __syncthreads();
+            pk_sync_some<S::WORKERS>();
             const float M = fmaxf(fmaxf(of_head[0], of_head[1]), fmaxf(of_head[2], of_head[3])), ref = M == -INFINITY ? 0.f : M;
             const float weight = pd_exp2(m - ref);
             float *const mine_o = merge + ((ht * 4 + w4) * 8 + head) * S::ROW + quad * 2;
@@ -323,7 +376,7 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
                 of_head[8] = M;
                 of_head[9] = L;
             }
-            __syncthreads();
+            pk_sync_some<S::WORKERS>();
             const int heads_here = min(8 * HT, P.group - (at.vh % P.splits) * (8 * HT)), head0 = (at.vh / P.splits) * P.group + (at.vh % P.splits) * (8 * HT);
             const bool whole = ends && first_tile == 0;
             // the CTAs that share the segment, and this one's record: the first of its two where the segment began before it
@@ -337,7 +390,7 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
                 else *reinterpret_cast<uint2 *>(out) = make_uint2(pk_pack<Q>(v.x * inv, v.y * inv), pk_pack<Q>(v.z * inv, v.w * inv));
                 if (d == 0 && P.lse) P.lse[(size_t)at.row * P.heads + head0 + h] = L > 0.f ? (M - PD_BIAS + log2f(L)) * 0.6931471805599453f : L != L ? L : -INFINITY;
             };
-            for (int e = tid; e < heads_here * (D / 4); e += S::THREADS) {
+            for (int e = tid; e < heads_here * (D / 4); e += S::WORKERS) {
                 const int h = e / (D / 4), d = e % (D / 4) * 4;
                 const float *const from = merge + ((h >> 3) * 32 + (h & 7)) * S::ROW + d;
                 float4 v = *reinterpret_cast<const float4 *>(from);
@@ -357,7 +410,7 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
             }
             if (!whole) {
                 __threadfence();
-                __syncthreads();
+                pk_sync_some<S::WORKERS>();
                 if (tid == 0) {
                     unsigned *const count = reinterpret_cast<unsigned *>(P.workspace + PD_WS_HEAD) + cta0;
                     const bool last = atomicAdd(count, 1u) == (unsigned)parts - 1;
@@ -365,12 +418,12 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
                     *note = last;
                     __threadfence();
                 }
-                __syncthreads();
+                pk_sync_some<S::WORKERS>();
                 if (*note) {
                     // ---- join: part p is of CTA cta0 + p, its second record for p = 0 and its first one after that ----
                     const float *const base = reinterpret_cast<const float *>(P.workspace + PD_WS_RECORDS);
                     auto part = [&](int p, int h) { return base + ((size_t)2 * (cta0 + p) + (p == 0 ? 1 : 0)) * (S::RECORD / 4) + h * (D + 4); };
-                    for (int h = warp; h < heads_here; h += S::THREADS / 32) {
+                    for (int h = warp; h < heads_here; h += S::WORKERS / 32) {
                         float M_h = -INFINITY, L_h = 0.f;
                         for (int p = lane; p < parts; p += 32) M_h = fmaxf(M_h, ld_l2(part(p, h)));
                         M_h = warp_max(M_h);
@@ -387,8 +440,8 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
                             ml[h * 10 + 9] = L_h;
                         }
                     }
-                    __syncthreads();
-                    for (int e = tid; e < heads_here * (D / 4); e += S::THREADS) {
+                    pk_sync_some<S::WORKERS>();
+                    for (int e = tid; e < heads_here * (D / 4); e += S::WORKERS) {
                         const int h = e / (D / 4), d = e % (D / 4) * 4;
                         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                         for (int p0 = 0; p0 < parts; p0 += 8) {
@@ -410,7 +463,6 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P) {
         }
         advance(at);
     }
-    pd_wait<0>();
 }
 #endif  // __CUDACC__
 
