@@ -5,8 +5,8 @@
 
 #include "launch_k.hpp"
 #include "paged.cuh"
-#include "paged_attention_plain.cuh"
 #include "paged_decode.cuh"
+#include "paged_prefill.cuh"
 
 namespace rnb {
 
@@ -151,8 +151,8 @@ struct PkAttention {   // a checked call
     void *out, *workspace;
     float *lse;
 };
-// the mark, the counters, and two records for every CTA of the decode kernel (16 heads of 128 dims are the largest)
-constexpr size_t PK_WORKSPACE_BYTES = PD_WS_RECORDS + 2 * PD_MAX_GRID * PdShape<128, 1>::RECORD;
+// the mark and the counters; two records for every CTA of the decode kernel, or 256 rows of sums for every CTA of the prompts' kernel in clusters
+constexpr size_t PK_WORKSPACE_BYTES = PD_WS_RECORDS + (size_t)148 * 256 * 128 * sizeof(float);
 static_assert(PD_WS_RECORDS % 256 == 0, "records are read by 16 bytes");
 
 static int pk_check_attention(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type, const void *q, size_t q_stride, size_t num_heads,
@@ -188,15 +188,8 @@ static int pk_check_attention(const rnb_b200_paged_cache *cache, const rnb_b200_
     return RNB_B200_OK;
 }
 
-template <class Q, class C>
-static int pk_attention_plain(const PkAttention &a, cudaStream_t s, int *err) {
-    const size_t items = (size_t)a.b.n_tokens * a.heads;
-    const dim3 grid((unsigned)((items + 3) / 4));
-    auto kernel = a.c.head_dim == 64 ? paged_attention_plain_kernel<Q, C, 64> : paged_attention_plain_kernel<Q, C, 128>;
-    RNB_CU(launch_k(kernel, grid, dim3(128), 0, s, a.c, a.b, (const Q *)a.q, a.q_stride, a.heads, a.scale, a.window, a.sinks, (Q *)a.out, a.out_stride, a.lse, err));
-    return RNB_B200_OK;
-}
-static int pk_encode(PkTensorMap *out, void *base, const PkAttention &a) {
+// keys: positions of a box; parts: 64-element parts of a row in it
+static int pk_encode(PkTensorMap *out, void *base, const PkAttention &a, int keys, int parts) {
     static_assert(sizeof(PkTensorMap) == sizeof(CUtensorMap) && alignof(PkTensorMap) >= alignof(CUtensorMap), "descriptor size");
     typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                     const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -213,7 +206,7 @@ static int pk_encode(PkTensorMap *out, void *base, const PkAttention &a) {
     const cuuint64_t page = (cuuint64_t)1 << c.page_shift;
     const cuuint64_t dims[5] = {64, page, (cuuint64_t)c.head_dim / 64, (cuuint64_t)c.kv_heads, (cuuint64_t)c.n_pages};
     const cuuint64_t strides[4] = {step(c.pos_stride, page), 128, step(c.head_stride, c.kv_heads), step(c.page_stride, c.n_pages)};
-    const cuuint32_t box[5] = {64, (cuuint32_t)std::min<cuuint64_t>(page, PD_TILE), (cuuint32_t)c.head_dim / 64, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+    const cuuint32_t box[5] = {64, (cuuint32_t)std::min<cuuint64_t>(page, keys), (cuuint32_t)parts, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
     const CUresult r = encode(reinterpret_cast<CUtensorMap *>(out), a.c_type == RNB_B200_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                               base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -244,8 +237,8 @@ static int pk_decode_launch(const PkAttention &a, cudaStream_t s, State &st) {
     const int grid = std::min(std::min(st.sm_count, 148) * S::PER_SM, PD_MAX_GRID);
     static_assert(148 * S::PER_SM * 2 * S::RECORD <= PK_WORKSPACE_BYTES - PD_WS_RECORDS, "records");
     PkMaps maps;
-    RNB_TRY(pk_encode(&maps.k, a.c.k, a));
-    RNB_TRY(pk_encode(&maps.v, a.c.v, a));
+    RNB_TRY(pk_encode(&maps.k, a.c.k, a, PD_TILE, D / 64));
+    RNB_TRY(pk_encode(&maps.v, a.c.v, a, PD_TILE, D / 64));
     RNB_CU(launch_k(paged_decode_kernel<Q, C, D, HT>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s, a.c, a.b, P, maps));
     return RNB_B200_OK;
 }
@@ -256,17 +249,53 @@ static int pk_decode(const PkAttention &a, cudaStream_t s, State &st) {
     if (a.c.head_dim == 64) return many ? pk_decode_launch<Q, C, 64, 2>(a, s, st) : pk_decode_launch<Q, C, 64, 1>(a, s, st);
     return many ? pk_decode_launch<Q, C, 128, 2>(a, s, st) : pk_decode_launch<Q, C, 128, 1>(a, s, st);
 }
+template <class Q, class C, int D>
+static int pk_prefill(const PkAttention &a, cudaStream_t s, State &st) {
+    using S = PpShape<Q, D>;
+    static bool ready = false;
+    if (!ready) RNB_CU(cudaFuncSetAttribute(paged_prefill_kernel<Q, C, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM));
+    ready = true;
+    PpParams P{};
+    P.q = a.q;
+    P.q_stride = a.q_stride;
+    P.out_stride = a.out_stride;
+    P.heads = a.heads;
+    P.group = a.heads / a.c.kv_heads;
+    P.blocks = (P.group + 127) / 128;
+    P.per_block = (P.group + P.blocks - 1) / P.blocks;
+    P.queries = 128 / P.per_block;
+    P.window = a.window;
+    P.sinks = a.sinks;
+    P.scale = a.scale;
+    P.out = a.out;
+    P.lse = a.lse;
+    P.sums = (float *)((uint8_t *)a.workspace + PD_WS_RECORDS);
+    P.err = st.dev_error;
+    PkMaps maps;
+    RNB_TRY(pk_encode(&maps.k, a.c.k, a, PP_KEYS, 1));
+    RNB_TRY(pk_encode(&maps.v, a.c.v, a, PP_KEYS, 1));
+    // Pairs of row blocks: the starts are on the device, so there is one more per sequence than the tokens could need.
+    const size_t pairs = std::min<size_t>((size_t)a.b.n_tokens, (size_t)a.b.n_tokens / (2 * P.queries) + (size_t)a.b.n_seq) * a.c.kv_heads * P.blocks;
+    if (pairs > 0x7fffffffu) return fail(RNB_B200_UNSUPPORTED, "paged attention: %zu blocks of rows are more than a launch can have", pairs);
+    // Keys are shared out where the launch leaves most of the chip idle and a share is at least two tiles of the longest table.
+    const long long tiles = (((long long)a.b.max_pages << a.c.page_shift) + PP_KEYS - 1) / PP_KEYS;
+    unsigned ranks = 1;
+    while (ranks < PP_MAX_CLUSTER && pairs * ranks * 2 <= (size_t)std::min(st.sm_count, 148) && tiles >= 4 * (long long)ranks) ranks *= 2;
+    if (ranks == 1) RNB_CU(launch_k(paged_prefill_kernel<Q, C, D>, dim3((unsigned)pairs), dim3(PP_THREADS), S::SMEM, s, a.c, a.b, P, maps));
+    else RNB_CU(launch_k_cluster(paged_prefill_kernel<Q, C, D>, dim3((unsigned)pairs * ranks), dim3(PP_THREADS), S::SMEM, s, dim3(ranks), a.c, a.b, P, maps));
+    return RNB_B200_OK;
+}
+template <class Q, class C>
+static int pk_attention_of(const PkAttention &a, cudaStream_t s, State &st) {
+    if (!a.b.q_start) return pk_decode<Q, C>(a, s, st);
+    return a.c.head_dim == 64 ? pk_prefill<Q, C, 64>(a, s, st) : pk_prefill<Q, C, 128>(a, s, st);
+}
 static int pk_attention(const PkAttention &a, cudaStream_t s) {
     if (a.b.n_tokens == 0 || a.b.n_seq == 0) return RNB_B200_OK;
     PkCall call;
     RNB_TRY(call.rc);
-    if (!a.b.q_start) {
-        if (a.q_type == RNB_B200_TYPE_F32) return pk_decode<float, F16>(a, s, call.st);
-        return a.q_type == RNB_B200_TYPE_F16 ? pk_decode<F16, F16>(a, s, call.st) : pk_decode<Bf16, Bf16>(a, s, call.st);
-    }
-    int *err = call.st.dev_error;
-    if (a.q_type == RNB_B200_TYPE_F32) return pk_attention_plain<float, F16>(a, s, err);
-    return a.q_type == RNB_B200_TYPE_F16 ? pk_attention_plain<F16, F16>(a, s, err) : pk_attention_plain<Bf16, Bf16>(a, s, err);
+    if (a.q_type == RNB_B200_TYPE_F32) return pk_attention_of<float, F16>(a, s, call.st);
+    return a.q_type == RNB_B200_TYPE_F16 ? pk_attention_of<F16, F16>(a, s, call.st) : pk_attention_of<Bf16, Bf16>(a, s, call.st);
 }
 
 // Nothing is thrown through the C entries.

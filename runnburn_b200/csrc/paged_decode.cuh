@@ -61,9 +61,9 @@ struct PkMaps {
 };
 
 #ifdef __CUDACC__
-__device__ __forceinline__ void pk_tma_5d(uint32_t dst, const PkTensorMap *map, int pos, int head, int page, uint64_t *bar) {
+__device__ __forceinline__ void pk_tma_5d(uint32_t dst, const PkTensorMap *map, int pos, int part, int head, int page, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-                 ::"r"(dst), "l"(map), "r"(0), "r"(pos), "r"(0), "r"(head), "r"(page), "r"(smem_u32(bar))
+                 ::"r"(dst), "l"(map), "r"(0), "r"(pos), "r"(part), "r"(head), "r"(page), "r"(smem_u32(bar))
                  : "memory");
 }
 // the workers of a CTA, without its copying warp
@@ -216,7 +216,7 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
             const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, now)) * (uint32_t)box * (D * 2);
             if (lane == 0) mbar_arrive_expect_tx(&full[stage], bytes);
             __syncwarp();
-            if (now) pk_tma_5d(dst + stage * 2 * S::TILE_BYTES, map, at_pos, at_head, at_page, &full[stage]);
+            if (now) pk_tma_5d(dst + stage * 2 * S::TILE_BYTES, map, at_pos, 0, at_head, at_page, &full[stage]);
             if (++stage == S::STAGES) stage = 0, phase ^= 1;
         }
         if (!ok && lane == 0) {

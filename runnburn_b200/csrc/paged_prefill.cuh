@@ -1,0 +1,584 @@
+// Causal attention of prompts over a paged cache on the 5th-generation tensor cores.
+//
+// A CTA owns two blocks of 128 (query, head) rows of one key head - a block is 128 / group consecutive queries of a sequence times the group's
+// heads - and walks the keys that some of its queries sees in tiles of 128.  Both blocks use a tile while it is in shared memory.  A
+// row is a tensor-memory lane and belongs to one thread of its block's four warps, so a row's maximum and sum need no shuffles.  Warp 8 issues the products:
+// scores from queries and keys in shared memory, then probabilities from tensor memory, where they take the scores' place, times
+// values.  It takes the blocks in turn, P V of block a, the next scores of a, P V of b, the next scores of b, so that one block's softmax runs under the
+// other's products.  Products of one thread run in the order of issue: scores that have arrived say that the product before them is through, and may
+// overwrite the probabilities that it has read.  Warp 9 copies K0 V0 K1 V1 ... into a ring, a box per page and 64 dims, its lanes
+// following the table.
+//
+// f32 queries enter as f16 "hi" + remainder "lo" (scaled by a power of two per row into f16's range), and so do the probabilities: every product is made
+// twice and keeps 22 bits; 16-bit queries are exact and their probabilities are rounded once to the cache's type, half a step of the output's own rounding.
+// Probabilities are scaled by 2^BIAS so that small ones keep their bits, and the output is scaled only when a row's
+// maximum has grown by more than 2^GROWTH.  The tensor cores cut sums off at every step, which adds up over long rows: f32 outputs are taken out of
+// tensor memory every FLUSH tiles and summed in f32.
+//
+// Few rows behind many keys: a cluster of up to eight CTAs shares the keys, and joins maxima, sums and outputs over distributed shared memory.
+#pragma once
+#include "paged_attention_plain.cuh"
+#include "paged_decode.cuh"
+#include "prefill_attention_tiled.cuh"
+
+namespace rnb {
+
+constexpr int PP_KEYS = 128;
+constexpr int PP_THREADS = 320;
+constexpr float PP_BIAS = 8.f, PP_GROWTH = 7.f;   // log2; together below f16's 2^16
+constexpr int PP_FLUSH = 16;
+constexpr int PP_MAX_CLUSTER = 8;
+constexpr uint32_t PP_PANEL = 128 * 128;          // 128 rows of 64 elements, 128-byte swizzle
+
+template <class Q, int D>
+struct PpShape {
+    static constexpr int TERMS = sizeof(Q) == 4 ? 2 : 1, PANELS = D / 64;
+    static constexpr uint32_t Q_BYTES = 2 * TERMS * PANELS * PP_PANEL, TILE_BYTES = PANELS * PP_PANEL;
+    static constexpr int SLOTS = (int)((224 * 1024 - Q_BYTES) / TILE_BYTES) < 8 ? (int)((224 * 1024 - Q_BYTES) / TILE_BYTES) : 8;
+    static constexpr size_t TAIL = 256 + 256 * 4;                                     // barriers; a factor per row
+    static constexpr size_t JOIN = 256 * (D + 4) * 4 + 256 * 8 + 256 * PP_MAX_CLUSTER * 4 + 256 * 8;   // outputs; maximum, sum; weights; joined
+    static constexpr size_t RING = Q_BYTES + (size_t)SLOTS * TILE_BYTES;
+    static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + TAIL;
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+struct PpParams {
+    const void *q;
+    size_t q_stride, out_stride;
+    int heads, group, blocks, per_block, queries, window, sinks;   // blocks of per_block heads per key head; queries of a row block
+    float scale;
+    void *out;
+    float *lse;
+    float *sums;   // cluster launches: 256 rows of D floats per CTA, for the f32 sums of long rows
+    int *err;
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float pp_ld_remote(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 pp_ld_remote4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// V as the second operand: dims contiguous, 8 keys x 64 dims are 1024 bytes, the other 64 dims are a panel further
+__device__ __forceinline__ uint64_t pp_v_desc(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3ffffu) >> 4) | ((uint64_t)(PP_PANEL >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// D = f32, A and B of the cache's type, M = 128
+template <class C>
+constexpr uint32_t pp_idesc(int n, bool b_mn_major) {
+    return (1u << 4) | (std::is_same<C, Bf16>::value ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// The tiles of PP_KEYS keys that queries see who see 0 .. sink - 1 and from .. len - 1.
+struct PpSeen {
+    int len, from, sink, lead, skip, tiles;
+    __device__ __forceinline__ int start(int i) const { return PP_KEYS * (i < lead ? i : i + skip); }
+    __device__ __forceinline__ bool has(int pos) const { return pos < len && (pos >= from || pos < sink); }
+};
+
+template <class Q, class C, int D>
+RNB_GLOBAL void __launch_bounds__(PP_THREADS, 1)
+paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ PkMaps maps) {
+    using S = PpShape<Q, D>;
+    extern __shared__ __align__(1024) uint8_t pp_smem[];
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint64_t *const bars = reinterpret_cast<uint64_t *>(pp_smem + S::SMEM - S::TAIL);
+    uint64_t *const full = bars, *const empty = bars + 8, *const q_full = bars + 16, *const s_full = bars + 18, *const p_full = bars + 20, *const o_full = bars + 22;   // two each
+    volatile uint32_t *const tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + 24);
+    volatile int *const failed = reinterpret_cast<volatile int *>(bars + 25);
+    volatile int *const found = reinterpret_cast<volatile int *>(bars + 26);   // sequence, first query, queries of the sequence, first row of its tokens
+    float *const factor = reinterpret_cast<float *>(pp_smem + S::SMEM - S::TAIL + 256);
+    uint32_t rank, ranks;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    if (tid == 0) {
+        for (int s = 0; s < S::SLOTS; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int x = 0; x < 2; x++) {
+            mbar_init(&q_full[x], 4);
+            mbar_init(&s_full[x], 1);
+            mbar_init(&p_full[x], 4);
+            mbar_init(&o_full[x], 1);
+        }
+        mbar_fence_init();
+        *failed = (smem_u32(pp_smem) & 1023u) != 0;
+    }
+    pdl_wait();   // tensor memory too is asked for when no earlier launch can still hold it
+    if (blockIdx.x == 0) pk_check_starts(b, P.err);
+    const int VH = c.kv_heads * P.blocks, item = (int)(blockIdx.x / ranks), vh = item % VH, head = vh / P.blocks, head0 = (vh % P.blocks) * P.per_block;
+    const int heads_here = min(P.per_block, P.group - head0);
+    if (warp == 0) {
+        // which queries: the launch's pairs of row blocks are numbered through from the last to the first, long rows before short ones
+        auto span = [&](int s, int &start) {   // tokens of a sequence; starts out of order are cut to the matrices
+            start = min(max(b.q_start[s], 0), b.n_tokens);
+            return max(0, min(b.q_start[s + 1], b.n_tokens) - start);
+        };
+        int total = 0, x;
+        for (int s = lane; s < b.n_seq; s += 32) total += (span(s, x) + 2 * P.queries - 1) / (2 * P.queries);
+        total = __reduce_add_sync(0xffffffffu, total);
+        const int want = total - 1 - item / VH;
+        int before = 0, seq = -1, first = 0, n = 0, start = 0;
+        for (int s0 = 0; s0 < b.n_seq && want >= 0 && seq < 0; s0 += 32) {
+            int st = 0;
+            const int len = s0 + lane < b.n_seq ? span(s0 + lane, st) : 0, pairs = (len + 2 * P.queries - 1) / (2 * P.queries);
+            int up = pairs;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, up, o);
+                if (lane >= o) up += y;
+            }
+            const unsigned behind = __ballot_sync(0xffffffffu, before + up > want);
+            if (behind) {
+                const int l = __ffs(behind) - 1;
+                seq = s0 + l;
+                n = __shfl_sync(0xffffffffu, len, l);
+                start = __shfl_sync(0xffffffffu, st, l);
+                first = (want - before - __shfl_sync(0xffffffffu, up - pairs, l)) * 2 * P.queries;
+            }
+            before += __shfl_sync(0xffffffffu, up, 31);
+        }
+        if (lane == 0) {
+            found[0] = seq;
+            found[1] = first;
+            found[2] = n;
+            found[3] = start;
+        }
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t *>(tmem_slot))), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pg_fence_before();
+    __syncthreads();
+    pg_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int seq = found[0], first = found[1], n_new = found[2], token0 = found[3];
+    bool ok = *failed == 0;
+    // block x holds queries first + x * queries ..; query i sits at position shift + i
+    const int shift = seq >= 0 ? pk_length(b, c.page_shift, seq, P.err) - n_new : 0;
+    const int live_a = seq >= 0 ? min(P.queries, n_new - first) : 0, live_b = seq >= 0 ? max(0, min(P.queries, n_new - first - P.queries)) : 0;
+    PpSeen seen;
+    seen.len = max(0, shift + first + live_a + live_b);
+    seen.from = P.window ? max(0, shift + first - P.window + 1) : 0;
+    seen.sink = min(P.sinks, seen.from);
+    seen.lead = min((seen.sink + PP_KEYS - 1) / PP_KEYS, seen.from / PP_KEYS);
+    seen.skip = seen.from / PP_KEYS - seen.lead;
+    seen.tiles = max(0, (seen.len + PP_KEYS - 1) / PP_KEYS - seen.skip);
+    // this CTA's share of the tiles, and of these the ones that block a sees some of (block b is behind it and sees something of all)
+    const int per = (seen.tiles + (int)ranks - 1) / (int)ranks, t0 = min(seen.tiles, per * (int)rank), n_tiles = min(per, seen.tiles - t0);
+    const int tiles_a = max(0, (shift + first + live_a + PP_KEYS - 1) / PP_KEYS - (shift + first + live_a > 0 ? seen.skip : 0));
+    const int n_a = live_b > 0 ? min(max(tiles_a - t0, 0), n_tiles) : n_tiles, n_b = live_b > 0 ? n_tiles : 0;
+
+    if (warp < 8) {
+        const int x = warp >> 2, w = warp & 3, mine = x ? n_b : n_a, live = x ? live_b : live_a, q0 = first + x * P.queries;
+        // ---- queries: a warp takes its 32 rows, several in flight ----
+        {
+            constexpr int E = sizeof(Q) == 4 ? 4 : 8, LANES = D / E, ROWS = 32 / LANES, BATCH = 8;   // elements of a lane, lanes of a row, rows of a load
+            const float sign = P.scale > 0.f ? 1.f : P.scale == 0.f ? 0.f : -1.f;   // the softmax takes maxima of unscaled scores: it needs a positive scale
+            const int d0 = lane % LANES * E;
+            for (int i = 0; i < 32 / ROWS && mine > 0 && ok; i += BATCH) {
+                uint4 raw[BATCH];
+#pragma unroll
+                for (int j = 0; j < BATCH; j++) {
+                    const int r = w * 32 + (i + j) * ROWS + lane / LANES, ql = r / heads_here;
+                    raw[j] = make_uint4(0, 0, 0, 0);
+                    if (ql < live)
+                        raw[j] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const Q *>(P.q) + (size_t)(token0 + q0 + ql) * P.q_stride +
+                                                                  (size_t)(head * P.group + head0 + r % heads_here) * D + d0);
+                }
+#pragma unroll
+                for (int j = 0; j < BATCH; j++) {
+                    const int r = w * 32 + (i + j) * ROWS + lane / LANES;
+                    uint8_t *const at = pp_smem + (uint32_t)(x * S::TERMS * S::PANELS + d0 / 64) * PP_PANEL + (uint32_t)(r >> 3) * 1024u + (uint32_t)(r & 7) * 128u +
+                                        (((uint32_t)(d0 % 64 / 8) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(d0 & 7) * 2u;
+                    if constexpr (sizeof(Q) == 4) {
+                        float v[4] = {__uint_as_float(raw[j].x), __uint_as_float(raw[j].y), __uint_as_float(raw[j].z), __uint_as_float(raw[j].w)};
+                        float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+                        for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                        // 2^e with largest * 2^-e in 1 .. 2
+                        int e = (int)((__float_as_uint(most) >> 23) & 255u) - 127;
+                        e = most == 0.f ? 0 : max(-126, min(126, e));
+                        const float down = __uint_as_float((uint32_t)(127 - e) << 23) * sign;
+                        if (lane % LANES == 0) factor[x * 128 + r] = __uint_as_float((uint32_t)(127 + e) << 23);
+                        uint2 hi, lo;
+                        pk_split<C>(v[0] * down, v[1] * down, hi.x, lo.x);
+                        pk_split<C>(v[2] * down, v[3] * down, hi.y, lo.y);
+                        *reinterpret_cast<uint2 *>(at) = hi;
+                        *reinterpret_cast<uint2 *>(at + S::PANELS * PP_PANEL) = lo;
+                    } else {
+                        auto turn = [&](uint32_t v) {   // exact
+                            const float2 f = pk_unpack<C>(v);
+                            return pk_pack<C>(f.x * sign, f.y * sign);
+                        };
+                        if (sign == 1.f) *reinterpret_cast<uint4 *>(at) = raw[j];
+                        else *reinterpret_cast<uint4 *>(at) = make_uint4(turn(raw[j].x), turn(raw[j].y), turn(raw[j].z), turn(raw[j].w));
+                    }
+                }
+            }
+            pg_proxy_fence();
+            __syncwarp();
+            if (lane == 0) pg_arrive(&q_full[x]);
+        }
+        // ---- softmax: this thread's row ----
+        const int r = w * 32 + lane, ql = r / heads_here;
+        const bool alive = ql < live;
+        const int pos = shift + q0 + min(ql, max(live - 1, 0));                       // dead rows see what the last one sees, and are not stored
+        const int pos0 = shift + q0, pos1 = shift + q0 + live - 1;                    // the block's positions
+        const uint32_t lanes = (uint32_t)(w * 32) << 16, t_s = tmem + (uint32_t)x * 128u + lanes, t_o = tmem + 256u + (uint32_t)x * 128u + lanes;
+        const float abs_scale = P.scale == 0.f ? 1.f : fabsf(P.scale);
+        const float sl2 = abs_scale * 1.4426950408889634f * (sizeof(Q) == 4 ? factor[x * 128 + r] : 1.f);   // log2 units
+        const size_t row = (size_t)(token0 + q0 + min(ql, max(live - 1, 0)));
+        const int q_head = head * P.group + head0 + r % heads_here;
+        Q *const out = reinterpret_cast<Q *>(P.out) + row * P.out_stride + (size_t)q_head * D;
+        float m_ref = -INFINITY, l_run = 0.f, m_sums = 0.f;
+        float *const sums = sizeof(Q) != 4 ? nullptr : ranks > 1 ? P.sums + ((size_t)blockIdx.x * 256 + x * 128 + r) * D : reinterpret_cast<float *>(out);
+        bool summed = false;
+        for (int t = 0; t < mine && ok; t++) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (uint32_t)(t & 1)));
+            if (!ok) break;
+            pg_fence_after();
+            uint32_t s[128];
+            {
+                uint32_t(&lo)[64] = *reinterpret_cast<uint32_t(*)[64]>(s), (&hi)[64] = *reinterpret_cast<uint32_t(*)[64]>(s + 64);
+                pat_tmem_ld64(t_s, lo);
+                pat_tmem_ld64(t_s + 64, hi);
+            }
+            const int k0 = seen.start(t0 + t);
+            if (!(k0 + PP_KEYS - 1 <= pos0 && (P.window == 0 || k0 > pos1 - P.window || k0 + PP_KEYS <= P.sinks))) {
+                // keys a .. z of the tile, and those before the end of the sinks
+                const int z = pos - k0, a = P.window ? pos - P.window + 1 - k0 : 0, k = P.sinks - k0;
+#pragma unroll
+                for (int i = 0; i < 128; i++)
+                    if (i > z || (i < a && i >= k)) s[i] = 0xff800000u;   // -inf
+            }
+            float mxs[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) mxs[j] = __uint_as_float(s[j]);
+#pragma unroll
+            for (int i = 4; i < 128; i++) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(s[i]));
+            const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * sl2;
+            float corr = 1.f;
+            if (mx > m_ref + PP_GROWTH || m_ref == -INFINITY) {
+                const float m_new = fmaxf(mx, m_ref);
+                corr = exp2f(m_ref - (m_new == -INFINITY ? 0.f : m_new));
+                m_ref = m_new;
+            }
+            const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+            const uint64_t sl22 = pg_pair_f32(sl2, sl2), nm2 = pg_pair_f32(PP_BIAS - m_use, PP_BIAS - m_use);
+            uint64_t sum[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 64; i++) {
+                const float2 y = pat_fma2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), sl22, nm2);
+                const float p0 = pat_exp2(y.x), p1 = pat_exp2(y.y);
+                pat_add2(sum[i & 1], p0, p1);
+                if constexpr (S::TERMS == 2) {
+                    uint32_t hi, lo;
+                    pk_split<C>(p0, p1, hi, lo);
+                    s[2 * i] = hi;
+                    s[2 * i + 1] = lo;
+                } else {
+                    s[2 * i] = pk_pack<C>(p0, p1);
+                }
+            }
+            l_run = fmaf(l_run, corr, pat_total(sum[0], sum[1]));
+            const bool flush = sizeof(Q) == 4 && t > 0 && t % PP_FLUSH == 0;
+            if (flush) {
+                // the tiles' sum so far joins the f32 sums; the next product starts from zero
+                const float old = summed ? exp2f(m_sums - m_use) : 0.f;
+#pragma unroll 1
+                for (int k = 0; k < D / 32; k++) {
+                    uint32_t v[32];
+                    pg_tmem_ld32(t_o + (uint32_t)k * 32u, v);
+                    if (alive) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            float4 *const at = reinterpret_cast<float4 *>(sums + k * 32 + i);
+                            const float4 a = summed ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+                            *at = make_float4(fmaf(a.x, old, __uint_as_float(v[i]) * corr), fmaf(a.y, old, __uint_as_float(v[i + 1]) * corr),
+                                              fmaf(a.z, old, __uint_as_float(v[i + 2]) * corr), fmaf(a.w, old, __uint_as_float(v[i + 3]) * corr));
+                        }
+                    }
+                }
+                summed = true;
+                m_sums = m_use;
+            } else if (t > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll 1
+                for (int k = 0; k < D / 32; k++) {
+                    uint32_t v[32];
+                    pg_tmem_ld32(t_o + (uint32_t)k * 32u, v);
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
+                    pat_tmem_st32(t_o + (uint32_t)k * 32u, v);
+                }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 2 * S::TERMS; k++) {   // 64 keys of a term are 32 columns
+                uint32_t v[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) v[i] = s[2 * ((k & 1) * 32 + i) + (k >> 1)];
+                pat_tmem_st32(t_s + (uint32_t)k * 32u, v);
+            }
+            pat_tmem_st_wait();
+            pg_fence_before();
+            __syncwarp();
+            if (lane == 0) pg_arrive(&p_full[x]);
+        }
+        if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_full[x], 0u));
+        pg_fence_after();
+        // ---- the row's end ----
+        const float m_use = m_ref == -INFINITY ? 0.f : m_ref, old = summed ? exp2f(m_sums - m_use) : 0.f;
+        auto output = [&](int k, float (&o)[32]) {   // unscaled dims 32 k ..
+            if (mine > 0 && ok) {
+                uint32_t v[32];
+                pg_tmem_ld32(t_o + (uint32_t)k * 32u, v);
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[i] = __uint_as_float(v[i]);
+                if (summed && alive) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 a = *reinterpret_cast<const float4 *>(sums + k * 32 + i);
+                        o[i] = fmaf(a.x, old, o[i]), o[i + 1] = fmaf(a.y, old, o[i + 1]), o[i + 2] = fmaf(a.z, old, o[i + 2]), o[i + 3] = fmaf(a.w, old, o[i + 3]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[i] = 0.f;
+            }
+        };
+        auto store4 = [](Q *to, float a, float b2, float c2, float d) {
+            if constexpr (sizeof(Q) == 4) *reinterpret_cast<float4 *>(to) = make_float4(a, b2, c2, d);
+            else *reinterpret_cast<uint2 *>(to) = make_uint2(pk_pack<Q>(a, b2), pk_pack<Q>(c2, d));
+        };
+        auto again = [&](bool strange, int row_pos, size_t token, int h) {   // rows that came out infinite or undefined, one by one
+            unsigned todo = __ballot_sync(0xffffffffu, strange);
+            while (todo) {
+                const int l = __ffs(todo) - 1;
+                todo &= todo - 1;
+                const int p = __shfl_sync(0xffffffffu, row_pos, l), hh = __shfl_sync(0xffffffffu, h, l);
+                const size_t tk = (size_t)__shfl_sync(0xffffffffu, (unsigned long long)token, l);
+                pk_plain_row<Q, C, D>(c, b, reinterpret_cast<const Q *>(P.q) + tk * P.q_stride + (size_t)hh * D, seq, p, head, P.scale, P.window, P.sinks,
+                                      reinterpret_cast<Q *>(P.out) + tk * P.out_stride + (size_t)hh * D, P.lse ? P.lse + tk * P.heads + hh : nullptr, P.err);
+            }
+        };
+        if (ranks == 1) {
+            const float inv = l_run > 0.f ? 1.f / l_run : l_run != l_run ? l_run : 0.f;
+            bool strange = false;
+#pragma unroll 1
+            for (int k = 0; k < D / 32; k++) {
+                float o[32];
+                output(k, o);
+                if (alive && ok) {
+                    float check = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        o[i] *= inv;
+                        check = fmaf(o[i], 0.f, check);   // stays zero while all are finite
+                    }
+                    strange |= check != 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) store4(out + k * 32 + i, o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            }
+            if (alive && ok && P.lse) P.lse[row * P.heads + q_head] = l_run > 0.f ? (m_use - PP_BIAS + log2f(l_run)) * 0.6931471805599453f : l_run != l_run ? l_run : -INFINITY;
+            __syncwarp();
+            again(strange, pos, row, q_head);
+        } else {
+            // ---- a cluster's shares: outputs, maxima and sums in shared memory, where the tiles were ----
+            if (!ok) *failed = 1;
+            asm volatile("bar.sync 1, 256;" ::: "memory");   // both blocks' products are through (each block's warps have waited for its own)
+            float *const o_all = reinterpret_cast<float *>(pp_smem), *const ml = o_all + 256 * (D + 4);
+#pragma unroll 1
+            for (int k = 0; k < D / 32; k++) {
+                float o[32];
+                output(k, o);
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(o_all + (x * 128 + r) * (D + 4) + k * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+            *reinterpret_cast<float2 *>(ml + 2 * (x * 128 + r)) = make_float2(m_ref, ok ? l_run : 0.f);
+            __syncwarp();
+            ps_cluster_sync();
+            // this CTA joins rows [rank * n, (rank + 1) * n)
+            const int n = 256 / (int)ranks;
+            float *const weights = ml + 512, *const joined = weights + 256 * PP_MAX_CLUSTER;
+            const uint32_t o_addr = smem_u32(o_all), ml_addr = smem_u32(ml);
+            if (tid < n) {
+                const int R = (int)rank * n + tid;
+                float m[PP_MAX_CLUSTER], l[PP_MAX_CLUSTER], M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int p = 0; p < PP_MAX_CLUSTER; p++) {
+                    m[p] = -INFINITY, l[p] = 0.f;
+                    if (p < (int)ranks) {
+                        const uint32_t at = ps_map(ml_addr + 8u * (uint32_t)R, p);
+                        m[p] = pp_ld_remote(at);
+                        l[p] = pp_ld_remote(at + 4);
+                        M = fmaxf(M, m[p]);
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < PP_MAX_CLUSTER; p++) {
+                    const float wgt = exp2f(m[p] - (M == -INFINITY ? 0.f : M));
+                    weights[tid * PP_MAX_CLUSTER + p] = wgt;
+                    L += wgt * l[p];
+                }
+                *reinterpret_cast<float2 *>(joined + 2 * tid) = make_float2(M == -INFINITY ? 0.f : M, L);
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const bool good = *failed == 0;
+            for (int e = warp; e < n; e += 8) {   // a warp per row
+                const int R = (int)rank * n + e, bx = R >> 7, rr = R & 127, rq = rr / heads_here;
+                if (rq >= (bx ? live_b : live_a) || !good) continue;
+                const float2 ML = *reinterpret_cast<const float2 *>(joined + 2 * e);
+                const float inv = ML.y > 0.f ? 1.f / ML.y : ML.y != ML.y ? ML.y : 0.f;
+                const size_t token = (size_t)(token0 + first + bx * P.queries + rq);
+                const int h = head * P.group + head0 + rr % heads_here;
+                bool strange = false;
+                if (lane < D / 4) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int p = 0; p < (int)ranks; p++) {
+                        const float wgt = weights[e * PP_MAX_CLUSTER + p];
+                        const float4 a = pp_ld_remote4(ps_map(o_addr + (uint32_t)(R * (D + 4) + lane * 4) * 4u, p));
+                        v = make_float4(fmaf(wgt, a.x, v.x), fmaf(wgt, a.y, v.y), fmaf(wgt, a.z, v.z), fmaf(wgt, a.w, v.w));
+                    }
+                    v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                    strange = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, v.w * 0.f))) != 0.f;
+                    store4(reinterpret_cast<Q *>(P.out) + token * P.out_stride + (size_t)h * D + lane * 4, v.x, v.y, v.z, v.w);
+                }
+                if (lane == 0 && P.lse) P.lse[token * P.heads + h] = ML.y > 0.f ? (ML.x - PP_BIAS + log2f(ML.y)) * 0.6931471805599453f : ML.y != ML.y ? ML.y : -INFINITY;
+                strange = __any_sync(0xffffffffu, strange);
+                again(strange && lane == 0, shift + first + bx * P.queries + rq, token, h);
+            }
+            __syncwarp();
+            ps_cluster_sync();
+        }
+    } else if (warp == 8) {
+        // ---- products: K of tile t is item 2t of the ring, V item 2t + 1 ----
+        const uint32_t base = smem_u32(pp_smem), ring = base + S::Q_BYTES;
+        const int last = n_b > 0 ? 1 : 0;   // the block that uses a tile last
+        auto arrived = [&](int i) { return __all_sync(0xffffffffu, mbar_wait_bounded(&full[i % S::SLOTS], (uint32_t)(i / S::SLOTS) & 1u)); };
+        auto scores = [&](int x, int t) {
+            if (pg_elect()) {
+                const int slot = 2 * t % S::SLOTS;
+                const uint32_t kt = ring + (uint32_t)slot * S::TILE_BYTES;
+#pragma unroll
+                for (int term = S::TERMS - 1; term >= 0; term--)   // remainders first: the accumulator cuts off what it adds, and adds less often to full sums
+#pragma unroll
+                    for (int p = 0; p < S::PANELS; p++) {
+                        const uint64_t dq = pg_smem_desc(base + (uint32_t)((x * S::TERMS + term) * S::PANELS + p) * PP_PANEL), dk = pg_smem_desc(kt + (uint32_t)p * PP_PANEL);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) ps_mma(tmem + (uint32_t)x * 128u, dq + 2u * k, dk + 2u * k, pp_idesc<C>(128, false), (S::TERMS - 1 - term) | p | k);
+                    }
+                pg_commit(&s_full[x]);
+                if (x == last) pg_commit(&empty[slot]);
+            }
+            __syncwarp();
+        };
+        if (n_tiles > 0) {
+            ok = ok && arrived(0);
+            for (int x = 0; x < 2 && ok; x++) {
+                if ((x ? n_b : n_a) == 0) continue;
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&q_full[x], 0u));
+                pg_fence_after();
+                if (ok) scores(x, 0);
+            }
+        }
+        for (int t = 0; t < n_tiles && ok; t++) {
+            const int slot = (2 * t + 1) % S::SLOTS, k0 = seen.start(t0 + t);
+            const uint32_t vt = ring + (uint32_t)slot * S::TILE_BYTES;
+            ok = arrived(2 * t + 1);
+            if (!ok) break;
+            if (k0 + PP_KEYS > seen.len || (k0 < seen.from && k0 + PP_KEYS > seen.sink)) {
+                // values that nobody sees become zeros: whatever they were, zero times it has to be zero
+                for (int e = lane; e < PP_KEYS * S::PANELS * 8; e += 32) {
+                    const int key = e / (S::PANELS * 8), ch = e % (S::PANELS * 8);
+                    if (!seen.has(k0 + key))
+                        *reinterpret_cast<uint4 *>(pp_smem + S::Q_BYTES + (uint32_t)slot * S::TILE_BYTES + (uint32_t)(ch >> 3) * PP_PANEL + (uint32_t)key * 128u + (uint32_t)(ch & 7) * 16u) =
+                            make_uint4(0, 0, 0, 0);
+                }
+                pg_proxy_fence();
+                __syncwarp();
+            }
+            for (int x = 0; x < 2 && ok; x++) {
+                const int mine = x ? n_b : n_a;
+                if (t >= mine) continue;
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&p_full[x], (uint32_t)(t & 1)));
+                if (!ok) break;
+                pg_fence_after();
+                if (pg_elect()) {
+                    const uint64_t dv = pp_v_desc(vt);
+                    const uint32_t tp = tmem + (uint32_t)x * 128u, to = tmem + 256u + (uint32_t)x * 128u;
+                    const uint32_t more = t > 0 && !(S::TERMS == 2 && t % PP_FLUSH == 0);
+#pragma unroll
+                    for (int k = 0; k < PP_KEYS / 16; k++) {   // 16 keys: 2048 bytes of a panel of V, eight columns of probabilities
+                        pat_mma_ta(to, tp + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), more | (k != 0));
+                        if constexpr (S::TERMS == 2) pat_mma_ta(to, tp + 64u + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), 1u);
+                    }
+                    if (t == mine - 1) pg_commit(&o_full[x]);
+                    if (x == last) pg_commit(&empty[slot]);
+                }
+                __syncwarp();
+                if (t + 1 < mine) {
+                    ok = arrived(2 * t + 2);
+                    if (ok) scores(x, t + 1);
+                }
+            }
+        }
+    } else {
+        // ---- copies: lane i has box i / PANELS of a tile, 64 dims of it ----
+        const int box = min(1 << c.page_shift, PP_KEYS), blk = lane / S::PANELS * box, part = lane % S::PANELS;
+        const uint32_t dst = smem_u32(pp_smem) + S::Q_BYTES + (uint32_t)part * PP_PANEL + (uint32_t)blk * 128u;
+        auto look_up = [&](int t, int &pos, bool &live) {
+            pos = seen.start(t0 + t) + blk;
+            live = blk < PP_KEYS && pos < seen.len && (pos + box > seen.from || pos < seen.sink);
+            return live ? b.table[(size_t)seq * b.table_stride + (pos >> c.page_shift)] : 0;
+        };
+        uint32_t it = 0;
+        int pos = 0, page = 0;
+        bool live = false;
+        if (n_tiles > 0) page = look_up(0, pos, live);
+        for (int t = 0; t < n_tiles && ok; t++) {
+            if (live && (unsigned)page >= (unsigned)c.n_pages) {
+                atomicExch(P.err, DEV_ERR_BAD_PAGE);
+                live = false;
+            }
+            const bool now = live;
+            const int at_pos = pos & ((1 << c.page_shift) - 1), at_page = page;
+            if (t + 1 < n_tiles) page = look_up(t + 1, pos, live);
+            const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, now)) * (uint32_t)box * 128u;
+            for (int v = 0; v < 2; v++) {
+                const uint32_t slot = it % S::SLOTS;
+                ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&empty[slot], ((it / S::SLOTS) & 1u) ^ 1u));
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
+                __syncwarp();
+                if (now) pk_tma_5d(dst + slot * S::TILE_BYTES, v ? &maps.v : &maps.k, at_pos, part, head, at_page, &full[slot]);
+                it++;
+            }
+        }
+        pg_drain(full, it, S::SLOTS);
+    }
+    __syncwarp();
+    if (warp >= 8 && ranks > 1) {
+        ps_cluster_sync();
+        ps_cluster_sync();
+    }
+    if (!ok) *failed = 1;
+    __syncwarp();
+    pg_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        if (lane == 0 && *failed) atomicExch(P.err, DEV_ERR_MBAR_TIMEOUT);
+    }
+}
+#endif  // __CUDACC__
+
+}  // namespace rnb
