@@ -9,7 +9,7 @@ namespace rnb {
 #ifdef __CUDACC__
 // q, out: the row's D elements; position `pos` of sequence `seq`, key head `head`; lse may be null.
 template <class Q, class C, int D>
-static __device__ __noinline__ void pk_plain_row(const PkCache &c, const PkBatch &b, const Q *q, int seq, int pos, int head, float scale, int window, int sinks, Q *out, float *lse,
+__device__ __forceinline__ void pk_plain_row(const PkCache &c, const PkBatch &b, const Q *q, int seq, int pos, int head, float scale, int window, int sinks, Q *out, float *lse,
                                                  int *err) {
     constexpr int PER = D / 32;   // dims of a lane
     const int lane = threadIdx.x & 31;
@@ -17,6 +17,7 @@ static __device__ __noinline__ void pk_plain_row(const PkCache &c, const PkBatch
 #pragma unroll
     for (int i = 0; i < PER; i++) x[i] = pk_value<Q>(q[lane * PER + i]);
     const int from = window ? max(0, pos - window + 1) : 0;
+#pragma unroll 1
     for (int j = min(sinks, from) > 0 ? 0 : from; j <= pos; j++) {
         if (j < from && j >= sinks) j = from;
         const int page = pk_page(b, c, seq, j, err);

@@ -24,7 +24,9 @@
 namespace rnb {
 
 constexpr int PP_KEYS = 128;
-constexpr int PP_THREADS = 320;
+constexpr int PP_THREADS = 384;   // warps 10 and 11 are there for the register split alone: setmaxnreg goes by four warps
+constexpr int PP_SOFTMAX_REGS = 208, PP_OTHER_REGS = 88;
+static_assert(256 * PP_SOFTMAX_REGS + 128 * PP_OTHER_REGS <= 384 * 168, "what the block is launched with");
 constexpr float PP_BIAS = 8.f, PP_GROWTH = 7.f;   // log2; together below f16's 2^16
 constexpr int PP_FLUSH = 16;
 constexpr int PP_MAX_CLUSTER = 8;
@@ -35,7 +37,7 @@ struct PpShape {
     static constexpr int TERMS = sizeof(Q) == 4 ? 2 : 1, PANELS = D / 64;
     static constexpr uint32_t Q_BYTES = 2 * TERMS * PANELS * PP_PANEL, TILE_BYTES = PANELS * PP_PANEL;
     static constexpr int SLOTS = (int)((224 * 1024 - Q_BYTES) / TILE_BYTES) < 8 ? (int)((224 * 1024 - Q_BYTES) / TILE_BYTES) : 8;
-    static constexpr size_t TAIL = 256 + 256 * 4;                                     // barriers; a factor per row
+    static constexpr size_t TAIL = 512 + 256 * 4;                                     // barriers; a factor per row
     static constexpr size_t JOIN = 256 * (D + 4) * 4 + 256 * 8 + 256 * PP_MAX_CLUSTER * 4 + 256 * 8;   // outputs; maximum, sum; weights; joined
     static constexpr size_t RING = Q_BYTES + (size_t)SLOTS * TILE_BYTES;
     static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + TAIL;
@@ -63,6 +65,42 @@ __device__ __forceinline__ float4 pp_ld_remote4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
+}
+// 128 columns of this thread's lane: four loads under way at once
+__device__ __forceinline__ void pp_tmem_ld128(uint32_t taddr, uint32_t (&v)[128]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%129];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%130];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%131];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
+          "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
+          "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]), "=r"(v[32]), "=r"(v[33]),
+          "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]), "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]),
+          "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]), "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]),
+          "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63]), "=r"(v[64]), "=r"(v[65]), "=r"(v[66]),
+          "=r"(v[67]), "=r"(v[68]), "=r"(v[69]), "=r"(v[70]), "=r"(v[71]), "=r"(v[72]), "=r"(v[73]), "=r"(v[74]), "=r"(v[75]), "=r"(v[76]), "=r"(v[77]),
+          "=r"(v[78]), "=r"(v[79]), "=r"(v[80]), "=r"(v[81]), "=r"(v[82]), "=r"(v[83]), "=r"(v[84]), "=r"(v[85]), "=r"(v[86]), "=r"(v[87]), "=r"(v[88]),
+          "=r"(v[89]), "=r"(v[90]), "=r"(v[91]), "=r"(v[92]), "=r"(v[93]), "=r"(v[94]), "=r"(v[95]), "=r"(v[96]), "=r"(v[97]), "=r"(v[98]), "=r"(v[99]),
+          "=r"(v[100]), "=r"(v[101]), "=r"(v[102]), "=r"(v[103]), "=r"(v[104]), "=r"(v[105]), "=r"(v[106]), "=r"(v[107]), "=r"(v[108]), "=r"(v[109]),
+          "=r"(v[110]), "=r"(v[111]), "=r"(v[112]), "=r"(v[113]), "=r"(v[114]), "=r"(v[115]), "=r"(v[116]), "=r"(v[117]), "=r"(v[118]), "=r"(v[119]),
+          "=r"(v[120]), "=r"(v[121]), "=r"(v[122]), "=r"(v[123]), "=r"(v[124]), "=r"(v[125]), "=r"(v[126]), "=r"(v[127])
+        : "r"(taddr), "r"(taddr + 32u), "r"(taddr + 64u), "r"(taddr + 96u)
+        : "memory");
+}
+template <int N>
+__device__ __forceinline__ void pp_registers(bool more) {
+    if (more) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// (x, y) in two terms by cutting x and y to the first one's bits: f16 has ten behind the point, bf16 seven
+template <class T>
+__device__ __forceinline__ void pp_cut(float x, float y, uint32_t &hi, uint32_t &lo) {
+    constexpr uint32_t MASK = std::is_same<T, F16>::value ? 0xffffe000u : 0xffff0000u;
+    const float a = __uint_as_float(__float_as_uint(x) & MASK), b = __uint_as_float(__float_as_uint(y) & MASK);
+    hi = pk_pack<T>(a, b);
+    lo = pk_pack<T>(x - a, y - b);
 }
 // V as the second operand: dims contiguous, 8 keys x 64 dims are 1024 bytes, the other 64 dims are a panel further
 __device__ __forceinline__ uint64_t pp_v_desc(uint32_t saddr) {
@@ -92,7 +130,8 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     volatile uint32_t *const tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + 24);
     volatile int *const failed = reinterpret_cast<volatile int *>(bars + 25);
     volatile int *const found = reinterpret_cast<volatile int *>(bars + 26);   // sequence, first query, queries of the sequence, first row of its tokens
-    float *const factor = reinterpret_cast<float *>(pp_smem + S::SMEM - S::TAIL + 256);
+    unsigned *const todo = reinterpret_cast<unsigned *>(bars + 28);   // rows of each warp to be done again
+    float *const factor = reinterpret_cast<float *>(pp_smem + S::SMEM - S::TAIL + 512);
     uint32_t rank, ranks;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
@@ -109,6 +148,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
         }
         mbar_fence_init();
         *failed = (smem_u32(pp_smem) & 1023u) != 0;
+        for (int i = 0; i < 8; i++) todo[i] = 0;
     }
     pdl_wait();   // tensor memory too is asked for when no earlier launch can still hold it
     if (blockIdx.x == 0) pk_check_starts(b, P.err);
@@ -176,11 +216,14 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     const int tiles_a = max(0, (shift + first + live_a + PP_KEYS - 1) / PP_KEYS - (shift + first + live_a > 0 ? seen.skip : 0));
     const int n_a = live_b > 0 ? min(max(tiles_a - t0, 0), n_tiles) : n_tiles, n_b = live_b > 0 ? n_tiles : 0;
 
+    // (one instruction for all warps of a warpgroup)
+    if (warp < 8) pp_registers<PP_SOFTMAX_REGS>(true);
+    else pp_registers<PP_OTHER_REGS>(false);
     if (warp < 8) {
         const int x = warp >> 2, w = warp & 3, mine = x ? n_b : n_a, live = x ? live_b : live_a, q0 = first + x * P.queries;
         // ---- queries: a warp takes its 32 rows, several in flight ----
         {
-            constexpr int E = sizeof(Q) == 4 ? 4 : 8, LANES = D / E, ROWS = 32 / LANES, BATCH = 8;   // elements of a lane, lanes of a row, rows of a load
+            constexpr int E = sizeof(Q) == 4 ? 4 : 8, LANES = D / E, ROWS = 32 / LANES, BATCH = 32 / ROWS < 16 ? 32 / ROWS : 16;   // elements of a lane, lanes of a row, rows of a load
             const float sign = P.scale > 0.f ? 1.f : P.scale == 0.f ? 0.f : -1.f;   // the softmax takes maxima of unscaled scores: it needs a positive scale
             const int d0 = lane % LANES * E;
             for (int i = 0; i < 32 / ROWS && mine > 0 && ok; i += BATCH) {
@@ -246,18 +289,19 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             if (!ok) break;
             pg_fence_after();
             uint32_t s[128];
-            {
-                uint32_t(&lo)[64] = *reinterpret_cast<uint32_t(*)[64]>(s), (&hi)[64] = *reinterpret_cast<uint32_t(*)[64]>(s + 64);
-                pat_tmem_ld64(t_s, lo);
-                pat_tmem_ld64(t_s + 64, hi);
-            }
+            pp_tmem_ld128(t_s, s);
             const int k0 = seen.start(t0 + t);
             if (!(k0 + PP_KEYS - 1 <= pos0 && (P.window == 0 || k0 > pos1 - P.window || k0 + PP_KEYS <= P.sinks))) {
                 // keys a .. z of the tile, and those before the end of the sinks
                 const int z = pos - k0, a = P.window ? pos - P.window + 1 - k0 : 0, k = P.sinks - k0;
+                auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };   // bits 0 .. n - 1
 #pragma unroll
-                for (int i = 0; i < 128; i++)
-                    if (i > z || (i < a && i >= k)) s[i] = 0xff800000u;   // -inf
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t keep = below(z + 1 - 32 * j) & (~below(a - 32 * j) | below(k - 32 * j));
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (!(keep & (1u << i))) s[32 * j + i] = 0xff800000u;   // -inf
+                }
             }
             float mxs[4];
 #pragma unroll
@@ -281,7 +325,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 pat_add2(sum[i & 1], p0, p1);
                 if constexpr (S::TERMS == 2) {
                     uint32_t hi, lo;
-                    pk_split<C>(p0, p1, hi, lo);
+                    pp_cut<C>(p0, p1, hi, lo);
                     s[2 * i] = hi;
                     s[2 * i + 1] = lo;
                 } else {
@@ -358,17 +402,6 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             if constexpr (sizeof(Q) == 4) *reinterpret_cast<float4 *>(to) = make_float4(a, b2, c2, d);
             else *reinterpret_cast<uint2 *>(to) = make_uint2(pk_pack<Q>(a, b2), pk_pack<Q>(c2, d));
         };
-        auto again = [&](bool strange, int row_pos, size_t token, int h) {   // rows that came out infinite or undefined, one by one
-            unsigned todo = __ballot_sync(0xffffffffu, strange);
-            while (todo) {
-                const int l = __ffs(todo) - 1;
-                todo &= todo - 1;
-                const int p = __shfl_sync(0xffffffffu, row_pos, l), hh = __shfl_sync(0xffffffffu, h, l);
-                const size_t tk = (size_t)__shfl_sync(0xffffffffu, (unsigned long long)token, l);
-                pk_plain_row<Q, C, D>(c, b, reinterpret_cast<const Q *>(P.q) + tk * P.q_stride + (size_t)hh * D, seq, p, head, P.scale, P.window, P.sinks,
-                                      reinterpret_cast<Q *>(P.out) + tk * P.out_stride + (size_t)hh * D, P.lse ? P.lse + tk * P.heads + hh : nullptr, P.err);
-            }
-        };
         if (ranks == 1) {
             const float inv = l_run > 0.f ? 1.f / l_run : l_run != l_run ? l_run : 0.f;
             bool strange = false;
@@ -389,8 +422,8 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 }
             }
             if (alive && ok && P.lse) P.lse[row * P.heads + q_head] = l_run > 0.f ? (m_use - PP_BIAS + log2f(l_run)) * 0.6931471805599453f : l_run != l_run ? l_run : -INFINITY;
+            if (strange) atomicOr(&todo[x * 4 + w], 1u << lane);
             __syncwarp();
-            again(strange, pos, row, q_head);
         } else {
             // ---- a cluster's shares: outputs, maxima and sums in shared memory, where the tiles were ----
             if (!ok) *failed = 1;
@@ -453,11 +486,18 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                     store4(reinterpret_cast<Q *>(P.out) + token * P.out_stride + (size_t)h * D + lane * 4, v.x, v.y, v.z, v.w);
                 }
                 if (lane == 0 && P.lse) P.lse[token * P.heads + h] = ML.y > 0.f ? (ML.x - PP_BIAS + log2f(ML.y)) * 0.6931471805599453f : ML.y != ML.y ? ML.y : -INFINITY;
-                strange = __any_sync(0xffffffffu, strange);
-                again(strange && lane == 0, shift + first + bx * P.queries + rq, token, h);
+                if (__any_sync(0xffffffffu, strange) && lane == 0) atomicOr(&todo[warp], 1u << (e >> 3));
             }
             __syncwarp();
             ps_cluster_sync();
+        }
+        // ---- rows that came out infinite or undefined, one by one ----
+        const int step = ranks == 1 ? 1 : 8, row0 = ranks == 1 ? warp * 32 : (int)rank * (256 / (int)ranks) + warp;
+        for (unsigned left = todo[warp]; left; left &= left - 1) {
+            const int R = row0 + (__ffs(left) - 1) * step, bx = R >> 7, rq = (R & 127) / heads_here, h = head * P.group + head0 + (R & 127) % heads_here;
+            const size_t token = (size_t)(token0 + first + bx * P.queries + rq);
+            pk_plain_row<Q, C, D>(c, b, reinterpret_cast<const Q *>(P.q) + token * P.q_stride + (size_t)h * D, seq, shift + first + bx * P.queries + rq, head, P.scale, P.window,
+                                  P.sinks, reinterpret_cast<Q *>(P.out) + token * P.out_stride + (size_t)h * D, P.lse ? P.lse + token * P.heads + h : nullptr, P.err);
         }
     } else if (warp == 8) {
         // ---- products: K of tile t is item 2t of the ring, V item 2t + 1 ----
@@ -531,7 +571,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 }
             }
         }
-    } else {
+    } else if (warp == 9) {
         // ---- copies: lane i has box i / PANELS of a tile, 64 dims of it ----
         const int box = min(1 << c.page_shift, PP_KEYS), blk = lane / S::PANELS * box, part = lane % S::PANELS;
         const uint32_t dst = smem_u32(pp_smem) + S::Q_BYTES + (uint32_t)part * PP_PANEL + (uint32_t)blk * 128u;
