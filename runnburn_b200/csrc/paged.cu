@@ -188,12 +188,11 @@ static int pk_check_attention(const rnb_b200_paged_cache *cache, const rnb_b200_
     return RNB_B200_OK;
 }
 
-// keys: positions of a box; parts: 64-element parts of a row in it
-static int pk_encode(PkTensorMap *out, void *base, const PkAttention &a, int keys, int parts) {
+static int pk_encode_tiled(PkTensorMap *out, void *base, uint32_t type, uint32_t rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box, const char *what) {
     static_assert(sizeof(PkTensorMap) == sizeof(CUtensorMap) && alignof(PkTensorMap) >= alignof(CUtensorMap), "descriptor size");
     typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                     const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static EncodeTiled encode = nullptr;
+    static EncodeTiled encode = nullptr;   // under the library's lock
     if (!encode) {
         void *fn = nullptr;
         cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
@@ -201,17 +200,22 @@ static int pk_encode(PkTensorMap *out, void *base, const PkAttention &a, int key
         if (q != cudaDriverEntryPointSuccess || !fn) return fail(RNB_B200_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
         encode = reinterpret_cast<EncodeTiled>(fn);
     }
+    const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+    const CUresult r = encode(reinterpret_cast<CUtensorMap *>(out), type == RNB_B200_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, base, dims,
+                              strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(RNB_B200_CUDA_ERROR, "cuTensorMapEncodeTiled(%s) failed with driver code %d", what, (int)r);
+    return RNB_B200_OK;
+}
+// keys: positions of a box; parts: 64-element parts of a row in it
+static int pk_encode(PkTensorMap *out, void *base, const PkAttention &a, int keys, int parts) {
     const PkCache &c = a.c;
     auto step = [](uint64_t stride, uint64_t n) { return (cuuint64_t)(n > 1 ? stride * 2 : 128); };   // of one entry only: never stepped
     const cuuint64_t page = (cuuint64_t)1 << c.page_shift;
     const cuuint64_t dims[5] = {64, page, (cuuint64_t)c.head_dim / 64, (cuuint64_t)c.kv_heads, (cuuint64_t)c.n_pages};
     const cuuint64_t strides[4] = {step(c.pos_stride, page), 128, step(c.head_stride, c.kv_heads), step(c.page_stride, c.n_pages)};
-    const cuuint32_t box[5] = {64, (cuuint32_t)std::min<cuuint64_t>(page, keys), (cuuint32_t)parts, 1, 1}, ones[5] = {1, 1, 1, 1, 1};
-    const CUresult r = encode(reinterpret_cast<CUtensorMap *>(out), a.c_type == RNB_B200_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
-                              base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(RNB_B200_CUDA_ERROR, "cuTensorMapEncodeTiled(pages) failed with driver code %d", (int)r);
-    return RNB_B200_OK;
+    const cuuint32_t box[5] = {64, (cuuint32_t)std::min<cuuint64_t>(page, keys), (cuuint32_t)parts, 1, 1};
+    return pk_encode_tiled(out, base, a.c_type, 5, dims, strides, box, "pages");
 }
 
 template <class Q, class C, int D, int HT>
@@ -271,9 +275,15 @@ static int pk_prefill(const PkAttention &a, cudaStream_t s, State &st) {
     P.lse = a.lse;
     P.sums = (float *)((uint8_t *)a.workspace + PD_WS_RECORDS);
     P.err = st.dev_error;
-    PkMaps maps;
+    P.by_heads = (65536 + P.per_block - 1) / P.per_block;
+    PpMaps maps{};
     RNB_TRY(pk_encode(&maps.k, a.c.k, a, PP_KEYS, 1));
     RNB_TRY(pk_encode(&maps.v, a.c.v, a, PP_KEYS, 1));
+    if (sizeof(Q) == 2) {
+        const cuuint64_t dims[4] = {64, (cuuint64_t)a.heads, (cuuint64_t)a.b.n_tokens, D / 64}, strides[3] = {D * 2, (cuuint64_t)(a.b.n_tokens > 1 ? a.q_stride * 2 : 128), 128};
+        const cuuint32_t box[4] = {64, (cuuint32_t)P.per_block, (cuuint32_t)P.queries, 1};
+        RNB_TRY(pk_encode_tiled(&maps.q, const_cast<void *>(a.q), a.c_type, 4, dims, strides, box, "queries"));
+    }
     // Pairs of row blocks: the starts are on the device, so there is one more per sequence than the tokens could need.
     const size_t pairs = std::min<size_t>((size_t)a.b.n_tokens, (size_t)a.b.n_tokens / (2 * P.queries) + (size_t)a.b.n_seq) * a.c.kv_heads * P.blocks;
     if (pairs > 0x7fffffffu) return fail(RNB_B200_UNSUPPORTED, "paged attention: %zu blocks of rows are more than a launch can have", pairs);

@@ -5,7 +5,7 @@
 // row is a tensor-memory lane and belongs to one thread of its block's four warps, so a row's maximum and sum need no shuffles.  Warp 8 issues the products:
 // scores from queries and keys in shared memory, then probabilities from tensor memory, where they take the scores' place, times
 // values.  It takes the blocks in turn, P V of block a, the next scores of a, P V of b, the next scores of b, so that one block's softmax runs under the
-// other's products.  Products of one thread run in the order of issue: scores that have arrived say that the product before them is through, and may
+// other's products; P V starts when half of a tile's probabilities are there.  Products of one thread run in the order of issue: scores that have arrived say that the product before them is through, and may
 // overwrite the probabilities that it has read.  Warp 9 copies K0 V0 K1 V1 ... into a ring, a box per page and 64 dims, its lanes
 // following the table.
 //
@@ -44,10 +44,15 @@ struct PpShape {
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
+struct PpMaps {
+    PkTensorMap k, v;
+    PkTensorMap q;   // 16-bit queries [token][head][64-element part]: boxes of a row block, 64 dims
+};
 struct PpParams {
     const void *q;
     size_t q_stride, out_stride;
     int heads, group, blocks, per_block, queries, window, sinks;   // blocks of per_block heads per key head; queries of a row block
+    uint32_t by_heads;   // 2^16 / per_block, rounded up: row / per_block = row * by_heads >> 16
     float scale;
     void *out;
     float *lse;
@@ -102,6 +107,20 @@ __device__ __forceinline__ void pp_cut(float x, float y, uint32_t &hi, uint32_t 
     hi = pk_pack<T>(a, b);
     lo = pk_pack<T>(x - a, y - b);
 }
+__device__ __forceinline__ void pp_tma_4d(uint32_t dst, const PkTensorMap *map, int head, int token, int part, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(0), "r"(head), "r"(token), "r"(part), "r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ float2 pp_mul2(float x, float y, uint64_t m) {
+    float2 r;
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%2, %3};\n\tmul.rn.f32x2 t, t, %4;\n\tmov.b64 {%0, %1}, t;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(x), "f"(y), "l"(m));
+    return r;
+}
+// check += {x, y} * 0: zeros stay zeros (of any sign) while both are finite
+__device__ __forceinline__ void pp_check2(uint64_t &check, float x, float y) {
+    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(check) : "f"(x), "f"(y), "l"(0ull));
+}
 // V as the second operand: dims contiguous, 8 keys x 64 dims are 1024 bytes, the other 64 dims are a panel further
 __device__ __forceinline__ uint64_t pp_v_desc(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3ffffu) >> 4) | ((uint64_t)(PP_PANEL >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
@@ -120,17 +139,17 @@ struct PpSeen {
 
 template <class Q, class C, int D>
 RNB_GLOBAL void __launch_bounds__(PP_THREADS, 1)
-paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ PkMaps maps) {
+paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ PpMaps maps) {
     using S = PpShape<Q, D>;
     extern __shared__ __align__(1024) uint8_t pp_smem[];
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint64_t *const bars = reinterpret_cast<uint64_t *>(pp_smem + S::SMEM - S::TAIL);
-    uint64_t *const full = bars, *const empty = bars + 8, *const q_full = bars + 16, *const s_full = bars + 18, *const p_full = bars + 20, *const o_full = bars + 22;   // two each
-    volatile uint32_t *const tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + 24);
-    volatile int *const failed = reinterpret_cast<volatile int *>(bars + 25);
-    volatile int *const found = reinterpret_cast<volatile int *>(bars + 26);   // sequence, first query, queries of the sequence, first row of its tokens
-    unsigned *const todo = reinterpret_cast<unsigned *>(bars + 28);   // rows of each warp to be done again
+    uint64_t *const full = bars, *const empty = bars + 8, *const q_full = bars + 16, *const s_full = bars + 18, *const p_full = bars + 20, *const o_full = bars + 24;   // two each, p_full 2 x 2
+    volatile uint32_t *const tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + 26);
+    volatile int *const failed = reinterpret_cast<volatile int *>(bars + 27);
+    volatile int *const found = reinterpret_cast<volatile int *>(bars + 28);   // sequence, first query, queries of the sequence, first row of its tokens, its positions
+    unsigned *const todo = reinterpret_cast<unsigned *>(bars + 32);   // rows of each warp to be done again
     float *const factor = reinterpret_cast<float *>(pp_smem + S::SMEM - S::TAIL + 512);
     uint32_t rank, ranks;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -141,9 +160,10 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             mbar_init(&empty[s], 1);
         }
         for (int x = 0; x < 2; x++) {
-            mbar_init(&q_full[x], 4);
+            mbar_init(&q_full[x], S::TERMS == 2 ? 4 : 1);
             mbar_init(&s_full[x], 1);
-            mbar_init(&p_full[x], 4);
+            mbar_init(&p_full[2 * x], 4);
+            mbar_init(&p_full[2 * x + 1], 4);
             mbar_init(&o_full[x], 1);
         }
         mbar_fence_init();
@@ -153,7 +173,9 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     pdl_wait();   // tensor memory too is asked for when no earlier launch can still hold it
     if (blockIdx.x == 0) pk_check_starts(b, P.err);
     const int VH = c.kv_heads * P.blocks, item = (int)(blockIdx.x / ranks), vh = item % VH, head = vh / P.blocks, head0 = (vh % P.blocks) * P.per_block;
+    // rows of a block: (query, head) = (row / per_block, row % per_block), by multiplication, exact for rows below 128; the last of several head blocks may have fewer heads
     const int heads_here = min(P.per_block, P.group - head0);
+    auto query_of = [&](int row) { return (int)((uint32_t)row * P.by_heads >> 16); };
     if (warp == 0) {
         // which queries: the launch's pairs of row blocks are numbered through from the last to the first, long rows before short ones
         auto span = [&](int s, int &start) {   // tokens of a sequence; starts out of order are cut to the matrices
@@ -189,6 +211,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             found[1] = first;
             found[2] = n;
             found[3] = start;
+            found[4] = seq >= 0 ? pk_length(b, c.page_shift, seq, P.err) : 0;
         }
     }
     if (warp == 8) {
@@ -202,7 +225,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     const int seq = found[0], first = found[1], n_new = found[2], token0 = found[3];
     bool ok = *failed == 0;
     // block x holds queries first + x * queries ..; query i sits at position shift + i
-    const int shift = seq >= 0 ? pk_length(b, c.page_shift, seq, P.err) - n_new : 0;
+    const int shift = found[4] - n_new;
     const int live_a = seq >= 0 ? min(P.queries, n_new - first) : 0, live_b = seq >= 0 ? max(0, min(P.queries, n_new - first - P.queries)) : 0;
     PpSeen seen;
     seen.len = max(0, shift + first + live_a + live_b);
@@ -221,49 +244,42 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     else pp_registers<PP_OTHER_REGS>(false);
     if (warp < 8) {
         const int x = warp >> 2, w = warp & 3, mine = x ? n_b : n_a, live = x ? live_b : live_a, q0 = first + x * P.queries;
-        // ---- queries: a warp takes its 32 rows, several in flight ----
-        {
-            constexpr int E = sizeof(Q) == 4 ? 4 : 8, LANES = D / E, ROWS = 32 / LANES, BATCH = 32 / ROWS < 16 ? 32 / ROWS : 16;   // elements of a lane, lanes of a row, rows of a load
-            const float sign = P.scale > 0.f ? 1.f : P.scale == 0.f ? 0.f : -1.f;   // the softmax takes maxima of unscaled scores: it needs a positive scale
-            const int d0 = lane % LANES * E;
-            for (int i = 0; i < 32 / ROWS && mine > 0 && ok; i += BATCH) {
-                uint4 raw[BATCH];
+        uint8_t *const q_smem = pp_smem + (uint32_t)(x * S::TERMS * S::PANELS) * PP_PANEL;   // this block's; rows w * 32 .. of every panel are this warp's
+        if constexpr (S::TERMS == 2) {
+            // ---- f32 queries in two terms: a warp takes its 32 rows, several under way ----
+            constexpr int LANES = D / 4, ROWS = 32 / LANES, LOADS = 32 / ROWS;   // lanes of a row, rows of a load
+            const int d0 = lane % LANES * 4;
+            const float *const q = reinterpret_cast<const float *>(P.q) + (size_t)(token0 + q0) * P.q_stride + (size_t)(head * P.group + head0) * D + d0;
+            if (mine > 0) {
+                float4 raw[LOADS];
 #pragma unroll
-                for (int j = 0; j < BATCH; j++) {
-                    const int r = w * 32 + (i + j) * ROWS + lane / LANES, ql = r / heads_here;
-                    raw[j] = make_uint4(0, 0, 0, 0);
-                    if (ql < live)
-                        raw[j] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const Q *>(P.q) + (size_t)(token0 + q0 + ql) * P.q_stride +
-                                                                  (size_t)(head * P.group + head0 + r % heads_here) * D + d0);
+                for (int j = 0; j < LOADS; j++) {
+                    const int row = w * 32 + j * ROWS + lane / LANES, ql = query_of(row), h = row - ql * P.per_block;
+                    raw[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (ql < live && h < heads_here) raw[j] = *reinterpret_cast<const float4 *>(q + (size_t)ql * P.q_stride + (size_t)h * D);
                 }
+                uint8_t *const to = q_smem + (uint32_t)(d0 / 64) * PP_PANEL + (uint32_t)(w * 32 + lane / LANES) * 128u + (uint32_t)(d0 & 7) * 2u;
 #pragma unroll
-                for (int j = 0; j < BATCH; j++) {
-                    const int r = w * 32 + (i + j) * ROWS + lane / LANES;
-                    uint8_t *const at = pp_smem + (uint32_t)(x * S::TERMS * S::PANELS + d0 / 64) * PP_PANEL + (uint32_t)(r >> 3) * 1024u + (uint32_t)(r & 7) * 128u +
-                                        (((uint32_t)(d0 % 64 / 8) ^ (uint32_t)(r & 7)) << 4) + (uint32_t)(d0 & 7) * 2u;
-                    if constexpr (sizeof(Q) == 4) {
-                        float v[4] = {__uint_as_float(raw[j].x), __uint_as_float(raw[j].y), __uint_as_float(raw[j].z), __uint_as_float(raw[j].w)};
-                        float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+                for (int j = 0; j < LOADS; j++) {
+                    const float4 v = raw[j];
+                    float most = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+                    if constexpr (LANES == 32) {
+                        most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));   // of values that are not negative, as whole numbers
+                    } else {
 #pragma unroll
                         for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                        // 2^e with largest * 2^-e in 1 .. 2
-                        int e = (int)((__float_as_uint(most) >> 23) & 255u) - 127;
-                        e = most == 0.f ? 0 : max(-126, min(126, e));
-                        const float down = __uint_as_float((uint32_t)(127 - e) << 23) * sign;
-                        if (lane % LANES == 0) factor[x * 128 + r] = __uint_as_float((uint32_t)(127 + e) << 23);
-                        uint2 hi, lo;
-                        pk_split<C>(v[0] * down, v[1] * down, hi.x, lo.x);
-                        pk_split<C>(v[2] * down, v[3] * down, hi.y, lo.y);
-                        *reinterpret_cast<uint2 *>(at) = hi;
-                        *reinterpret_cast<uint2 *>(at + S::PANELS * PP_PANEL) = lo;
-                    } else {
-                        auto turn = [&](uint32_t v) {   // exact
-                            const float2 f = pk_unpack<C>(v);
-                            return pk_pack<C>(f.x * sign, f.y * sign);
-                        };
-                        if (sign == 1.f) *reinterpret_cast<uint4 *>(at) = raw[j];
-                        else *reinterpret_cast<uint4 *>(at) = make_uint4(turn(raw[j].x), turn(raw[j].y), turn(raw[j].z), turn(raw[j].w));
                     }
+                    // 2^e with largest * 2^-e in 1 .. 2
+                    int e = (int)((__float_as_uint(most) >> 23) & 255u) - 127;
+                    e = most == 0.f ? 0 : max(-126, min(126, e));
+                    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                    if (lane % LANES == 0) factor[x * 128 + w * 32 + j * ROWS + lane / LANES] = __uint_as_float((uint32_t)(127 + e) << 23);
+                    uint2 hi, lo;
+                    pp_cut<C>(v.x * down, v.y * down, hi.x, lo.x);
+                    pp_cut<C>(v.z * down, v.w * down, hi.y, lo.y);
+                    uint8_t *const at = to + j * ROWS * 128 + (((d0 % 64 / 8) ^ ((j * ROWS + lane / LANES) & 7)) << 4);
+                    *reinterpret_cast<uint2 *>(at) = hi;
+                    *reinterpret_cast<uint2 *>(at + S::PANELS * PP_PANEL) = lo;
                 }
             }
             pg_proxy_fence();
@@ -271,18 +287,18 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             if (lane == 0) pg_arrive(&q_full[x]);
         }
         // ---- softmax: this thread's row ----
-        const int r = w * 32 + lane, ql = r / heads_here;
-        const bool alive = ql < live;
+        const int r = w * 32 + lane, ql = query_of(r);
+        const bool alive = ql < live && r - ql * P.per_block < heads_here;
         const int pos = shift + q0 + min(ql, max(live - 1, 0));                       // dead rows see what the last one sees, and are not stored
         const int pos0 = shift + q0, pos1 = shift + q0 + live - 1;                    // the block's positions
         const uint32_t lanes = (uint32_t)(w * 32) << 16, t_s = tmem + (uint32_t)x * 128u + lanes, t_o = tmem + 256u + (uint32_t)x * 128u + lanes;
-        const float abs_scale = P.scale == 0.f ? 1.f : fabsf(P.scale);
-        const float sl2 = abs_scale * 1.4426950408889634f * (sizeof(Q) == 4 ? factor[x * 128 + r] : 1.f);   // log2 units
+        const float turned = P.scale > 0.f ? 1.f : P.scale == 0.f ? 0.f : -1.f;   // maxima are of unscaled scores: they need a positive scale
+        const float sl2 = (P.scale == 0.f ? 1.f : fabsf(P.scale)) * 1.4426950408889634f * (S::TERMS == 2 && mine > 0 ? factor[x * 128 + r] : 1.f);   // to log2 units
         const size_t row = (size_t)(token0 + q0 + min(ql, max(live - 1, 0)));
-        const int q_head = head * P.group + head0 + r % heads_here;
-        Q *const out = reinterpret_cast<Q *>(P.out) + row * P.out_stride + (size_t)q_head * D;
+        const int q_head = head * P.group + head0 + r - ql * P.per_block;
+        Q *const out0 = reinterpret_cast<Q *>(P.out) + (size_t)(token0 + q0) * P.out_stride + (size_t)(head * P.group + head0) * D;   // the block's first row
         float m_ref = -INFINITY, l_run = 0.f, m_sums = 0.f;
-        float *const sums = sizeof(Q) != 4 ? nullptr : ranks > 1 ? P.sums + ((size_t)blockIdx.x * 256 + x * 128 + r) * D : reinterpret_cast<float *>(out);
+        float *const sums = sizeof(Q) != 4 ? nullptr : ranks > 1 ? P.sums + ((size_t)blockIdx.x * 256 + x * 128 + r) * D : reinterpret_cast<float *>(out0 + (size_t)ql * P.out_stride + (size_t)(r - ql * P.per_block) * D);
         bool summed = false;
         for (int t = 0; t < mine && ok; t++) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (uint32_t)(t & 1)));
@@ -290,6 +306,10 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             pg_fence_after();
             uint32_t s[128];
             pp_tmem_ld128(t_s, s);
+            if (turned != 1.f) {
+#pragma unroll
+                for (int i = 0; i < 128; i++) s[i] = __float_as_uint(__uint_as_float(s[i]) * turned);
+            }
             const int k0 = seen.start(t0 + t);
             if (!(k0 + PP_KEYS - 1 <= pos0 && (P.window == 0 || k0 > pos1 - P.window || k0 + PP_KEYS <= P.sinks))) {
                 // keys a .. z of the tile, and those before the end of the sinks
@@ -316,23 +336,6 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 m_ref = m_new;
             }
             const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-            const uint64_t sl22 = pg_pair_f32(sl2, sl2), nm2 = pg_pair_f32(PP_BIAS - m_use, PP_BIAS - m_use);
-            uint64_t sum[2] = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 64; i++) {
-                const float2 y = pat_fma2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), sl22, nm2);
-                const float p0 = pat_exp2(y.x), p1 = pat_exp2(y.y);
-                pat_add2(sum[i & 1], p0, p1);
-                if constexpr (S::TERMS == 2) {
-                    uint32_t hi, lo;
-                    pp_cut<C>(p0, p1, hi, lo);
-                    s[2 * i] = hi;
-                    s[2 * i + 1] = lo;
-                } else {
-                    s[2 * i] = pk_pack<C>(p0, p1);
-                }
-            }
-            l_run = fmaf(l_run, corr, pat_total(sum[0], sum[1]));
             const bool flush = sizeof(Q) == 4 && t > 0 && t % PP_FLUSH == 0;
             if (flush) {
                 // the tiles' sum so far joins the f32 sums; the next product starts from zero
@@ -364,17 +367,27 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 }
             }
             __syncwarp();
+            const uint64_t sl22 = pg_pair_f32(sl2, sl2), nm2 = pg_pair_f32(PP_BIAS - m_use, PP_BIAS - m_use);
+            uint64_t sum[2] = {0, 0};
 #pragma unroll
-            for (int k = 0; k < 2 * S::TERMS; k++) {   // 64 keys of a term are 32 columns
-                uint32_t v[32];
+            for (int half = 0; half < 2; half++) {   // 64 keys: 32 columns of a term
+                uint32_t hi[32], lo[32];
 #pragma unroll
-                for (int i = 0; i < 32; i++) v[i] = s[2 * ((k & 1) * 32 + i) + (k >> 1)];
-                pat_tmem_st32(t_s + (uint32_t)k * 32u, v);
+                for (int i = 0; i < 32; i++) {
+                    const float2 y = pat_fma2(__uint_as_float(s[64 * half + 2 * i]), __uint_as_float(s[64 * half + 2 * i + 1]), sl22, nm2);
+                    const float p0 = pat_exp2(y.x), p1 = pat_exp2(y.y);
+                    pat_add2(sum[i & 1], p0, p1);
+                    if constexpr (S::TERMS == 2) pp_cut<C>(p0, p1, hi[i], lo[i]);
+                    else hi[i] = pk_pack<C>(p0, p1);
+                }
+                pat_tmem_st32(t_s + (uint32_t)half * 32u, hi);
+                if constexpr (S::TERMS == 2) pat_tmem_st32(t_s + 64u + (uint32_t)half * 32u, lo);
+                pat_tmem_st_wait();
+                pg_fence_before();
+                __syncwarp();
+                if (lane == 0) pg_arrive(&p_full[2 * x + half]);
             }
-            pat_tmem_st_wait();
-            pg_fence_before();
-            __syncwarp();
-            if (lane == 0) pg_arrive(&p_full[x]);
+            l_run = fmaf(l_run, corr, pat_total(sum[0], sum[1]));
         }
         if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_full[x], 0u));
         pg_fence_after();
@@ -403,24 +416,52 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             else *reinterpret_cast<uint2 *>(to) = make_uint2(pk_pack<Q>(a, b2), pk_pack<Q>(c2, d));
         };
         if (ranks == 1) {
+            // 128 bytes of every row at a time through shared memory, where this warp's queries were, so that eight lanes store a row's
             const float inv = l_run > 0.f ? 1.f / l_run : l_run != l_run ? l_run : 0.f;
-            bool strange = false;
+            const uint64_t inv2 = pg_pair_f32(inv, inv);
+            uint64_t check = 0;   // stays zero while all are finite
+            Q *to[8];             // the rows that this lane stores 16 bytes of
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int rr = w * 32 + 4 * k + (lane >> 3), rq = query_of(rr), h = rr - rq * P.per_block;
+                to[k] = rq < live && h < heads_here && ok ? out0 + (size_t)rq * P.out_stride + (size_t)h * D + (lane & 7) * (16 / (int)sizeof(Q)) : nullptr;
+            }
+            constexpr int COLS = 128 / (int)sizeof(Q);
 #pragma unroll 1
-            for (int k = 0; k < D / 32; k++) {
-                float o[32];
-                output(k, o);
-                if (alive && ok) {
-                    float check = 0.f;
+            for (int k = 0; k < D / COLS; k++) {
+                uint8_t *const box = q_smem + (uint32_t)(k & (S::TERMS * S::PANELS > 1)) * PP_PANEL + (uint32_t)(w * 32) * 128u;
+                __syncwarp();   // a row's sums are read by now, and what was stored out of the box
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        o[i] *= inv;
-                        check = fmaf(o[i], 0.f, check);   // stays zero while all are finite
+                for (int j = 0; j < COLS / 32; j++) {
+                    float o[32];
+                    output(k * (COLS / 32) + j, o);
+                    uint32_t v[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 y = pp_mul2(o[i], o[i + 1], inv2);
+                        pp_check2(check, y.x, y.y);
+                        if constexpr (sizeof(Q) == 4) {
+                            v[i] = __float_as_uint(y.x);
+                            v[i + 1] = __float_as_uint(y.y);
+                        } else {
+                            v[i / 2] = pk_pack<Q>(y.x, y.y);
+                        }
                     }
-                    strange |= check != 0.f;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) store4(out + k * 32 + i, o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    for (int i = 0; i < 8 / (COLS / 32); i++) {
+                        const int ch = j * 4 + i;
+                        *reinterpret_cast<uint4 *>(box + lane * 128 + ((ch ^ (lane & 7)) << 4)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int rr = 4 * i + (lane >> 3);
+                    const uint4 y = *reinterpret_cast<const uint4 *>(box + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+                    if (to[i]) *reinterpret_cast<uint4 *>(to[i] + k * COLS) = y;
                 }
             }
+            const bool strange = alive && ok && !((uint32_t)check << 1 == 0 && (uint32_t)(check >> 32) << 1 == 0);
             if (alive && ok && P.lse) P.lse[row * P.heads + q_head] = l_run > 0.f ? (m_use - PP_BIAS + log2f(l_run)) * 0.6931471805599453f : l_run != l_run ? l_run : -INFINITY;
             if (strange) atomicOr(&todo[x * 4 + w], 1u << lane);
             __syncwarp();
@@ -467,12 +508,12 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const bool good = *failed == 0;
             for (int e = warp; e < n; e += 8) {   // a warp per row
-                const int R = (int)rank * n + e, bx = R >> 7, rr = R & 127, rq = rr / heads_here;
-                if (rq >= (bx ? live_b : live_a) || !good) continue;
+                const int R = (int)rank * n + e, bx = R >> 7, rr = R & 127, rq = query_of(rr);
+                if (rq >= (bx ? live_b : live_a) || rr - rq * P.per_block >= heads_here || !good) continue;
                 const float2 ML = *reinterpret_cast<const float2 *>(joined + 2 * e);
                 const float inv = ML.y > 0.f ? 1.f / ML.y : ML.y != ML.y ? ML.y : 0.f;
                 const size_t token = (size_t)(token0 + first + bx * P.queries + rq);
-                const int h = head * P.group + head0 + rr % heads_here;
+                const int h = head * P.group + head0 + rr - rq * P.per_block;
                 bool strange = false;
                 if (lane < D / 4) {
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -494,7 +535,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
         // ---- rows that came out infinite or undefined, one by one ----
         const int step = ranks == 1 ? 1 : 8, row0 = ranks == 1 ? warp * 32 : (int)rank * (256 / (int)ranks) + warp;
         for (unsigned left = todo[warp]; left; left &= left - 1) {
-            const int R = row0 + (__ffs(left) - 1) * step, bx = R >> 7, rq = (R & 127) / heads_here, h = head * P.group + head0 + (R & 127) % heads_here;
+            const int R = row0 + (__ffs(left) - 1) * step, bx = R >> 7, rq = query_of(R & 127), h = head * P.group + head0 + (R & 127) - rq * P.per_block;
             const size_t token = (size_t)(token0 + first + bx * P.queries + rq);
             pk_plain_row<Q, C, D>(c, b, reinterpret_cast<const Q *>(P.q) + token * P.q_stride + (size_t)h * D, seq, shift + first + bx * P.queries + rq, head, P.scale, P.window,
                                   P.sinks, reinterpret_cast<Q *>(P.out) + token * P.out_stride + (size_t)h * D, P.lse ? P.lse + token * P.heads + h : nullptr, P.err);
@@ -537,35 +578,42 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             if (!ok) break;
             if (k0 + PP_KEYS > seen.len || (k0 < seen.from && k0 + PP_KEYS > seen.sink)) {
                 // values that nobody sees become zeros: whatever they were, zero times it has to be zero
-                for (int e = lane; e < PP_KEYS * S::PANELS * 8; e += 32) {
-                    const int key = e / (S::PANELS * 8), ch = e % (S::PANELS * 8);
-                    if (!seen.has(k0 + key))
-                        *reinterpret_cast<uint4 *>(pp_smem + S::Q_BYTES + (uint32_t)slot * S::TILE_BYTES + (uint32_t)(ch >> 3) * PP_PANEL + (uint32_t)key * 128u + (uint32_t)(ch & 7) * 16u) =
-                            make_uint4(0, 0, 0, 0);
-                }
+                auto clear = [&](int lo, int hi) {
+                    for (int e = max(lo, 0) * 8 + lane; e < min(hi, PP_KEYS) * 8; e += 32)
+#pragma unroll
+                        for (int p = 0; p < S::PANELS; p++)
+                            *reinterpret_cast<uint4 *>(pp_smem + S::Q_BYTES + (uint32_t)slot * S::TILE_BYTES + (uint32_t)p * PP_PANEL + (uint32_t)e * 16u) = make_uint4(0, 0, 0, 0);
+                };
+                clear(seen.len - k0, PP_KEYS);
+                clear(seen.sink - k0, seen.from - k0);
                 pg_proxy_fence();
                 __syncwarp();
             }
             for (int x = 0; x < 2 && ok; x++) {
                 const int mine = x ? n_b : n_a;
                 if (t >= mine) continue;
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&p_full[x], (uint32_t)(t & 1)));
-                if (!ok) break;
-                pg_fence_after();
-                if (pg_elect()) {
-                    const uint64_t dv = pp_v_desc(vt);
-                    const uint32_t tp = tmem + (uint32_t)x * 128u, to = tmem + 256u + (uint32_t)x * 128u;
-                    const uint32_t more = t > 0 && !(S::TERMS == 2 && t % PP_FLUSH == 0);
+                const uint64_t dv = pp_v_desc(vt);
+                const uint32_t tp = tmem + (uint32_t)x * 128u, to = tmem + 256u + (uint32_t)x * 128u;
+                const uint32_t more = t > 0 && !(S::TERMS == 2 && t % PP_FLUSH == 0);
 #pragma unroll
-                    for (int k = 0; k < PP_KEYS / 16; k++) {   // 16 keys: 2048 bytes of a panel of V, eight columns of probabilities
-                        pat_mma_ta(to, tp + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), more | (k != 0));
-                        if constexpr (S::TERMS == 2) pat_mma_ta(to, tp + 64u + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), 1u);
+                for (int half = 0; half < 2; half++) {
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&p_full[2 * x + half], (uint32_t)(t & 1)));
+                    if (!ok) break;
+                    pg_fence_after();
+                    if (pg_elect()) {
+#pragma unroll
+                        for (int k = 4 * half; k < 4 * half + 4; k++) {   // 16 keys: 2048 bytes of a panel of V, eight columns of probabilities
+                            pat_mma_ta(to, tp + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), more | (k != 0));
+                            if constexpr (S::TERMS == 2) pat_mma_ta(to, tp + 64u + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), 1u);
+                        }
+                        if (half == 1) {
+                            if (t == mine - 1) pg_commit(&o_full[x]);
+                            if (x == last) pg_commit(&empty[slot]);
+                        }
                     }
-                    if (t == mine - 1) pg_commit(&o_full[x]);
-                    if (x == last) pg_commit(&empty[slot]);
+                    __syncwarp();
                 }
-                __syncwarp();
-                if (t + 1 < mine) {
+                if (ok && t + 1 < mine) {
                     ok = arrived(2 * t + 2);
                     if (ok) scores(x, t + 1);
                 }
@@ -584,6 +632,15 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
         int pos = 0, page = 0;
         bool live = false;
         if (n_tiles > 0) page = look_up(0, pos, live);
+        if constexpr (S::TERMS == 1) {   // 16-bit queries are copied as they are, with those of sequences behind this one where a block has room
+            for (int x = 0; x < 2; x++)
+                if ((x ? n_b : n_a) > 0) {
+                    if (lane == 0) mbar_arrive_expect_tx(&q_full[x], (uint32_t)(S::PANELS * P.queries * P.per_block) * 128u);
+                    __syncwarp();
+                    if (lane < S::PANELS)
+                        pp_tma_4d(smem_u32(pp_smem) + (uint32_t)(x * S::PANELS + lane) * PP_PANEL, &maps.q, head * P.group + head0, token0 + first + x * P.queries, lane, &q_full[x]);
+                }
+        }
         for (int t = 0; t < n_tiles && ok; t++) {
             if (live && (unsigned)page >= (unsigned)c.n_pages) {
                 atomicExch(P.err, DEV_ERR_BAD_PAGE);
@@ -603,6 +660,9 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 it++;
             }
         }
+        if constexpr (S::TERMS == 1)
+            for (int x = 0; x < 2; x++)
+                if ((x ? n_b : n_a) > 0) mbar_wait_bounded(&q_full[x], 0u);
         pg_drain(full, it, S::SLOTS);
     }
     __syncwarp();
