@@ -2,11 +2,10 @@
 //
 // A CTA owns two blocks of 128 (query, head) rows of one key head - a block is 128 / group consecutive queries of a sequence times the group's
 // heads - and walks the keys that some of its queries sees in tiles of 128.  Both blocks use a tile while it is in shared memory.  A
-// row is a tensor-memory lane and belongs to one thread of its block's four warps, so a row's maximum and sum need no shuffles.  Warp 8 issues the products:
+// row is a tensor-memory lane and has two threads, of two warps, which take half of a tile's keys each and tell each other their maxima.  Warp 16 issues the products:
 // scores from queries and keys in shared memory, then probabilities from tensor memory, where they take the scores' place, times
 // values.  It takes the blocks in turn, P V of block a, the next scores of a, P V of b, the next scores of b, so that one block's softmax runs under the
-// other's products; P V starts when half of a tile's probabilities are there.  Products of one thread run in the order of issue: scores that have arrived say that the product before them is through, and may
-// overwrite the probabilities that it has read.  Warp 9 copies K0 V0 K1 V1 ... into a ring, a box per page and 64 dims, its lanes
+// other's products.  Warp 17 copies K0 V0 K1 V1 ... into a ring, a box per page and 64 dims, its lanes
 // following the table.
 //
 // f32 queries enter as f16 "hi" + remainder "lo" (scaled by a power of two per row into f16's range), and so do the probabilities: every product is made
@@ -24,9 +23,9 @@
 namespace rnb {
 
 constexpr int PP_KEYS = 128;
-constexpr int PP_THREADS = 384;   // warps 10 and 11 are there for the register split alone: setmaxnreg goes by four warps
-constexpr int PP_SOFTMAX_REGS = 208, PP_OTHER_REGS = 88;
-static_assert(256 * PP_SOFTMAX_REGS + 128 * PP_OTHER_REGS <= 384 * 168, "what the block is launched with");
+constexpr int PP_SOFTMAX_WARPS = 16, PP_THREADS = 640;   // warp 19 is there for the register split alone: setmaxnreg goes by four warps
+constexpr int PP_SOFTMAX_REGS = 104, PP_OTHER_REGS = 64;
+static_assert(512 * PP_SOFTMAX_REGS + 128 * PP_OTHER_REGS <= 640 * 96, "what the block is launched with");
 constexpr float PP_BIAS = 8.f, PP_GROWTH = 7.f;   // log2; together below f16's 2^16
 constexpr int PP_FLUSH = 16;
 constexpr int PP_MAX_CLUSTER = 8;
@@ -36,8 +35,13 @@ template <class Q, int D>
 struct PpShape {
     static constexpr int TERMS = sizeof(Q) == 4 ? 2 : 1, PANELS = D / 64;
     static constexpr uint32_t Q_BYTES = 2 * TERMS * PANELS * PP_PANEL, TILE_BYTES = PANELS * PP_PANEL;
+    // tensor memory: where it has room, probabilities have columns of their own and the scores' columns serve both blocks in turn
+    static constexpr bool SHARED = 2 * D + 2 * TERMS * 64 + 128 <= 512;
+    static constexpr uint32_t scores_at(int x) { return SHARED ? 2 * D : (uint32_t)x * 128u; }
+    static constexpr uint32_t probabilities_at(int x) { return SHARED ? 2 * D + 128 + (uint32_t)(x * TERMS * 64) : (uint32_t)x * 128u; }
+    static constexpr uint32_t outputs_at(int x) { return (SHARED ? 0u : 256u) + (uint32_t)(x * D); }
     static constexpr int SLOTS = (int)((224 * 1024 - Q_BYTES) / TILE_BYTES) < 8 ? (int)((224 * 1024 - Q_BYTES) / TILE_BYTES) : 8;
-    static constexpr size_t TAIL = 512 + 256 * 4;                                     // barriers; a factor per row
+    static constexpr size_t TAIL = 512 + 512 * 4;                                     // barriers; what the threads of a row tell each other
     static constexpr size_t JOIN = 256 * (D + 4) * 4 + 256 * 8 + 256 * PP_MAX_CLUSTER * 4 + 256 * 8;   // outputs; maximum, sum; weights; joined
     static constexpr size_t RING = Q_BYTES + (size_t)SLOTS * TILE_BYTES;
     static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + TAIL;
@@ -70,29 +74,6 @@ __device__ __forceinline__ float4 pp_ld_remote4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
-}
-// 128 columns of this thread's lane: four loads under way at once
-__device__ __forceinline__ void pp_tmem_ld128(uint32_t taddr, uint32_t (&v)[128]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%128];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%129];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95}, [%130];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%131];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]),
-          "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]),
-          "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]), "=r"(v[32]), "=r"(v[33]),
-          "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]), "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]),
-          "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]), "=r"(v[49]), "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]),
-          "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]), "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63]), "=r"(v[64]), "=r"(v[65]), "=r"(v[66]),
-          "=r"(v[67]), "=r"(v[68]), "=r"(v[69]), "=r"(v[70]), "=r"(v[71]), "=r"(v[72]), "=r"(v[73]), "=r"(v[74]), "=r"(v[75]), "=r"(v[76]), "=r"(v[77]),
-          "=r"(v[78]), "=r"(v[79]), "=r"(v[80]), "=r"(v[81]), "=r"(v[82]), "=r"(v[83]), "=r"(v[84]), "=r"(v[85]), "=r"(v[86]), "=r"(v[87]), "=r"(v[88]),
-          "=r"(v[89]), "=r"(v[90]), "=r"(v[91]), "=r"(v[92]), "=r"(v[93]), "=r"(v[94]), "=r"(v[95]), "=r"(v[96]), "=r"(v[97]), "=r"(v[98]), "=r"(v[99]),
-          "=r"(v[100]), "=r"(v[101]), "=r"(v[102]), "=r"(v[103]), "=r"(v[104]), "=r"(v[105]), "=r"(v[106]), "=r"(v[107]), "=r"(v[108]), "=r"(v[109]),
-          "=r"(v[110]), "=r"(v[111]), "=r"(v[112]), "=r"(v[113]), "=r"(v[114]), "=r"(v[115]), "=r"(v[116]), "=r"(v[117]), "=r"(v[118]), "=r"(v[119]),
-          "=r"(v[120]), "=r"(v[121]), "=r"(v[122]), "=r"(v[123]), "=r"(v[124]), "=r"(v[125]), "=r"(v[126]), "=r"(v[127])
-        : "r"(taddr), "r"(taddr + 32u), "r"(taddr + 64u), "r"(taddr + 96u)
-        : "memory");
 }
 template <int N>
 __device__ __forceinline__ void pp_registers(bool more) {
@@ -134,7 +115,7 @@ constexpr uint32_t pp_idesc(int n, bool b_mn_major) {
 struct PpSeen {
     int len, from, sink, lead, skip, tiles;
     __device__ __forceinline__ int start(int i) const { return PP_KEYS * (i < lead ? i : i + skip); }
-    __device__ __forceinline__ bool has(int pos) const { return pos < len && (pos >= from || pos < sink); }
+    __device__ __forceinline__ bool ragged(int k0) const { return k0 + PP_KEYS > len || (k0 < from && k0 + PP_KEYS > sink); }   // not all of its keys are seen
 };
 
 template <class Q, class C, int D>
@@ -145,12 +126,12 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint64_t *const bars = reinterpret_cast<uint64_t *>(pp_smem + S::SMEM - S::TAIL);
-    uint64_t *const full = bars, *const empty = bars + 8, *const q_full = bars + 16, *const s_full = bars + 18, *const p_full = bars + 20, *const o_full = bars + 24;   // two each, p_full 2 x 2
+    uint64_t *const full = bars, *const empty = bars + 8, *const q_full = bars + 16, *const s_full = bars + 18, *const p_full = bars + 20, *const pv_done = bars + 22, *const s_free = bars + 24, *const cleared = bars + 40;   // two each of the first four
     volatile uint32_t *const tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + 26);
     volatile int *const failed = reinterpret_cast<volatile int *>(bars + 27);
     volatile int *const found = reinterpret_cast<volatile int *>(bars + 28);   // sequence, first query, queries of the sequence, first row of its tokens, its positions
     unsigned *const todo = reinterpret_cast<unsigned *>(bars + 32);   // rows of each warp to be done again
-    float *const factor = reinterpret_cast<float *>(pp_smem + S::SMEM - S::TAIL + 512);
+    float *const told = reinterpret_cast<float *>(pp_smem + S::SMEM - S::TAIL + 512);   // [block][half][row]
     uint32_t rank, ranks;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
@@ -160,15 +141,16 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             mbar_init(&empty[s], 1);
         }
         for (int x = 0; x < 2; x++) {
-            mbar_init(&q_full[x], S::TERMS == 2 ? 4 : 1);
+            mbar_init(&q_full[x], S::TERMS == 2 ? 8 : 1);
             mbar_init(&s_full[x], 1);
-            mbar_init(&p_full[2 * x], 4);
-            mbar_init(&p_full[2 * x + 1], 4);
-            mbar_init(&o_full[x], 1);
+            mbar_init(&p_full[x], 8);
+            mbar_init(&pv_done[x], 1);
         }
+        mbar_init(s_free, 8);
+        for (int i = 0; i < 8; i++) mbar_init(&cleared[i], 1);
         mbar_fence_init();
         *failed = (smem_u32(pp_smem) & 1023u) != 0;
-        for (int i = 0; i < 8; i++) todo[i] = 0;
+        for (int i = 0; i < PP_SOFTMAX_WARPS; i++) todo[i] = 0;
     }
     pdl_wait();   // tensor memory too is asked for when no earlier launch can still hold it
     if (blockIdx.x == 0) pk_check_starts(b, P.err);
@@ -214,7 +196,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             found[4] = seq >= 0 ? pk_length(b, c.page_shift, seq, P.err) : 0;
         }
     }
-    if (warp == 8) {
+    if (warp == PP_SOFTMAX_WARPS) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t *>(tmem_slot))), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -240,25 +222,27 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     const int n_a = live_b > 0 ? min(max(tiles_a - t0, 0), n_tiles) : n_tiles, n_b = live_b > 0 ? n_tiles : 0;
 
     // (one instruction for all warps of a warpgroup)
-    if (warp < 8) pp_registers<PP_SOFTMAX_REGS>(true);
+    if (warp < PP_SOFTMAX_WARPS) pp_registers<PP_SOFTMAX_REGS>(true);
     else pp_registers<PP_OTHER_REGS>(false);
-    if (warp < 8) {
-        const int x = warp >> 2, w = warp & 3, mine = x ? n_b : n_a, live = x ? live_b : live_a, q0 = first + x * P.queries;
-        uint8_t *const q_smem = pp_smem + (uint32_t)(x * S::TERMS * S::PANELS) * PP_PANEL;   // this block's; rows w * 32 .. of every panel are this warp's
+    if (warp < PP_SOFTMAX_WARPS) {
+        // a row has two threads: lane `lane` of the warps (x, half, w) with half 0 and 1, which take 64 of a tile's keys and half of the output each
+        const int x = warp >> 3, half = (warp >> 2) & 1, w = warp & 3, mine = x ? n_b : n_a, live = x ? live_b : live_a, q0 = first + x * P.queries;
+        auto both = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + x * 4 + w) : "memory"); };   // a row's two warps
+        uint8_t *const q_smem = pp_smem + (uint32_t)(x * S::TERMS * S::PANELS) * PP_PANEL;   // this block's
         if constexpr (S::TERMS == 2) {
-            // ---- f32 queries in two terms: a warp takes its 32 rows, several under way ----
-            constexpr int LANES = D / 4, ROWS = 32 / LANES, LOADS = 32 / ROWS;   // lanes of a row, rows of a load
-            const int d0 = lane % LANES * 4;
+            // ---- f32 queries in two terms: a warp takes 16 rows, all under way ----
+            constexpr int LANES = D / 4, ROWS = 32 / LANES, LOADS = 16 / ROWS;   // lanes of a row, rows of a load
+            const int d0 = lane % LANES * 4, row0 = (half * 4 + w) * 16;
             const float *const q = reinterpret_cast<const float *>(P.q) + (size_t)(token0 + q0) * P.q_stride + (size_t)(head * P.group + head0) * D + d0;
             if (mine > 0) {
                 float4 raw[LOADS];
 #pragma unroll
                 for (int j = 0; j < LOADS; j++) {
-                    const int row = w * 32 + j * ROWS + lane / LANES, ql = query_of(row), h = row - ql * P.per_block;
+                    const int row = row0 + j * ROWS + lane / LANES, ql = query_of(row), h = row - ql * P.per_block;
                     raw[j] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (ql < live && h < heads_here) raw[j] = *reinterpret_cast<const float4 *>(q + (size_t)ql * P.q_stride + (size_t)h * D);
                 }
-                uint8_t *const to = q_smem + (uint32_t)(d0 / 64) * PP_PANEL + (uint32_t)(w * 32 + lane / LANES) * 128u + (uint32_t)(d0 & 7) * 2u;
+                uint8_t *const to = q_smem + (uint32_t)(d0 / 64) * PP_PANEL + (uint32_t)(row0 + lane / LANES) * 128u + (uint32_t)(d0 & 7) * 2u;
 #pragma unroll
                 for (int j = 0; j < LOADS; j++) {
                     const float4 v = raw[j];
@@ -273,7 +257,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                     int e = (int)((__float_as_uint(most) >> 23) & 255u) - 127;
                     e = most == 0.f ? 0 : max(-126, min(126, e));
                     const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                    if (lane % LANES == 0) factor[x * 128 + w * 32 + j * ROWS + lane / LANES] = __uint_as_float((uint32_t)(127 + e) << 23);
+                    if (lane % LANES < 2) told[(x * 2 + lane % LANES) * 128 + row0 + j * ROWS + lane / LANES] = __uint_as_float((uint32_t)(127 + e) << 23);   // to both threads of the row
                     uint2 hi, lo;
                     pp_cut<C>(v.x * down, v.y * down, hi.x, lo.x);
                     pp_cut<C>(v.z * down, v.w * down, hi.y, lo.y);
@@ -291,32 +275,43 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
         const bool alive = ql < live && r - ql * P.per_block < heads_here;
         const int pos = shift + q0 + min(ql, max(live - 1, 0));                       // dead rows see what the last one sees, and are not stored
         const int pos0 = shift + q0, pos1 = shift + q0 + live - 1;                    // the block's positions
-        const uint32_t lanes = (uint32_t)(w * 32) << 16, t_s = tmem + (uint32_t)x * 128u + lanes, t_o = tmem + 256u + (uint32_t)x * 128u + lanes;
+        const uint32_t lanes = (uint32_t)(w * 32) << 16, t_s = tmem + S::scores_at(x) + lanes, t_p = tmem + S::probabilities_at(x) + lanes, t_o = tmem + S::outputs_at(x) + (uint32_t)(half * (D / 2)) + lanes;
         const float turned = P.scale > 0.f ? 1.f : P.scale == 0.f ? 0.f : -1.f;   // maxima are of unscaled scores: they need a positive scale
-        const float sl2 = (P.scale == 0.f ? 1.f : fabsf(P.scale)) * 1.4426950408889634f * (S::TERMS == 2 && mine > 0 ? factor[x * 128 + r] : 1.f);   // to log2 units
+        float sl2 = (P.scale == 0.f ? 1.f : fabsf(P.scale)) * 1.4426950408889634f;   // to log2 units
+        float *const say = told + (x * 2 + half) * 128 + r, *const hear = told + (x * 2 + (half ^ 1)) * 128 + r;
         const size_t row = (size_t)(token0 + q0 + min(ql, max(live - 1, 0)));
         const int q_head = head * P.group + head0 + r - ql * P.per_block;
         Q *const out0 = reinterpret_cast<Q *>(P.out) + (size_t)(token0 + q0) * P.out_stride + (size_t)(head * P.group + head0) * D;   // the block's first row
         float m_ref = -INFINITY, l_run = 0.f, m_sums = 0.f;
-        float *const sums = sizeof(Q) != 4 ? nullptr : ranks > 1 ? P.sums + ((size_t)blockIdx.x * 256 + x * 128 + r) * D : reinterpret_cast<float *>(out0 + (size_t)ql * P.out_stride + (size_t)(r - ql * P.per_block) * D);
+        float *const sums = sizeof(Q) != 4 ? nullptr : ranks > 1 ? P.sums + ((size_t)blockIdx.x * 256 + x * 128 + r) * D + half * (D / 2)
+                                                          : reinterpret_cast<float *>(out0 + (size_t)ql * P.out_stride + (size_t)(r - ql * P.per_block) * D + half * (D / 2));
         bool summed = false;
-        for (int t = 0; t < mine && ok; t++) {
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (uint32_t)(t & 1)));
-            if (!ok) break;
+        for (int t = 0; t < mine; t++) {
+            ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (uint32_t)(t & 1)));
+            if (!ok) {   // the other half's warp meets this one in every tile, whatever has failed
+                both();
+                continue;
+            }
             pg_fence_after();
-            uint32_t s[128];
-            pp_tmem_ld128(t_s, s);
+            uint32_t s[64];
+            pat_tmem_ld64(t_s + (uint32_t)half * 64u, s);
+            if constexpr (S::SHARED) {   // the other block's turn
+                pg_fence_before();
+                __syncwarp();
+                if (lane == 0) pg_arrive(s_free);
+            }
+            if (S::TERMS == 2 && t == 0) sl2 *= *say;   // the row's factor, from before the scores' product
             if (turned != 1.f) {
 #pragma unroll
-                for (int i = 0; i < 128; i++) s[i] = __float_as_uint(__uint_as_float(s[i]) * turned);
+                for (int i = 0; i < 64; i++) s[i] = __float_as_uint(__uint_as_float(s[i]) * turned);
             }
-            const int k0 = seen.start(t0 + t);
-            if (!(k0 + PP_KEYS - 1 <= pos0 && (P.window == 0 || k0 > pos1 - P.window || k0 + PP_KEYS <= P.sinks))) {
-                // keys a .. z of the tile, and those before the end of the sinks
+            const int k0 = seen.start(t0 + t) + half * 64;
+            if (!(k0 + 63 <= pos0 && (P.window == 0 || k0 > pos1 - P.window || k0 + 64 <= P.sinks))) {
+                // keys a .. z of the half, and those before the end of the sinks
                 const int z = pos - k0, a = P.window ? pos - P.window + 1 - k0 : 0, k = P.sinks - k0;
                 auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };   // bits 0 .. n - 1
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+                for (int j = 0; j < 2; j++) {
                     const uint32_t keep = below(z + 1 - 32 * j) & (~below(a - 32 * j) | below(k - 32 * j));
 #pragma unroll
                     for (int i = 0; i < 32; i++)
@@ -327,8 +322,13 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
 #pragma unroll
             for (int j = 0; j < 4; j++) mxs[j] = __uint_as_float(s[j]);
 #pragma unroll
-            for (int i = 4; i < 128; i++) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(s[i]));
-            const float mx = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])) * sl2;
+            for (int i = 4; i < 64; i++) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(s[i]));
+            // the other half's maximum; once both have their scores, probabilities may take the scores' place
+            *say = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
+            pg_fence_before();
+            both();
+            pg_fence_after();
+            const float mx = fmaxf(*say, *hear) * sl2;
             float corr = 1.f;
             if (mx > m_ref + PP_GROWTH || m_ref == -INFINITY) {
                 const float m_new = fmaxf(mx, m_ref);
@@ -337,11 +337,19 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             }
             const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
             const bool flush = sizeof(Q) == 4 && t > 0 && t % PP_FLUSH == 0;
+            // the product before this one is through: with scores in their probabilities' place that is said already
+            auto through = [&]() {
+                if (S::SHARED && t > 0) {
+                    ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[x], (uint32_t)((t - 1) & 1)));
+                    pg_fence_after();
+                }
+            };
             if (flush) {
+                through();
                 // the tiles' sum so far joins the f32 sums; the next product starts from zero
                 const float old = summed ? exp2f(m_sums - m_use) : 0.f;
 #pragma unroll 1
-                for (int k = 0; k < D / 32; k++) {
+                for (int k = 0; k < D / 64; k++) {
                     uint32_t v[32];
                     pg_tmem_ld32(t_o + (uint32_t)k * 32u, v);
                     if (alive) {
@@ -357,8 +365,9 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 summed = true;
                 m_sums = m_use;
             } else if (t > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+                through();
 #pragma unroll 1
-                for (int k = 0; k < D / 32; k++) {
+                for (int k = 0; k < D / 64; k++) {
                     uint32_t v[32];
                     pg_tmem_ld32(t_o + (uint32_t)k * 32u, v);
 #pragma unroll
@@ -369,31 +378,35 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             __syncwarp();
             const uint64_t sl22 = pg_pair_f32(sl2, sl2), nm2 = pg_pair_f32(PP_BIAS - m_use, PP_BIAS - m_use);
             uint64_t sum[2] = {0, 0};
+            uint32_t hi[32], lo[32];   // 64 keys: 32 columns of a term
 #pragma unroll
-            for (int half = 0; half < 2; half++) {   // 64 keys: 32 columns of a term
-                uint32_t hi[32], lo[32];
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    const float2 y = pat_fma2(__uint_as_float(s[64 * half + 2 * i]), __uint_as_float(s[64 * half + 2 * i + 1]), sl22, nm2);
-                    const float p0 = pat_exp2(y.x), p1 = pat_exp2(y.y);
-                    pat_add2(sum[i & 1], p0, p1);
-                    if constexpr (S::TERMS == 2) pp_cut<C>(p0, p1, hi[i], lo[i]);
-                    else hi[i] = pk_pack<C>(p0, p1);
-                }
-                pat_tmem_st32(t_s + (uint32_t)half * 32u, hi);
-                if constexpr (S::TERMS == 2) pat_tmem_st32(t_s + 64u + (uint32_t)half * 32u, lo);
+            for (int i = 0; i < 32; i++) {
+                const float2 y = pat_fma2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), sl22, nm2);
+                const float p0 = pat_exp2(y.x), p1 = pat_exp2(y.y);
+                pat_add2(sum[i & 1], p0, p1);
+                if constexpr (S::TERMS == 2) pp_cut<C>(p0, p1, hi[i], lo[i]);
+                else hi[i] = pk_pack<C>(p0, p1);
+            }
+            through();
+            if (ok) {
+                pat_tmem_st32(t_p + (uint32_t)half * 32u, hi);
+                if constexpr (S::TERMS == 2) pat_tmem_st32(t_p + 64u + (uint32_t)half * 32u, lo);
                 pat_tmem_st_wait();
                 pg_fence_before();
                 __syncwarp();
-                if (lane == 0) pg_arrive(&p_full[2 * x + half]);
+                if (lane == 0) pg_arrive(&p_full[x]);
             }
             l_run = fmaf(l_run, corr, pat_total(sum[0], sum[1]));
         }
-        if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_full[x], 0u));
+        if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[x], (uint32_t)((mine - 1) & 1)));
         pg_fence_after();
         // ---- the row's end ----
+        both();
+        *say = l_run;
+        both();
+        l_run += *hear;
         const float m_use = m_ref == -INFINITY ? 0.f : m_ref, old = summed ? exp2f(m_sums - m_use) : 0.f;
-        auto output = [&](int k, float (&o)[32]) {   // unscaled dims 32 k ..
+        auto output = [&](int k, float (&o)[32]) {   // unscaled, dims 32 k .. of this thread's half
             if (mine > 0 && ok) {
                 uint32_t v[32];
                 pg_tmem_ld32(t_o + (uint32_t)k * 32u, v);
@@ -416,68 +429,64 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             else *reinterpret_cast<uint2 *>(to) = make_uint2(pk_pack<Q>(a, b2), pk_pack<Q>(c2, d));
         };
         if (ranks == 1) {
-            // 128 bytes of every row at a time through shared memory, where this warp's queries were, so that eight lanes store a row's
+            // BYTES of every row's half at a time through shared memory, where the queries were, so that a few lanes store a row's
+            constexpr int BYTES = D / 2 * (int)sizeof(Q) < 128 ? D / 2 * (int)sizeof(Q) : 128, COLS = BYTES / (int)sizeof(Q), LANES = BYTES / 16;
+            uint8_t *const box = q_smem + (half * 4 + w) * (S::TERMS * S::PANELS * PP_PANEL / 8);
+            static_assert(32 * BYTES <= S::TERMS * S::PANELS * PP_PANEL / 8, "a box per warp");
             const float inv = l_run > 0.f ? 1.f / l_run : l_run != l_run ? l_run : 0.f;
             const uint64_t inv2 = pg_pair_f32(inv, inv);
             uint64_t check = 0;   // stays zero while all are finite
-            Q *to[8];             // the rows that this lane stores 16 bytes of
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int rr = w * 32 + 4 * k + (lane >> 3), rq = query_of(rr), h = rr - rq * P.per_block;
-                to[k] = rq < live && h < heads_here && ok ? out0 + (size_t)rq * P.out_stride + (size_t)h * D + (lane & 7) * (16 / (int)sizeof(Q)) : nullptr;
-            }
-            constexpr int COLS = 128 / (int)sizeof(Q);
 #pragma unroll 1
-            for (int k = 0; k < D / COLS; k++) {
-                uint8_t *const box = q_smem + (uint32_t)(k & (S::TERMS * S::PANELS > 1)) * PP_PANEL + (uint32_t)(w * 32) * 128u;
+            for (int k = 0; k < D / 2 / COLS; k++) {
                 __syncwarp();   // a row's sums are read by now, and what was stored out of the box
 #pragma unroll
                 for (int j = 0; j < COLS / 32; j++) {
                     float o[32];
                     output(k * (COLS / 32) + j, o);
-                    uint32_t v[32];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 y = pp_mul2(o[i], o[i + 1], inv2);
-                        pp_check2(check, y.x, y.y);
-                        if constexpr (sizeof(Q) == 4) {
-                            v[i] = __float_as_uint(y.x);
-                            v[i + 1] = __float_as_uint(y.y);
-                        } else {
-                            v[i / 2] = pk_pack<Q>(y.x, y.y);
+                    for (int i = 0; i < 32; i += 16 / (int)sizeof(Q)) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int e = 0; e < 16 / (int)sizeof(Q); e += 2) {
+                            const float2 y = pp_mul2(o[i + e], o[i + e + 1], inv2);
+                            pp_check2(check, y.x, y.y);
+                            if constexpr (sizeof(Q) == 4) {
+                                v[e] = __float_as_uint(y.x);
+                                v[e + 1] = __float_as_uint(y.y);
+                            } else {
+                                v[e / 2] = pk_pack<Q>(y.x, y.y);
+                            }
                         }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8 / (COLS / 32); i++) {
-                        const int ch = j * 4 + i;
-                        *reinterpret_cast<uint4 *>(box + lane * 128 + ((ch ^ (lane & 7)) << 4)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        const int ch = (j * 32 + i) * (int)sizeof(Q) / 16;
+                        *reinterpret_cast<uint4 *>(box + lane * BYTES + ((ch ^ (lane & (LANES - 1))) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
                     }
                 }
                 __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int rr = 4 * i + (lane >> 3);
-                    const uint4 y = *reinterpret_cast<const uint4 *>(box + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-                    if (to[i]) *reinterpret_cast<uint4 *>(to[i] + k * COLS) = y;
+                for (int i = 0; i < LANES; i++) {
+                    const int rr = (32 / LANES) * i + lane / LANES, ch = lane % LANES, R = w * 32 + rr, rq = query_of(R), h = R - rq * P.per_block;
+                    const uint4 y = *reinterpret_cast<const uint4 *>(box + rr * BYTES + ((ch ^ (rr & (LANES - 1))) << 4));
+                    if (rq < live && h < heads_here && ok)
+                        *reinterpret_cast<uint4 *>(out0 + (size_t)rq * P.out_stride + (size_t)h * D + half * (D / 2) + k * COLS + ch * (16 / (int)sizeof(Q))) = y;
                 }
             }
             const bool strange = alive && ok && !((uint32_t)check << 1 == 0 && (uint32_t)(check >> 32) << 1 == 0);
-            if (alive && ok && P.lse) P.lse[row * P.heads + q_head] = l_run > 0.f ? (m_use - PP_BIAS + log2f(l_run)) * 0.6931471805599453f : l_run != l_run ? l_run : -INFINITY;
+            if (alive && ok && half == 0 && P.lse) P.lse[row * P.heads + q_head] = l_run > 0.f ? (m_use - PP_BIAS + log2f(l_run)) * 0.6931471805599453f : l_run != l_run ? l_run : -INFINITY;
             if (strange) atomicOr(&todo[x * 4 + w], 1u << lane);
-            __syncwarp();
+            both();
         } else {
             // ---- a cluster's shares: outputs, maxima and sums in shared memory, where the tiles were ----
             if (!ok) *failed = 1;
-            asm volatile("bar.sync 1, 256;" ::: "memory");   // both blocks' products are through (each block's warps have waited for its own)
+            asm volatile("bar.sync 9, 512;" ::: "memory");   // both blocks' products are through (each block's warps have waited for its own)
             float *const o_all = reinterpret_cast<float *>(pp_smem), *const ml = o_all + 256 * (D + 4);
 #pragma unroll 1
-            for (int k = 0; k < D / 32; k++) {
+            for (int k = 0; k < D / 64; k++) {
                 float o[32];
                 output(k, o);
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(o_all + (x * 128 + r) * (D + 4) + k * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(o_all + (x * 128 + r) * (D + 4) + half * (D / 2) + k * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             }
-            *reinterpret_cast<float2 *>(ml + 2 * (x * 128 + r)) = make_float2(m_ref, ok ? l_run : 0.f);
+            if (half == 0) *reinterpret_cast<float2 *>(ml + 2 * (x * 128 + r)) = make_float2(m_ref, ok ? l_run : 0.f);
             __syncwarp();
             ps_cluster_sync();
             // this CTA joins rows [rank * n, (rank + 1) * n)
@@ -505,9 +514,9 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 }
                 *reinterpret_cast<float2 *>(joined + 2 * tid) = make_float2(M == -INFINITY ? 0.f : M, L);
             }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            asm volatile("bar.sync 9, 512;" ::: "memory");
             const bool good = *failed == 0;
-            for (int e = warp; e < n; e += 8) {   // a warp per row
+            for (int e = warp; e < n; e += PP_SOFTMAX_WARPS) {   // a warp per row
                 const int R = (int)rank * n + e, bx = R >> 7, rr = R & 127, rq = query_of(rr);
                 if (rq >= (bx ? live_b : live_a) || rr - rq * P.per_block >= heads_here || !good) continue;
                 const float2 ML = *reinterpret_cast<const float2 *>(joined + 2 * e);
@@ -527,26 +536,34 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                     store4(reinterpret_cast<Q *>(P.out) + token * P.out_stride + (size_t)h * D + lane * 4, v.x, v.y, v.z, v.w);
                 }
                 if (lane == 0 && P.lse) P.lse[token * P.heads + h] = ML.y > 0.f ? (ML.x - PP_BIAS + log2f(ML.y)) * 0.6931471805599453f : ML.y != ML.y ? ML.y : -INFINITY;
-                if (__any_sync(0xffffffffu, strange) && lane == 0) atomicOr(&todo[warp], 1u << (e >> 3));
+                if (__any_sync(0xffffffffu, strange) && lane == 0) atomicOr(&todo[warp], 1u << (e / PP_SOFTMAX_WARPS));
             }
             __syncwarp();
             ps_cluster_sync();
         }
         // ---- rows that came out infinite or undefined, one by one ----
-        const int step = ranks == 1 ? 1 : 8, row0 = ranks == 1 ? warp * 32 : (int)rank * (256 / (int)ranks) + warp;
-        for (unsigned left = todo[warp]; left; left &= left - 1) {
+        const int step = ranks == 1 ? 1 : PP_SOFTMAX_WARPS, row0 = ranks == 1 ? x * 128 + w * 32 : (int)rank * (256 / (int)ranks) + warp;
+        for (unsigned left = ranks > 1 ? todo[warp] : half == 0 ? todo[x * 4 + w] : 0; left; left &= left - 1) {
             const int R = row0 + (__ffs(left) - 1) * step, bx = R >> 7, rq = query_of(R & 127), h = head * P.group + head0 + (R & 127) - rq * P.per_block;
             const size_t token = (size_t)(token0 + first + bx * P.queries + rq);
             pk_plain_row<Q, C, D>(c, b, reinterpret_cast<const Q *>(P.q) + token * P.q_stride + (size_t)h * D, seq, shift + first + bx * P.queries + rq, head, P.scale, P.window,
                                   P.sinks, reinterpret_cast<Q *>(P.out) + token * P.out_stride + (size_t)h * D, P.lse ? P.lse + token * P.heads + h : nullptr, P.err);
         }
-    } else if (warp == 8) {
-        // ---- products: K of tile t is item 2t of the ring, V item 2t + 1 ----
-        const uint32_t base = smem_u32(pp_smem), ring = base + S::Q_BYTES;
-        const int last = n_b > 0 ? 1 : 0;   // the block that uses a tile last
-        auto arrived = [&](int i) { return __all_sync(0xffffffffu, mbar_wait_bounded(&full[i % S::SLOTS], (uint32_t)(i / S::SLOTS) & 1u)); };
-        auto scores = [&](int x, int t) {
-            if (pg_elect()) {
+    } else if (warp == PP_SOFTMAX_WARPS) {
+        // ---- products: K of tile t is item 2t of the ring, V item 2t + 1.  One thread waits and issues (votes of a warp around every wait took 100 to 200
+        // cycles each, in which the tensor cores had nothing to do) ----
+        if (pg_elect()) {
+            const uint32_t base = smem_u32(pp_smem), ring = base + S::Q_BYTES;
+            const int last = n_b > 0 ? 1 : 0;   // the block that uses a tile last
+            uint32_t turns = 0;                 // scores issued
+            auto arrived = [&](int i) { return mbar_wait_bounded(&full[i % S::SLOTS], (uint32_t)(i / S::SLOTS) & 1u); };
+            auto scores = [&](int x, int t) {
+                // their columns are free: the other block has read its scores, or the probabilities in them have been multiplied (nothing but its end orders a
+                // product behind one that reads what it overwrites)
+                ok = arrived(2 * t) && (S::SHARED ? turns == 0 || mbar_wait_bounded(s_free, (turns - 1) & 1u) : t == 0 || mbar_wait_bounded(&pv_done[x], (uint32_t)((t - 1) & 1)));
+                turns++;
+                if (!ok) return;
+                pg_fence_after();
                 const int slot = 2 * t % S::SLOTS;
                 const uint32_t kt = ring + (uint32_t)slot * S::TILE_BYTES;
 #pragma unroll
@@ -555,71 +572,68 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                     for (int p = 0; p < S::PANELS; p++) {
                         const uint64_t dq = pg_smem_desc(base + (uint32_t)((x * S::TERMS + term) * S::PANELS + p) * PP_PANEL), dk = pg_smem_desc(kt + (uint32_t)p * PP_PANEL);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) ps_mma(tmem + (uint32_t)x * 128u, dq + 2u * k, dk + 2u * k, pp_idesc<C>(128, false), (S::TERMS - 1 - term) | p | k);
+                        for (int k = 0; k < 4; k++) ps_mma(tmem + S::scores_at(x), dq + 2u * k, dk + 2u * k, pp_idesc<C>(128, false), (S::TERMS - 1 - term) | p | k);
                     }
                 pg_commit(&s_full[x]);
                 if (x == last) pg_commit(&empty[slot]);
-            }
-            __syncwarp();
-        };
-        if (n_tiles > 0) {
-            ok = ok && arrived(0);
+            };
+            auto outputs = [&](int x, int t, int mine, int slot) {
+                ok = mbar_wait_bounded(&p_full[x], (uint32_t)(t & 1));
+                if (!ok) return;
+                pg_fence_after();
+                const uint64_t dv = pp_v_desc(ring + (uint32_t)slot * S::TILE_BYTES);
+                const uint32_t tp = tmem + S::probabilities_at(x), to = tmem + S::outputs_at(x);
+                const uint32_t more = t > 0 && !(S::TERMS == 2 && t % PP_FLUSH == 0);
+#pragma unroll
+                for (int k = 0; k < PP_KEYS / 16; k++) {   // 16 keys: 2048 bytes of a panel of V, eight columns of probabilities
+                    pat_mma_ta(to, tp + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), more | (k != 0));
+                    if constexpr (S::TERMS == 2) pat_mma_ta(to, tp + 64u + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), 1u);
+                }
+                pg_commit(&pv_done[x]);
+                if (x == last) pg_commit(&empty[slot]);
+            };
             for (int x = 0; x < 2 && ok; x++) {
                 if ((x ? n_b : n_a) == 0) continue;
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&q_full[x], 0u));
-                pg_fence_after();
+                ok = mbar_wait_bounded(&q_full[x], 0u);
                 if (ok) scores(x, 0);
             }
+            for (int t = 0; t < n_tiles && ok; t++) {
+                const int slot = (2 * t + 1) % S::SLOTS;
+                for (int x = 0; x < 2 && ok; x++) {
+                    const int mine = x ? n_b : n_a;
+                    // in columns of their own the scores go first; in the probabilities' they have to wait for these to be read
+                    if (S::SHARED && t + 1 < mine) scores(x, t + 1);
+                    if (ok && t < mine) {
+                        if (x == 0 || n_a <= t) ok = mbar_wait_bounded(&cleared[t & 7], (uint32_t)(t >> 3) & 1u) && arrived(2 * t + 1);
+                        if (ok) outputs(x, t, mine, slot);
+                    }
+                    if (!S::SHARED && ok && t + 1 < mine) scores(x, t + 1);
+                }
+            }
         }
+        __syncwarp();
+    } else if (warp == PP_SOFTMAX_WARPS + 2) {
+        // ---- values that nobody sees become zeros: whatever they were, zero times it has to be zero.  (Every tile passes here: its product
+        // waits for this warp, so that it never falls behind the ring, and the ring keeps it less than eight tiles ahead) ----
         for (int t = 0; t < n_tiles && ok; t++) {
-            const int slot = (2 * t + 1) % S::SLOTS, k0 = seen.start(t0 + t);
-            const uint32_t vt = ring + (uint32_t)slot * S::TILE_BYTES;
-            ok = arrived(2 * t + 1);
+            const int k0 = seen.start(t0 + t), slot = (2 * t + 1) % S::SLOTS;
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[slot], (uint32_t)((2 * t + 1) / S::SLOTS) & 1u));
             if (!ok) break;
-            if (k0 + PP_KEYS > seen.len || (k0 < seen.from && k0 + PP_KEYS > seen.sink)) {
-                // values that nobody sees become zeros: whatever they were, zero times it has to be zero
-                auto clear = [&](int lo, int hi) {
-                    for (int e = max(lo, 0) * 8 + lane; e < min(hi, PP_KEYS) * 8; e += 32)
+            auto clear = [&](int lo, int hi) {
+                for (int e = max(lo, 0) * 8 + lane; e < min(hi, PP_KEYS) * 8; e += 32)
 #pragma unroll
-                        for (int p = 0; p < S::PANELS; p++)
-                            *reinterpret_cast<uint4 *>(pp_smem + S::Q_BYTES + (uint32_t)slot * S::TILE_BYTES + (uint32_t)p * PP_PANEL + (uint32_t)e * 16u) = make_uint4(0, 0, 0, 0);
-                };
+                    for (int p = 0; p < S::PANELS; p++)
+                        *reinterpret_cast<uint4 *>(pp_smem + S::Q_BYTES + (uint32_t)slot * S::TILE_BYTES + (uint32_t)p * PP_PANEL + (uint32_t)e * 16u) = make_uint4(0, 0, 0, 0);
+            };
+            if (seen.ragged(k0)) {
                 clear(seen.len - k0, PP_KEYS);
                 clear(seen.sink - k0, seen.from - k0);
                 pg_proxy_fence();
-                __syncwarp();
             }
-            for (int x = 0; x < 2 && ok; x++) {
-                const int mine = x ? n_b : n_a;
-                if (t >= mine) continue;
-                const uint64_t dv = pp_v_desc(vt);
-                const uint32_t tp = tmem + (uint32_t)x * 128u, to = tmem + 256u + (uint32_t)x * 128u;
-                const uint32_t more = t > 0 && !(S::TERMS == 2 && t % PP_FLUSH == 0);
-#pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&p_full[2 * x + half], (uint32_t)(t & 1)));
-                    if (!ok) break;
-                    pg_fence_after();
-                    if (pg_elect()) {
-#pragma unroll
-                        for (int k = 4 * half; k < 4 * half + 4; k++) {   // 16 keys: 2048 bytes of a panel of V, eight columns of probabilities
-                            pat_mma_ta(to, tp + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), more | (k != 0));
-                            if constexpr (S::TERMS == 2) pat_mma_ta(to, tp + 64u + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), 1u);
-                        }
-                        if (half == 1) {
-                            if (t == mine - 1) pg_commit(&o_full[x]);
-                            if (x == last) pg_commit(&empty[slot]);
-                        }
-                    }
-                    __syncwarp();
-                }
-                if (ok && t + 1 < mine) {
-                    ok = arrived(2 * t + 2);
-                    if (ok) scores(x, t + 1);
-                }
-            }
+            __syncwarp();
+            if (lane == 0) pg_arrive(&cleared[t & 7]);
         }
-    } else if (warp == 9) {
+    } else if (warp == PP_SOFTMAX_WARPS + 1) {
         // ---- copies: lane i has box i / PANELS of a tile, 64 dims of it ----
         const int box = min(1 << c.page_shift, PP_KEYS), blk = lane / S::PANELS * box, part = lane % S::PANELS;
         const uint32_t dst = smem_u32(pp_smem) + S::Q_BYTES + (uint32_t)part * PP_PANEL + (uint32_t)blk * 128u;
@@ -666,7 +680,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
         pg_drain(full, it, S::SLOTS);
     }
     __syncwarp();
-    if (warp >= 8 && ranks > 1) {
+    if (warp >= PP_SOFTMAX_WARPS && ranks > 1) {
         ps_cluster_sync();
         ps_cluster_sync();
     }
@@ -674,7 +688,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     __syncwarp();
     pg_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == PP_SOFTMAX_WARPS) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
         if (lane == 0 && *failed) atomicExch(P.err, DEV_ERR_MBAR_TIMEOUT);
     }
