@@ -2,10 +2,10 @@
 //
 // A CTA owns two blocks of 128 (query, head) rows of one key head - a block is 128 / group consecutive queries of a sequence times the group's
 // heads - and walks the keys that some of its queries sees in tiles of 128.  Both blocks use a tile while it is in shared memory.  A
-// row is a tensor-memory lane and has two threads, of two warps, which take half of a tile's keys each and tell each other their maxima.  Warp 16 issues the products:
+// row is a tensor-memory lane and has two threads, of two warps, which take half of a tile's keys each and tell each other their maxima.  One thread issues the products:
 // scores from queries and keys in shared memory, then probabilities from tensor memory, where they take the scores' place, times
 // values.  It takes the blocks in turn, P V of block a, the next scores of a, P V of b, the next scores of b, so that one block's softmax runs under the
-// other's products.  Warp 17 copies K0 V0 K1 V1 ... into a ring, a box per page and 64 dims, its lanes
+// other's products.  One warp copies K0 V0 K1 V1 ... into a ring, a box per page and 64 dims, its lanes
 // following the table.
 //
 // f32 queries enter as f16 "hi" + remainder "lo" (scaled by a power of two per row into f16's range), and so do the probabilities: every product is made
@@ -23,9 +23,10 @@
 namespace rnb {
 
 constexpr int PP_KEYS = 128;
-constexpr int PP_SOFTMAX_WARPS = 16, PP_THREADS = 640;   // warp 19 is there for the register split alone: setmaxnreg goes by four warps
+constexpr int PP_WAYS = 2;   // threads of a row
+constexpr int PP_SOFTMAX_WARPS = 8 * PP_WAYS, PP_THREADS = PP_SOFTMAX_WARPS * 32 + 128;   // the last warp is there for the register split alone: setmaxnreg goes by four warps
 constexpr int PP_SOFTMAX_REGS = 104, PP_OTHER_REGS = 64;
-static_assert(512 * PP_SOFTMAX_REGS + 128 * PP_OTHER_REGS <= 640 * 96, "what the block is launched with");
+static_assert(PP_SOFTMAX_WARPS * 32 * PP_SOFTMAX_REGS + 128 * PP_OTHER_REGS <= PP_THREADS * 96, "what the block is launched with");
 constexpr float PP_BIAS = 8.f, PP_GROWTH = 7.f;   // log2; together below f16's 2^16
 constexpr int PP_FLUSH = 16;
 constexpr int PP_MAX_CLUSTER = 8;
@@ -37,6 +38,7 @@ struct PpShape {
     static constexpr uint32_t Q_BYTES = 2 * TERMS * PANELS * PP_PANEL, TILE_BYTES = PANELS * PP_PANEL;
     // tensor memory: where it has room, probabilities have columns of their own and the scores' columns serve both blocks in turn
     static constexpr bool SHARED = 2 * D + 2 * TERMS * 64 + 128 <= 512;
+    static constexpr int PARTS = SHARED ? 1 : 2;   // of a tile's probabilities, that are multiplied one after the other: where scores wait for the last of them
     static constexpr uint32_t scores_at(int x) { return SHARED ? 2 * D : (uint32_t)x * 128u; }
     static constexpr uint32_t probabilities_at(int x) { return SHARED ? 2 * D + 128 + (uint32_t)(x * TERMS * 64) : (uint32_t)x * 128u; }
     static constexpr uint32_t outputs_at(int x) { return (SHARED ? 0u : 256u) + (uint32_t)(x * D); }
@@ -74,6 +76,12 @@ __device__ __forceinline__ float4 pp_ld_remote4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
+}
+__device__ __forceinline__ void pp_tmem_st(uint32_t taddr, const uint32_t (&v)[32]) { pat_tmem_st32(taddr, v); }
+__device__ __forceinline__ void pp_tmem_st(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
 }
 template <int N>
 __device__ __forceinline__ void pp_registers(bool more) {
@@ -126,11 +134,11 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint64_t *const bars = reinterpret_cast<uint64_t *>(pp_smem + S::SMEM - S::TAIL);
-    uint64_t *const full = bars, *const empty = bars + 8, *const q_full = bars + 16, *const s_full = bars + 18, *const p_full = bars + 20, *const pv_done = bars + 22, *const s_free = bars + 24, *const cleared = bars + 40;   // two each of the first four
-    volatile uint32_t *const tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + 26);
-    volatile int *const failed = reinterpret_cast<volatile int *>(bars + 27);
-    volatile int *const found = reinterpret_cast<volatile int *>(bars + 28);   // sequence, first query, queries of the sequence, first row of its tokens, its positions
-    unsigned *const todo = reinterpret_cast<unsigned *>(bars + 32);   // rows of each warp to be done again
+    uint64_t *const full = bars, *const empty = bars + 8, *const q_full = bars + 16, *const s_full = bars + 18, *const p_full = bars + 20, *const pv_done = bars + 24, *const s_free = bars + 26, *const cleared = bars + 44;   // two each of the first four, p_full 2 x 2
+    volatile uint32_t *const tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + 27);
+    volatile int *const failed = reinterpret_cast<volatile int *>(bars + 28);
+    volatile int *const found = reinterpret_cast<volatile int *>(bars + 29);   // sequence, first query, queries of the sequence, first row of its tokens, its positions
+    unsigned *const todo = reinterpret_cast<unsigned *>(bars + 33);   // rows of each warp to be done again
     float *const told = reinterpret_cast<float *>(pp_smem + S::SMEM - S::TAIL + 512);   // [block][half][row]
     uint32_t rank, ranks;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -141,12 +149,13 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             mbar_init(&empty[s], 1);
         }
         for (int x = 0; x < 2; x++) {
-            mbar_init(&q_full[x], S::TERMS == 2 ? 8 : 1);
+            mbar_init(&q_full[x], S::TERMS == 2 ? 4 * PP_WAYS : 1);
             mbar_init(&s_full[x], 1);
-            mbar_init(&p_full[x], 8);
+            mbar_init(&p_full[2 * x], 4 * PP_WAYS);
+            mbar_init(&p_full[2 * x + 1], 4 * PP_WAYS);
             mbar_init(&pv_done[x], 1);
         }
-        mbar_init(s_free, 8);
+        mbar_init(s_free, 4 * PP_WAYS);
         for (int i = 0; i < 8; i++) mbar_init(&cleared[i], 1);
         mbar_fence_init();
         *failed = (smem_u32(pp_smem) & 1023u) != 0;
@@ -225,14 +234,17 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     if (warp < PP_SOFTMAX_WARPS) pp_registers<PP_SOFTMAX_REGS>(true);
     else pp_registers<PP_OTHER_REGS>(false);
     if (warp < PP_SOFTMAX_WARPS) {
-        // a row has two threads: lane `lane` of the warps (x, half, w) with half 0 and 1, which take 64 of a tile's keys and half of the output each
-        const int x = warp >> 3, half = (warp >> 2) & 1, w = warp & 3, mine = x ? n_b : n_a, live = x ? live_b : live_a, q0 = first + x * P.queries;
-        auto both = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + x * 4 + w) : "memory"); };   // a row's two warps
+        // a row's threads: lane `lane` of the warps (x, half, w), which take KEYS of a tile's keys and COLS of the output's dims each
+        constexpr int KEYS = PP_KEYS / PP_WAYS, DIMS = D / PP_WAYS;
+        const int x = warp / (4 * PP_WAYS), half = (warp >> 2) % PP_WAYS, w = warp & 3, mine = x ? n_b : n_a, live = x ? live_b : live_a, q0 = first + x * P.queries;
+        auto both = [&]() {   // a row's warps meet
+            if constexpr (PP_WAYS > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + x * 4 + w), "n"(32 * PP_WAYS) : "memory");
+        };
         uint8_t *const q_smem = pp_smem + (uint32_t)(x * S::TERMS * S::PANELS) * PP_PANEL;   // this block's
         if constexpr (S::TERMS == 2) {
-            // ---- f32 queries in two terms: a warp takes 16 rows, all under way ----
-            constexpr int LANES = D / 4, ROWS = 32 / LANES, LOADS = 16 / ROWS;   // lanes of a row, rows of a load
-            const int d0 = lane % LANES * 4, row0 = (half * 4 + w) * 16;
+            // ---- f32 queries in two terms: a warp takes its share of the rows, all under way ----
+            constexpr int LANES = D / 4, ROWS = 32 / LANES, LOADS = 32 / PP_WAYS / ROWS;   // lanes of a row, rows of a load
+            const int d0 = lane % LANES * 4, row0 = (half * 4 + w) * (32 / PP_WAYS);
             const float *const q = reinterpret_cast<const float *>(P.q) + (size_t)(token0 + q0) * P.q_stride + (size_t)(head * P.group + head0) * D + d0;
             if (mine > 0) {
                 float4 raw[LOADS];
@@ -275,7 +287,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
         const bool alive = ql < live && r - ql * P.per_block < heads_here;
         const int pos = shift + q0 + min(ql, max(live - 1, 0));                       // dead rows see what the last one sees, and are not stored
         const int pos0 = shift + q0, pos1 = shift + q0 + live - 1;                    // the block's positions
-        const uint32_t lanes = (uint32_t)(w * 32) << 16, t_s = tmem + S::scores_at(x) + lanes, t_p = tmem + S::probabilities_at(x) + lanes, t_o = tmem + S::outputs_at(x) + (uint32_t)(half * (D / 2)) + lanes;
+        const uint32_t lanes = (uint32_t)(w * 32) << 16, t_s = tmem + S::scores_at(x) + lanes, t_p = tmem + S::probabilities_at(x) + lanes, t_o = tmem + S::outputs_at(x) + (uint32_t)(half * DIMS) + lanes;
         const float turned = P.scale > 0.f ? 1.f : P.scale == 0.f ? 0.f : -1.f;   // maxima are of unscaled scores: they need a positive scale
         float sl2 = (P.scale == 0.f ? 1.f : fabsf(P.scale)) * 1.4426950408889634f;   // to log2 units
         float *const say = told + (x * 2 + half) * 128 + r, *const hear = told + (x * 2 + (half ^ 1)) * 128 + r;
@@ -283,8 +295,8 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
         const int q_head = head * P.group + head0 + r - ql * P.per_block;
         Q *const out0 = reinterpret_cast<Q *>(P.out) + (size_t)(token0 + q0) * P.out_stride + (size_t)(head * P.group + head0) * D;   // the block's first row
         float m_ref = -INFINITY, l_run = 0.f, m_sums = 0.f;
-        float *const sums = sizeof(Q) != 4 ? nullptr : ranks > 1 ? P.sums + ((size_t)blockIdx.x * 256 + x * 128 + r) * D + half * (D / 2)
-                                                          : reinterpret_cast<float *>(out0 + (size_t)ql * P.out_stride + (size_t)(r - ql * P.per_block) * D + half * (D / 2));
+        float *const sums = sizeof(Q) != 4 ? nullptr : ranks > 1 ? P.sums + ((size_t)blockIdx.x * 256 + x * 128 + r) * D + half * DIMS
+                                                          : reinterpret_cast<float *>(out0 + (size_t)ql * P.out_stride + (size_t)(r - ql * P.per_block) * D + half * DIMS);
         bool summed = false;
         for (int t = 0; t < mine; t++) {
             ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (uint32_t)(t & 1)));
@@ -293,8 +305,9 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 continue;
             }
             pg_fence_after();
-            uint32_t s[64];
-            pat_tmem_ld64(t_s + (uint32_t)half * 64u, s);
+            static_assert(KEYS == 64, "columns per load");
+            uint32_t s[KEYS];
+            pat_tmem_ld64(t_s + (uint32_t)(half * KEYS), s);
             if constexpr (S::SHARED) {   // the other block's turn
                 pg_fence_before();
                 __syncwarp();
@@ -303,15 +316,15 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             if (S::TERMS == 2 && t == 0) sl2 *= *say;   // the row's factor, from before the scores' product
             if (turned != 1.f) {
 #pragma unroll
-                for (int i = 0; i < 64; i++) s[i] = __float_as_uint(__uint_as_float(s[i]) * turned);
+                for (int i = 0; i < KEYS; i++) s[i] = __float_as_uint(__uint_as_float(s[i]) * turned);
             }
-            const int k0 = seen.start(t0 + t) + half * 64;
-            if (!(k0 + 63 <= pos0 && (P.window == 0 || k0 > pos1 - P.window || k0 + 64 <= P.sinks))) {
-                // keys a .. z of the half, and those before the end of the sinks
+            const int k0 = seen.start(t0 + t) + half * KEYS;
+            if (!(k0 + KEYS - 1 <= pos0 && (P.window == 0 || k0 > pos1 - P.window || k0 + KEYS <= P.sinks))) {
+                // keys a .. z of these, and those before the end of the sinks
                 const int z = pos - k0, a = P.window ? pos - P.window + 1 - k0 : 0, k = P.sinks - k0;
                 auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };   // bits 0 .. n - 1
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
+                for (int j = 0; j < KEYS / 32; j++) {
                     const uint32_t keep = below(z + 1 - 32 * j) & (~below(a - 32 * j) | below(k - 32 * j));
 #pragma unroll
                     for (int i = 0; i < 32; i++)
@@ -322,13 +335,16 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
 #pragma unroll
             for (int j = 0; j < 4; j++) mxs[j] = __uint_as_float(s[j]);
 #pragma unroll
-            for (int i = 4; i < 64; i++) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(s[i]));
-            // the other half's maximum; once both have their scores, probabilities may take the scores' place
-            *say = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
-            pg_fence_before();
-            both();
-            pg_fence_after();
-            const float mx = fmaxf(*say, *hear) * sl2;
+            for (int i = 4; i < KEYS; i++) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(s[i]));
+            float top = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
+            if constexpr (PP_WAYS > 1) {   // the other half's; once both have their scores, probabilities may take the scores' place
+                *say = top;
+                pg_fence_before();
+                both();
+                pg_fence_after();
+                top = fmaxf(top, *hear);
+            }
+            const float mx = top * sl2;
             float corr = 1.f;
             if (mx > m_ref + PP_GROWTH || m_ref == -INFINITY) {
                 const float m_new = fmaxf(mx, m_ref);
@@ -349,7 +365,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 // the tiles' sum so far joins the f32 sums; the next product starts from zero
                 const float old = summed ? exp2f(m_sums - m_use) : 0.f;
 #pragma unroll 1
-                for (int k = 0; k < D / 64; k++) {
+                for (int k = 0; k < DIMS / 32; k++) {
                     uint32_t v[32];
                     pg_tmem_ld32(t_o + (uint32_t)k * 32u, v);
                     if (alive) {
@@ -367,7 +383,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             } else if (t > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
                 through();
 #pragma unroll 1
-                for (int k = 0; k < D / 64; k++) {
+                for (int k = 0; k < DIMS / 32; k++) {
                     uint32_t v[32];
                     pg_tmem_ld32(t_o + (uint32_t)k * 32u, v);
 #pragma unroll
@@ -378,33 +394,39 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             __syncwarp();
             const uint64_t sl22 = pg_pair_f32(sl2, sl2), nm2 = pg_pair_f32(PP_BIAS - m_use, PP_BIAS - m_use);
             uint64_t sum[2] = {0, 0};
-            uint32_t hi[32], lo[32];   // 64 keys: 32 columns of a term
 #pragma unroll
-            for (int i = 0; i < 32; i++) {
-                const float2 y = pat_fma2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), sl22, nm2);
-                const float p0 = pat_exp2(y.x), p1 = pat_exp2(y.y);
-                pat_add2(sum[i & 1], p0, p1);
-                if constexpr (S::TERMS == 2) pp_cut<C>(p0, p1, hi[i], lo[i]);
-                else hi[i] = pk_pack<C>(p0, p1);
-            }
-            through();
-            if (ok) {
-                pat_tmem_st32(t_p + (uint32_t)half * 32u, hi);
-                if constexpr (S::TERMS == 2) pat_tmem_st32(t_p + 64u + (uint32_t)half * 32u, lo);
+            for (int part = 0; part < S::PARTS; part++) {
+                constexpr int PAIRS = KEYS / 2 / S::PARTS;   // columns of a term
+                uint32_t hi[PAIRS], lo[PAIRS];
+#pragma unroll
+                for (int i = 0; i < PAIRS; i++) {
+                    const float2 y = pat_fma2(__uint_as_float(s[2 * (part * PAIRS + i)]), __uint_as_float(s[2 * (part * PAIRS + i) + 1]), sl22, nm2);
+                    const float p0 = pat_exp2(y.x), p1 = pat_exp2(y.y);
+                    pat_add2(sum[i & 1], p0, p1);
+                    if constexpr (S::TERMS == 2) pp_cut<C>(p0, p1, hi[i], lo[i]);
+                    else hi[i] = pk_pack<C>(p0, p1);
+                }
+                if (part == 0) through();
+                if (!ok) continue;
+                const uint32_t to = t_p + (uint32_t)(half * (KEYS / 2) + part * PAIRS);
+                pp_tmem_st(to, hi);
+                if constexpr (S::TERMS == 2) pp_tmem_st(to + 64u, lo);
                 pat_tmem_st_wait();
                 pg_fence_before();
                 __syncwarp();
-                if (lane == 0) pg_arrive(&p_full[x]);
+                if (lane == 0) pg_arrive(&p_full[2 * x + part]);
             }
             l_run = fmaf(l_run, corr, pat_total(sum[0], sum[1]));
         }
         if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[x], (uint32_t)((mine - 1) & 1)));
         pg_fence_after();
         // ---- the row's end ----
-        both();
-        *say = l_run;
-        both();
-        l_run += *hear;
+        if constexpr (PP_WAYS > 1) {
+            both();
+            *say = l_run;
+            both();
+            l_run += *hear;
+        }
         const float m_use = m_ref == -INFINITY ? 0.f : m_ref, old = summed ? exp2f(m_sums - m_use) : 0.f;
         auto output = [&](int k, float (&o)[32]) {   // unscaled, dims 32 k .. of this thread's half
             if (mine > 0 && ok) {
@@ -429,15 +451,15 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             else *reinterpret_cast<uint2 *>(to) = make_uint2(pk_pack<Q>(a, b2), pk_pack<Q>(c2, d));
         };
         if (ranks == 1) {
-            // BYTES of every row's half at a time through shared memory, where the queries were, so that a few lanes store a row's
-            constexpr int BYTES = D / 2 * (int)sizeof(Q) < 128 ? D / 2 * (int)sizeof(Q) : 128, COLS = BYTES / (int)sizeof(Q), LANES = BYTES / 16;
-            uint8_t *const box = q_smem + (half * 4 + w) * (S::TERMS * S::PANELS * PP_PANEL / 8);
-            static_assert(32 * BYTES <= S::TERMS * S::PANELS * PP_PANEL / 8, "a box per warp");
+            // BYTES of every row (of its half) at a time through shared memory, where the queries were, so that a few lanes store a row's
+            constexpr int BYTES = DIMS * (int)sizeof(Q) < 128 ? DIMS * (int)sizeof(Q) : 128, COLS = BYTES / (int)sizeof(Q), LANES = BYTES / 16;
+            uint8_t *const box = q_smem + (half * 4 + w) * (S::TERMS * S::PANELS * PP_PANEL / (4 * PP_WAYS));
+            static_assert(32 * BYTES <= S::TERMS * S::PANELS * PP_PANEL / (4 * PP_WAYS), "a box per warp");
             const float inv = l_run > 0.f ? 1.f / l_run : l_run != l_run ? l_run : 0.f;
             const uint64_t inv2 = pg_pair_f32(inv, inv);
             uint64_t check = 0;   // stays zero while all are finite
 #pragma unroll 1
-            for (int k = 0; k < D / 2 / COLS; k++) {
+            for (int k = 0; k < DIMS / COLS; k++) {
                 __syncwarp();   // a row's sums are read by now, and what was stored out of the box
 #pragma unroll
                 for (int j = 0; j < COLS / 32; j++) {
@@ -467,24 +489,25 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                     const int rr = (32 / LANES) * i + lane / LANES, ch = lane % LANES, R = w * 32 + rr, rq = query_of(R), h = R - rq * P.per_block;
                     const uint4 y = *reinterpret_cast<const uint4 *>(box + rr * BYTES + ((ch ^ (rr & (LANES - 1))) << 4));
                     if (rq < live && h < heads_here && ok)
-                        *reinterpret_cast<uint4 *>(out0 + (size_t)rq * P.out_stride + (size_t)h * D + half * (D / 2) + k * COLS + ch * (16 / (int)sizeof(Q))) = y;
+                        *reinterpret_cast<uint4 *>(out0 + (size_t)rq * P.out_stride + (size_t)h * D + half * DIMS + k * COLS + ch * (16 / (int)sizeof(Q))) = y;
                 }
             }
             const bool strange = alive && ok && !((uint32_t)check << 1 == 0 && (uint32_t)(check >> 32) << 1 == 0);
             if (alive && ok && half == 0 && P.lse) P.lse[row * P.heads + q_head] = l_run > 0.f ? (m_use - PP_BIAS + log2f(l_run)) * 0.6931471805599453f : l_run != l_run ? l_run : -INFINITY;
             if (strange) atomicOr(&todo[x * 4 + w], 1u << lane);
+            __syncwarp();
             both();
         } else {
             // ---- a cluster's shares: outputs, maxima and sums in shared memory, where the tiles were ----
             if (!ok) *failed = 1;
-            asm volatile("bar.sync 9, 512;" ::: "memory");   // both blocks' products are through (each block's warps have waited for its own)
+            asm volatile("bar.sync 9, %0;" ::"n"(32 * PP_SOFTMAX_WARPS) : "memory");   // both blocks' products are through (each block's warps have waited for its own)
             float *const o_all = reinterpret_cast<float *>(pp_smem), *const ml = o_all + 256 * (D + 4);
 #pragma unroll 1
-            for (int k = 0; k < D / 64; k++) {
+            for (int k = 0; k < DIMS / 32; k++) {
                 float o[32];
                 output(k, o);
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(o_all + (x * 128 + r) * (D + 4) + half * (D / 2) + k * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(o_all + (x * 128 + r) * (D + 4) + half * DIMS + k * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             }
             if (half == 0) *reinterpret_cast<float2 *>(ml + 2 * (x * 128 + r)) = make_float2(m_ref, ok ? l_run : 0.f);
             __syncwarp();
@@ -514,7 +537,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 }
                 *reinterpret_cast<float2 *>(joined + 2 * tid) = make_float2(M == -INFINITY ? 0.f : M, L);
             }
-            asm volatile("bar.sync 9, 512;" ::: "memory");
+            asm volatile("bar.sync 9, %0;" ::"n"(32 * PP_SOFTMAX_WARPS) : "memory");
             const bool good = *failed == 0;
             for (int e = warp; e < n; e += PP_SOFTMAX_WARPS) {   // a warp per row
                 const int R = (int)rank * n + e, bx = R >> 7, rr = R & 127, rq = query_of(rr);
@@ -578,16 +601,21 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 if (x == last) pg_commit(&empty[slot]);
             };
             auto outputs = [&](int x, int t, int mine, int slot) {
-                ok = mbar_wait_bounded(&p_full[x], (uint32_t)(t & 1));
-                if (!ok) return;
-                pg_fence_after();
                 const uint64_t dv = pp_v_desc(ring + (uint32_t)slot * S::TILE_BYTES);
                 const uint32_t tp = tmem + S::probabilities_at(x), to = tmem + S::outputs_at(x);
                 const uint32_t more = t > 0 && !(S::TERMS == 2 && t % PP_FLUSH == 0);
 #pragma unroll
-                for (int k = 0; k < PP_KEYS / 16; k++) {   // 16 keys: 2048 bytes of a panel of V, eight columns of probabilities
-                    pat_mma_ta(to, tp + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), more | (k != 0));
-                    if constexpr (S::TERMS == 2) pat_mma_ta(to, tp + 64u + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), 1u);
+                for (int part = 0; part < S::PARTS; part++) {
+                    ok = mbar_wait_bounded(&p_full[2 * x + part], (uint32_t)(t & 1));
+                    if (!ok) return;
+                    pg_fence_after();
+#pragma unroll
+                    for (int i = 0; i < 8 / S::PARTS; i++) {   // 16 keys: 2048 bytes of a panel of V, eight columns of probabilities
+                        constexpr int RUN = 8 / S::PARTS / PP_WAYS;   // of one half's part
+                        const int k = i / RUN * (8 / PP_WAYS) + part * RUN + i % RUN;
+                        pat_mma_ta(to, tp + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), more | (uint32_t)((part | i) != 0));
+                        if constexpr (S::TERMS == 2) pat_mma_ta(to, tp + 64u + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), 1u);
+                    }
                 }
                 pg_commit(&pv_done[x]);
                 if (x == last) pg_commit(&empty[slot]);
