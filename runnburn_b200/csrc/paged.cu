@@ -238,6 +238,10 @@ static int pk_decode_launch(const PkAttention &a, cudaStream_t s, State &st) {
     P.lse = a.lse;
     P.workspace = (uint8_t *)a.workspace;
     P.err = st.dev_error;
+    // tiles are counted in 31 bits: of a sequence at most what its table holds, or its window and sinks with the tiles that they begin in
+    const uint64_t held = (((uint64_t)a.b.max_pages << a.c.page_shift) + PD_TILE - 1) / PD_TILE, seen = ((uint64_t)a.window + a.sinks) / PD_TILE + 4;
+    if ((uint64_t)a.b.n_seq * (a.window ? std::min(held, seen) : held) * P.splits * a.c.kv_heads > 0x7fffffffu)
+        return fail(RNB_B200_UNSUPPORTED, "paged attention: %d sequences with tables of %d pages are more than a launch can have", a.b.n_seq, a.b.max_pages);
     const int grid = std::min(std::min(st.sm_count, 148) * S::PER_SM, PD_MAX_GRID);
     static_assert(148 * S::PER_SM * 2 * S::RECORD <= PK_WORKSPACE_BYTES - PD_WS_RECORDS, "records");
     PkMaps maps;

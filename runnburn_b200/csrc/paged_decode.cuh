@@ -66,6 +66,12 @@ __device__ __forceinline__ void pk_tma_5d(uint32_t dst, const PkTensorMap *map, 
                  ::"r"(dst), "l"(map), "r"(0), "r"(pos), "r"(part), "r"(head), "r"(page), "r"(smem_u32(bar))
                  : "memory");
 }
+// One more arrival at a counter: what the CTA wrote before the barrier ahead of this is visible to whoever reads the count afterwards.
+__device__ __forceinline__ unsigned pk_arrive_gpu(unsigned *count) {
+    unsigned before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+    return before;
+}
 // the workers of a CTA, without its copying warp
 template <int N>
 __device__ __forceinline__ void pk_sync_some() {
@@ -117,59 +123,62 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
     const int VH = c.kv_heads * P.splits;
 
     // ---- this CTA's run: units [begin, end) of VH * (tiles of all sequences) ----
+    volatile int *const found = reinterpret_cast<volatile int *>(pd_smem);
     if (warp == 0) {
-        long long sum = 0;
-        for (int r = lane; r < b.n_seq; r += 32) sum += pd_seen(pk_length(b, c.page_shift, r, P.err), P.window, P.sinks).tiles;
+        const unsigned mark = lane == 0 ? ld_l2(reinterpret_cast<const uint32_t *>(P.workspace)) : 0;
+        auto tiles_of = [&](int r) { return r < b.n_seq ? pd_seen(pk_length(b, c.page_shift, r, P.err), P.window, P.sinks).tiles : 0; };
+        const int first32 = tiles_of(lane);
+        int sum = first32, most = first32;
+        for (int r = lane + 32; r < b.n_seq; r += 32) {
+            const int n = tiles_of(r);
+            sum += n;
+            most = max(most, n);
+        }
+        const unsigned units = (unsigned)__reduce_add_sync(0xffffffffu, sum) * VH;   // (the host has seen to it that this fits)
+        // short sequences are not cut, nor put behind one another while there are CTAs for each
+        const unsigned per = max((units + gridDim.x - 1) / gridDim.x, (unsigned)min(PD_MIN_TILES, __reduce_max_sync(0xffffffffu, most))), begin = per * blockIdx.x;
+        if (begin < units) {   // the sequence that unit `begin` lies in
+            unsigned before = 0;
+            for (int r0 = 0;; r0 += 32) {
+                const unsigned n = r0 == 0 ? first32 : tiles_of(r0 + lane);
+                unsigned up = n;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const long long units = sum * VH, per = max((units + gridDim.x - 1) / gridDim.x, (long long)PD_MIN_TILES), begin = per * blockIdx.x;
-        // the sequence that unit `begin` lies in
-        long long before = 0;
-        int row = 0;
-        for (int r0 = 0; r0 < b.n_seq && begin < units; r0 += 32) {
-            const int n = r0 + lane < b.n_seq ? pd_seen(pk_length(b, c.page_shift, r0 + lane, P.err), P.window, P.sinks).tiles : 0;
-            long long up = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, up, o);
-                if (lane >= o) up += x;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned x = __shfl_up_sync(0xffffffffu, up, o);
+                    if (lane >= o) up += x;
+                }
+                const unsigned behind = __ballot_sync(0xffffffffu, (before + up) * VH > begin);
+                if (behind) {
+                    const int l = __ffs(behind) - 1;
+                    if (lane == l) {
+                        const unsigned rest = begin - (before + up - n) * VH;
+                        found[2] = r0 + l;
+                        found[3] = (int)(rest / n);
+                        found[4] = (int)(rest % n);
+                    }
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, up, 31);
             }
-            const unsigned behind = __ballot_sync(0xffffffffu, (before + up) * VH > begin);
-            if (behind) {
-                const int l = __ffs(behind) - 1;
-                row = r0 + l;
-                before += __shfl_sync(0xffffffffu, up - n, l);
-                break;
-            }
-            before += __shfl_sync(0xffffffffu, up, 31);
         }
         if (lane == 0) {
-            const bool ready = *reinterpret_cast<volatile unsigned *>(P.workspace) == PD_WS_MARK;
-            if (!ready) atomicExch(P.err, DEV_ERR_BAD_WORKSPACE);
-            long long *const w = reinterpret_cast<long long *>(pd_smem);
-            w[0] = ready && begin < units ? min(per, units - begin) : 0;
-            w[1] = begin;
-            w[2] = begin - before * VH;   // unit within the sequence
-            w[3] = per;
-            w[4] = row;
+            if (mark != PD_WS_MARK) atomicExch(P.err, DEV_ERR_BAD_WORKSPACE);
+            found[0] = mark == PD_WS_MARK && begin < units ? (int)min(per, units - begin) : 0;
+            found[1] = (int)per;
         }
     }
     __syncthreads();
-    const long long *const found = reinterpret_cast<const long long *>(pd_smem);
-    const long long n_units = found[0], begin = found[1], per = found[3];
+    const int n_units = found[0], per = found[1], begin = per * (int)blockIdx.x;
     struct Walk {
         int row, vh, i;
         PdSeen s;
     } at;
-    at.row = (int)found[4];
-    at.s = pd_seen(0, 0, 0);
-    if (n_units > 0) {
-        at.s = pd_seen(pk_length(b, c.page_shift, at.row, P.err), P.window, P.sinks);
-        at.vh = (int)(found[2] / at.s.tiles);
-        at.i = (int)(found[2] % at.s.tiles);
-    }
+    at.row = found[2];
+    at.vh = found[3];
+    at.i = found[4];
     __syncthreads();
     if (n_units == 0) return;
+    at.s = pd_seen(pk_length(b, c.page_shift, at.row, P.err), P.window, P.sinks);
     auto advance = [&](Walk &w) {
         if (++w.i < w.s.tiles) return;
         w.i = 0;
@@ -188,8 +197,7 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
         const PkTensorMap *const map = lane & 1 ? &maps.v : &maps.k;
         const uint32_t dst = smem_u32(pd_smem) + (lane & 1) * S::TILE_BYTES + mine * (D * 2);
         bool ok = note[1] == 0;
-        long long u = 0;
-        int stage = 0;
+        int u = 0, stage = 0;
         uint32_t phase = 1;   // of the empty barriers: a fresh one counts as passed
         auto look_up = [&](int &pos, bool &live) {   // the page of this lane's box of tile `at`
             pos = start(at) + mine;
@@ -244,10 +252,9 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
     uint32_t phase = 0;
     bool ok = note[1] == 0;
     bool fresh = true;   // a segment begins
-    long long unit = begin;
-    int first_tile = at.i;
+    int unit = begin, first_tile = at.i;
     int stage = 0;
-    for (long long u = 0; u < n_units; u++, unit++) {
+    for (int u = 0; u < n_units; u++, unit++) {
         const int group0 = (at.vh % P.splits) * (8 * HT) + ht * 8, mine = group0 + head, q_head = (at.vh / P.splits) * P.group + mine;
         if (fresh) {
             fresh = false;
@@ -298,16 +305,17 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
             atomicExch(P.err, DEV_ERR_MBAR_TIMEOUT);
         }
         if (p0 < at.s.len && (p0 + 15 >= at.s.from || p0 < at.s.sink)) {
-            float s0[4] = {}, s1[4] = {};
+            float s0[2][4] = {}, s1[2][4] = {};   // even and odd steps: shorter chains
             const uint32_t kt = k_base + stage * 2 * S::TILE_BYTES, vt = v_base + stage * 2 * S::TILE_BYTES;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 uint32_t r[4];
                 pk_ldmatrix(r, kt + (k >> 2) * part + (((2 * (k & 3) + k_c) ^ k_x) << 4));
-                pk_mma<C>(s0, qa[k], r[0], r[1]);
-                pk_mma<C>(s1, qa[k], r[2], r[3]);
+                pk_mma<C>(s0[k & 1], qa[k], r[0], r[1]);
+                pk_mma<C>(s1[k & 1], qa[k], r[2], r[3]);
             }
-            float t[4] = {s0[0] + s0[2], s0[1] + s0[3], s1[0] + s1[2], s1[1] + s1[3]};
+            float t[4] = {(s0[0][0] + s0[1][0]) + (s0[0][2] + s0[1][2]), (s0[0][1] + s0[1][1]) + (s0[0][3] + s0[1][3]), (s1[0][0] + s1[1][0]) + (s1[0][2] + s1[1][2]),
+                          (s1[0][1] + s1[1][1]) + (s1[0][3] + s1[1][3])};
             float mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -380,8 +388,7 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
             const int heads_here = min(8 * HT, P.group - (at.vh % P.splits) * (8 * HT)), head0 = (at.vh / P.splits) * P.group + (at.vh % P.splits) * (8 * HT);
             const bool whole = ends && first_tile == 0;
             // the CTAs that share the segment, and this one's record: the first of its two where the segment began before it
-            const long long seg = unit - at.i;
-            const int cta0 = (int)(seg / per), parts = (int)((seg + at.s.tiles - 1) / per) - cta0 + 1;
+            const int seg = unit - at.i, cta0 = seg / per, parts = (seg + at.s.tiles - 1) / per - cta0 + 1;
             float *const record = reinterpret_cast<float *>(P.workspace + PD_WS_RECORDS + (size_t)(2 * blockIdx.x + (first_tile == 0 ? 1 : 0)) * S::RECORD);
             auto put = [&](int h, int d, float4 v, float M, float L) {   // four dims of an output
                 const float inv = L > 0.f ? 1.f / L : L != L ? L : 0.f;
@@ -409,34 +416,46 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
                 }
             }
             if (!whole) {
-                __threadfence();
                 pk_sync_some<S::WORKERS>();
                 if (tid == 0) {
                     unsigned *const count = reinterpret_cast<unsigned *>(P.workspace + PD_WS_HEAD) + cta0;
-                    const bool last = atomicAdd(count, 1u) == (unsigned)parts - 1;
+                    const bool last = pk_arrive_gpu(count) == (unsigned)parts - 1;   // all threads' records before it, the others' behind it
                     if (last) *count = 0;   // for the next launch
                     *note = last;
-                    __threadfence();
                 }
                 pk_sync_some<S::WORKERS>();
                 if (*note) {
                     // ---- join: part p is of CTA cta0 + p, its second record for p = 0 and its first one after that ----
                     const float *const base = reinterpret_cast<const float *>(P.workspace + PD_WS_RECORDS);
                     auto part = [&](int p, int h) { return base + ((size_t)2 * (cta0 + p) + (p == 0 ? 1 : 0)) * (S::RECORD / 4) + h * (D + 4); };
+                    // outputs of the first parts are asked for before their weights are known
+                    constexpr int AHEAD = 8;
+                    float4 x[AHEAD];
+                    auto ask = [&](int e, int p0) {
+#pragma unroll
+                        for (int i = 0; i < AHEAD; i++)
+                            if (p0 + i < parts && e < heads_here * (D / 4)) x[i] = ld_l2(reinterpret_cast<const float4 *>(part(p0 + i, e / (D / 4)) + 4 + e % (D / 4) * 4));
+                    };
+                    ask(tid, 0);
                     for (int h = warp; h < heads_here; h += S::WORKERS / 32) {
                         float M_h = -INFINITY, L_h = 0.f;
-                        for (int p = lane; p < parts; p += 32) M_h = fmaxf(M_h, ld_l2(part(p, h)));
-                        M_h = warp_max(M_h);
-                        const float ref_h = M_h == -INFINITY ? 0.f : M_h;
-                        for (int p = lane; p < parts; p += 32) {
-                            const float2 x = ld_l2(reinterpret_cast<const float2 *>(part(p, h)));
-                            const float w = pd_exp2(x.x - ref_h);
-                            merge[p * (8 * HT) + h] = w;
-                            L_h += w * x.y;
+                        for (int p0 = lane; p0 < parts; p0 += 128) {
+                            float2 y[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) y[i] = p0 + 32 * i < parts ? ld_l2(reinterpret_cast<const float2 *>(part(p0 + 32 * i, h))) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                if (p0 + 32 * i < parts) merge[(p0 + 32 * i) * (8 * HT) + h] = y[i].x;
+                                const float top = fmaxf(M_h, y[i].x), ref = top == -INFINITY ? 0.f : top;
+                                L_h = L_h * pd_exp2(M_h - ref) + y[i].y * pd_exp2(y[i].x - ref);
+                                M_h = top;
+                            }
                         }
-                        L_h = warp_sum(L_h);
+                        const float M_all = warp_max(M_h), ref_h = M_all == -INFINITY ? 0.f : M_all;
+                        L_h = warp_sum(L_h * pd_exp2(M_h - ref_h));
+                        for (int p = lane; p < parts; p += 32) merge[p * (8 * HT) + h] = pd_exp2(merge[p * (8 * HT) + h] - ref_h);
                         if (lane == 0) {
-                            ml[h * 10 + 8] = M_h;
+                            ml[h * 10 + 8] = M_all;
                             ml[h * 10 + 9] = L_h;
                         }
                     }
@@ -444,12 +463,10 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
                     for (int e = tid; e < heads_here * (D / 4); e += S::WORKERS) {
                         const int h = e / (D / 4), d = e % (D / 4) * 4;
                         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        for (int p0 = 0; p0 < parts; p0 += 8) {
-                            float4 x[8];
+                        for (int p0 = 0; p0 < parts; p0 += AHEAD) {
+                            if (p0 > 0 || e != tid) ask(e, p0);
 #pragma unroll
-                            for (int i = 0; i < 8; i++) x[i] = p0 + i < parts ? ld_l2(reinterpret_cast<const float4 *>(part(p0 + i, h) + 4 + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                            for (int i = 0; i < 8; i++)
+                            for (int i = 0; i < AHEAD; i++)
                                 if (p0 + i < parts) {
                                     const float w = merge[(p0 + i) * (8 * HT) + h];
                                     v = make_float4(fmaf(w, x[i].x, v.x), fmaf(w, x[i].y, v.y), fmaf(w, x[i].z, v.z), fmaf(w, x[i].w, v.w));

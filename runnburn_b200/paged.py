@@ -40,19 +40,30 @@ def _type(t) -> int:
         raise TypeError(f"expected float32, float16 or bfloat16, got {t.dtype}") from None
 
 
-def _on_device(*tensors):
-    device = tensors[0].device
+def _on_device(index: int, *tensors) -> None:
     for t in tensors:
-        if t.device != device or device.type != "cuda":
-            raise ValueError(f"tensors have to be on one CUDA device, got {t.device} and {device}")
-    return device
+        if t.get_device() != index:
+            raise ValueError(f"tensors have to be on one CUDA device, got {t.device} and cuda:{index}")
 
 
-def _stream(device, stream):
+def _index(t) -> int:
+    if not t.is_cuda:
+        raise ValueError(f"tensors have to be on a CUDA device, got {t.device}")
+    return t.get_device()
+
+
+_raw_stream = None
+
+
+def _stream(index: int, stream):
+    """The stream's handle; None: the current one of PyTorch (asked for by its number alone where that is offered: an object for it takes 2 us)."""
+    global _raw_stream
     if stream is not None:
         return stream
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _raw_stream(index)
 
 
 def _ints(t, what: str, ndim: int):
@@ -70,7 +81,8 @@ class PagedCache:
             raise ValueError("k and v have to be alike, [n_pages, page_size, kv_heads, head_dim] or with a dimension of layers before these")
         if k.shape[-1] > 1 and k.stride(-1) != 1:
             raise ValueError("the elements of a head's row have to be contiguous")
-        self.device = _on_device(k, v)
+        self.index = _index(k)
+        _on_device(self.index, v)
         self.k, self.v = k, v
         self.n_layers, self.layer_stride = (k.shape[0], k.stride(0)) if k.dim() == 5 else (1, 0)
         self.n_pages, self.page_size, self.kv_heads, self.head_dim = k.shape[-4:]
@@ -93,7 +105,8 @@ class PagedBatch:
         n_seq = table.shape[0]
         if kv_len.shape[0] != n_seq:
             raise ValueError(f"table has {n_seq} sequences, kv_len {kv_len.shape[0]}")
-        self.device = _on_device(table, kv_len, *(() if q_start is None else (q_start,)))
+        self.index = _index(table)
+        _on_device(self.index, kv_len, *(() if q_start is None else (q_start,)))
         if q_start is not None:
             if _ints(q_start, "q_start", 1).shape[0] != n_seq + 1:
                 raise ValueError(f"q_start has to have {n_seq + 1} entries, got {q_start.shape[0]}")
@@ -115,8 +128,8 @@ class Workspace:
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         n = load().rnb_b200_paged_workspace_bytes()
         self.buffer = torch.empty(n, dtype=torch.uint8, device=device)
-        self.device, self.ptr, self.bytes = self.buffer.device, self.buffer.data_ptr(), n
-        check(load().rnb_b200_paged_workspace_init(self.ptr, n, _stream(self.device, stream)))
+        self.index, self.ptr, self.bytes = _index(self.buffer), self.buffer.data_ptr(), n
+        check(load().rnb_b200_paged_workspace_init(self.ptr, n, _stream(self.index, stream)))
 
 
 def _rows(t, what: str, tokens: int, heads: int | None, dim: int):
@@ -139,14 +152,16 @@ def _attention(fn, cache, batch, q, scale, out, window, sinks, lse, workspace, s
     out_stride = _rows(out, "out", n, heads, dim)
     if out.dtype != q.dtype:
         raise ValueError(f"out has to have the queries' type {q.dtype}, got {out.dtype}")
-    device = _on_device(q, out, cache, batch, workspace)
+    index = cache.index
+    if batch.index != index or workspace.index != index or q.get_device() != index or out.get_device() != index:
+        raise ValueError(f"cache, batch, workspace, q and out have to be on one CUDA device, got {index}, {batch.index}, {workspace.index}, {q.device} and {out.device}")
     if lse is not None:
-        _on_device(q, lse)
+        _on_device(index, lse)
         if str(lse.dtype) != "torch.float32" or tuple(lse.shape) != (n, heads) or not lse.is_contiguous():
             raise ValueError(f"lse has to be a contiguous float32 tensor [{n}, {heads}]")
         lse = lse.data_ptr()
     check(fn(cache._ref, batch._ref, _type(q), q.data_ptr(), q_stride, heads, scale, window, sinks, workspace.ptr, workspace.bytes, out.data_ptr(), out_stride, lse,
-             _stream(device, stream)))
+             _stream(index, stream)))
     return out
 
 
@@ -168,8 +183,10 @@ def paged_kv_append(cache: PagedCache, batch: PagedBatch, k_new, v_new, *, strea
     stride = _rows(k_new, "k_new", batch.n_tokens, cache.kv_heads, cache.head_dim)
     if _rows(v_new, "v_new", batch.n_tokens, cache.kv_heads, cache.head_dim) != stride or k_new.dtype != v_new.dtype:
         raise ValueError("k_new and v_new have to be alike")
-    device = _on_device(k_new, v_new, cache, batch)
-    check(load().rnb_b200_dev_paged_kv_append(cache._ref, batch._ref, _type(k_new), k_new.data_ptr(), v_new.data_ptr(), stride, _stream(device, stream)))
+    index = cache.index
+    if batch.index != index or k_new.get_device() != index or v_new.get_device() != index:
+        raise ValueError(f"cache, batch and rows have to be on one CUDA device, got {index}, {batch.index}, {k_new.device} and {v_new.device}")
+    check(load().rnb_b200_dev_paged_kv_append(cache._ref, batch._ref, _type(k_new), k_new.data_ptr(), v_new.data_ptr(), stride, _stream(index, stream)))
 
 
 def _host(a) -> np.ndarray:
@@ -183,7 +200,7 @@ def paged_kv_copy(cache: PagedCache, src, dst, rows=None, *, stream=None) -> Non
     if src.size != dst.size or (rows is not None and rows.size != src.size):
         raise ValueError("src, dst and rows have to be equally long")
     check(load().rnb_b200_dev_paged_kv_copy(cache._ref, cache.n_layers, cache.layer_stride, src.ctypes.data, dst.ctypes.data, None if rows is None else rows.ctypes.data,
-                                            src.size, _stream(cache.device, stream)))
+                                            src.size, _stream(cache.index, stream)))
 
 
 class KvPages:
