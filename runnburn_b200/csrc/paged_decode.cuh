@@ -35,8 +35,10 @@ struct PdShape {
     static constexpr int ROW = D + 4;                                                    // floats between the heads of a partial output
     static constexpr uint32_t TILE_BYTES = PD_TILE * D * 2;
     static constexpr size_t MERGE = sizeof(float) * HT * 4 * 8 * ROW;                    // outputs of the warps; weights of the parts in a join
-    static constexpr size_t JOIN = sizeof(float) * HT * 8 * 148 * PER_SM;
-    static constexpr size_t SMEM = STAGES * 2 * TILE_BYTES + (MERGE > JOIN ? MERGE : JOIN) + sizeof(float) * HT * 8 * 10 + 128;
+    static constexpr int WEIGHTS = 256;                                                  // parts whose weights a join has at hand
+    static constexpr size_t SMEM = STAGES * 2 * TILE_BYTES + MERGE + sizeof(float) * HT * 8 * 10 + 128;
+    static_assert(WEIGHTS * 8 * HT * sizeof(float) <= MERGE, "they lie where the outputs were");
+    static_assert(PER_SM * (SMEM + 1024) <= 228 * 1024, "shared memory");
     static constexpr size_t RECORD = sizeof(float) * HT * 8 * (D + 4);                   // per head: maximum, sum, two unused, output
 };
 
@@ -445,7 +447,7 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
                             for (int i = 0; i < 4; i++) y[i] = p0 + 32 * i < parts ? ld_l2(reinterpret_cast<const float2 *>(part(p0 + 32 * i, h))) : make_float2(-INFINITY, 0.f);
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
-                                if (p0 + 32 * i < parts) merge[(p0 + 32 * i) * (8 * HT) + h] = y[i].x;
+                                if (p0 + 32 * i < min(parts, S::WEIGHTS)) merge[(p0 + 32 * i) * (8 * HT) + h] = y[i].x;
                                 const float top = fmaxf(M_h, y[i].x), ref = top == -INFINITY ? 0.f : top;
                                 L_h = L_h * pd_exp2(M_h - ref) + y[i].y * pd_exp2(y[i].x - ref);
                                 M_h = top;
@@ -453,7 +455,7 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
                         }
                         const float M_all = warp_max(M_h), ref_h = M_all == -INFINITY ? 0.f : M_all;
                         L_h = warp_sum(L_h * pd_exp2(M_h - ref_h));
-                        for (int p = lane; p < parts; p += 32) merge[p * (8 * HT) + h] = pd_exp2(merge[p * (8 * HT) + h] - ref_h);
+                        for (int p = lane; p < min(parts, S::WEIGHTS); p += 32) merge[p * (8 * HT) + h] = pd_exp2(merge[p * (8 * HT) + h] - ref_h);
                         if (lane == 0) {
                             ml[h * 10 + 8] = M_all;
                             ml[h * 10 + 9] = L_h;
@@ -463,16 +465,17 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
                     for (int e = tid; e < heads_here * (D / 4); e += S::WORKERS) {
                         const int h = e / (D / 4), d = e % (D / 4) * 4;
                         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        const float top = ml[h * 10 + 8], ref = top == -INFINITY ? 0.f : top;
                         for (int p0 = 0; p0 < parts; p0 += AHEAD) {
                             if (p0 > 0 || e != tid) ask(e, p0);
 #pragma unroll
                             for (int i = 0; i < AHEAD; i++)
                                 if (p0 + i < parts) {
-                                    const float w = merge[(p0 + i) * (8 * HT) + h];
+                                    const float w = p0 < S::WEIGHTS ? merge[(p0 + i) * (8 * HT) + h] : pd_exp2(ld_l2(part(p0 + i, h)) - ref);
                                     v = make_float4(fmaf(w, x[i].x, v.x), fmaf(w, x[i].y, v.y), fmaf(w, x[i].z, v.z), fmaf(w, x[i].w, v.w));
                                 }
                         }
-                        put(h, d, v, ml[h * 10 + 8], ml[h * 10 + 9]);
+                        put(h, d, v, top, ml[h * 10 + 9]);
                     }
                 }
             }
