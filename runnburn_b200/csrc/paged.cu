@@ -152,7 +152,8 @@ struct PkAttention {   // a checked call
     float *lse;
 };
 // the mark and the counters; two records for every CTA of the decode kernel, or 256 rows of sums for every CTA of the prompts' kernel in clusters
-constexpr size_t PK_WORKSPACE_BYTES = PD_WS_RECORDS + (size_t)148 * 256 * 128 * sizeof(float);
+constexpr int PK_MAX_SMS = 148;
+constexpr size_t PK_WORKSPACE_BYTES = PD_WS_RECORDS + (size_t)PK_MAX_SMS * 256 * 128 * sizeof(float);
 static_assert(PD_WS_RECORDS % 256 == 0, "records are read by 16 bytes");
 
 static int pk_check_attention(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type, const void *q, size_t q_stride, size_t num_heads,
@@ -242,8 +243,8 @@ static int pk_decode_launch(const PkAttention &a, cudaStream_t s, State &st) {
     const uint64_t held = (((uint64_t)a.b.max_pages << a.c.page_shift) + PD_TILE - 1) / PD_TILE, seen = ((uint64_t)a.window + a.sinks) / PD_TILE + 4;
     if ((uint64_t)a.b.n_seq * (a.window ? std::min(held, seen) : held) * P.splits * a.c.kv_heads > 0x7fffffffu)
         return fail(RNB_B200_UNSUPPORTED, "paged attention: %d sequences with tables of %d pages are more than a launch can have", a.b.n_seq, a.b.max_pages);
-    const int grid = std::min(std::min(st.sm_count, 148) * S::PER_SM, PD_MAX_GRID);
-    static_assert(148 * S::PER_SM * 2 * S::RECORD <= PK_WORKSPACE_BYTES - PD_WS_RECORDS, "records");
+    const int grid = std::min(st.sm_count, PK_MAX_SMS) * S::PER_SM;
+    static_assert(PK_MAX_SMS * S::PER_SM <= PD_MAX_GRID && PK_MAX_SMS * S::PER_SM * 2 * S::RECORD <= PK_WORKSPACE_BYTES - PD_WS_RECORDS, "records");
     PkMaps maps;
     RNB_TRY(pk_encode(&maps.k, a.c.k, a, PD_TILE, D / 64));
     RNB_TRY(pk_encode(&maps.v, a.c.v, a, PD_TILE, D / 64));
@@ -291,10 +292,12 @@ static int pk_prefill(const PkAttention &a, cudaStream_t s, State &st) {
     // Pairs of row blocks: the starts are on the device, so there is one more per sequence than the tokens could need.
     const size_t pairs = std::min<size_t>((size_t)a.b.n_tokens, (size_t)a.b.n_tokens / (2 * P.queries) + (size_t)a.b.n_seq) * a.c.kv_heads * P.blocks;
     if (pairs > 0x7fffffffu) return fail(RNB_B200_UNSUPPORTED, "paged attention: %zu blocks of rows are more than a launch can have", pairs);
-    // Keys are shared out where the launch leaves most of the chip idle and a share is at least two tiles of the longest table.
-    const long long tiles = (((long long)a.b.max_pages << a.c.page_shift) + PP_KEYS - 1) / PP_KEYS;
+    // Keys are shared out where the launch leaves most of the chip idle, down to one tile of what a pair could see for each: a join costs less than a tile
+    // (33 tokens behind 300 positions: 14.0 us, without 16.5).
+    long long tiles = (((long long)a.b.max_pages << a.c.page_shift) + PP_KEYS - 1) / PP_KEYS;
+    if (a.window) tiles = std::min(tiles, ((long long)a.window + a.sinks + 2 * P.queries) / PP_KEYS + 3);
     unsigned ranks = 1;
-    while (ranks < PP_MAX_CLUSTER && pairs * ranks * 2 <= (size_t)std::min(st.sm_count, 148) && tiles >= 4 * (long long)ranks) ranks *= 2;
+    while (ranks < PP_MAX_CLUSTER && pairs * ranks * 2 <= (size_t)std::min(st.sm_count, PK_MAX_SMS) && tiles > (long long)ranks) ranks *= 2;
     if (ranks == 1) RNB_CU(launch_k(paged_prefill_kernel<Q, C, D>, dim3((unsigned)pairs), dim3(PP_THREADS), S::SMEM, s, a.c, a.b, P, maps));
     else RNB_CU(launch_k_cluster(paged_prefill_kernel<Q, C, D>, dim3((unsigned)pairs * ranks), dim3(PP_THREADS), S::SMEM, s, dim3(ranks), a.c, a.b, P, maps));
     return RNB_B200_OK;

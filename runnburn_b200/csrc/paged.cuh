@@ -46,10 +46,10 @@ __device__ __forceinline__ PkRow pk_row(const PkBatch &b, int page_shift, int ro
     if (row < start || row >= end) return {-1, -1};   // starts out of order
     return {lo, pk_length(b, page_shift, lo, err) - (end - row)};
 }
-// One block of a launch looks through the starts: from 0, not descending, within the token matrices.
-__device__ __forceinline__ void pk_check_starts(const PkBatch &b, int *err) {
+// Some threads of a launch look through the starts: from 0, not descending, within the token matrices.
+__device__ __forceinline__ void pk_check_starts(const PkBatch &b, int thread, int threads, int *err) {
     if (!b.q_start) return;
-    for (int i = threadIdx.x; i <= b.n_seq; i += blockDim.x) {
+    for (int i = thread; i <= b.n_seq; i += threads) {
         const int x = b.q_start[i];
         if (i == 0 ? x != 0 : x < b.q_start[i - 1]) atomicExch(err, DEV_ERR_BAD_PAGE);
         if (i == b.n_seq && x > b.n_tokens) atomicExch(err, DEV_ERR_BAD_PAGE);
@@ -61,6 +61,13 @@ __device__ __forceinline__ int pk_page(const PkBatch &b, const PkCache &c, int s
     if ((unsigned)page < (unsigned)c.n_pages) return page;
     atomicExch(err, DEV_ERR_BAD_PAGE);
     return -1;
+}
+
+// A power of two `up` that a row's largest absolute value is one to two times, and its reciprocal; the extremes of f32 stay in range.
+__device__ __forceinline__ void pk_factor(float most, float &down, float &up) {
+    const uint32_t e = min(max(__float_as_uint(most) & 0x7f800000u, 0x00800000u), 0x7e800000u);
+    up = __uint_as_float(e);
+    down = __uint_as_float(0x7f000000u - e);
 }
 
 // ---- append -----------------------------------------------------------------------------------------
@@ -80,7 +87,7 @@ RNB_GLOBAL void paged_append_kernel(PkCache c, PkBatch b, const Src *k_new, cons
     pdl_launch_dependents();
     pdl_wait();
     const int row = blockIdx.x;
-    if (row == 0) pk_check_starts(b, err);
+    if (row == 0) pk_check_starts(b, threadIdx.x, blockDim.x, err);
     const PkRow at = pk_row(b, c.page_shift, row, err);
     if (at.seq < 0) return;
     if (at.pos < 0) {   // more tokens than positions

@@ -125,11 +125,11 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
     const int VH = c.kv_heads * P.splits;
 
     // ---- this CTA's run: units [begin, end) of VH * (tiles of all sequences) ----
-    volatile int *const found = reinterpret_cast<volatile int *>(pd_smem);
+    volatile int *const found = note + 2;
     if (warp == 0) {
         const unsigned mark = lane == 0 ? ld_l2(reinterpret_cast<const uint32_t *>(P.workspace)) : 0;
         auto tiles_of = [&](int r) { return r < b.n_seq ? pd_seen(pk_length(b, c.page_shift, r, P.err), P.window, P.sinks).tiles : 0; };
-        const int first32 = tiles_of(lane);
+        const int len32 = lane < b.n_seq ? pk_length(b, c.page_shift, lane, P.err) : 0, first32 = lane < b.n_seq ? pd_seen(len32, P.window, P.sinks).tiles : 0;
         int sum = first32, most = first32;
         for (int r = lane + 32; r < b.n_seq; r += 32) {
             const int n = tiles_of(r);
@@ -157,6 +157,7 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
                         found[2] = r0 + l;
                         found[3] = (int)(rest / n);
                         found[4] = (int)(rest % n);
+                        found[5] = r0 == 0 ? len32 : pk_length(b, c.page_shift, r0 + lane, P.err);
                     }
                     break;
                 }
@@ -175,12 +176,11 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
         int row, vh, i;
         PdSeen s;
     } at;
+    if (n_units == 0) return;
     at.row = found[2];
     at.vh = found[3];
     at.i = found[4];
-    __syncthreads();
-    if (n_units == 0) return;
-    at.s = pd_seen(pk_length(b, c.page_shift, at.row, P.err), P.window, P.sinks);
+    at.s = pd_seen(found[5], P.window, P.sinks);
     auto advance = [&](Walk &w) {
         if (++w.i < w.s.tiles) return;
         w.i = 0;
@@ -285,11 +285,9 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
             if constexpr (sizeof(Q) == 4) {
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                // 2^e with largest * 2^-e in 1 .. 2; f32's own extremes stay in range
-                int e = (int)((__float_as_uint(most) >> 23) & 255u) - 127;
-                e = most == 0.f ? 0 : max(-126, min(126, e));
-                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                to_log2 = P.scale_log2 * __uint_as_float((uint32_t)(127 + e) << 23);
+                float down, up;
+                pk_factor(most, down, up);
+                to_log2 = P.scale_log2 * up;
 #pragma unroll
                 for (int k = 0; k < KS; k++)
 #pragma unroll

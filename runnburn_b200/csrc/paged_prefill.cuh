@@ -162,25 +162,36 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
         for (int i = 0; i < PP_SOFTMAX_WARPS; i++) todo[i] = 0;
     }
     pdl_wait();   // tensor memory too is asked for when no earlier launch can still hold it
-    if (blockIdx.x == 0) pk_check_starts(b, P.err);
     const int VH = c.kv_heads * P.blocks, item = (int)(blockIdx.x / ranks), vh = item % VH, head = vh / P.blocks, head0 = (vh % P.blocks) * P.per_block;
     // rows of a block: (query, head) = (row / per_block, row % per_block), by multiplication, exact for rows below 128; the last of several head blocks may have fewer heads
     const int heads_here = min(P.per_block, P.group - head0);
     auto query_of = [&](int row) { return (int)((uint32_t)row * P.by_heads >> 16); };
     if (warp == 0) {
         // which queries: the launch's pairs of row blocks are numbered through from the last to the first, long rows before short ones
-        auto span = [&](int s, int &start) {   // tokens of a sequence; starts out of order are cut to the matrices
-            start = min(max(b.q_start[s], 0), b.n_tokens);
-            return max(0, min(b.q_start[s + 1], b.n_tokens) - start);
+        struct Span {
+            int start, n, len;
         };
-        int total = 0, x;
-        for (int s = lane; s < b.n_seq; s += 32) total += (span(s, x) + 2 * P.queries - 1) / (2 * P.queries);
+        auto span = [&](int s) {   // a sequence's tokens; starts out of order are cut to the matrices
+            Span v{0, 0, 0};
+            if (s >= b.n_seq) return v;
+            const int from = b.q_start[s], to = b.q_start[s + 1];
+            v.len = pk_length(b, c.page_shift, s, P.err);
+            v.start = min(max(from, 0), b.n_tokens);
+            v.n = max(0, min(to, b.n_tokens) - v.start);
+            return v;
+        };
+        auto pairs_of = [&](const Span &v) { return (v.n + 2 * P.queries - 1) / (2 * P.queries); };
+        const Span first32 = span(lane);
+        int total = pairs_of(first32);
+        for (int s = lane + 32; s < b.n_seq; s += 32) total += pairs_of(span(s));
         total = __reduce_add_sync(0xffffffffu, total);
         const int want = total - 1 - item / VH;
-        int before = 0, seq = -1, first = 0, n = 0, start = 0;
-        for (int s0 = 0; s0 < b.n_seq && want >= 0 && seq < 0; s0 += 32) {
-            int st = 0;
-            const int len = s0 + lane < b.n_seq ? span(s0 + lane, st) : 0, pairs = (len + 2 * P.queries - 1) / (2 * P.queries);
+        if (lane == 0) found[0] = -1;
+        __syncwarp();
+        int before = 0;
+        for (int s0 = 0; s0 < b.n_seq && want >= 0; s0 += 32) {
+            const Span v = s0 == 0 ? first32 : span(s0 + lane);
+            const int pairs = pairs_of(v);
             int up = pairs;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -189,20 +200,16 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             }
             const unsigned behind = __ballot_sync(0xffffffffu, before + up > want);
             if (behind) {
-                const int l = __ffs(behind) - 1;
-                seq = s0 + l;
-                n = __shfl_sync(0xffffffffu, len, l);
-                start = __shfl_sync(0xffffffffu, st, l);
-                first = (want - before - __shfl_sync(0xffffffffu, up - pairs, l)) * 2 * P.queries;
+                if (lane == __ffs(behind) - 1) {
+                    found[0] = s0 + lane;
+                    found[1] = (want - before - (up - pairs)) * 2 * P.queries;
+                    found[2] = v.n;
+                    found[3] = v.start;
+                    found[4] = v.len;
+                }
+                break;
             }
             before += __shfl_sync(0xffffffffu, up, 31);
-        }
-        if (lane == 0) {
-            found[0] = seq;
-            found[1] = first;
-            found[2] = n;
-            found[3] = start;
-            found[4] = seq >= 0 ? pk_length(b, c.page_shift, seq, P.err) : 0;
         }
     }
     if (warp == PP_SOFTMAX_WARPS) {
@@ -213,10 +220,10 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     __syncthreads();
     pg_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int seq = found[0], first = found[1], n_new = found[2], token0 = found[3];
+    const int seq = found[0];
+    const int first = seq < 0 ? 0 : found[1], n_new = seq < 0 ? 0 : found[2], token0 = seq < 0 ? 0 : found[3], shift = seq < 0 ? 0 : found[4] - n_new;
     bool ok = *failed == 0;
     // block x holds queries first + x * queries ..; query i sits at position shift + i
-    const int shift = found[4] - n_new;
     const int live_a = seq >= 0 ? min(P.queries, n_new - first) : 0, live_b = seq >= 0 ? max(0, min(P.queries, n_new - first - P.queries)) : 0;
     PpSeen seen;
     seen.len = max(0, shift + first + live_a + live_b);
@@ -265,11 +272,9 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
 #pragma unroll
                         for (int o = LANES / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                     }
-                    // 2^e with largest * 2^-e in 1 .. 2
-                    int e = (int)((__float_as_uint(most) >> 23) & 255u) - 127;
-                    e = most == 0.f ? 0 : max(-126, min(126, e));
-                    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                    if (lane % LANES < 2) told[(x * 2 + lane % LANES) * 128 + row0 + j * ROWS + lane / LANES] = __uint_as_float((uint32_t)(127 + e) << 23);   // to both threads of the row
+                    float down, up;
+                    pk_factor(most, down, up);
+                    if (lane % LANES < 2) told[(x * 2 + lane % LANES) * 128 + row0 + j * ROWS + lane / LANES] = up;   // to both threads of the row
                     uint2 hi, lo;
                     pp_cut<C>(v.x * down, v.y * down, hi.x, lo.x);
                     pp_cut<C>(v.z * down, v.w * down, hi.y, lo.y);
@@ -706,6 +711,8 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             for (int x = 0; x < 2; x++)
                 if ((x ? n_b : n_a) > 0) mbar_wait_bounded(&q_full[x], 0u);
         pg_drain(full, it, S::SLOTS);
+    } else if (blockIdx.x == 0) {
+        pk_check_starts(b, lane, 32, P.err);
     }
     __syncwarp();
     if (warp >= PP_SOFTMAX_WARPS && ranks > 1) {
