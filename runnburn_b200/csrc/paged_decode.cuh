@@ -29,14 +29,14 @@ constexpr unsigned PD_WS_MARK = 0x5a5a5a5au;
 
 template <int D, int HT>
 struct PdShape {
-    static constexpr int WORKERS = 128 * HT, THREADS = WORKERS + 32;
+    static constexpr int WORKERS = 128 * HT, THREADS = WORKERS + 64;
     static constexpr int STAGES = D == 128 ? (HT == 1 ? 3 : 5) : 4;
     static constexpr int PER_SM = HT == 1 ? (D == 128 ? 2 : 3) : (D == 128 ? 1 : 2);
     static constexpr int ROW = D + 4;                                                    // floats between the heads of a partial output
     static constexpr uint32_t TILE_BYTES = PD_TILE * D * 2;
     static constexpr size_t MERGE = sizeof(float) * HT * 4 * 8 * ROW;                    // outputs of the warps; weights of the parts in a join
     static constexpr int WEIGHTS = 256;                                                  // parts whose weights a join has at hand
-    static constexpr size_t SMEM = STAGES * 2 * TILE_BYTES + MERGE + sizeof(float) * HT * 8 * 10 + 128;
+    static constexpr size_t SMEM = STAGES * 2 * TILE_BYTES + MERGE + sizeof(float) * HT * 8 * 10 + 192;
     static_assert(WEIGHTS * 8 * HT * sizeof(float) <= MERGE, "they lie where the outputs were");
     static_assert(PER_SM * (SMEM + 1024) <= 228 * 1024, "shared memory");
     static constexpr size_t RECORD = sizeof(float) * HT * 8 * (D + 4);                   // per head: maximum, sum, two unused, output
@@ -108,9 +108,10 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
     constexpr int KS = D / 16;
     extern __shared__ __align__(1024) uint8_t pd_smem[];
     float *const merge = reinterpret_cast<float *>(pd_smem + S::STAGES * 2 * S::TILE_BYTES);
-    float *const ml = reinterpret_cast<float *>(pd_smem + S::SMEM - 128 - sizeof(float) * HT * 8 * 10);   // [head][m of 4 warps, l of 4 warps, M, L]
-    uint64_t *const full = reinterpret_cast<uint64_t *>(pd_smem + S::SMEM - 128), *const empty = full + S::STAGES;
-    volatile int *const note = reinterpret_cast<volatile int *>(full + 2 * S::STAGES);
+    float *const ml = reinterpret_cast<float *>(pd_smem + S::SMEM - 192 - sizeof(float) * HT * 8 * 10);   // [head][m of 4 warps, l of 4 warps, M, L]
+    uint64_t *const full = reinterpret_cast<uint64_t *>(pd_smem + S::SMEM - 192), *const empty = full + S::STAGES;
+    volatile int *const note = reinterpret_cast<volatile int *>(full + 2 * S::STAGES);   // [1]: something gave up; [2] .. [7]: the run
+    volatile int *const jobs = note + 8;   // two cut segments: sequence, head block, first CTA, parts (0: none), whether this CTA came last
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::STAGES; i++) {
@@ -118,6 +119,7 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
             mbar_init(&empty[i], 4 * HT);
         }
         mbar_fence_init();
+        jobs[3] = jobs[8] = jobs[4] = jobs[9] = 0;
         note[1] = (smem_u32(pd_smem) & 1023u) != 0;   // a wait gave up (or the swizzle would not hold): no more waits, the results are void
     }
     pdl_wait();
@@ -241,6 +243,23 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
         return;
     }
 
+    // A warp that tells of cut segments: the workers' records have to be visible before the count, and behind loads that wait for the memory that took up to
+    // 10000 cycles, in which the workers go on.
+    if (warp == 4 * HT + 1) {
+        for (int k = 0; k < 2; k++) {
+            asm volatile("bar.sync %0, %1;" ::"r"(2 + k), "n"(S::WORKERS + 32) : "memory");
+            if (lane == 0 && jobs[5 * k + 3]) {
+                unsigned *const count = reinterpret_cast<unsigned *>(P.workspace + PD_WS_HEAD) + jobs[5 * k + 2];
+                const bool last = pk_arrive_gpu(count) == (unsigned)jobs[5 * k + 3] - 1;   // all workers' records before it, the others' behind it
+                if (last) *count = 0;   // for the next launch
+                jobs[5 * k + 4] = last;
+            }
+            __syncwarp();
+        }
+        asm volatile("bar.sync 4, %0;" ::"n"(S::WORKERS + 32) : "memory");
+        return;
+    }
+
     // ---- products ----
     const int head = lane >> 2, quad = lane & 3;   // of the rows and columns that this thread holds
     uint32_t qa[KS][4];
@@ -253,7 +272,16 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
     const uint32_t k_x = k_row & 7, v_x = v_row & 7, k_c = (lane >> 3) & 1, v_c = lane >> 4;
     uint32_t phase = 0;
     bool ok = note[1] == 0;
-    bool fresh = true;   // a segment begins
+    auto heads_of = [&](int vh) { return min(8 * HT, P.group - (vh % P.splits) * (8 * HT)); };
+    auto put = [&](int row, int vh, int h, int d, float4 v, float M, float L) {   // four dims of an output
+        const float inv = L > 0.f ? 1.f / L : L != L ? L : 0.f;
+        const int q_head = (vh / P.splits) * P.group + (vh % P.splits) * (8 * HT) + h;
+        Q *const out = reinterpret_cast<Q *>(P.out) + (size_t)row * P.out_stride + (size_t)q_head * D + d;
+        if constexpr (sizeof(Q) == 4) *reinterpret_cast<float4 *>(out) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        else *reinterpret_cast<uint2 *>(out) = make_uint2(pk_pack<Q>(v.x * inv, v.y * inv), pk_pack<Q>(v.z * inv, v.w * inv));
+        if (d == 0 && P.lse) P.lse[(size_t)row * P.heads + q_head] = L > 0.f ? (M - PD_BIAS + log2f(L)) * 0.6931471805599453f : L != L ? L : -INFINITY;
+    };
+    bool fresh = true, first_segment = true;   // a segment begins
     int unit = begin, first_tile = at.i;
     int stage = 0;
     for (int u = 0; u < n_units; u++, unit++) {
@@ -385,18 +413,11 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
                 of_head[9] = L;
             }
             pk_sync_some<S::WORKERS>();
-            const int heads_here = min(8 * HT, P.group - (at.vh % P.splits) * (8 * HT)), head0 = (at.vh / P.splits) * P.group + (at.vh % P.splits) * (8 * HT);
             const bool whole = ends && first_tile == 0;
             // the CTAs that share the segment, and this one's record: the first of its two where the segment began before it
             const int seg = unit - at.i, cta0 = seg / per, parts = (seg + at.s.tiles - 1) / per - cta0 + 1;
             float *const record = reinterpret_cast<float *>(P.workspace + PD_WS_RECORDS + (size_t)(2 * blockIdx.x + (first_tile == 0 ? 1 : 0)) * S::RECORD);
-            auto put = [&](int h, int d, float4 v, float M, float L) {   // four dims of an output
-                const float inv = L > 0.f ? 1.f / L : L != L ? L : 0.f;
-                Q *const out = reinterpret_cast<Q *>(P.out) + (size_t)at.row * P.out_stride + (size_t)(head0 + h) * D + d;
-                if constexpr (sizeof(Q) == 4) *reinterpret_cast<float4 *>(out) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-                else *reinterpret_cast<uint2 *>(out) = make_uint2(pk_pack<Q>(v.x * inv, v.y * inv), pk_pack<Q>(v.z * inv, v.w * inv));
-                if (d == 0 && P.lse) P.lse[(size_t)at.row * P.heads + head0 + h] = L > 0.f ? (M - PD_BIAS + log2f(L)) * 0.6931471805599453f : L != L ? L : -INFINITY;
-            };
+            const int heads_here = heads_of(at.vh);
             for (int e = tid; e < heads_here * (D / 4); e += S::WORKERS) {
                 const int h = e / (D / 4), d = e % (D / 4) * 4;
                 const float *const from = merge + ((h >> 3) * 32 + (h & 7)) * S::ROW + d;
@@ -408,78 +429,80 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
                 }
                 const float M_h = ml[h * 10 + 8], L_h = ml[h * 10 + 9];
                 if (whole) {
-                    put(h, d, v, M_h, L_h);
+                    put(at.row, at.vh, h, d, v, M_h, L_h);
                 } else {
                     float *const r = record + h * (D + 4);
                     if (d == 0) *reinterpret_cast<float2 *>(r) = make_float2(M_h, L_h);
                     *reinterpret_cast<float4 *>(r + 4 + d) = v;
                 }
             }
-            if (!whole) {
-                pk_sync_some<S::WORKERS>();
-                if (tid == 0) {
-                    unsigned *const count = reinterpret_cast<unsigned *>(P.workspace + PD_WS_HEAD) + cta0;
-                    const bool last = pk_arrive_gpu(count) == (unsigned)parts - 1;   // all threads' records before it, the others' behind it
-                    if (last) *count = 0;   // for the next launch
-                    *note = last;
-                }
-                pk_sync_some<S::WORKERS>();
-                if (*note) {
-                    // ---- join: part p is of CTA cta0 + p, its second record for p = 0 and its first one after that ----
-                    const float *const base = reinterpret_cast<const float *>(P.workspace + PD_WS_RECORDS);
-                    auto part = [&](int p, int h) { return base + ((size_t)2 * (cta0 + p) + (p == 0 ? 1 : 0)) * (S::RECORD / 4) + h * (D + 4); };
-                    // outputs of the first parts are asked for before their weights are known
-                    constexpr int AHEAD = 8;
-                    float4 x[AHEAD];
-                    auto ask = [&](int e, int p0) {
-#pragma unroll
-                        for (int i = 0; i < AHEAD; i++)
-                            if (p0 + i < parts && e < heads_here * (D / 4)) x[i] = ld_l2(reinterpret_cast<const float4 *>(part(p0 + i, e / (D / 4)) + 4 + e % (D / 4) * 4));
-                    };
-                    ask(tid, 0);
-                    for (int h = warp; h < heads_here; h += S::WORKERS / 32) {
-                        float M_h = -INFINITY, L_h = 0.f;
-                        for (int p0 = lane; p0 < parts; p0 += 128) {
-                            float2 y[4];
-#pragma unroll
-                            for (int i = 0; i < 4; i++) y[i] = p0 + 32 * i < parts ? ld_l2(reinterpret_cast<const float2 *>(part(p0 + 32 * i, h))) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                if (p0 + 32 * i < min(parts, S::WEIGHTS)) merge[(p0 + 32 * i) * (8 * HT) + h] = y[i].x;
-                                const float top = fmaxf(M_h, y[i].x), ref = top == -INFINITY ? 0.f : top;
-                                L_h = L_h * pd_exp2(M_h - ref) + y[i].y * pd_exp2(y[i].x - ref);
-                                M_h = top;
-                            }
-                        }
-                        const float M_all = warp_max(M_h), ref_h = M_all == -INFINITY ? 0.f : M_all;
-                        L_h = warp_sum(L_h * pd_exp2(M_h - ref_h));
-                        for (int p = lane; p < min(parts, S::WEIGHTS); p += 32) merge[p * (8 * HT) + h] = pd_exp2(merge[p * (8 * HT) + h] - ref_h);
-                        if (lane == 0) {
-                            ml[h * 10 + 8] = M_all;
-                            ml[h * 10 + 9] = L_h;
-                        }
-                    }
-                    pk_sync_some<S::WORKERS>();
-                    for (int e = tid; e < heads_here * (D / 4); e += S::WORKERS) {
-                        const int h = e / (D / 4), d = e % (D / 4) * 4;
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        const float top = ml[h * 10 + 8], ref = top == -INFINITY ? 0.f : top;
-                        for (int p0 = 0; p0 < parts; p0 += AHEAD) {
-                            if (p0 > 0 || e != tid) ask(e, p0);
-#pragma unroll
-                            for (int i = 0; i < AHEAD; i++)
-                                if (p0 + i < parts) {
-                                    const float w = p0 < S::WEIGHTS ? merge[(p0 + i) * (8 * HT) + h] : pd_exp2(ld_l2(part(p0 + i, h)) - ref);
-                                    v = make_float4(fmaf(w, x[i].x, v.x), fmaf(w, x[i].y, v.y), fmaf(w, x[i].z, v.z), fmaf(w, x[i].w, v.w));
-                                }
-                        }
-                        put(h, d, v, top, ml[h * 10 + 9]);
-                    }
-                }
+            if (!whole && tid == 0) {
+                volatile int *const job = jobs + (first_tile == 0 ? 5 : 0);
+                job[0] = at.row, job[1] = at.vh, job[2] = cta0, job[3] = parts;
             }
+            if (first_segment) asm volatile("bar.arrive 2, %0;" ::"n"(S::WORKERS + 32) : "memory");
+            if (u == n_units - 1) asm volatile("bar.arrive 3, %0;" ::"n"(S::WORKERS + 32) : "memory");
+            first_segment = false;
             fresh = true;
         }
         advance(at);
+    }
+    asm volatile("bar.sync 4, %0;" ::"n"(S::WORKERS + 32) : "memory");   // the counts are in
+    for (int k = 0; k < 2; k++) {
+        volatile const int *const job = jobs + 5 * k;
+        if (!job[4]) continue;
+        const int row = job[0], vh = job[1], cta0 = job[2], parts = job[3], heads_here = heads_of(vh);
+        pk_sync_some<S::WORKERS>();   // the weights' place and the maxima are free
+        // ---- join: part p is of CTA cta0 + p, its second record for p = 0 and its first one after that ----
+        const float *const base = reinterpret_cast<const float *>(P.workspace + PD_WS_RECORDS);
+        auto part = [&](int p, int h) { return base + ((size_t)2 * (cta0 + p) + (p == 0 ? 1 : 0)) * (S::RECORD / 4) + h * (D + 4); };
+        // outputs of the first parts are asked for before their weights are known
+        constexpr int AHEAD = 8;
+        float4 x[AHEAD];
+        auto ask = [&](int e, int p0) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+                if (p0 + i < parts && e < heads_here * (D / 4)) x[i] = ld_l2(reinterpret_cast<const float4 *>(part(p0 + i, e / (D / 4)) + 4 + e % (D / 4) * 4));
+        };
+        ask(tid, 0);
+        for (int h = warp; h < heads_here; h += S::WORKERS / 32) {
+            float M_h = -INFINITY, L_h = 0.f;
+            for (int p0 = lane; p0 < parts; p0 += 128) {
+                float2 y[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[i] = p0 + 32 * i < parts ? ld_l2(reinterpret_cast<const float2 *>(part(p0 + 32 * i, h))) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (p0 + 32 * i < min(parts, S::WEIGHTS)) merge[(p0 + 32 * i) * (8 * HT) + h] = y[i].x;
+                    const float top = fmaxf(M_h, y[i].x), ref = top == -INFINITY ? 0.f : top;
+                    L_h = L_h * pd_exp2(M_h - ref) + y[i].y * pd_exp2(y[i].x - ref);
+                    M_h = top;
+                }
+            }
+            const float M_all = warp_max(M_h), ref_h = M_all == -INFINITY ? 0.f : M_all;
+            L_h = warp_sum(L_h * pd_exp2(M_h - ref_h));
+            for (int p = lane; p < min(parts, S::WEIGHTS); p += 32) merge[p * (8 * HT) + h] = pd_exp2(merge[p * (8 * HT) + h] - ref_h);
+            if (lane == 0) {
+                ml[h * 10 + 8] = M_all;
+                ml[h * 10 + 9] = L_h;
+            }
+        }
+        pk_sync_some<S::WORKERS>();
+        for (int e = tid; e < heads_here * (D / 4); e += S::WORKERS) {
+            const int h = e / (D / 4), d = e % (D / 4) * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float top = ml[h * 10 + 8], ref = top == -INFINITY ? 0.f : top;
+            for (int p0 = 0; p0 < parts; p0 += AHEAD) {
+                if (p0 > 0 || e != tid) ask(e, p0);
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++)
+                    if (p0 + i < parts) {
+                        const float w = p0 < S::WEIGHTS ? merge[(p0 + i) * (8 * HT) + h] : pd_exp2(ld_l2(part(p0 + i, h)) - ref);
+                        v = make_float4(fmaf(w, x[i].x, v.x), fmaf(w, x[i].y, v.y), fmaf(w, x[i].z, v.z), fmaf(w, x[i].w, v.w));
+                    }
+            }
+            put(row, vh, h, d, v, top, ml[h * 10 + 9]);
+        }
     }
 }
 #endif  // __CUDACC__
