@@ -151,9 +151,10 @@ struct PkAttention {   // a checked call
     void *out, *workspace;
     float *lse;
 };
-// the mark and the counters; two records for every CTA of the decode kernel, or 256 rows of sums for every CTA of the prompts' kernel in clusters
+// the mark and the counters, and two records for every CTA of the decode kernel; the prompts' kernel joins in shared memory
 constexpr int PK_MAX_SMS = 148;
-constexpr size_t PK_WORKSPACE_BYTES = PD_WS_RECORDS + (size_t)PK_MAX_SMS * 256 * 128 * sizeof(float);
+constexpr size_t PK_WORKSPACE_BYTES = PD_WS_RECORDS + (size_t)PK_MAX_SMS * 2 * std::max({PdShape<64, 1>::PER_SM * PdShape<64, 1>::RECORD, PdShape<64, 2>::PER_SM * PdShape<64, 2>::RECORD,
+                                                                                         PdShape<128, 1>::PER_SM * PdShape<128, 1>::RECORD, PdShape<128, 2>::PER_SM * PdShape<128, 2>::RECORD});
 static_assert(PD_WS_RECORDS % 256 == 0, "records are read by 16 bytes");
 
 static int pk_check_attention(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type, const void *q, size_t q_stride, size_t num_heads,
@@ -278,7 +279,6 @@ static int pk_prefill(const PkAttention &a, cudaStream_t s, State &st) {
     P.scale = a.scale;
     P.out = a.out;
     P.lse = a.lse;
-    P.sums = (float *)((uint8_t *)a.workspace + PD_WS_RECORDS);
     P.err = st.dev_error;
     P.by_heads = (65536 + P.per_block - 1) / P.per_block;
     PpMaps maps{};
@@ -290,12 +290,12 @@ static int pk_prefill(const PkAttention &a, cudaStream_t s, State &st) {
         RNB_TRY(pk_encode_tiled(&maps.q, const_cast<void *>(a.q), a.c_type, 4, dims, strides, box, "queries"));
     }
     // Pairs of row blocks: the starts are on the device, so there is one more per sequence than the tokens could need.
-    const size_t pairs = std::min<size_t>((size_t)a.b.n_tokens, (size_t)a.b.n_tokens / (2 * P.queries) + (size_t)a.b.n_seq) * a.c.kv_heads * P.blocks;
+    const size_t pairs = std::min<size_t>((size_t)a.b.n_tokens, (size_t)a.b.n_tokens / (S::BLOCKS * P.queries) + (size_t)a.b.n_seq) * a.c.kv_heads * P.blocks;
     if (pairs > 0x7fffffffu) return fail(RNB_B200_UNSUPPORTED, "paged attention: %zu blocks of rows are more than a launch can have", pairs);
     // Keys are shared out where the launch leaves most of the chip idle, down to one tile of what a pair could see for each: a join costs less than a tile
     // (33 tokens behind 300 positions: 14.0 us, without 16.5).
     long long tiles = (((long long)a.b.max_pages << a.c.page_shift) + PP_KEYS - 1) / PP_KEYS;
-    if (a.window) tiles = std::min(tiles, ((long long)a.window + a.sinks + 2 * P.queries) / PP_KEYS + 3);
+    if (a.window) tiles = std::min(tiles, ((long long)a.window + a.sinks + S::BLOCKS * P.queries) / PP_KEYS + 3);
     unsigned ranks = 1;
     while (ranks < PP_MAX_CLUSTER && pairs * ranks * 2 <= (size_t)std::min(st.sm_count, PK_MAX_SMS) && tiles > (long long)ranks) ranks *= 2;
     if (ranks == 1) RNB_CU(launch_k(paged_prefill_kernel<Q, C, D>, dim3((unsigned)pairs), dim3(PP_THREADS), S::SMEM, s, a.c, a.b, P, maps));

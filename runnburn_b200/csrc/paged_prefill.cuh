@@ -1,19 +1,22 @@
 // Causal attention of prompts over a paged cache on the 5th-generation tensor cores.
 //
-// A CTA owns two blocks of 128 (query, head) rows of one key head - a block is 128 / group consecutive queries of a sequence times the group's
-// heads - and walks the keys that some of its queries sees in tiles of 128.  Both blocks use a tile while it is in shared memory.  A
-// row is a tensor-memory lane and has two threads, of two warps, which take half of a tile's keys each and tell each other their maxima.  One thread issues the products:
-// scores from queries and keys in shared memory, then probabilities from tensor memory, where they take the scores' place, times
-// values.  It takes the blocks in turn, P V of block a, the next scores of a, P V of b, the next scores of b, so that one block's softmax runs under the
-// other's products.  One warp copies K0 V0 K1 V1 ... into a ring, a box per page and 64 dims, its lanes
-// following the table.
+// A CTA owns blocks of 128 (query, head) rows of one key head - a block is 128 / group consecutive queries of a sequence times the group's heads - and
+// walks the keys that some of its queries sees in tiles of 128.  A row is a tensor-memory lane; its threads, of as many warps, take a part of a tile's
+// keys each and tell each other their maxima.  One thread issues the products: scores from queries and keys in shared memory, then
+// probabilities from tensor memory times values.  One warp copies K0 V0 K1 V1 ... into a ring, a box per page and 64 dims, its lanes following
+// the table; another sets values that nobody sees to zero.
 //
-// f32 queries enter as f16 "hi" + remainder "lo" (scaled by a power of two per row into f16's range), and so do the probabilities: every product is made
-// twice and keeps 22 bits; 16-bit queries are exact and their probabilities are rounded once to the cache's type, half a step of the output's own rounding.
-// Probabilities are scaled by 2^BIAS so that small ones keep their bits, and the output is scaled only when a row's
-// maximum has grown by more than 2^GROWTH.  The tensor cores cut sums off at every step, which adds up over long rows: f32 outputs are taken out of
-// tensor memory every FLUSH tiles and summed in f32.
+// 16-bit queries: two blocks, which use a tile while it is in shared memory, two threads a row.  One block's softmax runs under the other's
+// products.  Tensor memory holds two outputs and probabilities, and scores of one block at a time: as soon as they are read it is the other's turn.
+// What sets the pace is this turn: 1650 cycles from one block's reading to the other's (the exponentials take 1024 of a block's tile, its products 1100).
+// Queries are exact; probabilities are rounded once to the cache's type, half a step of the output's own rounding.
 //
+// f32 queries: one block, four threads a row.  Queries enter as f16 "hi" + remainder "lo" (scaled by a power of two per row into f16's range), and so do the
+// probabilities: every product is made twice and keeps 22 bits, so the products set the pace.  Three tiles' scores are under way, and probabilities take their place.
+// The tensor cores cut sums off at every step, which adds up over long rows: outputs are taken out of tensor memory every FLUSH tiles and summed in f32
+// registers (error against 64 bits at 2048 tokens 6.3e-7, at 60000 positions 9.4e-7; summed there throughout 1.6e-6 and more).
+//
+// Probabilities are scaled by 2^BIAS so that small ones keep their bits, and the output is scaled only when a row's maximum has grown by more than 2^GROWTH.
 // Few rows behind many keys: a cluster of up to eight CTAs shares the keys, and joins maxima, sums and outputs over distributed shared memory.
 #pragma once
 #include "paged_attention_plain.cuh"
@@ -23,28 +26,29 @@
 namespace rnb {
 
 constexpr int PP_KEYS = 128;
-constexpr int PP_WAYS = 2;   // threads of a row
-constexpr int PP_SOFTMAX_WARPS = 8 * PP_WAYS, PP_THREADS = PP_SOFTMAX_WARPS * 32 + 128;   // the last warp is there for the register split alone: setmaxnreg goes by four warps
+constexpr int PP_SOFTMAX_WARPS = 16, PP_THREADS = PP_SOFTMAX_WARPS * 32 + 128;   // the last warp is there for the register split, which goes by four warps
 constexpr int PP_SOFTMAX_REGS = 104, PP_OTHER_REGS = 64;
 static_assert(PP_SOFTMAX_WARPS * 32 * PP_SOFTMAX_REGS + 128 * PP_OTHER_REGS <= PP_THREADS * 96, "what the block is launched with");
 constexpr float PP_BIAS = 8.f, PP_GROWTH = 7.f;   // log2; together below f16's 2^16
-constexpr int PP_FLUSH = 16;
+constexpr int PP_FLUSH = 2;
 constexpr int PP_MAX_CLUSTER = 8;
 constexpr uint32_t PP_PANEL = 128 * 128;          // 128 rows of 64 elements, 128-byte swizzle
 
 template <class Q, int D>
 struct PpShape {
     static constexpr int TERMS = sizeof(Q) == 4 ? 2 : 1, PANELS = D / 64;
-    static constexpr uint32_t Q_BYTES = 2 * TERMS * PANELS * PP_PANEL, TILE_BYTES = PANELS * PP_PANEL;
-    // tensor memory: where it has room, probabilities have columns of their own and the scores' columns serve both blocks in turn
-    static constexpr bool SHARED = 2 * D + 2 * TERMS * 64 + 128 <= 512;
-    static constexpr int PARTS = SHARED ? 1 : 2;   // of a tile's probabilities, that are multiplied one after the other: where scores wait for the last of them
-    static constexpr uint32_t scores_at(int x) { return SHARED ? 2 * D : (uint32_t)x * 128u; }
-    static constexpr uint32_t probabilities_at(int x) { return SHARED ? 2 * D + 128 + (uint32_t)(x * TERMS * 64) : (uint32_t)x * 128u; }
-    static constexpr uint32_t outputs_at(int x) { return (SHARED ? 0u : 256u) + (uint32_t)(x * D); }
+    static constexpr int BLOCKS = TERMS == 2 ? 1 : 2, ROWS = 128 * BLOCKS, WAYS = PP_SOFTMAX_WARPS / (4 * BLOCKS);   // threads of a row
+    static constexpr uint32_t Q_BYTES = BLOCKS * TERMS * PANELS * PP_PANEL, TILE_BYTES = PANELS * PP_PANEL;
+    // tensor memory.  One block: scores of three tiles, in whose place their probabilities come, and the output.  Two: outputs, scores of one of them, probabilities
+    static constexpr bool TURNS = BLOCKS == 2;
+    static constexpr int BUFFERS = TURNS ? 1 : 3;
+    static __device__ __forceinline__ uint32_t scores_at(int t) { return TURNS ? 2 * D : (uint32_t)(t % BUFFERS) * 128u; }
+    static __device__ __forceinline__ uint32_t probabilities_at(int x, int t) { return TURNS ? 2 * D + 128 + (uint32_t)x * 64u : scores_at(t); }
+    static constexpr uint32_t outputs_at(int x) { return TURNS ? (uint32_t)(x * D) : 384u; }
+    static_assert(TURNS ? 2 * D + 256 <= 512 : 384 + D <= 512, "tensor memory");
     static constexpr int SLOTS = (int)((224 * 1024 - Q_BYTES) / TILE_BYTES) < 8 ? (int)((224 * 1024 - Q_BYTES) / TILE_BYTES) : 8;
     static constexpr size_t TAIL = 512 + 512 * 4;                                     // barriers; what the threads of a row tell each other
-    static constexpr size_t JOIN = 256 * (D + 4) * 4 + 256 * 8 + 256 * PP_MAX_CLUSTER * 4 + 256 * 8;   // outputs; maximum, sum; weights; joined
+    static constexpr size_t JOIN = ROWS * (D + 4) * 4 + ROWS * 8 + ROWS * PP_MAX_CLUSTER * 4 + ROWS * 8;   // outputs; maximum, sum; weights; joined
     static constexpr size_t RING = Q_BYTES + (size_t)SLOTS * TILE_BYTES;
     static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + TAIL;
     static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -62,7 +66,6 @@ struct PpParams {
     float scale;
     void *out;
     float *lse;
-    float *sums;   // cluster launches: 256 rows of D floats per CTA, for the f32 sums of long rows
     int *err;
 };
 
@@ -83,6 +86,10 @@ __device__ __forceinline__ void pp_tmem_st(uint32_t taddr, const uint32_t (&v)[1
                  "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
 }
+// 16, 32 or 64 columns of this thread's lane
+__device__ __forceinline__ void pp_tmem_ld(uint32_t taddr, uint32_t (&v)[64]) { pat_tmem_ld64(taddr, v); }
+__device__ __forceinline__ void pp_tmem_ld(uint32_t taddr, uint32_t (&v)[32]) { pg_tmem_ld32(taddr, v); }
+__device__ __forceinline__ void pp_tmem_ld(uint32_t taddr, uint32_t (&v)[16]) { ps_tmem_ld<16>(taddr, v); }
 template <int N>
 __device__ __forceinline__ void pp_registers(bool more) {
     if (more) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -134,12 +141,12 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint64_t *const bars = reinterpret_cast<uint64_t *>(pp_smem + S::SMEM - S::TAIL);
-    uint64_t *const full = bars, *const empty = bars + 8, *const q_full = bars + 16, *const s_full = bars + 18, *const p_full = bars + 20, *const pv_done = bars + 24, *const s_free = bars + 26, *const cleared = bars + 44;   // two each of the first four, p_full 2 x 2
-    volatile uint32_t *const tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + 27);
-    volatile int *const failed = reinterpret_cast<volatile int *>(bars + 28);
-    volatile int *const found = reinterpret_cast<volatile int *>(bars + 29);   // sequence, first query, queries of the sequence, first row of its tokens, its positions
-    unsigned *const todo = reinterpret_cast<unsigned *>(bars + 33);   // rows of each warp to be done again
-    float *const told = reinterpret_cast<float *>(pp_smem + S::SMEM - S::TAIL + 512);   // [block][half][row]
+    uint64_t *const full = bars, *const empty = bars + 8, *const q_full = bars + 16, *const s_full = bars + 18, *const p_full = bars + 21, *const pv_done = bars + 24, *const s_free = bars + 27, *const cleared = bars + 44;   // s_full, p_full, pv_done: per block, or per buffer of one
+    volatile uint32_t *const tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + 28);
+    volatile int *const failed = reinterpret_cast<volatile int *>(bars + 29);
+    volatile int *const found = reinterpret_cast<volatile int *>(bars + 30);   // sequence, first query, queries of the sequence, first row of its tokens, its positions
+    unsigned *const todo = reinterpret_cast<unsigned *>(bars + 34);   // rows of each warp to be done again
+    float *const told = reinterpret_cast<float *>(pp_smem + S::SMEM - S::TAIL + 512);   // [block][way][row]
     uint32_t rank, ranks;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
@@ -148,14 +155,13 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int x = 0; x < 2; x++) {
-            mbar_init(&q_full[x], S::TERMS == 2 ? 4 * PP_WAYS : 1);
-            mbar_init(&s_full[x], 1);
-            mbar_init(&p_full[2 * x], 4 * PP_WAYS);
-            mbar_init(&p_full[2 * x + 1], 4 * PP_WAYS);
-            mbar_init(&pv_done[x], 1);
+        for (int i = 0; i < 2; i++) mbar_init(&q_full[i], S::TERMS == 2 ? PP_SOFTMAX_WARPS : 1);
+        for (int i = 0; i < 3; i++) {
+            mbar_init(&pv_done[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4 * S::WAYS);
         }
-        mbar_init(s_free, 4 * PP_WAYS);
+        mbar_init(s_free, 4 * S::WAYS);
         for (int i = 0; i < 8; i++) mbar_init(&cleared[i], 1);
         mbar_fence_init();
         *failed = (smem_u32(pp_smem) & 1023u) != 0;
@@ -167,7 +173,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     const int heads_here = min(P.per_block, P.group - head0);
     auto query_of = [&](int row) { return (int)((uint32_t)row * P.by_heads >> 16); };
     if (warp == 0) {
-        // which queries: the launch's pairs of row blocks are numbered through from the last to the first, long rows before short ones
+        // which queries: the launch's CTAs' worth of row blocks are numbered through from the last to the first, long rows before short ones
         struct Span {
             int start, n, len;
         };
@@ -180,7 +186,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             v.n = max(0, min(to, b.n_tokens) - v.start);
             return v;
         };
-        auto pairs_of = [&](const Span &v) { return (v.n + 2 * P.queries - 1) / (2 * P.queries); };
+        auto pairs_of = [&](const Span &v) { return (v.n + S::BLOCKS * P.queries - 1) / (S::BLOCKS * P.queries); };
         const Span first32 = span(lane);
         int total = pairs_of(first32);
         for (int s = lane + 32; s < b.n_seq; s += 32) total += pairs_of(span(s));
@@ -202,7 +208,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             if (behind) {
                 if (lane == __ffs(behind) - 1) {
                     found[0] = s0 + lane;
-                    found[1] = (want - before - (up - pairs)) * 2 * P.queries;
+                    found[1] = (want - before - (up - pairs)) * S::BLOCKS * P.queries;
                     found[2] = v.n;
                     found[3] = v.start;
                     found[4] = v.len;
@@ -220,11 +226,17 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     __syncthreads();
     pg_fence_after();
     const uint32_t tmem = *tmem_slot;
+    // The barriers of block x's tile t.  With several buffers nobody is more than their number of tiles ahead, so each has its own: a phase of one barrier for
+    // all would be taken for the one two tiles on.
+    auto passed = [&](uint64_t *bar, int x, int t) {
+        return S::TURNS ? mbar_wait_bounded(&bar[x], (uint32_t)(t & 1)) : mbar_wait_bounded(&bar[t % S::BUFFERS], (uint32_t)(t / S::BUFFERS) & 1u);
+    };
+    auto of_tile = [&](uint64_t *bar, int x, int t) { return &bar[S::TURNS ? x : t % S::BUFFERS]; };
     const int seq = found[0];
     const int first = seq < 0 ? 0 : found[1], n_new = seq < 0 ? 0 : found[2], token0 = seq < 0 ? 0 : found[3], shift = seq < 0 ? 0 : found[4] - n_new;
     bool ok = *failed == 0;
     // block x holds queries first + x * queries ..; query i sits at position shift + i
-    const int live_a = seq >= 0 ? min(P.queries, n_new - first) : 0, live_b = seq >= 0 ? max(0, min(P.queries, n_new - first - P.queries)) : 0;
+    const int live_a = seq >= 0 ? min(P.queries, n_new - first) : 0, live_b = S::BLOCKS == 2 && seq >= 0 ? max(0, min(P.queries, n_new - first - P.queries)) : 0;
     PpSeen seen;
     seen.len = max(0, shift + first + live_a + live_b);
     seen.from = P.window ? max(0, shift + first - P.window + 1) : 0;
@@ -241,17 +253,15 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     if (warp < PP_SOFTMAX_WARPS) pp_registers<PP_SOFTMAX_REGS>(true);
     else pp_registers<PP_OTHER_REGS>(false);
     if (warp < PP_SOFTMAX_WARPS) {
-        // a row's threads: lane `lane` of the warps (x, half, w), which take KEYS of a tile's keys and COLS of the output's dims each
-        constexpr int KEYS = PP_KEYS / PP_WAYS, DIMS = D / PP_WAYS;
-        const int x = warp / (4 * PP_WAYS), half = (warp >> 2) % PP_WAYS, w = warp & 3, mine = x ? n_b : n_a, live = x ? live_b : live_a, q0 = first + x * P.queries;
-        auto both = [&]() {   // a row's warps meet
-            if constexpr (PP_WAYS > 1) asm volatile("bar.sync %0, %1;" ::"r"(1 + x * 4 + w), "n"(32 * PP_WAYS) : "memory");
-        };
+        // a row's threads: lane `lane` of the warps (x, way, w), which take KEYS of a tile's keys and DIMS of the output's dims each
+        constexpr int KEYS = PP_KEYS / S::WAYS, DIMS = D / S::WAYS;
+        const int x = warp / (4 * S::WAYS), way = (warp >> 2) % S::WAYS, w = warp & 3, mine = x ? n_b : n_a, live = x ? live_b : live_a, q0 = first + x * P.queries;
+        auto meet = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + x * 4 + w), "n"(32 * S::WAYS) : "memory"); };   // a row's warps
         uint8_t *const q_smem = pp_smem + (uint32_t)(x * S::TERMS * S::PANELS) * PP_PANEL;   // this block's
         if constexpr (S::TERMS == 2) {
             // ---- f32 queries in two terms: a warp takes its share of the rows, all under way ----
-            constexpr int LANES = D / 4, ROWS = 32 / LANES, LOADS = 32 / PP_WAYS / ROWS;   // lanes of a row, rows of a load
-            const int d0 = lane % LANES * 4, row0 = (half * 4 + w) * (32 / PP_WAYS);
+            constexpr int LANES = D / 4, ROWS = 32 / LANES, LOADS = 32 / S::WAYS / ROWS < 1 ? 1 : 32 / S::WAYS / ROWS;   // lanes of a row, rows of a load
+            const int d0 = lane % LANES * 4, row0 = (way * 4 + w) * (32 / S::WAYS);
             const float *const q = reinterpret_cast<const float *>(P.q) + (size_t)(token0 + q0) * P.q_stride + (size_t)(head * P.group + head0) * D + d0;
             if (mine > 0) {
                 float4 raw[LOADS];
@@ -274,7 +284,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                     }
                     float down, up;
                     pk_factor(most, down, up);
-                    if (lane % LANES < 2) told[(x * 2 + lane % LANES) * 128 + row0 + j * ROWS + lane / LANES] = up;   // to both threads of the row
+                    if (lane % LANES < S::WAYS) told[lane % LANES * 128 + row0 + j * ROWS + lane / LANES] = up;   // to all threads of the row
                     uint2 hi, lo;
                     pp_cut<C>(v.x * down, v.y * down, hi.x, lo.x);
                     pp_cut<C>(v.z * down, v.w * down, hi.y, lo.y);
@@ -292,28 +302,39 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
         const bool alive = ql < live && r - ql * P.per_block < heads_here;
         const int pos = shift + q0 + min(ql, max(live - 1, 0));                       // dead rows see what the last one sees, and are not stored
         const int pos0 = shift + q0, pos1 = shift + q0 + live - 1;                    // the block's positions
-        const uint32_t lanes = (uint32_t)(w * 32) << 16, t_s = tmem + S::scores_at(x) + lanes, t_p = tmem + S::probabilities_at(x) + lanes, t_o = tmem + S::outputs_at(x) + (uint32_t)(half * DIMS) + lanes;
+        const uint32_t lanes = (uint32_t)(w * 32) << 16, t_o = tmem + S::outputs_at(x) + (uint32_t)(way * DIMS) + lanes;
         const float turned = P.scale > 0.f ? 1.f : P.scale == 0.f ? 0.f : -1.f;   // maxima are of unscaled scores: they need a positive scale
         float sl2 = (P.scale == 0.f ? 1.f : fabsf(P.scale)) * 1.4426950408889634f;   // to log2 units
-        float *const say = told + (x * 2 + half) * 128 + r, *const hear = told + (x * 2 + (half ^ 1)) * 128 + r;
+        float *const say = told + (x * S::WAYS + way) * 128 + r;
+        auto heard = [&](int i) { return told[(x * S::WAYS + i) * 128 + r]; };
         const size_t row = (size_t)(token0 + q0 + min(ql, max(live - 1, 0)));
         const int q_head = head * P.group + head0 + r - ql * P.per_block;
         Q *const out0 = reinterpret_cast<Q *>(P.out) + (size_t)(token0 + q0) * P.out_stride + (size_t)(head * P.group + head0) * D;   // the block's first row
-        float m_ref = -INFINITY, l_run = 0.f, m_sums = 0.f;
-        float *const sums = sizeof(Q) != 4 ? nullptr : ranks > 1 ? P.sums + ((size_t)blockIdx.x * 256 + x * 128 + r) * D + half * DIMS
-                                                          : reinterpret_cast<float *>(out0 + (size_t)ql * P.out_stride + (size_t)(r - ql * P.per_block) * D + half * DIMS);
-        bool summed = false;
+        float m_ref = -INFINITY, l_run = 0.f, m_sums = -INFINITY;
+        float sums[S::TERMS == 2 ? DIMS : 1];   // f32 sums of the outputs up to the last flush, in units of 2^m_sums
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(sums) / 4); i++) sums[i] = 0.f;
+        // the output in tensor memory, in units of 2^m_ref, joins the sums (nothing seen yet: of no weight)
+        auto collect = [&]() {
+            if constexpr (S::TERMS == 2) {
+                const float old = exp2f(m_sums - (m_ref == -INFINITY ? 0.f : m_ref));
+                uint32_t v[DIMS];
+                pp_tmem_ld(t_o, v);
+#pragma unroll
+                for (int i = 0; i < DIMS; i++) sums[i] = fmaf(sums[i], old, __uint_as_float(v[i]));
+                m_sums = m_ref;
+            }
+        };
         for (int t = 0; t < mine; t++) {
-            ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (uint32_t)(t & 1)));
-            if (!ok) {   // the other half's warp meets this one in every tile, whatever has failed
-                both();
+            ok = ok && __all_sync(0xffffffffu, passed(s_full, x, t));
+            if (!ok) {   // a row's warps meet in every tile, whatever has failed
+                meet();
                 continue;
             }
             pg_fence_after();
-            static_assert(KEYS == 64, "columns per load");
             uint32_t s[KEYS];
-            pat_tmem_ld64(t_s + (uint32_t)(half * KEYS), s);
-            if constexpr (S::SHARED) {   // the other block's turn
+            pp_tmem_ld(tmem + S::scores_at(t) + lanes + (uint32_t)(way * KEYS), s);
+            if constexpr (S::TURNS) {   // the other block's turn
                 pg_fence_before();
                 __syncwarp();
                 if (lane == 0) pg_arrive(s_free);
@@ -323,7 +344,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
 #pragma unroll
                 for (int i = 0; i < KEYS; i++) s[i] = __float_as_uint(__uint_as_float(s[i]) * turned);
             }
-            const int k0 = seen.start(t0 + t) + half * KEYS;
+            const int k0 = seen.start(t0 + t) + way * KEYS;
             if (!(k0 + KEYS - 1 <= pos0 && (P.window == 0 || k0 > pos1 - P.window || k0 + KEYS <= P.sinks))) {
                 // keys a .. z of these, and those before the end of the sinks
                 const int z = pos - k0, a = P.window ? pos - P.window + 1 - k0 : 0, k = P.sinks - k0;
@@ -341,15 +362,27 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             for (int j = 0; j < 4; j++) mxs[j] = __uint_as_float(s[j]);
 #pragma unroll
             for (int i = 4; i < KEYS; i++) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(s[i]));
-            float top = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
-            if constexpr (PP_WAYS > 1) {   // the other half's; once both have their scores, probabilities may take the scores' place
-                *say = top;
-                pg_fence_before();
-                both();
-                pg_fence_after();
-                top = fmaxf(top, *hear);
-            }
+            // the row's maximum; once all its threads have their scores, probabilities may take the scores' place
+            *say = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
+            pg_fence_before();
+            meet();
+            pg_fence_after();
+            float top = heard(0);
+#pragma unroll
+            for (int i = 1; i < S::WAYS; i++) top = fmaxf(top, heard(i));
             const float mx = top * sl2;
+            // the product before this one is through, the output stands
+            bool waited = t == 0;
+            auto through = [&]() {
+                if (!waited) ok = ok && __all_sync(0xffffffffu, passed(pv_done, x, t - 1));
+                waited = true;
+                pg_fence_after();
+            };
+            const bool flush = S::TERMS == 2 && t > 0 && t % PP_FLUSH == 0;   // the next product starts from zero
+            if (flush) {
+                through();
+                collect();
+            }
             float corr = 1.f;
             if (mx > m_ref + PP_GROWTH || m_ref == -INFINITY) {
                 const float m_new = fmaxf(mx, m_ref);
@@ -357,98 +390,67 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 m_ref = m_new;
             }
             const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-            const bool flush = sizeof(Q) == 4 && t > 0 && t % PP_FLUSH == 0;
-            // the product before this one is through: with scores in their probabilities' place that is said already
-            auto through = [&]() {
-                if (S::SHARED && t > 0) {
-                    ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[x], (uint32_t)((t - 1) & 1)));
-                    pg_fence_after();
-                }
-            };
-            if (flush) {
+            if (t > 0 && !flush && __any_sync(0xffffffffu, corr != 1.f)) {
                 through();
-                // the tiles' sum so far joins the f32 sums; the next product starts from zero
-                const float old = summed ? exp2f(m_sums - m_use) : 0.f;
+                constexpr int SOME = DIMS < 32 ? DIMS : 32;
 #pragma unroll 1
-                for (int k = 0; k < DIMS / 32; k++) {
-                    uint32_t v[32];
-                    pg_tmem_ld32(t_o + (uint32_t)k * 32u, v);
-                    if (alive) {
+                for (int k = 0; k < DIMS; k += SOME) {
+                    uint32_t v[SOME];
+                    pp_tmem_ld(t_o + (uint32_t)k, v);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            float4 *const at = reinterpret_cast<float4 *>(sums + k * 32 + i);
-                            const float4 a = summed ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
-                            *at = make_float4(fmaf(a.x, old, __uint_as_float(v[i]) * corr), fmaf(a.y, old, __uint_as_float(v[i + 1]) * corr),
-                                              fmaf(a.z, old, __uint_as_float(v[i + 2]) * corr), fmaf(a.w, old, __uint_as_float(v[i + 3]) * corr));
-                        }
-                    }
-                }
-                summed = true;
-                m_sums = m_use;
-            } else if (t > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-                through();
-#pragma unroll 1
-                for (int k = 0; k < DIMS / 32; k++) {
-                    uint32_t v[32];
-                    pg_tmem_ld32(t_o + (uint32_t)k * 32u, v);
-#pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
-                    pat_tmem_st32(t_o + (uint32_t)k * 32u, v);
+                    for (int i = 0; i < SOME; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
+                    pp_tmem_st(t_o + (uint32_t)k, v);
                 }
             }
             __syncwarp();
             const uint64_t sl22 = pg_pair_f32(sl2, sl2), nm2 = pg_pair_f32(PP_BIAS - m_use, PP_BIAS - m_use);
             uint64_t sum[2] = {0, 0};
+            uint32_t hi[KEYS / 2], lo[KEYS / 2];   // columns of a term
 #pragma unroll
-            for (int part = 0; part < S::PARTS; part++) {
-                constexpr int PAIRS = KEYS / 2 / S::PARTS;   // columns of a term
-                uint32_t hi[PAIRS], lo[PAIRS];
-#pragma unroll
-                for (int i = 0; i < PAIRS; i++) {
-                    const float2 y = pat_fma2(__uint_as_float(s[2 * (part * PAIRS + i)]), __uint_as_float(s[2 * (part * PAIRS + i) + 1]), sl22, nm2);
-                    const float p0 = pat_exp2(y.x), p1 = pat_exp2(y.y);
-                    pat_add2(sum[i & 1], p0, p1);
-                    if constexpr (S::TERMS == 2) pp_cut<C>(p0, p1, hi[i], lo[i]);
-                    else hi[i] = pk_pack<C>(p0, p1);
-                }
-                if (part == 0) through();
-                if (!ok) continue;
-                const uint32_t to = t_p + (uint32_t)(half * (KEYS / 2) + part * PAIRS);
+            for (int i = 0; i < KEYS / 2; i++) {
+                const float2 y = pat_fma2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), sl22, nm2);
+                const float p0 = pat_exp2(y.x), p1 = pat_exp2(y.y);
+                pat_add2(sum[i & 1], p0, p1);
+                if constexpr (S::TERMS == 2) pp_cut<C>(p0, p1, hi[i], lo[i]);
+                else hi[i] = pk_pack<C>(p0, p1);
+            }
+            if (S::TURNS) through();   // (a buffer's own product was through before its scores came)
+            if (ok) {
+                const uint32_t to = tmem + S::probabilities_at(x, t) + lanes + (uint32_t)(way * (KEYS / 2));
                 pp_tmem_st(to, hi);
                 if constexpr (S::TERMS == 2) pp_tmem_st(to + 64u, lo);
                 pat_tmem_st_wait();
                 pg_fence_before();
                 __syncwarp();
-                if (lane == 0) pg_arrive(&p_full[2 * x + part]);
+                if (lane == 0) pg_arrive(of_tile(p_full, x, t));
             }
             l_run = fmaf(l_run, corr, pat_total(sum[0], sum[1]));
         }
-        if (ok && mine > 0) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[x], (uint32_t)((mine - 1) & 1)));
+        if (ok && mine > 0) ok = __all_sync(0xffffffffu, passed(pv_done, x, mine - 1));
         pg_fence_after();
         // ---- the row's end ----
-        if constexpr (PP_WAYS > 1) {
-            both();
-            *say = l_run;
-            both();
-            l_run += *hear;
-        }
-        const float m_use = m_ref == -INFINITY ? 0.f : m_ref, old = summed ? exp2f(m_sums - m_use) : 0.f;
-        auto output = [&](int k, float (&o)[32]) {   // unscaled, dims 32 k .. of this thread's half
-            if (mine > 0 && ok) {
-                uint32_t v[32];
-                pg_tmem_ld32(t_o + (uint32_t)k * 32u, v);
+        meet();
+        *say = l_run;
+        meet();
+        l_run = heard(0);
 #pragma unroll
-                for (int i = 0; i < 32; i++) o[i] = __uint_as_float(v[i]);
-                if (summed && alive) {
+        for (int i = 1; i < S::WAYS; i++) l_run += heard(i);
+        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+        if (S::TERMS == 2 && mine > 0 && ok) collect();
+        constexpr int SOME = DIMS < 32 ? DIMS : 32;
+        auto output = [&](int k, float (&o)[SOME]) {   // unscaled, dims SOME * k .. of this thread's
+            if constexpr (S::TERMS == 2) {
+                static_assert(S::TERMS == 1 || DIMS == SOME, "all of them");
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 a = *reinterpret_cast<const float4 *>(sums + k * 32 + i);
-                        o[i] = fmaf(a.x, old, o[i]), o[i + 1] = fmaf(a.y, old, o[i + 1]), o[i + 2] = fmaf(a.z, old, o[i + 2]), o[i + 3] = fmaf(a.w, old, o[i + 3]);
-                    }
-                }
+                for (int i = 0; i < SOME; i++) o[i] = sums[i];
+            } else if (mine > 0 && ok) {
+                uint32_t v[SOME];
+                pp_tmem_ld(t_o + (uint32_t)(k * SOME), v);
+#pragma unroll
+                for (int i = 0; i < SOME; i++) o[i] = __uint_as_float(v[i]);
             } else {
 #pragma unroll
-                for (int i = 0; i < 32; i++) o[i] = 0.f;
+                for (int i = 0; i < SOME; i++) o[i] = 0.f;
             }
         };
         auto store4 = [](Q *to, float a, float b2, float c2, float d) {
@@ -456,10 +458,10 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             else *reinterpret_cast<uint2 *>(to) = make_uint2(pk_pack<Q>(a, b2), pk_pack<Q>(c2, d));
         };
         if (ranks == 1) {
-            // BYTES of every row (of its half) at a time through shared memory, where the queries were, so that a few lanes store a row's
+            // BYTES of this thread's part of every row at a time through shared memory, where the queries were, so that a few lanes store a row's
             constexpr int BYTES = DIMS * (int)sizeof(Q) < 128 ? DIMS * (int)sizeof(Q) : 128, COLS = BYTES / (int)sizeof(Q), LANES = BYTES / 16;
-            uint8_t *const box = q_smem + (half * 4 + w) * (S::TERMS * S::PANELS * PP_PANEL / (4 * PP_WAYS));
-            static_assert(32 * BYTES <= S::TERMS * S::PANELS * PP_PANEL / (4 * PP_WAYS), "a box per warp");
+            uint8_t *const box = q_smem + (way * 4 + w) * (S::TERMS * S::PANELS * PP_PANEL / (4 * S::WAYS));
+            static_assert(32 * BYTES <= S::TERMS * S::PANELS * PP_PANEL / (4 * S::WAYS), "a box per warp");
             const float inv = l_run > 0.f ? 1.f / l_run : l_run != l_run ? l_run : 0.f;
             const uint64_t inv2 = pg_pair_f32(inv, inv);
             uint64_t check = 0;   // stays zero while all are finite
@@ -467,11 +469,11 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             for (int k = 0; k < DIMS / COLS; k++) {
                 __syncwarp();   // a row's sums are read by now, and what was stored out of the box
 #pragma unroll
-                for (int j = 0; j < COLS / 32; j++) {
-                    float o[32];
-                    output(k * (COLS / 32) + j, o);
+                for (int j = 0; j < COLS / SOME; j++) {
+                    float o[SOME];
+                    output(k * (COLS / SOME) + j, o);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 16 / (int)sizeof(Q)) {
+                    for (int i = 0; i < SOME; i += 16 / (int)sizeof(Q)) {
                         uint32_t v[4];
 #pragma unroll
                         for (int e = 0; e < 16 / (int)sizeof(Q); e += 2) {
@@ -484,7 +486,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                                 v[e / 2] = pk_pack<Q>(y.x, y.y);
                             }
                         }
-                        const int ch = (j * 32 + i) * (int)sizeof(Q) / 16;
+                        const int ch = (j * SOME + i) * (int)sizeof(Q) / 16;
                         *reinterpret_cast<uint4 *>(box + lane * BYTES + ((ch ^ (lane & (LANES - 1))) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
                     }
                 }
@@ -494,32 +496,32 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                     const int rr = (32 / LANES) * i + lane / LANES, ch = lane % LANES, R = w * 32 + rr, rq = query_of(R), h = R - rq * P.per_block;
                     const uint4 y = *reinterpret_cast<const uint4 *>(box + rr * BYTES + ((ch ^ (rr & (LANES - 1))) << 4));
                     if (rq < live && h < heads_here && ok)
-                        *reinterpret_cast<uint4 *>(out0 + (size_t)rq * P.out_stride + (size_t)h * D + half * DIMS + k * COLS + ch * (16 / (int)sizeof(Q))) = y;
+                        *reinterpret_cast<uint4 *>(out0 + (size_t)rq * P.out_stride + (size_t)h * D + way * DIMS + k * COLS + ch * (16 / (int)sizeof(Q))) = y;
                 }
             }
             const bool strange = alive && ok && !((uint32_t)check << 1 == 0 && (uint32_t)(check >> 32) << 1 == 0);
-            if (alive && ok && half == 0 && P.lse) P.lse[row * P.heads + q_head] = l_run > 0.f ? (m_use - PP_BIAS + log2f(l_run)) * 0.6931471805599453f : l_run != l_run ? l_run : -INFINITY;
+            if (alive && ok && way == 0 && P.lse) P.lse[row * P.heads + q_head] = l_run > 0.f ? (m_use - PP_BIAS + log2f(l_run)) * 0.6931471805599453f : l_run != l_run ? l_run : -INFINITY;
             if (strange) atomicOr(&todo[x * 4 + w], 1u << lane);
             __syncwarp();
-            both();
+            meet();
         } else {
             // ---- a cluster's shares: outputs, maxima and sums in shared memory, where the tiles were ----
             if (!ok) *failed = 1;
             asm volatile("bar.sync 9, %0;" ::"n"(32 * PP_SOFTMAX_WARPS) : "memory");   // both blocks' products are through (each block's warps have waited for its own)
-            float *const o_all = reinterpret_cast<float *>(pp_smem), *const ml = o_all + 256 * (D + 4);
+            float *const o_all = reinterpret_cast<float *>(pp_smem), *const ml = o_all + S::ROWS * (D + 4);
 #pragma unroll 1
-            for (int k = 0; k < DIMS / 32; k++) {
-                float o[32];
+            for (int k = 0; k < DIMS / SOME; k++) {
+                float o[SOME];
                 output(k, o);
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4 *>(o_all + (x * 128 + r) * (D + 4) + half * DIMS + k * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                for (int i = 0; i < SOME; i += 4) *reinterpret_cast<float4 *>(o_all + (x * 128 + r) * (D + 4) + way * DIMS + k * SOME + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             }
-            if (half == 0) *reinterpret_cast<float2 *>(ml + 2 * (x * 128 + r)) = make_float2(m_ref, ok ? l_run : 0.f);
+            if (way == 0) *reinterpret_cast<float2 *>(ml + 2 * (x * 128 + r)) = make_float2(m_ref, ok ? l_run : 0.f);
             __syncwarp();
             ps_cluster_sync();
             // this CTA joins rows [rank * n, (rank + 1) * n)
-            const int n = 256 / (int)ranks;
-            float *const weights = ml + 512, *const joined = weights + 256 * PP_MAX_CLUSTER;
+            const int n = S::ROWS / (int)ranks;
+            float *const weights = ml + 2 * S::ROWS, *const joined = weights + S::ROWS * PP_MAX_CLUSTER;
             const uint32_t o_addr = smem_u32(o_all), ml_addr = smem_u32(ml);
             if (tid < n) {
                 const int R = (int)rank * n + tid;
@@ -570,8 +572,8 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             ps_cluster_sync();
         }
         // ---- rows that came out infinite or undefined, one by one ----
-        const int step = ranks == 1 ? 1 : PP_SOFTMAX_WARPS, row0 = ranks == 1 ? x * 128 + w * 32 : (int)rank * (256 / (int)ranks) + warp;
-        for (unsigned left = ranks > 1 ? todo[warp] : half == 0 ? todo[x * 4 + w] : 0; left; left &= left - 1) {
+        const int step = ranks == 1 ? 1 : PP_SOFTMAX_WARPS, row0 = ranks == 1 ? x * 128 + w * 32 : (int)rank * (S::ROWS / (int)ranks) + warp;
+        for (unsigned left = ranks > 1 ? todo[warp] : way == 0 ? todo[x * 4 + w] : 0; left; left &= left - 1) {
             const int R = row0 + (__ffs(left) - 1) * step, bx = R >> 7, rq = query_of(R & 127), h = head * P.group + head0 + (R & 127) - rq * P.per_block;
             const size_t token = (size_t)(token0 + first + bx * P.queries + rq);
             pk_plain_row<Q, C, D>(c, b, reinterpret_cast<const Q *>(P.q) + token * P.q_stride + (size_t)h * D, seq, shift + first + bx * P.queries + rq, head, P.scale, P.window,
@@ -588,7 +590,8 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             auto scores = [&](int x, int t) {
                 // their columns are free: the other block has read its scores, or the probabilities in them have been multiplied (nothing but its end orders a
                 // product behind one that reads what it overwrites)
-                ok = arrived(2 * t) && (S::SHARED ? turns == 0 || mbar_wait_bounded(s_free, (turns - 1) & 1u) : t == 0 || mbar_wait_bounded(&pv_done[x], (uint32_t)((t - 1) & 1)));
+                ok = arrived(2 * t) && (S::TURNS ? turns == 0 || mbar_wait_bounded(s_free, (turns - 1) & 1u)
+                                                 : t < S::BUFFERS || passed(pv_done, x, t - S::BUFFERS));
                 turns++;
                 if (!ok) return;
                 pg_fence_after();
@@ -600,47 +603,43 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                     for (int p = 0; p < S::PANELS; p++) {
                         const uint64_t dq = pg_smem_desc(base + (uint32_t)((x * S::TERMS + term) * S::PANELS + p) * PP_PANEL), dk = pg_smem_desc(kt + (uint32_t)p * PP_PANEL);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) ps_mma(tmem + S::scores_at(x), dq + 2u * k, dk + 2u * k, pp_idesc<C>(128, false), (S::TERMS - 1 - term) | p | k);
+                        for (int k = 0; k < 4; k++) ps_mma(tmem + S::scores_at(t), dq + 2u * k, dk + 2u * k, pp_idesc<C>(128, false), (S::TERMS - 1 - term) | p | k);
                     }
-                pg_commit(&s_full[x]);
+                pg_commit(of_tile(s_full, x, t));
                 if (x == last) pg_commit(&empty[slot]);
             };
             auto outputs = [&](int x, int t, int mine, int slot) {
+                ok = passed(p_full, x, t);
+                if (!ok) return;
+                pg_fence_after();
                 const uint64_t dv = pp_v_desc(ring + (uint32_t)slot * S::TILE_BYTES);
-                const uint32_t tp = tmem + S::probabilities_at(x), to = tmem + S::outputs_at(x);
+                const uint32_t tp = tmem + S::probabilities_at(x, t), to = tmem + S::outputs_at(x);
                 const uint32_t more = t > 0 && !(S::TERMS == 2 && t % PP_FLUSH == 0);
 #pragma unroll
-                for (int part = 0; part < S::PARTS; part++) {
-                    ok = mbar_wait_bounded(&p_full[2 * x + part], (uint32_t)(t & 1));
-                    if (!ok) return;
-                    pg_fence_after();
-#pragma unroll
-                    for (int i = 0; i < 8 / S::PARTS; i++) {   // 16 keys: 2048 bytes of a panel of V, eight columns of probabilities
-                        constexpr int RUN = 8 / S::PARTS / PP_WAYS;   // of one half's part
-                        const int k = i / RUN * (8 / PP_WAYS) + part * RUN + i % RUN;
-                        pat_mma_ta(to, tp + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), more | (uint32_t)((part | i) != 0));
-                        if constexpr (S::TERMS == 2) pat_mma_ta(to, tp + 64u + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), 1u);
-                    }
+                for (int k = 0; k < PP_KEYS / 16; k++) {   // 16 keys: 2048 bytes of a panel of V, eight columns of probabilities
+                    pat_mma_ta(to, tp + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), more | (uint32_t)(k != 0));
+                    if constexpr (S::TERMS == 2) pat_mma_ta(to, tp + 64u + 8u * k, dv + (uint64_t)(k * (2048 >> 4)), pp_idesc<C>(D, true), 1u);
                 }
-                pg_commit(&pv_done[x]);
+                pg_commit(of_tile(pv_done, x, t));
                 if (x == last) pg_commit(&empty[slot]);
             };
-            for (int x = 0; x < 2 && ok; x++) {
+            constexpr int AHEAD = S::BLOCKS == 2 ? 1 : S::BUFFERS - 1;   // tiles whose scores are under way before a product of probabilities
+            for (int x = 0; x < S::BLOCKS && ok; x++) {
                 if ((x ? n_b : n_a) == 0) continue;
                 ok = mbar_wait_bounded(&q_full[x], 0u);
-                if (ok) scores(x, 0);
+                for (int t = 0; t < AHEAD && t < (x ? n_b : n_a) && ok; t++) scores(x, t);
             }
             for (int t = 0; t < n_tiles && ok; t++) {
                 const int slot = (2 * t + 1) % S::SLOTS;
-                for (int x = 0; x < 2 && ok; x++) {
+                for (int x = 0; x < S::BLOCKS && ok; x++) {
                     const int mine = x ? n_b : n_a;
-                    // in columns of their own the scores go first; in the probabilities' they have to wait for these to be read
-                    if (S::SHARED && t + 1 < mine) scores(x, t + 1);
+                    if (S::TURNS && t + AHEAD < mine) scores(x, t + AHEAD);
                     if (ok && t < mine) {
                         if (x == 0 || n_a <= t) ok = mbar_wait_bounded(&cleared[t & 7], (uint32_t)(t >> 3) & 1u) && arrived(2 * t + 1);
                         if (ok) outputs(x, t, mine, slot);
                     }
-                    if (!S::SHARED && ok && t + 1 < mine) scores(x, t + 1);
+                    // (behind the product: a flush waits for that one)
+                    if (!S::TURNS && ok && t + AHEAD < mine) scores(x, t + AHEAD);
                 }
             }
         }
