@@ -770,7 +770,7 @@ int rnb_b200_attention_decode_hd128_noalloc_status(int *status_out, void *stream
  * outside the pool; what the call writes for such a sequence is then not to be used.  Entries of pages
  * that no query sees are not read and may hold anything. */
 #define RNB_B200_DEVICE_BAD_PAGE 5
-#define RNB_B200_DEVICE_BAD_WORKSPACE 6 /* attention with a workspace that was not initialised: nothing is written */
+#define RNB_B200_DEVICE_BAD_WORKSPACE 6 /* decode attention with a workspace that was not initialised: nothing is written */
 typedef struct {
     uint32_t type;      /* RNB_B200_TYPE_F16 or _BF16 */
     int32_t head_dim;   /* a multiple of 8 up to 512; attention: 64 or 128 */
@@ -790,7 +790,7 @@ typedef struct {
     const int32_t *kv_len;  /* [n_seq] positions in the cache, the call's own tokens included; 0: none */
     /* [n_seq + 1] first row of every sequence's tokens, from 0 and not descending; null: row i is the one token of
      * sequence i.  The last tokens of a sequence's kv_len positions are the call's; rows from
-     * q_start[n_seq] on are padding: not read, and left as they are in outputs */
+     * q_start[n_seq] on are padding: without effect, and left as they are in outputs */
     const int32_t *q_start;
 } rnb_b200_paged_batch;
 /* K and V rows of the call's tokens to their places in the pages, rounded to the cache's type (to nearest,
@@ -811,11 +811,12 @@ int rnb_b200_dev_paged_kv_copy(const rnb_b200_paged_cache *cache, size_t n_layer
  * F16 cache, or the cache's type; `out` has the same type.  Sums, maxima and the softmax are f32, and f32 queries
  * keep f32 accuracy (queries and probabilities enter the products as two f16 terms).  q, out
  * [n_tokens][heads][head_dim], 16-byte aligned, q_stride / out_stride elements from one token to the next
- * (multiples of 8); heads a multiple of kv_heads.  lse (may be null): f32 [n_tokens][heads], the logarithm of
+ * (multiples of 8), that do not overlap; heads a multiple of kv_heads.  lse (may be null): f32 [n_tokens][heads], the logarithm of
  * the sum of exponentials, -inf for a query that sees nothing.
  * `workspace`: rnb_b200_paged_workspace_bytes() bytes, 256-byte aligned, initialised once by
  * rnb_b200_paged_workspace_init; one workspace serves any number of calls one after another (of any sizes, of both
- * calls, of captured graphs), but calls that may overlap on the GPU need one each.
+ * calls, of captured graphs), but calls that may overlap on the GPU need one each.  Decode keeps parts of long
+ * sequences there until they are joined; _prefill checks the argument and joins on the chip.
  * _decode: one new token per sequence (q_start null), the work split over the lengths so that few sequences
  * use the whole GPU too.  _prefill: the tokens of every sequence, causal. */
 size_t rnb_b200_paged_workspace_bytes(void);

@@ -157,6 +157,16 @@ constexpr size_t PK_WORKSPACE_BYTES = PD_WS_RECORDS + (size_t)PK_MAX_SMS * 2 * s
                                                                                          PdShape<128, 1>::PER_SM * PdShape<128, 1>::RECORD, PdShape<128, 2>::PER_SM * PdShape<128, 2>::RECORD});
 static_assert(PD_WS_RECORDS % 256 == 0, "records are read by 16 bytes");
 
+// Whether two matrices share bytes: their ranges do, unless their rows lie beside each other in rows of one length.  strides in elements.
+static bool pk_rows_meet(const void *x, size_t x_stride, const void *y, size_t y_stride, size_t row, size_t rows, size_t element) {
+    const uintptr_t a = (uintptr_t)x, b = (uintptr_t)y;
+    const size_t xs = x_stride * element, ys = y_stride * element;
+    if (a + (rows - 1) * xs + row <= b || b + (rows - 1) * ys + row <= a) return false;
+    if (xs != ys || rows == 1) return true;
+    const size_t d = a > b ? (a - b) % xs : (b - a) % xs;
+    return d < row || xs - d < row;
+}
+
 static int pk_check_attention(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type, const void *q, size_t q_stride, size_t num_heads,
                               float scale, int32_t window, int32_t sinks, void *workspace, size_t workspace_bytes, void *out, size_t out_stride, float *lse, PkAttention *a) {
     RNB_TRY(pk_check_cache(cache, &a->c));
@@ -175,6 +185,8 @@ static int pk_check_attention(const rnb_b200_paged_cache *cache, const rnb_b200_
         return fail(RNB_B200_VALIDATION_FAILED, "paged attention: q and out must be 16-byte aligned with strides that are multiples of 8, lse 4-byte aligned");
     if (a->b.n_tokens > 1 && (q_stride < num_heads * cache->head_dim || out_stride < num_heads * cache->head_dim))
         return fail(RNB_B200_VALIDATION_FAILED, "paged attention: q_stride and out_stride must be at least num_heads * head_dim");
+    if (a->b.n_tokens > 0 && pk_rows_meet(q, q_stride, out, out_stride, num_heads * cache->head_dim * (q_type == RNB_B200_TYPE_F32 ? 4 : 2), (size_t)a->b.n_tokens, q_type == RNB_B200_TYPE_F32 ? 4 : 2))
+        return fail(RNB_B200_VALIDATION_FAILED, "paged attention: q and out must not overlap");
     a->q_type = q_type;
     a->c_type = cache->type;
     a->q = q;

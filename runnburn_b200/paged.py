@@ -24,7 +24,7 @@ import numpy as np
 from . import _lib
 from ._lib import TYPE_BF16, TYPE_F16, TYPE_F32, check, load
 
-DEVICE_BAD_PAGE = 5
+DEVICE_BAD_PAGE, DEVICE_BAD_WORKSPACE = 5, 6   # what ops.dev_error_flag() tells of a call
 
 _types: dict = {}
 

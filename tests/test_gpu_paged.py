@@ -305,6 +305,35 @@ def test_what_points_outside_is_flagged(P, ws, new, kv):
         assert worst(got[:m], out[:m], tolerance(out, mass, got.dtype)[:m]) <= 1
 
 
+def test_a_workspace_that_was_not_initialised_is_flagged(P, ws):
+    """And nothing is written, to it or to the output; one that was initialised then serves."""
+    import torch
+    from runnburn_b200 import ops
+    c, bare = Case(P, [3000, 5, 0, 700]), P.Workspace()
+    bare.buffer.zero_()
+    out = torch.full_like(c.q, 3.0)
+    c.run(bare, out=out)
+    torch.cuda.synchronize()
+    assert ops.dev_error_flag() == P.DEVICE_BAD_WORKSPACE
+    assert bool((out == 3.0).all()) and bool((c.lse == 7.0).all()) and int(bare.buffer.count_nonzero()) == 0
+    c.check(c.run(ws, out=out))
+
+
+def test_streams_side_by_side(P):
+    """Calls on streams of their own, with a workspace each, that overlap as they like."""
+    import torch
+    cases = [Case(P, [20000, 9], seed=1), Case(P, [5, 9000, 0, 300], q="bf16", cache="bf16", dim=64, seed=2), Case(P, [900, 40], [700, 3], seed=3)]
+    streams, spaces = [torch.cuda.Stream() for _ in cases], [P.Workspace() for _ in cases]
+    torch.cuda.synchronize()
+    outs = [[c.run(w, stream=s) for c, s, w in zip(cases, streams, spaces)] for _ in range(4)]
+    torch.cuda.synchronize()
+    for turn in outs:
+        for c, out, first in zip(cases, turn, outs[0]):
+            assert torch.equal(out, first)
+    for c, out in zip(cases, outs[0]):
+        c.check(out)
+
+
 def test_offsets_past_32_bits(P, ws):
     """Pages 2^31 elements and more apart."""
     import torch

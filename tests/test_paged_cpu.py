@@ -195,7 +195,7 @@ BAD_BATCH = [
 ]
 
 
-def attend(L, c, b, q_type=0, q=ADDRESS, q_stride=512, heads=4, scale=0.1, window=0, sinks=0, ws=ADDRESS, ws_bytes=None, out=ADDRESS, out_stride=512, lse=None, prefill=False):
+def attend(L, c, b, q_type=0, q=ADDRESS, q_stride=512, heads=4, scale=0.1, window=0, sinks=0, ws=ADDRESS, ws_bytes=None, out=ADDRESS + (1 << 20), out_stride=512, lse=None, prefill=False):
     fn = L.rnb_b200_dev_attention_prefill_paged if prefill else L.rnb_b200_dev_attention_decode_paged
     n = L.rnb_b200_paged_workspace_bytes() if ws_bytes is None else ws_bytes
     return fn(C.byref(c) if c else None, C.byref(b) if b else None, q_type, q, q_stride, heads, scale, window, sinks, ws, n, out, out_stride, lse, None)
@@ -232,6 +232,17 @@ def test_attention_refuses(r, kw, status, what):
     L = r.load()
     for prefill in (False, True):
         refused(L, attend(L, cache(r), batch(r), prefill=prefill, **kw), status, what)
+
+
+@pytest.mark.parametrize("tokens,q_stride,out_stride,shift,ok", [
+    (2, 512, 512, 0, False), (2, 512, 512, 2048, False), (2, 512, 512, 4096, True), (2, 512, 512, -4096, True), (2, 512, 512, -4080, False), (1, 512, 512, 2048, True),
+    (1, 512, 512, 2032, False), (5, 1024, 1024, 2048, True), (5, 1024, 1024, -2048, True), (5, 1024, 1024, 2064, False), (5, 1024, 1024, 4096 * 3 + 2048, True),
+    (5, 1024, 1024, 2032, False), (5, 1024, 1032, 2048, False), (5, 1536, 1536, 2064, True), (5, 1536, 1536, 4112, False)])
+def test_queries_and_outputs_must_not_overlap(r, tokens, q_stride, out_stride, shift, ok):
+    """Rows of 4 * 128 f32, side by side in one matrix or apart; what is let through stops at the next check, the one for a sequence's one token."""
+    L, base = r.load(), ADDRESS + (1 << 20)
+    rc = attend(L, cache(r), batch(r, n_seq=tokens, n_tokens=tokens, q_start=ADDRESS), q=base, out=base + shift, q_stride=q_stride, out_stride=out_stride)
+    refused(L, rc, 2, "q_start" if ok else "overlap")
 
 
 def test_calls_refuse_what_only_they_can_see(r):
