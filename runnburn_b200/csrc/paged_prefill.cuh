@@ -314,15 +314,15 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
         float sums[S::TERMS == 2 ? DIMS : 1];   // f32 sums of the outputs up to the last flush, in units of 2^m_sums
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(sums) / 4); i++) sums[i] = 0.f;
-        // the output in tensor memory, in units of 2^m_ref, joins the sums (nothing seen yet: of no weight)
-        auto collect = [&]() {
+        // the output in tensor memory, in units of 2^m, joins the sums (nothing seen yet: of no weight)
+        auto collect = [&](float m) {
             if constexpr (S::TERMS == 2) {
-                const float old = exp2f(m_sums - (m_ref == -INFINITY ? 0.f : m_ref));
+                const float old = exp2f(m_sums - (m == -INFINITY ? 0.f : m));
                 uint32_t v[DIMS];
                 pp_tmem_ld(t_o, v);
 #pragma unroll
                 for (int i = 0; i < DIMS; i++) sums[i] = fmaf(sums[i], old, __uint_as_float(v[i]));
-                m_sums = m_ref;
+                m_sums = m;
             }
         };
         for (int t = 0; t < mine; t++) {
@@ -379,10 +379,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 pg_fence_after();
             };
             const bool flush = S::TERMS == 2 && t > 0 && t % PP_FLUSH == 0;   // the next product starts from zero
-            if (flush) {
-                through();
-                collect();
-            }
+            const float m_before = m_ref;
             float corr = 1.f;
             if (mx > m_ref + PP_GROWTH || m_ref == -INFINITY) {
                 const float m_new = fmaxf(mx, m_ref);
@@ -419,6 +416,12 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 const uint32_t to = tmem + S::probabilities_at(x, t) + lanes + (uint32_t)(way * (KEYS / 2));
                 pp_tmem_st(to, hi);
                 if constexpr (S::TERMS == 2) pp_tmem_st(to + 64u, lo);
+            }
+            if (flush) {   // (as late as the product allows, which is under way until now)
+                through();
+                collect(m_before);
+            }
+            if (ok) {
                 pat_tmem_st_wait();
                 pg_fence_before();
                 __syncwarp();
@@ -436,7 +439,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
 #pragma unroll
         for (int i = 1; i < S::WAYS; i++) l_run += heard(i);
         const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-        if (S::TERMS == 2 && mine > 0 && ok) collect();
+        if (S::TERMS == 2 && mine > 0 && ok) collect(m_ref);
         constexpr int SOME = DIMS < 32 ? DIMS : 32;
         auto output = [&](int k, float (&o)[SOME]) {   // unscaled, dims SOME * k .. of this thread's
             if constexpr (S::TERMS == 2) {
