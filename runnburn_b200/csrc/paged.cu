@@ -292,6 +292,8 @@ static int pk_prefill(const PkAttention &a, cudaStream_t s, State &st) {
     P.out = a.out;
     P.lse = a.lse;
     P.err = st.dev_error;
+    P.by_vh = pp_by((uint32_t)(a.c.kv_heads * P.blocks));
+    P.by_rows = pp_by((uint32_t)(S::BLOCKS * P.queries));
     P.by_heads = (65536 + P.per_block - 1) / P.per_block;
     PpMaps maps{};
     RNB_TRY(pk_encode(&maps.k, a.c.k, a, PP_KEYS, 1));

@@ -63,6 +63,9 @@ struct PpParams {
     size_t q_stride, out_stride;
     int heads, group, blocks, per_block, queries, window, sinks;   // blocks of per_block heads per key head; queries of a row block
     uint32_t by_heads;   // 2^16 / per_block, rounded up: row / per_block = row * by_heads >> 16
+    // 2^64 / d, rounded up (d = 1: 0), for d = key heads * blocks and the queries of a CTA: x / d = x * by >> 64 for all 32-bit x.  (A division by what
+    // is only known now takes a CTA 100 to 200 cycles, and there were six on the way to its first tile.)
+    uint64_t by_vh, by_rows;
     float scale;
     void *out;
     float *lse;
@@ -108,6 +111,7 @@ __device__ __forceinline__ void pp_tma_4d(uint32_t dst, const PkTensorMap *map, 
                  ::"r"(dst), "l"(map), "r"(0), "r"(head), "r"(token), "r"(part), "r"(smem_u32(bar))
                  : "memory");
 }
+__device__ __forceinline__ void pp_prefetch_map(const PkTensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ float2 pp_mul2(float x, float y, uint64_t m) {
     float2 r;
     asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%2, %3};\n\tmul.rn.f32x2 t, t, %4;\n\tmov.b64 {%0, %1}, t;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(x), "f"(y), "l"(m));
@@ -126,6 +130,8 @@ template <class C>
 constexpr uint32_t pp_idesc(int n, bool b_mn_major) {
     return (1u << 4) | (std::is_same<C, Bf16>::value ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
+__host__ __device__ inline uint64_t pp_by(uint32_t d) { return d == 1 ? 0 : ~0ull / d + 1; }
+__device__ __forceinline__ unsigned pp_over(unsigned x, uint64_t by) { return by ? (unsigned)__umul64hi(x, by) : x; }
 // The tiles of PP_KEYS keys that queries see who see 0 .. sink - 1 and from .. len - 1.
 struct PpSeen {
     int len, from, sink, lead, skip, tiles;
@@ -150,6 +156,11 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     uint32_t rank, ranks;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    if (tid == PP_THREADS - 1) {   // (the first box of a launch waits for its map otherwise)
+        pp_prefetch_map(&maps.k);
+        pp_prefetch_map(&maps.v);
+        if (S::TERMS == 1) pp_prefetch_map(&maps.q);
+    }
     if (tid == 0) {
         for (int s = 0; s < S::SLOTS; s++) {
             mbar_init(&full[s], 1);
@@ -168,7 +179,9 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
         for (int i = 0; i < PP_SOFTMAX_WARPS; i++) todo[i] = 0;
     }
     pdl_wait();   // tensor memory too is asked for when no earlier launch can still hold it
-    const int VH = c.kv_heads * P.blocks, item = (int)(blockIdx.x / ranks), vh = item % VH, head = vh / P.blocks, head0 = (vh % P.blocks) * P.per_block;
+    const int to_ranks = 31 - __clz((int)ranks);   // a power of two
+    const int VH = c.kv_heads * P.blocks, item = (int)(blockIdx.x >> to_ranks), turn = (int)pp_over((unsigned)item, P.by_vh), vh = item - turn * VH;
+    const int head = P.blocks == 1 ? vh : vh / P.blocks, head0 = (vh - head * P.blocks) * P.per_block;
     // rows of a block: (query, head) = (row / per_block, row % per_block), by multiplication, exact for rows below 128; the last of several head blocks may have fewer heads
     const int heads_here = min(P.per_block, P.group - head0);
     auto query_of = [&](int row) { return (int)((uint32_t)row * P.by_heads >> 16); };
@@ -186,12 +199,12 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             v.n = max(0, min(to, b.n_tokens) - v.start);
             return v;
         };
-        auto pairs_of = [&](const Span &v) { return (v.n + S::BLOCKS * P.queries - 1) / (S::BLOCKS * P.queries); };
+        auto pairs_of = [&](const Span &v) { return (int)pp_over((unsigned)(v.n + S::BLOCKS * P.queries - 1), P.by_rows); };
         const Span first32 = span(lane);
         int total = pairs_of(first32);
         for (int s = lane + 32; s < b.n_seq; s += 32) total += pairs_of(span(s));
         total = __reduce_add_sync(0xffffffffu, total);
-        const int want = total - 1 - item / VH;
+        const int want = total - 1 - turn;
         if (lane == 0) found[0] = -1;
         __syncwarp();
         int before = 0;
@@ -245,7 +258,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     seen.skip = seen.from / PP_KEYS - seen.lead;
     seen.tiles = max(0, (seen.len + PP_KEYS - 1) / PP_KEYS - seen.skip);
     // this CTA's share of the tiles, and of these the ones that block a sees some of (block b is behind it and sees something of all)
-    const int per = (seen.tiles + (int)ranks - 1) / (int)ranks, t0 = min(seen.tiles, per * (int)rank), n_tiles = min(per, seen.tiles - t0);
+    const int per = (seen.tiles + (int)ranks - 1) >> to_ranks, t0 = min(seen.tiles, per * (int)rank), n_tiles = min(per, seen.tiles - t0);
     const int tiles_a = max(0, (shift + first + live_a + PP_KEYS - 1) / PP_KEYS - (shift + first + live_a > 0 ? seen.skip : 0));
     const int n_a = live_b > 0 ? min(max(tiles_a - t0, 0), n_tiles) : n_tiles, n_b = live_b > 0 ? n_tiles : 0;
 
