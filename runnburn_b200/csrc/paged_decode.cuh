@@ -21,7 +21,11 @@ namespace rnb {
 
 constexpr int PD_TILE = 64;
 constexpr float PD_BIAS = 12.f;
-constexpr int PD_MIN_TILES = 4;   // of a run: a cut costs a join
+// The shortest run, in tiles: a join reads one of n parts after the other, a tile takes about as long as the reading of 16, so runs of sqrt(tiles) / 4 are best
+// where there are CTAs enough.  32 heads on 8 key heads, 128 dims: 300 positions 7.0 us, 600 8.1, 1000 8.7 (with runs of four tiles 10.6, 10.5, 9.9);
+// 32768 positions of one key head 19.8 us (with the shortest that give all CTAs work 35.5).
+constexpr float PD_RUN = 0.25f;
+constexpr int PD_WHOLE = 3;   // tiles of a sequence that is not cut at all (180 positions: 6.4 us, cut 6.9; 250: 7.2, cut 7.0)
 constexpr size_t PD_WS_HEAD = 256;                      // a mark that the workspace has been initialised
 constexpr int PD_MAX_GRID = 1024;                       // runs of a launch
 constexpr size_t PD_WS_RECORDS = PD_WS_HEAD + PD_MAX_GRID * sizeof(unsigned);
@@ -139,8 +143,8 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
             most = max(most, n);
         }
         const unsigned units = (unsigned)__reduce_add_sync(0xffffffffu, sum) * VH;   // (the host has seen to it that this fits)
-        // short sequences are not cut, nor put behind one another while there are CTAs for each
-        const unsigned per = max((units + gridDim.x - 1) / gridDim.x, (unsigned)min(PD_MIN_TILES, __reduce_max_sync(0xffffffffu, most))), begin = per * blockIdx.x;
+        const int longest = __reduce_max_sync(0xffffffffu, most);
+        const unsigned per = max((units + gridDim.x - 1) / gridDim.x, longest <= PD_WHOLE ? (unsigned)longest : (unsigned)(sqrtf((float)longest) * PD_RUN + 1.f)), begin = per * blockIdx.x;
         if (begin < units) {   // the sequence that unit `begin` lies in
             unsigned before = 0;
             for (int r0 = 0;; r0 += 32) {

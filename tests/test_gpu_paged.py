@@ -334,6 +334,13 @@ def test_streams_side_by_side(P):
         c.check(out)
 
 
+def test_a_sequence_in_more_parts_than_a_join_has_weights_for(P, ws):
+    """One key head and so many tiles that every CTA of the launch leaves a part."""
+    for dim, heads in ((64, 2), (128, 5)):
+        c = Case(P, [64 * 15000 + 3], heads=heads, kv_heads=1, dim=dim, page=256, nan=False)
+        c.check(c.run(ws))
+
+
 def test_offsets_past_32_bits(P, ws):
     """Pages 2^31 elements and more apart."""
     import torch
