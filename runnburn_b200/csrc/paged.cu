@@ -307,11 +307,16 @@ static int pk_prefill(const PkAttention &a, cudaStream_t s, State &st) {
     const size_t pairs = std::min<size_t>((size_t)a.b.n_tokens, (size_t)a.b.n_tokens / (S::BLOCKS * P.queries) + (size_t)a.b.n_seq) * a.c.kv_heads * P.blocks;
     if (pairs > 0x7fffffffu) return fail(RNB_B200_UNSUPPORTED, "paged attention: %zu blocks of rows are more than a launch can have", pairs);
     // Keys are shared out where the launch leaves most of the chip idle, down to one tile of what a pair could see for each: a join costs less than a tile
-    // (33 tokens behind 300 positions: 14.0 us, without 16.5).
+    // (33 tokens of f32 behind 300 positions: 11.3 us, without 16.5).
     long long tiles = (((long long)a.b.max_pages << a.c.page_shift) + PP_KEYS - 1) / PP_KEYS;
     if (a.window) tiles = std::min(tiles, ((long long)a.window + a.sinks + S::BLOCKS * P.queries) / PP_KEYS + 3);
     unsigned ranks = 1;
     while (ranks < PP_MAX_CLUSTER && pairs * ranks * 2 <= (size_t)std::min(st.sm_count, PK_MAX_SMS) && tiles > (long long)ranks) ranks *= 2;
+    // Several sequences are seldom of one length, and the longest decides: where it takes longer than all SMs need for halves of everything, lengths spread
+    // evenly from nothing on and a CTA costing FIXED tiles' time beside its tiles, two share (3 sequences of up to 512 tokens behind up to 6000, 32 heads on 8:
+    // 70 us, without 92; 10 of up to 100: 55, without 83; 9 of up to 512, which the rule leaves alone: 145, without 118.  Four alike of 200: 106, without 98).
+    constexpr long long FIXED = 6;
+    if (ranks == 1 && a.b.n_seq > 2 && (long long)pairs * (tiles + 4 * FIXED) * 10 < 17 * (tiles + FIXED) * std::min(st.sm_count, PK_MAX_SMS)) ranks = 2;
     if (ranks == 1) RNB_CU(launch_k(paged_prefill_kernel<Q, C, D>, dim3((unsigned)pairs), dim3(PP_THREADS), S::SMEM, s, a.c, a.b, P, maps));
     else RNB_CU(launch_k_cluster(paged_prefill_kernel<Q, C, D>, dim3((unsigned)pairs * ranks), dim3(PP_THREADS), S::SMEM, s, dim3(ranks), a.c, a.b, P, maps));
     return RNB_B200_OK;

@@ -73,9 +73,9 @@ struct PpParams {
 };
 
 #ifdef __CUDACC__
-__device__ __forceinline__ float pp_ld_remote(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float2 pp_ld_remote2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ float4 pp_ld_remote4(uint32_t addr) {
@@ -541,49 +541,67 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             const uint32_t o_addr = smem_u32(o_all), ml_addr = smem_u32(ml);
             if (tid < n) {
                 const int R = (int)rank * n + tid;
-                float m[PP_MAX_CLUSTER], l[PP_MAX_CLUSTER], M = -INFINITY, L = 0.f;
+                float2 y[PP_MAX_CLUSTER];
+                float M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int p = 0; p < PP_MAX_CLUSTER; p++) y[p] = pp_ld_remote2(ps_map(ml_addr + 8u * (uint32_t)R, p & ((int)ranks - 1)));   // (read twice: of no weight)
+#pragma unroll
+                for (int p = 0; p < PP_MAX_CLUSTER; p++) M = fmaxf(M, y[p].x);
 #pragma unroll
                 for (int p = 0; p < PP_MAX_CLUSTER; p++) {
-                    m[p] = -INFINITY, l[p] = 0.f;
-                    if (p < (int)ranks) {
-                        const uint32_t at = ps_map(ml_addr + 8u * (uint32_t)R, p);
-                        m[p] = pp_ld_remote(at);
-                        l[p] = pp_ld_remote(at + 4);
-                        M = fmaxf(M, m[p]);
-                    }
-                }
-#pragma unroll
-                for (int p = 0; p < PP_MAX_CLUSTER; p++) {
-                    const float wgt = exp2f(m[p] - (M == -INFINITY ? 0.f : M));
+                    const float wgt = exp2f(y[p].x - (M == -INFINITY ? 0.f : M));
                     weights[tid * PP_MAX_CLUSTER + p] = wgt;
-                    L += wgt * l[p];
+                    if (p < (int)ranks) L += wgt * y[p].y;
                 }
                 *reinterpret_cast<float2 *>(joined + 2 * tid) = make_float2(M == -INFINITY ? 0.f : M, L);
             }
             asm volatile("bar.sync 9, %0;" ::"n"(32 * PP_SOFTMAX_WARPS) : "memory");
             const bool good = *failed == 0;
-            for (int e = warp; e < n; e += PP_SOFTMAX_WARPS) {   // a warp per row
-                const int R = (int)rank * n + e, bx = R >> 7, rr = R & 127, rq = query_of(rr);
-                if (rq >= (bx ? live_b : live_a) || rr - rq * P.per_block >= heads_here || !good) continue;
-                const float2 ML = *reinterpret_cast<const float2 *>(joined + 2 * e);
-                const float inv = ML.y > 0.f ? 1.f / ML.y : ML.y != ML.y ? ML.y : 0.f;
-                const size_t token = (size_t)(token0 + first + bx * P.queries + rq);
-                const int h = head * P.group + head0 + rr - rq * P.per_block;
-                bool strange = false;
-                if (lane < D / 4) {
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int p = 0; p < (int)ranks; p++) {
-                        const float wgt = weights[e * PP_MAX_CLUSTER + p];
-                        const float4 a = pp_ld_remote4(ps_map(o_addr + (uint32_t)(R * (D + 4) + lane * 4) * 4u, p));
-                        v = make_float4(fmaf(wgt, a.x, v.x), fmaf(wgt, a.y, v.y), fmaf(wgt, a.z, v.z), fmaf(wgt, a.w, v.w));
+            // a warp per row, and as many rows at a time that eight parts are asked for before the first is used
+            auto join = [&](auto parts) {
+                constexpr int PARTS = decltype(parts)::value, AT_ONCE = PP_MAX_CLUSTER / PARTS;
+                for (int e0 = warp; e0 < n; e0 += AT_ONCE * PP_SOFTMAX_WARPS) {
+                    float4 a[AT_ONCE][PARTS];
+                    auto is_live = [&](int e) {
+                        const int R = (int)rank * n + e, rr = R & 127, rq = query_of(rr);
+                        return e < n && rq < (R >> 7 ? live_b : live_a) && rr - rq * P.per_block < heads_here && good;
+                    };
+#pragma unroll
+                    for (int j = 0; j < AT_ONCE; j++) {
+                        const int e = e0 + j * PP_SOFTMAX_WARPS;
+                        if (lane < D / 4 && is_live(e))
+#pragma unroll
+                            for (int p = 0; p < PARTS; p++) a[j][p] = pp_ld_remote4(ps_map(o_addr + (uint32_t)(((int)rank * n + e) * (D + 4) + lane * 4) * 4u, p));
                     }
-                    v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-                    strange = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, v.w * 0.f))) != 0.f;
-                    store4(reinterpret_cast<Q *>(P.out) + token * P.out_stride + (size_t)h * D + lane * 4, v.x, v.y, v.z, v.w);
+#pragma unroll
+                    for (int j = 0; j < AT_ONCE; j++) {
+                        const int e = e0 + j * PP_SOFTMAX_WARPS;
+                        if (!is_live(e)) continue;
+                        const int R = (int)rank * n + e, bx = R >> 7, rr = R & 127, rq = query_of(rr);
+                        const float2 ML = *reinterpret_cast<const float2 *>(joined + 2 * e);
+                        const float inv = ML.y > 0.f ? 1.f / ML.y : ML.y != ML.y ? ML.y : 0.f;
+                        const size_t token = (size_t)(token0 + first + bx * P.queries + rq);
+                        const int h = head * P.group + head0 + rr - rq * P.per_block;
+                        bool strange = false;
+                        if (lane < D / 4) {
+                            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                            for (int p = 0; p < PARTS; p++) {
+                                const float wgt = weights[e * PP_MAX_CLUSTER + p];
+                                v = make_float4(fmaf(wgt, a[j][p].x, v.x), fmaf(wgt, a[j][p].y, v.y), fmaf(wgt, a[j][p].z, v.z), fmaf(wgt, a[j][p].w, v.w));
+                            }
+                            v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                            strange = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, v.w * 0.f))) != 0.f;
+                            store4(reinterpret_cast<Q *>(P.out) + token * P.out_stride + (size_t)h * D + lane * 4, v.x, v.y, v.z, v.w);
+                        }
+                        if (lane == 0 && P.lse) P.lse[token * P.heads + h] = ML.y > 0.f ? (ML.x - PP_BIAS + log2f(ML.y)) * 0.6931471805599453f : ML.y != ML.y ? ML.y : -INFINITY;
+                        if (__any_sync(0xffffffffu, strange) && lane == 0) atomicOr(&todo[warp], 1u << (e / PP_SOFTMAX_WARPS));
+                    }
                 }
-                if (lane == 0 && P.lse) P.lse[token * P.heads + h] = ML.y > 0.f ? (ML.x - PP_BIAS + log2f(ML.y)) * 0.6931471805599453f : ML.y != ML.y ? ML.y : -INFINITY;
-                if (__any_sync(0xffffffffu, strange) && lane == 0) atomicOr(&todo[warp], 1u << (e / PP_SOFTMAX_WARPS));
-            }
+            };
+            if (ranks == 2) join(std::integral_constant<int, 2>());
+            else if (ranks == 4) join(std::integral_constant<int, 4>());
+            else join(std::integral_constant<int, 8>());
             __syncwarp();
             ps_cluster_sync();
         }
