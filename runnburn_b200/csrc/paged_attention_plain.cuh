@@ -27,11 +27,12 @@ __device__ __forceinline__ void pk_plain_row(const PkCache &c, const PkBatch &b,
 #pragma unroll
         for (int i = 0; i < PER; i++) s += x[i] * pk_value<C>(reinterpret_cast<const C *>(c.k)[e + i]);
         s = warp_sum(s) * scale;
-        const float m_new = fmaxf(m, s), corr = m_new == -INFINITY ? 1.f : expf(m - m_new), p = m_new == -INFINITY ? 0.f : expf(s - m_new);
+        const float m_new = fmaxf(m, s), corr = m_new == -INFINITY ? 1.f : expf(m - m_new), p = s != s ? s : m_new == -INFINITY ? 0.f : expf(s - m_new);
         m = m_new;
         l = l * corr + p;
 #pragma unroll
         for (int i = 0; i < PER; i++) o[i] = o[i] * corr + p * pk_value<C>(reinterpret_cast<const C *>(c.v)[e + i]);
+        if (l != l) break;   // an undefined score, or an infinite one: so is the whole row
     }
 #pragma unroll
     for (int i = 0; i < PER; i++) out[lane * PER + i] = pk_rounded<Q>(l == 0.f ? 0.f : o[i] / l);

@@ -346,8 +346,10 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
                 pk_mma<C>(s0[k & 1], qa[k], r[0], r[1]);
                 pk_mma<C>(s1[k & 1], qa[k], r[2], r[3]);
             }
-            float t[4] = {(s0[0][0] + s0[1][0]) + (s0[0][2] + s0[1][2]), (s0[0][1] + s0[1][1]) + (s0[0][3] + s0[1][3]), (s1[0][0] + s1[1][0]) + (s1[0][2] + s1[1][2]),
-                          (s1[0][1] + s1[1][1]) + (s1[0][3] + s1[1][3])};
+            // an infinite value is one already in the first term; its product with the remainder says nothing
+            auto both = [](float hi, float lo) { return fabsf(hi) < INFINITY ? hi + lo : hi; };
+            float t[4] = {both(s0[0][0] + s0[1][0], s0[0][2] + s0[1][2]), both(s0[0][1] + s0[1][1], s0[0][3] + s0[1][3]), both(s1[0][0] + s1[1][0], s1[0][2] + s1[1][2]),
+                          both(s1[0][1] + s1[1][1], s1[0][3] + s1[1][3])};
             float mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -382,8 +384,6 @@ paged_decode_kernel(PkCache c, PkBatch b, PdParams P, const __grid_constant__ Pk
                 float x0[4] = {}, x1[4] = {};
                 pk_mma<C>(x0, pa, r[0], r[1]);
                 pk_mma<C>(x1, pa, r[2], r[3]);
-                // an infinite value is one already in the first term; its product with the remainder says nothing
-                auto both = [](float hi, float lo) { return fabsf(hi) < INFINITY ? hi + lo : hi; };
                 o[2 * d][0] = fmaf(o[2 * d][0], corr, both(x0[0], x0[2]));
                 o[2 * d][1] = fmaf(o[2 * d][1], corr, both(x0[1], x0[3]));
                 o[2 * d + 1][0] = fmaf(o[2 * d + 1][0], corr, both(x1[0], x1[2]));

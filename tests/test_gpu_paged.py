@@ -305,6 +305,34 @@ def test_what_points_outside_is_flagged(P, ws, new, kv):
         assert worst(got[:m], out[:m], tolerance(out, mass, got.dtype)[:m]) <= 1
 
 
+@pytest.mark.parametrize("q,cache", PAIRS)
+@pytest.mark.parametrize("new,kv", BOTH)
+def test_scores_that_are_not_finite(P, ws, new, kv, q, cache):
+    """Undefined keys and queries, and scores of plus infinity, leave rows undefined in all dimensions; a score of minus infinity has no weight."""
+    import torch
+    c = Case(P, kv, new, heads=4, kv_heads=2, q=q, cache=cache)
+    keys = [(0, 290, 1, math.nan), (3, 1990, 0, math.inf), (3, 1855, 1, -math.inf), (2, 60, 0, math.inf)]   # sequence, position, head, its element 7
+    for s, j, h, x in keys:
+        c.k[c.table[s, j // c.page], j % c.page, h, 7] = x
+    c.q[c.starts[3], 2] = math.nan
+    c.q[c.starts[4] - 1, 1, 64] = math.nan
+    got = c.run(ws)
+    for s in range(len(c.kv)):
+        n = c.new[s]
+        if not n or not c.kv[s]:
+            continue
+        k, v = pu.rows_of(c.k, c.table[s], c.page, c.kv[s]), pu.rows_of(c.v, c.table[s], c.page, c.kv[s])
+        seen = pu.seen(torch.arange(c.kv[s] - n, c.kv[s], device="cuda"), c.kv[s], 0, 0, "cuda")
+        for h in range(4):
+            x = (c.q[c.starts[s]:c.starts[s + 1], h].double() @ k[:, h // 2].double().T * c.scale).masked_fill(~seen, -math.inf)
+            bad = (torch.isnan(x) | (x == math.inf)).any(1)
+            row, lse = got[c.starts[s]:c.starts[s + 1], h], c.lse[c.starts[s]:c.starts[s + 1], h]
+            assert torch.isnan(row[bad]).all() and torch.isnan(lse[bad]).all(), (s, h)
+            w = torch.softmax(x[~bad], 1)
+            out, mass = w @ v[:, h // 2].double(), w @ v[:, h // 2].double().abs()
+            assert worst(row[~bad], out, tolerance(out, mass, got.dtype)) <= 1, (s, h)
+
+
 def test_a_workspace_that_was_not_initialised_is_flagged(P, ws):
     """And nothing is written, to it or to the output; one that was initialised then serves."""
     import torch
