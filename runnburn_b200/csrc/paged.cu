@@ -113,7 +113,8 @@ static int pk_copy(const rnb_b200_paged_cache *cache, size_t n_layers, uint64_t 
     PkCache c{};
     RNB_TRY(pk_check_cache(cache, &c));
     if (n_layers < 1 || n_layers > 32767) return fail(RNB_B200_VALIDATION_FAILED, "paged cache: n_layers must be in 1..32767, got %zu", n_layers);
-    if (layer_stride % 8 || (n_layers > 1 && layer_stride < (uint64_t)c.head_dim)) return pk_bad("layer_stride must be a multiple of 8 and at least head_dim");
+    if (layer_stride % 8 || layer_stride > (uint64_t)1 << 38 || (n_layers > 1 && layer_stride < (uint64_t)c.head_dim))
+        return pk_bad("layer_stride must be a multiple of 8 below 2^38 and at least head_dim");
     if (n == 0) return RNB_B200_OK;
     if (!src || !dst) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
     if (n > (size_t)c.n_pages) return pk_bad("more copies than pages");

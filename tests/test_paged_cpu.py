@@ -276,7 +276,7 @@ def test_copies_refuse(r, src, dst, rows, what):
 
 def test_copies_refuse_bad_layers(r):
     L, z = r.load(), np.array([0, 1], np.int32)
-    for layers, stride in ((0, 0), (40000, 1 << 20), (2, 0), (2, 12)):
+    for layers, stride in ((0, 0), (40000, 1 << 20), (2, 0), (2, 12), (2, 1 << 40), (1, (1 << 64) - 8)):
         refused(L, L.rnb_b200_dev_paged_kv_copy(C.byref(cache(r)), layers, stride, z[:1].ctypes.data, z[1:].ctypes.data, None, 1, None), 2, "layer")
 
 
