@@ -16,7 +16,8 @@
 // f32 queries: one block, four threads a row.  Queries enter as f16 "hi" + remainder "lo" (scaled by a power of two per row into f16's range), and so do the
 // probabilities: every product is made twice and keeps 22 bits, so the products set the pace.  Three tiles' scores are under way, and probabilities take their place.
 // The tensor cores cut sums off at every step, which adds up over long rows: outputs are taken out of tensor memory every FLUSH tiles and summed in f32
-// registers, behind the next probabilities, while the last product is still under way (2048 tokens, 32 heads on 8: 78 us; error against 64 bits at 2048 tokens 6.3e-7, at 60000 positions 9.4e-7; summed there throughout 1.6e-6 and more).
+// registers, behind the next probabilities, while the last product is still under way (2048 tokens, 32 heads on 8: 78 us; error against 64 bits 6.3e-7, at
+// 60000 positions 9.4e-7; summed in tensor memory throughout 1.6e-6 and more).
 //
 // Probabilities are scaled by 2^BIAS so that small ones keep their bits, and the output is scaled only when a row's maximum has grown by more than 2^GROWTH.
 // Few rows behind many keys: a cluster of up to eight CTAs shares the keys, and joins maxima, sums and outputs over distributed shared memory.
@@ -32,7 +33,7 @@ constexpr int PP_SOFTMAX_WARPS = 16, PP_THREADS = PP_SOFTMAX_WARPS * 32 + 128;  
 constexpr int PP_SOFTMAX_REGS = 104, PP_OTHER_REGS = 64;
 static_assert(PP_SOFTMAX_WARPS * 32 * PP_SOFTMAX_REGS + 128 * PP_OTHER_REGS <= PP_THREADS * 96, "what the block is launched with");
 constexpr float PP_BIAS = 8.f, PP_GROWTH = 7.f;   // log2; together below f16's 2^16
-constexpr int PP_FLUSH = 2;
+constexpr int PP_FLUSH = 2;                       // 3: 76 us for 78 and errors of 7.6e-7 and 1.2e-6, in sums that are too small
 constexpr int PP_MAX_CLUSTER = 8;
 constexpr uint32_t PP_PANEL = 128 * 128;          // 128 rows of 64 elements, 128-byte swizzle
 
