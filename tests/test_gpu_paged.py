@@ -333,6 +333,26 @@ def test_scores_that_are_not_finite(P, ws, new, kv, q, cache):
             assert worst(row[~bad], out, tolerance(out, mass, got.dtype)) <= 1, (s, h)
 
 
+@pytest.mark.parametrize("q,cache", PAIRS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3)])
+@pytest.mark.parametrize("copies", [1, 40])
+def test_more_tokens_than_positions(P, ws, copies, window, sinks, q, cache):
+    """Tokens before the first position see nothing: zeros, with minus infinity for the sum; the others are as ever."""
+    new, kv = [40, 5, 300, 1] * copies, [10, 0, 280, 1] * copies
+    c = Case(P, kv, new, q=q, cache=cache, window=window, sinks=sinks, nan=False)
+    c.check(c.run(ws))
+
+
+@pytest.mark.parametrize("q,cache", PAIRS)
+@pytest.mark.parametrize("dim,window", [(64, 0), (128, 0), (128, 1500)])
+def test_prompts_whose_longest_decides(P, ws, dim, window, q, cache):
+    """Several prompts of very unlike lengths, whose keys pairs of CTAs share."""
+    new = [100, 1, 70, 33, 0, 5, 99, 128, 2, 64]
+    kv = [5001, 1, 70, 3000, 900, 4000, 131, 128, 2600, 65]
+    c = Case(P, kv, new, heads=16, kv_heads=8, dim=dim, page=32, q=q, cache=cache, window=window, sinks=4, padding=9)
+    c.check(c.run(ws))
+
+
 def test_a_workspace_that_was_not_initialised_is_flagged(P, ws):
     """And nothing is written, to it or to the output; one that was initialised then serves."""
     import torch
