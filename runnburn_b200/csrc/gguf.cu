@@ -474,10 +474,13 @@ int rnb_b200_decoder_load_gguf(rnb_b200_decoder *d, const rnb_b200_gguf *g, int 
     if (!d || !g) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
     rnb_b200_model_cfg c;
     RNB_TRY(rnb_b200_decoder_config(d, &c));
-    if (register_pages && g->data_start < g->len) {
+    if (register_pages && g->map && g->data_start < g->len) {
         // best effort: some file systems' read-only mappings cannot be pinned (the driver answers
         // "invalid argument"); the uploads then run as staged pageable copies, same bytes
-        if (rnb_b200_register_host_range(g->data + g->data_start, g->len - g->data_start) != RNB_B200_OK) cudaGetLastError();
+        // Whole pages around the section (the mapping begins with a page and ends with one): a copy from a range that is pinned in part is an
+        // "invalid argument" too.
+        const size_t page = 4096, from = g->data_start & ~(page - 1), to = (g->len + page - 1) & ~(page - 1);
+        if (rnb_b200_register_host_range(g->data + from, to - from) != RNB_B200_OK) cudaGetLastError();
     }
     auto quant = [&](const std::string &name, rnb_b200_qweight *out, bool required) -> int {
         const Tensor *t = g->tensor(name);
