@@ -345,6 +345,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             ok = ok && __all_sync(0xffffffffu, passed(s_full, x, t));
             if (!ok) {   // a row's warps meet in every tile, whatever has failed
                 meet();
+                meet();
                 continue;
             }
             pg_fence_after();
@@ -378,7 +379,9 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             for (int j = 0; j < 4; j++) mxs[j] = __uint_as_float(s[j]);
 #pragma unroll
             for (int i = 4; i < KEYS; i++) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(s[i]));
-            // the row's maximum; once all its threads have their scores, probabilities may take the scores' place
+            // the row's maximum, once all its threads have read the last tile's (no barrier of the products holds a warp back until then); when all have their scores,
+            // probabilities may take the scores' place
+            meet();
             *say = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
             pg_fence_before();
             meet();
