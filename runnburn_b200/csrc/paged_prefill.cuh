@@ -255,7 +255,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
     const int live_a = seq >= 0 ? min(P.queries, n_new - first) : 0, live_b = S::BLOCKS == 2 && seq >= 0 ? max(0, min(P.queries, n_new - first - P.queries)) : 0;
     PpSeen seen;
     seen.len = max(0, shift + first + live_a + live_b);
-    seen.from = P.window ? max(0, shift + first - P.window + 1) : 0;
+    seen.from = P.window && shift + first >= P.window ? shift + first - P.window + 1 : 0;   // (positions may be below 0, and a window up to 2^31 - 1)
     seen.sink = min(P.sinks, seen.from);
     seen.lead = min((seen.sink + PP_KEYS - 1) / PP_KEYS, seen.from / PP_KEYS);
     seen.skip = seen.from / PP_KEYS - seen.lead;
@@ -362,9 +362,9 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 for (int i = 0; i < KEYS; i++) s[i] = __float_as_uint(__uint_as_float(s[i]) * turned);
             }
             const int k0 = seen.start(t0 + t) + way * KEYS;
-            if (!(k0 + KEYS - 1 <= pos0 && (P.window == 0 || k0 > pos1 - P.window || k0 + KEYS <= P.sinks))) {
+            if (!(k0 + KEYS - 1 <= pos0 && (P.window == 0 || pos1 - k0 < P.window || k0 + KEYS <= P.sinks))) {
                 // keys a .. z of these, and those before the end of the sinks
-                const int z = pos - k0, a = P.window ? pos - P.window + 1 - k0 : 0, k = P.sinks - k0;
+                const int z = pos - k0, a = P.window && z >= P.window ? z - P.window + 1 : 0, k = P.sinks - k0;
                 auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };   // bits 0 .. n - 1
 #pragma unroll
                 for (int j = 0; j < KEYS / 32; j++) {

@@ -344,6 +344,16 @@ def test_more_tokens_than_positions(P, ws, copies, window, sinks, q, cache):
 
 
 @pytest.mark.parametrize("q,cache", PAIRS)
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 0), (2 ** 31 - 1, 3), (2 ** 31 - 6, 0), (2 ** 31 - 41, 0)])
+def test_windows_without_an_end(P, ws, window, sinks, q, cache):
+    """Windows near 2^31 hide nothing, in front of the first position neither."""
+    c = Case(P, [10, 0, 280, 1], [40, 5, 300, 1], window=window, sinks=sinks, q=q, cache=cache, nan=False)
+    c.check(c.run(ws))
+    c = Case(P, [10, 0, 280, 1], window=window, sinks=sinks, q=q, cache=cache)
+    c.check(c.run(ws))
+
+
+@pytest.mark.parametrize("q,cache", PAIRS)
 @pytest.mark.parametrize("dim,window", [(64, 0), (128, 0), (128, 1500)])
 def test_prompts_whose_longest_decides(P, ws, dim, window, q, cache):
     """Several prompts of very unlike lengths, whose keys pairs of CTAs share."""
