@@ -787,7 +787,7 @@ typedef struct {
     int32_t table_stride, max_pages;
     int32_t n_seq;
     int32_t n_tokens;       /* rows of the call's token matrices */
-    const int32_t *kv_len;  /* [n_seq] positions in the cache, the call's own tokens included; 0: none */
+    const int32_t *kv_len;  /* [n_seq] positions in the cache, the call's own tokens included, at most 2^31 - 256; 0: none */
     /* [n_seq + 1] first row of every sequence's tokens, from 0 and not descending; null: row i is the one token of
      * sequence i.  The last tokens of a sequence's kv_len positions are the call's; rows from
      * q_start[n_seq] on are padding: without effect, and left as they are in outputs */

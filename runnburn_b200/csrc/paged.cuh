@@ -19,10 +19,11 @@ struct PkBatch {
 };
 
 #ifdef __CUDACC__
-// Positions of a sequence, within what its table can hold.
+// Positions of a sequence, within what its table can hold, and so far below 2^31 that the end of a tile or page behind the last one is a position too.
+constexpr int PK_MAX_POSITIONS = 0x7fffff00;
 __device__ __forceinline__ int pk_length(const PkBatch &b, int page_shift, int seq, int *err) {
     const int n = b.kv_len[seq];
-    const long long most = (long long)b.max_pages << page_shift;
+    const long long most = min((long long)b.max_pages << page_shift, (long long)PK_MAX_POSITIONS);
     if (n < 0 || n > most) {
         atomicExch(err, DEV_ERR_BAD_PAGE);
         return n < 0 ? 0 : (int)most;

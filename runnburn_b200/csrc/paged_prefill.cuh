@@ -222,9 +222,10 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             }
             const unsigned behind = __ballot_sync(0xffffffffu, before + up > want);
             if (behind) {
-                if (lane == __ffs(behind) - 1) {
+                const int i = want - before - (up - pairs);
+                if (lane == __ffs(behind) - 1 && i >= 0 && i < pairs) {   // (starts out of order may add up to more than 31 bits: then there is no such place)
                     found[0] = s0 + lane;
-                    found[1] = (want - before - (up - pairs)) * S::BLOCKS * P.queries;
+                    found[1] = i * S::BLOCKS * P.queries;
                     found[2] = v.n;
                     found[3] = v.start;
                     found[4] = v.len;

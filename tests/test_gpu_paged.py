@@ -420,6 +420,26 @@ def test_offsets_past_32_bits(P, ws):
     assert torch.equal(k[1], k[2]) and torch.equal(v[1], v[2])
 
 
+@pytest.mark.parametrize("prompt", [False, True])
+def test_positions_up_to_the_last(P, ws, prompt):
+    """A table of 2^31 positions, all in one page: 2^31 - 256 of them are a length, more are flagged."""
+    import torch
+    from runnburn_b200 import ops
+    page, window, dim, i32 = 256, 300, 64, dict(dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(1, page, 1, dim, device="cuda").half() for _ in range(2))
+    q = torch.randn(1, 2, dim, device="cuda")
+    cache, table = P.PagedCache(k, v), torch.zeros(1, 1 << 23, **i32)
+    j = torch.arange(2 ** 31 - 256 - window, 2 ** 31 - 256) % page
+    for n in (2 ** 31 - 256, 2 ** 31 - 255, 2 ** 31 - 1):
+        batch = P.PagedBatch(table, torch.tensor([n], **i32), torch.tensor([0, 1], **i32) if prompt else None, 1)
+        got = (P.attention_prefill_paged if prompt else P.attention_decode_paged)(cache, batch, q, 0.125, window=window, workspace=ws)
+        torch.cuda.synchronize()
+        assert ops.dev_error_flag() == (0 if n == 2 ** 31 - 256 else P.DEVICE_BAD_PAGE)
+        if n == 2 ** 31 - 256:
+            w, vv = torch.softmax(q[0].double() @ k[0, j, 0].double().T * 0.125, 1), v[0, j, 0].double()
+            assert worst(got[0], w @ vv, tolerance(w @ vv, w @ vv.abs(), got.dtype)) <= 1
+
+
 # ---- append and copy ----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("src,cache", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
 @pytest.mark.parametrize("page,kv_heads,dim,order", [(16, 8, 128, "page pos head"), (8, 1, 64, "page head pos"), (64, 3, 8, "head page pos"), (256, 5, 200, "pos head page"),
