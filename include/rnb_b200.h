@@ -808,8 +808,9 @@ int rnb_b200_dev_paged_kv_copy(const rnb_b200_paged_cache *cache, size_t n_layer
                                const int32_t *dst, const int32_t *rows, size_t n_pages, void *stream);
 /* softmax(scale q.K^T) V over the pages.  A query at position p sees positions j <= p with window = 0, else
  * those with j > p - window or j < sinks.  A query that sees nothing (kv_len 0) gets zeros.  q_type: F32 with an
- * F16 cache, or the cache's type; `out` has the same type.  Sums, maxima and the softmax are f32, and f32 queries
- * keep f32 accuracy (queries and probabilities enter the products as two f16 terms).  q, out
+ * F16 cache, or the cache's type; `out` has the same type.  Sums, maxima and the softmax are f32.  f32 queries and
+ * their probabilities enter the products as two f16 terms: 22 bits are kept of elements down to 2^-17 of their row's
+ * largest, 19 bits down to 2^-20, and outputs are some 6e-7 off where f32 throughout gives 4e-7.  q, out
  * [n_tokens][heads][head_dim], 16-byte aligned, q_stride / out_stride elements from one token to the next
  * (multiples of 8), that do not overlap; heads a multiple of kv_heads.  lse (may be null): f32 [n_tokens][heads], the logarithm of
  * the sum of exponentials, -inf for a query that sees nothing.

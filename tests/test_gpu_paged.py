@@ -181,6 +181,18 @@ def test_f32_queries_of_any_size(P, ws, new, kv, gain):
 
 
 @pytest.mark.parametrize("new,kv", BOTH)
+@pytest.mark.parametrize("factor", [1e2, 1e3, 1e4, 1e5, 1e6])
+@pytest.mark.parametrize("gain", [1.0, 1e-30, 1e20])
+def test_f32_queries_with_one_large_element(P, ws, new, kv, factor, gain):
+    """Where the keys have nothing it says nothing about the score, which keeps the bound of 19 bits of every other element (2^20 times smaller)."""
+    c = Case(P, kv, new, gain=gain)
+    c.scale = 128 ** -0.5 / gain
+    c.q[..., 77] *= factor
+    c.k[..., 77] = 0
+    c.check(c.run(ws))
+
+
+@pytest.mark.parametrize("new,kv", BOTH)
 @pytest.mark.parametrize("q,cache", PAIRS)
 @pytest.mark.parametrize("way", ["growing", "falling", "sharp"])
 def test_maxima_that_move(P, ws, new, kv, q, cache, way):
