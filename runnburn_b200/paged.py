@@ -1,8 +1,9 @@
 """A key-value cache in pages: attention over it, its writes and copies, and the book-keeping of its pages.
 
 The functions take device tensors of PyTorch (anything with `data_ptr`, `shape`, `stride`, `dtype` and `device` will do) and run on
-the given stream, else on PyTorch's current one; they do not synchronise and allocate nothing but a missing `out`, so calls with `out`
-can be captured into graphs.  Tables, lengths and starts are read when the work runs.  What they hold is checked on the
+the given stream (a stream of PyTorch or its handle), else on PyTorch's current one; they do not synchronise and allocate nothing but a missing `out`, so
+calls with `out` can be captured into graphs.  A missing `out` is allocated on the stream that writes it.  Tensors that the caller brings are used as they
+are: those of another stream than the call's have to be kept until it is through (`record_stream`), as ever in PyTorch.  Tables, lengths and starts are read when the work runs.  What they hold is checked on the
 device: a page outside the pool, a length that the table cannot hold or a start out of order sets the device error word
 (`ops.dev_error_flag()` returns 5) instead of touching memory outside.  The C ABI behind it is declared in include/rnb_b200.h.
 
@@ -17,6 +18,7 @@ device: a page outside the pool, a length that the table cannot hold or a start 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -55,15 +57,29 @@ def _index(t) -> int:
 _raw_stream = None
 
 
-def _stream(index: int, stream):
+def _stream(index: int, stream) -> int:
     """The stream's handle; None: the current one of PyTorch (asked for by its number alone where that is offered: an object for it takes 2 us)."""
     global _raw_stream
     if stream is not None:
-        return stream
+        handle = getattr(stream, "cuda_stream", stream)
+        return getattr(handle, "value", handle) or 0
     if _raw_stream is None:
         import torch
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
     return _raw_stream(index)
+
+
+def _stream_object(index: int, handle: int):
+    import torch
+    return torch.cuda.ExternalStream(handle, device=index) if handle else torch.cuda.default_stream(index)
+
+
+def _allocating(index: int, stream):
+    """In this context PyTorch allocates memory in the order of `stream`, and takes it back in that order."""
+    if stream is None:
+        return contextlib.nullcontext()
+    import torch
+    return torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream) else _stream_object(index, _stream(index, stream)))
 
 
 def _ints(t, what: str, ndim: int):
@@ -121,15 +137,26 @@ class PagedBatch:
 
 
 class Workspace:
-    """Scratch of the attention calls.  Calls that may overlap on the GPU (other streams) need one each."""
+    """Scratch of the attention calls, allocated on the given stream and initialised when this returns (unless the stream is being captured).  Calls that may
+    overlap on the GPU (other streams) need one each."""
 
     def __init__(self, device=None, stream=None):
         import torch
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         n = load().rnb_b200_paged_workspace_bytes()
-        self.buffer = torch.empty(n, dtype=torch.uint8, device=device)
-        self.index, self.ptr, self.bytes = _index(self.buffer), self.buffer.data_ptr(), n
-        check(load().rnb_b200_paged_workspace_init(self.ptr, n, _stream(self.index, stream)))
+        with torch.cuda.device(device), _allocating(device.index, stream):
+            self.buffer = torch.empty(n, dtype=torch.uint8, device=device)
+            self.index, self.ptr, self.bytes = _index(self.buffer), self.buffer.data_ptr(), n
+            on = _stream(self.index, stream)
+            check(load().rnb_b200_paged_workspace_init(self.ptr, n, on))
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(self.index).synchronize()   # it may be used on any stream from here on
+        self._streams = {on}
+
+    def _used_on(self, handle: int) -> None:
+        """The memory is not given to others before this stream's work is through, either."""
+        self.buffer.record_stream(_stream_object(self.index, handle))
+        self._streams.add(handle)
 
 
 def _rows(t, what: str, tokens: int, heads: int | None, dim: int):
@@ -148,7 +175,8 @@ def _attention(fn, cache, batch, q, scale, out, window, sinks, lse, workspace, s
     q_stride = _rows(q, "q", n, None, dim)
     heads = q.shape[1]
     if out is None:
-        out = q.new_empty(q.shape)
+        with _allocating(cache.index, stream):
+            out = q.new_empty(q.shape)
     out_stride = _rows(out, "out", n, heads, dim)
     if out.dtype != q.dtype:
         raise ValueError(f"out has to have the queries' type {q.dtype}, got {out.dtype}")
@@ -160,8 +188,10 @@ def _attention(fn, cache, batch, q, scale, out, window, sinks, lse, workspace, s
         if str(lse.dtype) != "torch.float32" or tuple(lse.shape) != (n, heads) or not lse.is_contiguous():
             raise ValueError(f"lse has to be a contiguous float32 tensor [{n}, {heads}]")
         lse = lse.data_ptr()
-    check(fn(cache._ref, batch._ref, _type(q), q.data_ptr(), q_stride, heads, scale, window, sinks, workspace.ptr, workspace.bytes, out.data_ptr(), out_stride, lse,
-             _stream(index, stream)))
+    on = _stream(index, stream)
+    if on not in workspace._streams:
+        workspace._used_on(on)
+    check(fn(cache._ref, batch._ref, _type(q), q.data_ptr(), q_stride, heads, scale, window, sinks, workspace.ptr, workspace.bytes, out.data_ptr(), out_stride, lse, on))
     return out
 
 

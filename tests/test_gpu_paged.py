@@ -404,6 +404,55 @@ def test_streams_side_by_side(P):
         c.check(out)
 
 
+@pytest.mark.parametrize("new,kv", BOTH)
+@pytest.mark.parametrize("number", [False, True])
+def test_memory_of_a_given_stream(P, ws, new, kv, number):
+    """What a call allocates is of the stream that writes it, not a block that work of the current stream may still be using."""
+    import torch
+    c, s = Case(P, kv, new), torch.cuda.Stream()
+    stream = s.cuda_stream if number else s
+    torch.cuda.synchronize()
+    block = torch.empty_like(c.q)   # the block that the next one of its size on the current stream gets
+    at = block.data_ptr()
+    del block
+    out = c.run(ws, stream=stream)
+    assert out.data_ptr() != at
+    s.synchronize()
+    c.check(out)
+    space = P.Workspace()
+    at = space.ptr
+    del space
+    assert P.Workspace(stream=stream).ptr != at
+    torch.cuda.synchronize()
+
+
+def test_a_workspace_that_goes_while_another_stream_uses_it(P):
+    import torch
+    c, s, space = Case(P, [3000, 5]), torch.cuda.Stream(), P.Workspace()
+    out, at, n = torch.empty_like(c.q), space.ptr, space.bytes
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(50_000_000)
+    c.run(space, out=out, stream=s)
+    del space
+    block = torch.empty(n, dtype=torch.uint8, device="cuda")
+    assert block.data_ptr() != at
+    s.synchronize()
+    c.check(out)
+
+
+def test_a_new_workspace_serves_any_stream(P):
+    """Without a wait of the caller's between its making and its use."""
+    import torch
+    c = Case(P, [9000, 3])
+    torch.cuda.synchronize()
+    torch.cuda._sleep(50_000_000)
+    space, s = P.Workspace(), torch.cuda.Stream()
+    out = c.run(space, stream=s)
+    s.synchronize()
+    c.check(out)
+
+
 def test_a_sequence_in_more_parts_than_a_join_has_weights_for(P, ws):
     """One key head and so many tiles that every CTA of the launch leaves a part."""
     for dim, heads in ((64, 2), (128, 5)):
