@@ -55,6 +55,8 @@ void rnb_b200_close(void);
 /* cuda_memory_info — api/cache_api.rs:97 */
 int rnb_b200_cuda_memory_info(size_t *free_bytes, size_t *total_bytes);
 int rnb_b200_device_sm_count(int *sm_count);
+/* The CUDA device that the library runs on, or would run on if it were opened now (RNB_CUDA_DEVICE, else 0).  Opens nothing. */
+int rnb_b200_device_index(int *device);
 
 /* ---- resident weight cache -------------------------------------------------------------- */
 /* cuda_cache_snapshot / cuda_weight_residency_counters — api/cache_api.rs:114,147;

@@ -120,6 +120,7 @@ def load() -> C.CDLL:
         "rnb_b200_open": [],
         "rnb_b200_cuda_memory_info": [vp, vp],
         "rnb_b200_device_sm_count": [vp],
+        "rnb_b200_device_index": [vp],
         "rnb_b200_cuda_cache_snapshot": [vp],
         "rnb_b200_clear_q4k_cache": [],
         "rnb_b200_reset_state_for_engine_init": [],

@@ -105,6 +105,11 @@ int gemv_kernel_setup() {
 // ---------------------------------------------------------------------------------------------
 // State
 // ---------------------------------------------------------------------------------------------
+static int chosen_device() {
+    const char *env = getenv("RNB_CUDA_DEVICE");
+    return env ? atoi(env) : 0;
+}
+
 int State::open() {
     if (is_open) return RNB_B200_OK;
     int n = 0;
@@ -114,8 +119,7 @@ int State::open() {
         return fail(RNB_B200_CUDA_ERROR, "no usable CUDA device (%s); this library has no CPU fallback",
                     e == cudaSuccess ? "device count is 0" : cudaGetErrorString(e));
     }
-    const char *env = getenv("RNB_CUDA_DEVICE");
-    device = env ? atoi(env) : 0;
+    device = chosen_device();
     if (device < 0 || device >= n) return fail(RNB_B200_VALIDATION_FAILED, "RNB_CUDA_DEVICE=%d out of range (%d devices)", device, n);
     RNB_CU(cudaSetDevice(device));
     cudaDeviceProp prop;
@@ -561,6 +565,12 @@ int rnb_b200_device_sm_count(int *sm_count) {
     Locked L;
     RNB_TRY(L.st.open());
     if (sm_count) *sm_count = L.st.sm_count;
+    return RNB_B200_OK;
+}
+int rnb_b200_device_index(int *device) {
+    if (!device) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
+    Locked L;
+    *device = L.st.is_open ? L.st.device : chosen_device();
     return RNB_B200_OK;
 }
 int rnb_b200_cuda_cache_snapshot(rnb_b200_cache_snapshot *out) {

@@ -58,6 +58,13 @@ def device_sm_count() -> int:
     return n.value
 
 
+def device_index() -> int:
+    """The CUDA device that the library runs on, or would run on if it were opened now."""
+    n = C.c_int()
+    check(load().rnb_b200_device_index(C.byref(n)))
+    return n.value
+
+
 def cuda_cache_snapshot() -> dict:
     s = _lib.CacheSnapshot()
     check(load().rnb_b200_cuda_cache_snapshot(C.byref(s)))

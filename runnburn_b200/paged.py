@@ -1,11 +1,13 @@
 """A key-value cache in pages: attention over it, its writes and copies, and the book-keeping of its pages.
 
-The functions take device tensors of PyTorch (anything with `data_ptr`, `shape`, `stride`, `dtype` and `device` will do) and run on
-the given stream (a stream of PyTorch or its handle), else on PyTorch's current one; they do not synchronise and allocate nothing but a missing `out`, so
-calls with `out` can be captured into graphs.  A missing `out` is allocated on the stream that writes it.  Tensors that the caller brings are used as they
-are: those of another stream than the call's have to be kept until it is through (`record_stream`), as ever in PyTorch.  Tables, lengths and starts are read when the work runs.  What they hold is checked on the
-device: a page outside the pool, a length that the table cannot hold or a start out of order sets the device error word
-(`ops.dev_error_flag()` returns 5) instead of touching memory outside.  The C ABI behind it is declared in include/rnb_b200.h.
+The functions take device tensors of PyTorch (anything with its `data_ptr`, `shape`, `stride`, `dtype`, `device` and the like will do)
+on the library's device (`ops.device_index()`), whatever device is current, and run on the given stream (a stream of PyTorch or its
+handle), else on PyTorch's current one; they do not synchronise and allocate nothing but a missing `out`, so calls with `out` can be
+captured into graphs.  A missing `out` is allocated on the stream that writes it.  Tensors that the caller brings are used as they are:
+those of another stream than the call's have to be kept until it is through (`record_stream`), as ever in PyTorch.  Tables, lengths and
+starts are read when the work runs.  What they hold is checked on the device: a page outside the pool, a length that the table cannot
+hold or a start out of order sets the device error word (`ops.dev_error_flag()` returns 5) instead of touching memory outside.  The C
+ABI behind it is declared in include/rnb_b200.h.
 
     pages = KvPages(n_pages, page_size)                    # host: who holds which page
     cache = PagedCache(k, v)                               # [n_pages, page_size, kv_heads, head_dim] each, any strides
@@ -23,7 +25,7 @@ import ctypes as C
 
 import numpy as np
 
-from . import _lib
+from . import _lib, ops
 from ._lib import TYPE_BF16, TYPE_F16, TYPE_F32, check, load
 
 DEVICE_BAD_PAGE, DEVICE_BAD_WORKSPACE = 5, 6   # what ops.dev_error_flag() tells of a call
@@ -52,6 +54,14 @@ def _index(t) -> int:
     if not t.is_cuda:
         raise ValueError(f"tensors have to be on a CUDA device, got {t.device}")
     return t.get_device()
+
+
+def _library_index(t) -> int:
+    """The tensor's device, which has to be the one that the library launches on."""
+    index, own = _index(t), ops.device_index()
+    if index != own:
+        raise ValueError(f"the library runs on cuda:{own} (RNB_CUDA_DEVICE), got a tensor on {t.device}")
+    return index
 
 
 _raw_stream = None
@@ -97,7 +107,7 @@ class PagedCache:
             raise ValueError("k and v have to be alike, [n_pages, page_size, kv_heads, head_dim] or with a dimension of layers before these")
         if k.shape[-1] > 1 and k.stride(-1) != 1:
             raise ValueError("the elements of a head's row have to be contiguous")
-        self.index = _index(k)
+        self.index = _library_index(k)
         _on_device(self.index, v)
         self.k, self.v = k, v
         self.n_layers, self.layer_stride = (k.shape[0], k.stride(0)) if k.dim() == 5 else (1, 0)
@@ -137,16 +147,16 @@ class PagedBatch:
 
 
 class Workspace:
-    """Scratch of the attention calls, allocated on the given stream and initialised when this returns (unless the stream is being captured).  Calls that may
+    """Scratch of the attention calls, on the library's device, allocated on the given stream and initialised when this returns (unless the stream is being captured).  Calls that may
     overlap on the GPU (other streams) need one each."""
 
     def __init__(self, device=None, stream=None):
         import torch
-        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        device = torch.device("cuda", ops.device_index()) if device is None else torch.device(device)
         n = load().rnb_b200_paged_workspace_bytes()
         with torch.cuda.device(device), _allocating(device.index, stream):
             self.buffer = torch.empty(n, dtype=torch.uint8, device=device)
-            self.index, self.ptr, self.bytes = _index(self.buffer), self.buffer.data_ptr(), n
+            self.index, self.ptr, self.bytes = _library_index(self.buffer), self.buffer.data_ptr(), n
             on = _stream(self.index, stream)
             check(load().rnb_b200_paged_workspace_init(self.ptr, n, on))
             if not torch.cuda.is_current_stream_capturing():

@@ -280,6 +280,43 @@ def test_copies_refuse_bad_layers(r):
         refused(L, L.rnb_b200_dev_paged_kv_copy(C.byref(cache(r)), layers, stride, z[:1].ctypes.data, z[1:].ctypes.data, None, 1, None), 2, "layer")
 
 
+class OnDevice:
+    """As much of a tensor on a CUDA device as is looked at before anything runs."""
+    is_cuda = True
+
+    def __init__(self, index, shape=(4, 16, 2, 64), dtype=None):
+        import torch
+        self.index, self.like, self.device = index, torch.empty(shape, dtype=dtype or torch.float16), f"cuda:{index}"
+        self.shape, self.dtype, self.dim, self.stride = self.like.shape, self.like.dtype, self.like.dim, self.like.stride
+
+    def get_device(self):
+        return self.index
+
+    def data_ptr(self):
+        return ADDRESS
+
+
+def test_tensors_on_another_device_than_the_library_s_are_refused(r):
+    """The launch goes to the library's device, whatever device the tensors are on."""
+    here = r.ops.device_index()
+    assert r.paged.PagedCache(OnDevice(here), OnDevice(here)).index == here
+    with pytest.raises(ValueError, match=f"runs on cuda:{here}.*cuda:{here + 1}"):
+        r.paged.PagedCache(OnDevice(here + 1), OnDevice(here + 1))
+    with pytest.raises(ValueError, match="one CUDA device"):
+        r.paged.PagedCache(OnDevice(here), OnDevice(here + 1))
+
+
+def test_the_device_is_the_one_that_would_be_opened(r):
+    """Asked for in a process of its own, where nothing is open."""
+    import os
+    import subprocess
+    import sys
+    for env, want in ((None, "0"), ("3", "3")):
+        e = {k: v for k, v in os.environ.items() if k != "RNB_CUDA_DEVICE"} | ({"RNB_CUDA_DEVICE": env} if env else {})
+        got = subprocess.run([sys.executable, "-c", "from runnburn_b200 import ops; print(ops.device_index())"], capture_output=True, text=True, env=e, cwd=r._lib.PKG.parent)
+        assert got.stdout.strip() == want, got.stderr
+
+
 def test_nothing_to_do_is_no_call(r):
     """No tokens, no sequences, no copies: fine without a GPU."""
     L = r.load()
