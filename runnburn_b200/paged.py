@@ -92,6 +92,12 @@ def _allocating(index: int, stream):
     return torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream) else _stream_object(index, _stream(index, stream)))
 
 
+def _int(x, what: str):
+    if not -2 ** 31 <= x < 2 ** 31:
+        raise ValueError(f"{what}: {x} does not fit 32 bits")
+    return x
+
+
 def _ints(t, what: str, ndim: int):
     if str(t.dtype) != "torch.int32" or t.dim() != ndim or (t.shape[-1] > 1 and t.stride(-1) != 1):
         raise ValueError(f"{what} has to be an int32 tensor of {ndim} dimension(s), its last one contiguous")
@@ -141,7 +147,8 @@ class PagedBatch:
         elif n_tokens is None:
             n_tokens = n_seq
         self.table, self.kv_len, self.q_start, self.n_tokens = table, kv_len, q_start, n_tokens
-        self._c = _lib.PagedBatch(table.data_ptr(), max(table.stride(0), table.shape[1]) if n_seq < 2 else table.stride(0), table.shape[1], n_seq, n_tokens, kv_len.data_ptr(),
+        stride = max(table.stride(0), table.shape[1]) if n_seq < 2 else table.stride(0)
+        self._c = _lib.PagedBatch(table.data_ptr(), _int(stride, "table"), _int(table.shape[1], "table"), n_seq, _int(n_tokens, "n_tokens"), kv_len.data_ptr(),
                                   None if q_start is None else q_start.data_ptr())
         self._ref = C.byref(self._c)
 
@@ -201,7 +208,7 @@ def _attention(fn, cache, batch, q, scale, out, window, sinks, lse, workspace, s
     on = _stream(index, stream)
     if on not in workspace._streams:
         workspace._used_on(on)
-    check(fn(cache._ref, batch._ref, _type(q), q.data_ptr(), q_stride, heads, scale, window, sinks, workspace.ptr, workspace.bytes, out.data_ptr(), out_stride, lse, on))
+    check(fn(cache._ref, batch._ref, _type(q), q.data_ptr(), q_stride, heads, scale, _int(window, "window"), _int(sinks, "sinks"), workspace.ptr, workspace.bytes, out.data_ptr(), out_stride, lse, on))
     return out
 
 
@@ -229,14 +236,20 @@ def paged_kv_append(cache: PagedCache, batch: PagedBatch, k_new, v_new, *, strea
     check(load().rnb_b200_dev_paged_kv_append(cache._ref, batch._ref, _type(k_new), k_new.data_ptr(), v_new.data_ptr(), stride, _stream(index, stream)))
 
 
-def _host(a) -> np.ndarray:
+def _host(a, what: str) -> np.ndarray:
+    """A list of whole numbers as int32; what would be cut on the way is refused."""
+    a = np.asarray(a)
+    if a.dtype != np.int32 and a.size:
+        if a.dtype.kind not in "iu":
+            raise TypeError(f"{what} has to hold whole numbers, got {a.dtype}")
+        _int(a.min(), what), _int(a.max(), what)
     return np.ascontiguousarray(a, dtype=np.int32).ravel()
 
 
 def paged_kv_copy(cache: PagedCache, src, dst, rows=None, *, stream=None) -> None:
     """Copies page src[i] to page dst[i] in all layers, its first rows[i] positions (None: all).  The lists are host integers.  A page may
     be copied to several places; one that is written must be written once and not read."""
-    src, dst, rows = _host(src), _host(dst), None if rows is None else _host(rows)
+    src, dst, rows = _host(src, "src"), _host(dst, "dst"), None if rows is None else _host(rows, "rows")
     if src.size != dst.size or (rows is not None and rows.size != src.size):
         raise ValueError("src, dst and rows have to be equally long")
     check(load().rnb_b200_dev_paged_kv_copy(cache._ref, cache.n_layers, cache.layer_stride, src.ctypes.data, dst.ctypes.data, None if rows is None else rows.ctypes.data,
@@ -249,7 +262,7 @@ class KvPages:
 
     def __init__(self, n_pages: int, page_size: int):
         h = C.c_void_p()
-        check(load().rnb_b200_kv_pages_create(n_pages, page_size, C.byref(h)))
+        check(load().rnb_b200_kv_pages_create(_int(n_pages, "n_pages"), _int(page_size, "page_size"), C.byref(h)))
         self._h, self.n_pages, self.page_size = h, n_pages, page_size
 
     def close(self) -> None:
@@ -272,23 +285,23 @@ class KvPages:
     def extend(self, seq: int, n_new: int):
         """Room for n_new more positions; ([], [], []) or the one copy that parts a shared last page."""
         n, src, dst, rows = (C.c_int32() for _ in range(4))
-        check(load().rnb_b200_kv_pages_extend(self._h, seq, n_new, C.byref(n), C.byref(src), C.byref(dst), C.byref(rows)))
+        check(load().rnb_b200_kv_pages_extend(self._h, _int(seq, "seq"), _int(n_new, "n_new"), C.byref(n), C.byref(src), C.byref(dst), C.byref(rows)))
         return ([src.value], [dst.value], [rows.value]) if n.value else ([], [], [])
 
     def fork(self, seq: int) -> int:
         s = C.c_int32()
-        check(load().rnb_b200_kv_pages_fork(self._h, seq, C.byref(s)))
+        check(load().rnb_b200_kv_pages_fork(self._h, _int(seq, "seq"), C.byref(s)))
         return s.value
 
     def truncate(self, seq: int, length: int) -> None:
-        check(load().rnb_b200_kv_pages_truncate(self._h, seq, length))
+        check(load().rnb_b200_kv_pages_truncate(self._h, _int(seq, "seq"), _int(length, "length")))
 
     def release(self, seq: int, window: int, sinks: int = 0) -> None:
         """Frees the pages that neither the window of the next token nor the sinks reach."""
-        check(load().rnb_b200_kv_pages_release(self._h, seq, window, sinks))
+        check(load().rnb_b200_kv_pages_release(self._h, _int(seq, "seq"), _int(window, "window"), _int(sinks, "sinks")))
 
     def free(self, seq: int) -> None:
-        check(load().rnb_b200_kv_pages_free(self._h, seq))
+        check(load().rnb_b200_kv_pages_free(self._h, _int(seq, "seq")))
 
     def compact(self):
         """Moves the used pages to the front of the pool; (src, dst, None)."""
@@ -299,11 +312,12 @@ class KvPages:
 
     def tables(self, seqs, max_pages: int | None = None):
         """(int32 [n, max_pages], int32 [n]): page tables and lengths on the host, unused entries -1."""
-        seqs = _host(seqs)
+        seqs = _host(seqs, "seqs")
         lens = np.empty(seqs.size, np.int32)
         check(load().rnb_b200_kv_pages_tables(self._h, seqs.ctypes.data, seqs.size, None, 0, lens.ctypes.data))
         if max_pages is None:
             max_pages = max(1, -(-int(lens.max(initial=0)) // self.page_size))
+        _int(max_pages, "max_pages")
         table = np.empty((seqs.size, max_pages), np.int32)
         check(load().rnb_b200_kv_pages_tables(self._h, seqs.ctypes.data, seqs.size, table.ctypes.data, max_pages, None))
         return table, lens

@@ -274,6 +274,45 @@ def test_copies_refuse(r, src, dst, rows, what):
     refused(L, L.rnb_b200_dev_paged_kv_copy(C.byref(cache(r)), 1, 0, a[0].ctypes.data, a[1].ctypes.data, a[2].ctypes.data if rows else None, len(src), None), 2, what)
 
 
+@pytest.mark.parametrize("bad,error", [
+    (np.array([0, 2 ** 32 + 1]), ValueError), (np.array([0, -2 ** 32 + 1]), ValueError), (np.array([0, 2 ** 31], np.uint64), ValueError), ([0, 2 ** 32 + 1], ValueError),
+    (np.array([0.0, 1.0]), TypeError), ([0, 1.5], TypeError), (np.array([False, True]), TypeError), ([0, 2 ** 70], TypeError), (["0", "1"], TypeError)])
+def test_lists_are_whole_numbers_of_32_bits(r, bad, error):
+    """Cut to 32 bits, or to whole numbers, they would be pages and sequences that nobody named."""
+    here = r.ops.device_index()
+    cache, p = r.paged.PagedCache(OnDevice(here), OnDevice(here)), r.paged.KvPages(8, 8)
+    p.extend(p.new(), 5), p.extend(p.new(), 6)
+    good = [2, 3]
+    for lists in ((bad, good, None), (good, bad, None), ([0, 1], good, bad)):
+        with pytest.raises(error, match="src|dst|rows"):
+            r.paged.paged_kv_copy(cache, *lists)
+    with pytest.raises(error, match="seqs"):
+        p.tables(bad)
+    import torch
+    for fine in ([0, 1], np.array([0, 1]), np.array([0, 1], np.uint8), torch.tensor([0, 1])):
+        assert p.tables(fine)[1].tolist() == [5, 6]
+    assert p.tables([])[0].shape == (0, 1)
+
+
+def test_numbers_of_more_than_32_bits_are_refused(r):
+    """Cut to 32 bits they would be other ones."""
+    p = r.paged.KvPages(8, 8)
+    s = p.new()
+    p.extend(s, 20)
+    far = 2 ** 32
+    for call in (lambda: p.extend(s, far + 1), lambda: p.extend(far + s, 1), lambda: p.truncate(s, far + 8), lambda: p.release(s, far + 4), lambda: p.release(s, 4, far),
+                 lambda: p.fork(far + s), lambda: p.free(far + s), lambda: r.paged.KvPages(far + 8, 8), lambda: r.paged.KvPages(8, far + 8), lambda: p.tables([s], far + 3)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+    assert p.info() == dict(n_pages=8, page_size=8, free_pages=5, n_seqs=1)
+    import torch
+    here = r.ops.device_index()
+    table, lens, start = (OnDevice(here, shape, torch.int32) for shape in ((2, 4), (2,), (3,)))
+    assert r.paged.PagedBatch(table, lens, start, 9).n_tokens == 9
+    with pytest.raises(ValueError, match="32 bits"):
+        r.paged.PagedBatch(table, lens, start, far + 9)
+
+
 def test_copies_refuse_bad_layers(r):
     L, z = r.load(), np.array([0, 1], np.int32)
     for layers, stride in ((0, 0), (40000, 1 << 20), (2, 0), (2, 12), (2, 1 << 40), (1, (1 << 64) - 8)):
