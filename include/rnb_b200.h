@@ -657,8 +657,8 @@ int rnb_b200_decoder_set_exact_attention_max(rnb_b200_decoder *d, int max_positi
  * little-endian only, u64 counts, KV metadata, tensor infos with dims stored innermost first,
  * `general.alignment` (default 32, a power of two), data section at the next aligned offset;
  * limits and messages as the reference's); type ids — gguf/types.rs:5-40.  `open` maps the file
- * read-only; `parse` reads a buffer the caller keeps alive.  Tensor data is never copied on the
- * host. */
+ * read-only; `parse` reads a buffer the caller keeps alive.  Tensor data is not copied on the
+ * host, but for the tensors at the edges of a buffer of which the whole pages are pinned. */
 typedef struct rnb_b200_gguf rnb_b200_gguf;
 typedef struct {
     char name[64];
@@ -692,8 +692,8 @@ int rnb_b200_gguf_tensor_at(const rnb_b200_gguf *g, size_t index, rnb_b200_gguf_
 int rnb_b200_gguf_model_config(const rnb_b200_gguf *g, int max_ctx, rnb_b200_model_cfg *cfg);
 /* Tensor names of crates/rnb-loader/src/arch/llama.rs:33-155 (`token_embd`, `blk.N.attn_q`, ...,
  * `output_norm`, `output`; a file without `output.weight` ties the LM head to the embedding)
- * uploaded from the mapped pages; register_pages != 0 pins the data section first
- * (rnb_b200_register_host_range) where the mapping can be pinned: best effort. */
+ * uploaded from the mapped pages or the buffer; register_pages != 0 pins the data section first
+ * (rnb_b200_register_host_range) where it can be pinned: best effort. */
 int rnb_b200_decoder_load_gguf(rnb_b200_decoder *d, const rnb_b200_gguf *g, int register_pages);
 
 /* ---- device-pointer tier (no host copies, no synchronisation; for callers that keep

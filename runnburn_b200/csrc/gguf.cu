@@ -467,21 +467,31 @@ int rnb_b200_gguf_model_config(const rnb_b200_gguf *g, int max_ctx, rnb_b200_mod
 }
 
 // Points the decoder at the file's tensors (names of arch/llama.rs:33-155; the expert stacks of the
-// MoE families are `ffn_gate_inp`, `ffn_{gate,up,down}_exps`).  With register_pages the mapped
-// tensor-data section is pinned first, where the mapping allows it, so the uploads run as
-// asynchronous DMA from the page cache.
-int rnb_b200_decoder_load_gguf(rnb_b200_decoder *d, const rnb_b200_gguf *g, int register_pages) {
-    if (!d || !g) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
+// MoE families are `ffn_gate_inp`, `ffn_{gate,up,down}_exps`).  With register_pages the pages of the
+// tensor-data section are pinned first, where they can be, so the uploads run as
+// asynchronous DMA from them (2 GB of a caller's memory: 92 ms, 40 of them the pinning, without 191).
+static int load_tensors(rnb_b200_decoder *d, const rnb_b200_gguf *g, int register_pages) {
     rnb_b200_model_cfg c;
     RNB_TRY(rnb_b200_decoder_config(d, &c));
-    if (register_pages && g->map && g->data_start < g->len) {
-        // best effort: some file systems' read-only mappings cannot be pinned (the driver answers
-        // "invalid argument"); the uploads then run as staged pageable copies, same bytes
-        // Whole pages around the section (the mapping begins with a page and ends with one): a copy from a range that is pinned in part is an
-        // "invalid argument" too.
-        const size_t page = 4096, from = g->data_start & ~(page - 1), to = (g->len + page - 1) & ~(page - 1);
-        if (rnb_b200_register_host_range(g->data + from, to - from) != RNB_B200_OK) cudaGetLastError();
+    const uint8_t *pinned = nullptr, *pinned_end = nullptr;
+    std::vector<std::vector<uint8_t>> staged;
+    if (register_pages && g->data_start < g->len) {
+        // Best effort: some file systems' read-only mappings cannot be pinned (the driver answers "invalid argument"); the uploads then run as staged pageable
+        // copies, same bytes.  Of a mapping, whole pages around the section (it begins with a page and ends with one).  Of a caller's memory, the pages that lie
+        // within it: what shares the others is not ours to pin.
+        const uintptr_t page = 4096, from = (uintptr_t)g->data + g->data_start, to = (uintptr_t)g->data + g->len;
+        const uintptr_t first = g->map ? from & ~(page - 1) : (from + page - 1) & ~(page - 1), last = g->map ? (to + page - 1) & ~(page - 1) : to & ~(page - 1);
+        if (first < last) {
+            if (rnb_b200_register_host_range((const void *)first, last - first) == RNB_B200_OK) pinned = (const uint8_t *)first, pinned_end = (const uint8_t *)last;
+            else cudaGetLastError();
+        }
     }
+    // Where a tensor is uploaded from: a copy from a range that is pinned in part is an "invalid argument", so a tensor at an edge goes by way of memory that is not.
+    auto source = [&](const uint8_t *p, size_t n) {
+        if (p + n <= pinned || p >= pinned_end || (p >= pinned && p + n <= pinned_end)) return p;
+        staged.emplace_back(p, p + n);
+        return (const uint8_t *)staged.back().data();
+    };
     auto quant = [&](const std::string &name, rnb_b200_qweight *out, bool required) -> int {
         const Tensor *t = g->tensor(name);
         if (!t) {
@@ -497,7 +507,7 @@ int rnb_b200_decoder_load_gguf(rnb_b200_decoder *d, const rnb_b200_gguf *g, int 
         RNB_TRY(fill_tensor_info(g, *t, &ti));
         if (ti.n_bytes == 0) return fail(RNB_B200_UNSUPPORTED, "tensor '%s' has GGML type %u, which this decoder cannot size", name.c_str(), ti.ggml_type);
         out->type = ti.ggml_type;
-        out->data = ti.data;
+        out->data = source((const uint8_t *)ti.data, (size_t)ti.n_bytes);
         out->len = (size_t)ti.n_bytes;
         return RNB_B200_OK;
     };
@@ -508,7 +518,7 @@ int rnb_b200_decoder_load_gguf(rnb_b200_decoder *d, const rnb_b200_gguf *g, int 
         RNB_TRY(fill_tensor_info(g, *t, &ti));
         if (ti.ggml_type != 0 || ti.n_elements != n) return fail(RNB_B200_VALIDATION_FAILED, "tensor '%s' must be %zu f32 values (type %u, %llu elements found)", name.c_str(), n, ti.ggml_type, (unsigned long long)ti.n_elements);
         if ((uintptr_t)ti.data & 3u) return fail(RNB_B200_VALIDATION_FAILED, "tensor '%s' is not 4-byte aligned in the file", name.c_str());
-        *out = reinterpret_cast<const float *>(ti.data);
+        *out = reinterpret_cast<const float *>(source((const uint8_t *)ti.data, (size_t)ti.n_bytes));
         return RNB_B200_OK;
     };
     for (int l = 0; l < c.n_layer; l++) {
@@ -540,6 +550,14 @@ int rnb_b200_decoder_load_gguf(rnb_b200_decoder *d, const rnb_b200_gguf *g, int 
     RNB_TRY(quant("output.weight", &output, false));
     if (!output.data) output = embd;   // tied embeddings: no separate LM head in the file
     return rnb_b200_decoder_set_globals(d, embd, out_norm, output);
+}
+int rnb_b200_decoder_load_gguf(rnb_b200_decoder *d, const rnb_b200_gguf *g, int register_pages) {
+    if (!d || !g) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
+    try {
+        return load_tensors(d, g, register_pages);
+    } catch (const std::bad_alloc &) {
+        return fail(RNB_B200_OUT_OF_MEMORY, "GGUF weights: out of host memory");
+    }
 }
 
 }  // extern "C"
