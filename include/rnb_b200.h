@@ -692,8 +692,8 @@ int rnb_b200_gguf_tensor_at(const rnb_b200_gguf *g, size_t index, rnb_b200_gguf_
 int rnb_b200_gguf_model_config(const rnb_b200_gguf *g, int max_ctx, rnb_b200_model_cfg *cfg);
 /* Tensor names of crates/rnb-loader/src/arch/llama.rs:33-155 (`token_embd`, `blk.N.attn_q`, ...,
  * `output_norm`, `output`; a file without `output.weight` ties the LM head to the embedding)
- * uploaded from the mapped pages or the buffer; register_pages != 0 pins the data section first
- * (rnb_b200_register_host_range) where it can be pinned: best effort. */
+ * uploaded from the mapped pages or the buffer; register_pages != 0 pins the data section for the
+ * length of the call where it can be pinned: best effort. */
 int rnb_b200_decoder_load_gguf(rnb_b200_decoder *d, const rnb_b200_gguf *g, int register_pages);
 
 /* ---- device-pointer tier (no host copies, no synchronisation; for callers that keep

@@ -162,7 +162,7 @@ void State::close() {
         cudaFree(kv.second.dv);
     }
     kv_mirrors.clear();
-    for (auto &r : registered) cudaHostUnregister(r.first);
+    for (auto &r : registered) cudaHostUnregister(r.p);
     registered.clear();
     DevBuf *bufs[] = {&in_f32, &xq, &xq2, &out_f32, &mid_a, &mid_b, &mid_c, &jobs, &partials, &misc, &xb};
     for (DevBuf *b : bufs) b->release();
@@ -272,6 +272,51 @@ int State::resident_ptr(const uint8_t *host, size_t len, bool pin, const uint8_t
     ctr.h2d_bytes += len;
     *dev_out = dev;
     return RNB_B200_OK;
+}
+
+// only whole pages strictly inside a range can be pinned
+static bool whole_pages(const void *p, size_t n, void **first, size_t *bytes) {
+    const uintptr_t page = 4096, b = ((uintptr_t)p + page - 1) & ~(page - 1), e = ((uintptr_t)p + n) & ~(page - 1);
+    *first = (void *)b;
+    *bytes = e > b ? e - b : 0;
+    return e > b;
+}
+int State::pin(const void *p, size_t n, bool *held) {
+    void *first;
+    size_t bytes;
+    if (held) *held = false;
+    if (!whole_pages(p, n, &first, &bytes)) return RNB_B200_OK;
+    for (Pinned &r : registered)
+        if (r.p == first && r.n == bytes) {
+            r.holders++;
+            if (held) *held = true;
+            return RNB_B200_OK;
+        }
+    cudaError_t err = cudaHostRegister(first, bytes, cudaHostRegisterReadOnly);
+    if (err == cudaErrorNotSupported || err == cudaErrorInvalidValue) {
+        cudaGetLastError();
+        err = cudaHostRegister(first, bytes, cudaHostRegisterDefault);
+    }
+    if (err == cudaErrorHostMemoryAlreadyRegistered) {
+        cudaGetLastError();
+        return RNB_B200_OK;
+    }
+    if (err != cudaSuccess) return fail_cuda(err, "cudaHostRegister");
+    registered.push_back({first, bytes, 1});
+    if (held) *held = true;
+    return RNB_B200_OK;
+}
+void State::unpin(const void *p, size_t n) {
+    void *first;
+    size_t bytes;
+    if (!whole_pages(p, n, &first, &bytes)) return;
+    for (size_t i = 0; i < registered.size(); i++)
+        if (registered[i].p == first && registered[i].n == bytes) {
+            if (--registered[i].holders > 0) return;
+            if (cudaHostUnregister(first) != cudaSuccess) cudaGetLastError();
+            registered.erase(registered.begin() + i);
+            return;
+        }
 }
 
 int State::h2d(void *dst, const void *src, size_t n, PinnedBuf &stage, size_t stage_off) {
@@ -645,28 +690,14 @@ int rnb_b200_register_host_range(const void *ptr, size_t len) {
     Locked L;
     RNB_TRY(L.st.open());
     RNB_CU(cudaSetDevice(L.st.device));
-    // only whole pages strictly inside the range can be pinned
-    const uintptr_t page = 4096, b = ((uintptr_t)ptr + page - 1) & ~(page - 1), e = ((uintptr_t)ptr + len) & ~(page - 1);
-    if (e <= b) return RNB_B200_OK;
-    cudaError_t err = cudaHostRegister((void *)b, e - b, cudaHostRegisterReadOnly);
-    if (err == cudaErrorNotSupported || err == cudaErrorInvalidValue) {
-        cudaGetLastError();
-        err = cudaHostRegister((void *)b, e - b, cudaHostRegisterDefault);
-    }
-    if (err == cudaErrorHostMemoryAlreadyRegistered) {
-        cudaGetLastError();
-        return RNB_B200_OK;
-    }
-    if (err != cudaSuccess) return fail_cuda(err, "cudaHostRegister");
-    L.st.registered.push_back(std::make_pair((void *)b, (size_t)(e - b)));
-    return RNB_B200_OK;
+    return L.st.pin(ptr, len, nullptr);
 }
 int rnb_b200_clear_host_registered_ranges(void) {
     Locked L;
     if (!L.st.is_open) return RNB_B200_OK;
     RNB_CU(cudaSetDevice(L.st.device));
     RNB_CU(cudaStreamSynchronize(L.st.stream));
-    for (auto &r : L.st.registered) cudaHostUnregister(r.first);
+    for (auto &r : L.st.registered) cudaHostUnregister(r.p);
     L.st.registered.clear();
     return RNB_B200_OK;
 }

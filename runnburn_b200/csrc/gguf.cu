@@ -6,7 +6,7 @@
 // and its Llama-family metadata extraction (crates/rnb-loader/src/arch/mod.rs:304-560) and tensor
 // names (crates/rnb-loader/src/arch/llama.rs:33-155).  The file is mapped read-only; tensor data
 // is never copied on the host: the decoder uploads straight from the mapped pages, optionally
-// pinned for DMA first (rnb_b200_register_host_range).
+// pinned for DMA meanwhile.
 #include <fcntl.h>
 #include <sys/mman.h>
 #include <sys/stat.h>
@@ -470,25 +470,37 @@ int rnb_b200_gguf_model_config(const rnb_b200_gguf *g, int max_ctx, rnb_b200_mod
 // MoE families are `ffn_gate_inp`, `ffn_{gate,up,down}_exps`).  With register_pages the pages of the
 // tensor-data section are pinned first, where they can be, so the uploads run as
 // asynchronous DMA from them (2 GB of a caller's memory: 92 ms, 40 of them the pinning, without 191).
-static int load_tensors(rnb_b200_decoder *d, const rnb_b200_gguf *g, int register_pages) {
-    rnb_b200_model_cfg c;
-    RNB_TRY(rnb_b200_decoder_config(d, &c));
-    const uint8_t *pinned = nullptr, *pinned_end = nullptr;
-    std::vector<std::vector<uint8_t>> staged;
-    if (register_pages && g->data_start < g->len) {
+// The pages are pinned for the length of the call only: behind a mapping that ends, its address may be another file's.
+struct PinnedSection {
+    const uint8_t *first = nullptr, *last = nullptr;   // what lies between them is pinned
+    bool ours = false;
+    void pin(const rnb_b200_gguf *g) {
         // Best effort: some file systems' read-only mappings cannot be pinned (the driver answers "invalid argument"); the uploads then run as staged pageable
         // copies, same bytes.  Of a mapping, whole pages around the section (it begins with a page and ends with one).  Of a caller's memory, the pages that lie
         // within it: what shares the others is not ours to pin.
         const uintptr_t page = 4096, from = (uintptr_t)g->data + g->data_start, to = (uintptr_t)g->data + g->len;
-        const uintptr_t first = g->map ? from & ~(page - 1) : (from + page - 1) & ~(page - 1), last = g->map ? (to + page - 1) & ~(page - 1) : to & ~(page - 1);
-        if (first < last) {
-            if (rnb_b200_register_host_range((const void *)first, last - first) == RNB_B200_OK) pinned = (const uint8_t *)first, pinned_end = (const uint8_t *)last;
-            else cudaGetLastError();
-        }
+        const uintptr_t begin = g->map ? from & ~(page - 1) : (from + page - 1) & ~(page - 1), end = g->map ? (to + page - 1) & ~(page - 1) : to & ~(page - 1);
+        if (begin >= end) return;
+        std::lock_guard<std::mutex> lock(state_mutex());
+        if (state().open() != RNB_B200_OK || cudaSetDevice(state().device) != cudaSuccess || state().pin((const void *)begin, end - begin, &ours) != RNB_B200_OK) return;
+        first = (const uint8_t *)begin;
+        last = (const uint8_t *)end;
     }
+    void unpin(bool loaded) {
+        if (!ours) return;
+        std::lock_guard<std::mutex> lock(state_mutex());
+        if (!state().is_open) return;   // closed: nothing is pinned any more
+        if (cudaSetDevice(state().device) != cudaSuccess || (!loaded && cudaDeviceSynchronize() != cudaSuccess)) cudaGetLastError();   // (every upload of a load that came to its end has been waited for)
+        state().unpin(first, (size_t)(last - first));
+    }
+};
+static int load_tensors(rnb_b200_decoder *d, const rnb_b200_gguf *g, const PinnedSection &section) {
+    rnb_b200_model_cfg c;
+    RNB_TRY(rnb_b200_decoder_config(d, &c));
+    std::vector<std::vector<uint8_t>> staged;
     // Where a tensor is uploaded from: a copy from a range that is pinned in part is an "invalid argument", so a tensor at an edge goes by way of memory that is not.
     auto source = [&](const uint8_t *p, size_t n) {
-        if (p + n <= pinned || p >= pinned_end || (p >= pinned && p + n <= pinned_end)) return p;
+        if (p + n <= section.first || p >= section.last || (p >= section.first && p + n <= section.last)) return p;
         staged.emplace_back(p, p + n);
         return (const uint8_t *)staged.back().data();
     };
@@ -553,11 +565,16 @@ static int load_tensors(rnb_b200_decoder *d, const rnb_b200_gguf *g, int registe
 }
 int rnb_b200_decoder_load_gguf(rnb_b200_decoder *d, const rnb_b200_gguf *g, int register_pages) {
     if (!d || !g) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
+    PinnedSection section;
+    int rc;
     try {
-        return load_tensors(d, g, register_pages);
+        if (register_pages && g->data_start < g->len) section.pin(g);
+        rc = load_tensors(d, g, section);
     } catch (const std::bad_alloc &) {
-        return fail(RNB_B200_OUT_OF_MEMORY, "GGUF weights: out of host memory");
+        rc = fail(RNB_B200_OUT_OF_MEMORY, "GGUF weights: out of host memory");
     }
+    section.unpin(rc == RNB_B200_OK);
+    return rc;
 }
 
 }  // extern "C"

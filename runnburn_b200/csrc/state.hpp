@@ -134,7 +134,12 @@ struct State {
     PinnedBuf pin_in, pin_out, pin_jobs;
     int *dev_error = nullptr;
     std::map<size_t, KvMirror> kv_mirrors;
-    std::vector<std::pair<void *, size_t>> registered;
+    struct Pinned {
+        void *p;
+        size_t n;
+        int holders;   // calls of pin() that are not undone
+    };
+    std::vector<Pinned> registered;
     int fail_next_allocs = 0;  // host-side fault injection for tests (fake OOM)
 
     int open();
@@ -144,6 +149,8 @@ struct State {
     void evict_all(bool include_pinned);
     int h2d(void *dst, const void *src, size_t n, PinnedBuf &stage, size_t stage_off = 0);
     int check_dev_error();
+    int pin(const void *p, size_t n, bool *held);   // the whole pages within a host range; held: unpin undoes it (false: others have pinned some of it)
+    void unpin(const void *p, size_t n);            // by then nothing is being copied from it
 };
 
 State &state();

@@ -55,6 +55,16 @@ def in_memory(path, offset):
     return room[start:start + data.size]
 
 
+def is_pinned(address):
+    import ctypes as C
+
+    class Attributes(C.Structure):
+        _fields_ = [("type", C.c_int), ("device", C.c_int), ("device_pointer", C.c_void_p), ("host_pointer", C.c_void_p)]
+    a = Attributes()
+    assert C.CDLL("libcudart.so.12").cudaPointerGetAttributes(C.byref(a), C.c_void_p(address)) == 0
+    return a.type != 0
+
+
 def logits(dec):
     return np.concatenate([dec.step(t, i, want_logits=True)[1] for i, t in enumerate((5, 900, 77, 3))])
 
@@ -77,3 +87,64 @@ def test_weights_of_a_caller_s_memory_are_uploaded_from_pinned_pages(tmp_path, o
     ops.clear_host_registered_ranges()
     assert np.array_equal(got[0], got[1]) and np.isfinite(got[0]).all()
     f.close()
+
+
+@pytest.mark.parametrize("where", ["memory", "file", "file in memory"])
+def test_nothing_stays_pinned_behind_a_load(tmp_path, where):
+    """Pages that stay pinned when the file is closed would be taken for those of the next file at their address.  (Whether a mapped
+    file can be pinned goes by the file system.)"""
+    import os
+    from runnburn_b200 import Decoder, RnbError, build, ops
+    from runnburn_b200.gguf import GgufFile, check, load
+    build.build_library()
+    ops.open()
+    path = f"/dev/shm/runnburn-{os.getpid()}.gguf" if where == "file in memory" else str(tmp_path / "m.gguf")
+    try:
+        small_file(path, 12)
+        data = in_memory(path, 32)
+        f = GgufFile(data=memoryview(data)) if where == "memory" else GgufFile(path)
+    finally:
+        if where == "file in memory":
+            os.unlink(path)
+    tensor = f.tensor("blk.0.attn_q.weight")["data"]
+    cfg = f.model_config()
+    dec = Decoder(cfg)
+    check(load().rnb_b200_decoder_load_gguf(dec._h, f._h, 1))
+    assert not is_pinned(tensor)
+    want = logits(dec)
+    # nor behind one that fails
+    with pytest.raises(RnbError, match="already running"):
+        check(load().rnb_b200_decoder_load_gguf(dec._h, f._h, 1))
+    assert not is_pinned(tensor)
+    dec.close()
+    # but what the caller has pinned does
+    if where == "memory":
+        section = data[f.info()["data_start"]:]
+        ops.register_host_range(section)
+        dec = Decoder(cfg)
+        check(load().rnb_b200_decoder_load_gguf(dec._h, f._h, 1))
+        assert is_pinned(tensor) and np.array_equal(logits(dec), want)
+        dec.close()
+        ops.clear_host_registered_ranges()
+        assert not is_pinned(tensor)
+    f.close()
+
+
+def test_files_one_after_another(tmp_path):
+    """Each decoder has its own file's weights, wherever the files are mapped."""
+    from runnburn_b200 import build, ops
+    from runnburn_b200.gguf import load_decoder
+    build.build_library()
+    ops.open()
+    got = []
+    for pin in (False, True):
+        for seed in (21, 22, 23):
+            small_file(tmp_path / "m.gguf", seed)
+            dec, f = load_decoder(str(tmp_path / "m.gguf"), register_pages=pin)
+            (tmp_path / "m.gguf").unlink()
+            f.close()
+            got.append(logits(dec))
+            dec.close()
+    for a, b in zip(got[:3], got[3:]):
+        assert np.array_equal(a, b)
+    assert not np.array_equal(got[0], got[1])
