@@ -850,7 +850,9 @@ int rnb_b200_kv_pages_new(rnb_b200_kv_pages *p, int32_t *seq_out);
 int rnb_b200_kv_pages_extend(rnb_b200_kv_pages *p, int32_t seq, int32_t n_new, int32_t *n_copies, int32_t *src, int32_t *dst, int32_t *rows);
 /* a sequence with the same positions, sharing all pages */
 int rnb_b200_kv_pages_fork(rnb_b200_kv_pages *p, int32_t seq, int32_t *seq_out);
-/* keeps the first `len` positions */
+/* Keeps the first `len` positions.  Refused (RNB_B200_VALIDATION_FAILED) where the next token, at position len, would see a released
+ * page by the window and sinks of the sequence's last release: a program that takes tokens back releases with a window larger by
+ * as many. */
 int rnb_b200_kv_pages_truncate(rnb_b200_kv_pages *p, int32_t seq, int32_t len);
 /* Frees pages that the next token, at position len, and later ones do not see: those whose positions all lie in
  * sinks .. len - window.  Their entries become -1. */

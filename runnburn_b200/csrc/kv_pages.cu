@@ -13,7 +13,8 @@ struct rnb_b200_kv_pages {
     struct Seq {
         bool used = false;
         int32_t len = 0;
-        std::vector<int32_t> pages;   // -1: released
+        int32_t window = 0, sinks = 0;   // of the last release
+        std::vector<int32_t> pages;      // -1: released
     };
     mutable std::mutex mutex;
     int32_t n_pages, page_size;
@@ -151,6 +152,12 @@ int rnb_b200_kv_pages_truncate(rnb_b200_kv_pages *p, int32_t seq, int32_t len) {
     if (len < 0 || len > s->len) return fail(RNB_B200_VALIDATION_FAILED, "KV pages: cannot keep %d of %d positions", len, s->len);
     const size_t keep = (size_t)((len + (int64_t)p->page_size - 1) / p->page_size);
     if (len % p->page_size && s->pages[keep - 1] < 0) return fail(RNB_B200_VALIDATION_FAILED, "KV pages: position %d lies in a released page", len - 1);
+    for (size_t i = 0; i < keep; i++) {   // the window comes back with the positions
+        const int64_t from = (int64_t)i * p->page_size, last = std::min<int64_t>(from + p->page_size, len) - 1;
+        if (s->pages[i] < 0 && (last > (int64_t)len - s->window || from < s->sinks))
+            return fail(RNB_B200_VALIDATION_FAILED, "KV pages: a token at position %d sees position %lld (window %d, %d sinks), which lies in a released page", len,
+                        (long long)(from < s->sinks ? from : last), s->window, s->sinks);
+    }
     for (size_t i = keep; i < s->pages.size(); i++) p->give(s->pages[i]);
     s->pages.resize(keep);
     s->len = len;
@@ -168,6 +175,8 @@ int rnb_b200_kv_pages_release(rnb_b200_kv_pages *p, int32_t seq, int32_t window,
         p->give(s->pages[i]);
         s->pages[i] = -1;
     }
+    s->window = window;
+    s->sinks = sinks;
     return RNB_B200_OK;
 }
 

@@ -294,6 +294,7 @@ class KvPages:
         return s.value
 
     def truncate(self, seq: int, length: int) -> None:
+        """Keeps the first `length` positions; refused where the next token would see a released page (by the last release's window and sinks)."""
         check(load().rnb_b200_kv_pages_truncate(self._h, _int(seq, "seq"), _int(length, "length")))
 
     def release(self, seq: int, window: int, sinks: int = 0) -> None:

@@ -118,6 +118,91 @@ def test_release_keeps_what_later_tokens_see(r, window, sinks, n):
     assert p.info()["free_pages"] == 20
 
 
+def seen_by_the_next_token(length, window, sinks):
+    return [j for j in range(length) if j > length - window or j < sinks]
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (5, 0), (16, 3), (16, 8), (30, 20), (33, 0)])
+def test_truncate_keeps_what_the_next_token_sees(r, window, sinks):
+    """Positions that are taken back bring the window back too: where it reaches a released page the sequence could not go on."""
+    for n in (40, 100, 104):
+        p = r.paged.KvPages(30, 8)
+        for keep in range(n, -1, -1):
+            s = p.new()
+            p.extend(s, n)
+            p.release(s, window, sinks)
+            table = p.tables([s])[0][0]
+            gone = any(table[j // 8] < 0 for j in seen_by_the_next_token(keep, window, sinks)) or (keep % 8 and table[keep // 8] < 0)
+            if gone:
+                before = p.info(), p.tables([s])[0].tolist()
+                with pytest.raises(r.RnbError, match="released page") as e:
+                    p.truncate(s, keep)
+                assert e.value.status == 2 and (p.info(), p.tables([s])[0].tolist()) == before and p.tables([s])[1][0] == n
+            else:
+                p.truncate(s, keep)
+                assert p.tables([s])[1][0] == keep
+                f = p.fork(s)   # and its fork is bound by the same
+                p.extend(f, 9)
+                p.free(f)
+            p.free(s)
+
+
+def test_a_fork_remembers_what_was_released(r):
+    p = r.paged.KvPages(30, 8)
+    s = p.new()
+    p.extend(s, 100)
+    p.release(s, 16)
+    f = p.fork(s)
+    for x in (s, f):
+        with pytest.raises(r.RnbError, match="released page"):
+            p.truncate(x, 90)   # sees from 75 on, and 72 .. 79 are gone
+        p.truncate(x, 96)
+    p.free(s)
+    t = p.new()   # the number of a freed sequence, without its past
+    assert t == s
+    p.extend(t, 100)
+    p.truncate(t, 90)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_sequences_under_a_window_can_always_go_on(r, seed):
+    """Random steps with releases among them: what the next token sees is there, or the step was refused and changed nothing."""
+    rng, m, window, sinks, page = random.Random(seed), Model(r.paged.KvPages(60, 8), r), 20 + seed, seed, 8
+    stamp, told = iter(range(10 ** 9)), {}
+    for _ in range(400):
+        seqs = list(m.want)
+        act = rng.choice(["new", "extend", "extend", "extend", "fork", "truncate", "release", "release", "free", "compact"])
+        s = rng.choice(seqs) if seqs else None
+        try:
+            if act == "new" and len(seqs) < 8:
+                s = m.p.new()
+                m.want[s], told[s] = [], False
+            elif act == "extend" and seqs:
+                m.extend(s, [next(stamp) for _ in range(rng.choice([1, 2, page, 3 * page + 1]))])
+            elif act == "fork" and seqs and len(seqs) < 8:
+                f = m.p.fork(s)
+                m.want[f], told[f] = list(m.want[s]), told[s]
+            elif act == "release" and seqs:
+                m.p.release(s, window, sinks)
+                told[s] = True
+            elif act == "truncate" and seqs:
+                n = max(0, len(m.want[s]) - rng.choice([0, 1, 3, 9, 30]))
+                m.p.truncate(s, n)
+                m.want[s] = m.want[s][:n]
+            elif act == "free" and seqs and rng.random() < 0.4:
+                m.p.free(s)
+                del m.want[s], told[s]
+            elif act == "compact":
+                m.copy(*m.p.compact())
+        except r.RnbError as e:
+            assert "pages needed" in str(e) or (act == "truncate" and "released page" in str(e))
+        for s, want in m.want.items():
+            table, lens = m.p.tables([s])
+            assert lens[0] == len(want)
+            for j in seen_by_the_next_token(len(want), window, sinks) if told[s] else range(len(want)):
+                assert table[0, j // page] >= 0 and m.cache[int(table[0, j // page]), j % page] == want[j]
+
+
 def test_shared_pages_are_freed_once(r):
     p = r.paged.KvPages(4, 8)
     a = p.new()
