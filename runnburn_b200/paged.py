@@ -126,6 +126,10 @@ class PagedCache:
         """The cache of one layer, for the calls that take one."""
         return PagedCache(self.k[i], self.v[i])
 
+    def _one(self) -> None:
+        if self.n_layers != 1:
+            raise ValueError(f"this call takes the cache of one layer, layer(i) of these {self.n_layers}")
+
 
 class PagedBatch:
     """Sequences of a call: their page tables [n_seq, max_pages], positions in the cache [n_seq] (the call's own tokens included) and, unless
@@ -188,6 +192,7 @@ def _rows(t, what: str, tokens: int, heads: int | None, dim: int):
 
 
 def _attention(fn, cache, batch, q, scale, out, window, sinks, lse, workspace, stream):
+    cache._one()
     n, dim = batch.n_tokens, cache.head_dim
     q_stride = _rows(q, "q", n, None, dim)
     heads = q.shape[1]
@@ -227,6 +232,7 @@ def attention_prefill_paged(cache: PagedCache, batch: PagedBatch, q, scale: floa
 
 def paged_kv_append(cache: PagedCache, batch: PagedBatch, k_new, v_new, *, stream=None) -> None:
     """Writes the rows of the batch's tokens, [n_tokens, kv_heads, head_dim], to their places in the pages, rounded to the cache's type."""
+    cache._one()
     stride = _rows(k_new, "k_new", batch.n_tokens, cache.kv_heads, cache.head_dim)
     if _rows(v_new, "v_new", batch.n_tokens, cache.kv_heads, cache.head_dim) != stride or k_new.dtype != v_new.dtype:
         raise ValueError("k_new and v_new have to be alike")

@@ -430,6 +430,21 @@ def test_tensors_on_another_device_than_the_library_s_are_refused(r):
         r.paged.PagedCache(OnDevice(here), OnDevice(here + 1))
 
 
+def test_calls_of_one_layer_refuse_a_cache_of_several(r):
+    """They would take the first one, whichever was meant."""
+    import torch
+    here = r.ops.device_index()
+    at = lambda *shape, t=torch.float16: OnDevice(here, shape, t)  # noqa: E731
+    cache = r.paged.PagedCache(at(3, 4, 16, 2, 64), at(3, 4, 16, 2, 64))
+    assert cache.n_layers == 3
+    batch = r.paged.PagedBatch(at(2, 4, t=torch.int32), at(2, t=torch.int32))
+    rows = at(2, 2, 64)
+    for call in (lambda: r.paged.attention_decode_paged(cache, batch, rows, 0.1, workspace=None, out=rows), lambda: r.paged.paged_kv_append(cache, batch, rows, rows),
+                 lambda: r.paged.attention_prefill_paged(cache, batch, rows, 0.1, workspace=None, out=rows)):
+        with pytest.raises(ValueError, match=r"layer\(i\)"):
+            call()
+
+
 def test_the_device_is_the_one_that_would_be_opened(r):
     """Asked for in a process of its own, where nothing is open."""
     import os
