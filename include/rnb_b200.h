@@ -779,8 +779,8 @@ typedef struct {
     int32_t kv_heads;
     int32_t page_size;  /* positions per page: a power of two from 8 to 256 */
     int32_t n_pages;
-    /* elements from one page, position and head to the next: multiples of 8, at least head_dim.  Rows of
-     * head_dim elements are contiguous and must not overlap; any order of the three is taken */
+    /* elements from one page, position and head to the next: multiples of 8, at least head_dim (of one page or one
+     * head only: anything).  Rows of head_dim elements are contiguous and must not overlap; any order of the three is taken */
     uint64_t page_stride, pos_stride, head_stride;
     void *k, *v;        /* 16-byte aligned */
 } rnb_b200_paged_cache;

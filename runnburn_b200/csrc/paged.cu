@@ -46,8 +46,8 @@ static int pk_check_cache(const rnb_b200_paged_cache *c, PkCache *out) {
     std::sort(steps, steps + 3, [](const Step &a, const Step &b) { return a.stride < b.stride; });
     uint64_t span = dim;
     for (const Step &s : steps) {
-        if (s.stride % 8 || s.stride > (uint64_t)1 << 38) return pk_bad("strides must be multiples of 8 elements below 2^38");
         if (s.n == 1) continue;
+        if (s.stride % 8 || s.stride > (uint64_t)1 << 38) return pk_bad("strides must be multiples of 8 elements, at most 2^38");
         if (s.stride < span) return pk_bad("rows overlap: a stride is smaller than what lies below it");
         span = s.stride * (s.n - 1) + span;
     }

@@ -273,6 +273,9 @@ BAD_CACHE = [
     (dict(v=ADDRESS + 2), 2, "16-byte"), (dict(pos_stride=260), 2, "strides"), (dict(page_stride=2 ** 40), 2, "strides"), (dict(head_stride=64), 2, "overlap"),
     (dict(pos_stride=128), 2, "overlap"), (dict(page_stride=4088), 2, "overlap"), (dict(pos_stride=0), 2, "overlap"),
 ]
+# strides that are never stepped, of one head or one page, say nothing
+FINE_CACHE = [dict(kv_heads=1, head_stride=0), dict(kv_heads=1, head_stride=5), dict(kv_heads=1, head_stride=1 << 40), dict(n_pages=1, page_stride=12), dict(n_pages=1, page_stride=0),
+              dict(n_pages=1, page_stride=3, kv_heads=1, head_stride=1)]
 BAD_BATCH = [
     (dict(n_seq=-1), 2, "negative"), (dict(n_tokens=-1), 2, "negative"), (dict(n_tokens=3), 2, "one token per sequence"), (dict(table=None), 2, "null"),
     (dict(kv_len=None), 2, "null"), (dict(max_pages=0), 2, "max_pages"), (dict(table_stride=3), 2, "table_stride"), (dict(table=ADDRESS + 2), 2, "4-byte"),
@@ -297,6 +300,15 @@ def test_a_bad_cache_is_refused(r, kw, status, what):
     refused(L, attend(L, c, b, prefill=True), status, what)
     refused(L, L.rnb_b200_dev_paged_kv_append(C.byref(c), C.byref(b), 0, ADDRESS, ADDRESS, 256, None), status, what)
     refused(L, L.rnb_b200_dev_paged_kv_copy(C.byref(c), 1, 0, one.ctypes.data, one.ctypes.data, None, 1, None), status, what)
+
+
+@pytest.mark.parametrize("kw", FINE_CACHE)
+def test_strides_that_are_never_stepped_may_be_anything(r, kw):
+    """What is let through stops at the next check, the one for a sequence's one token, or of the batch."""
+    L, c, one = r.load(), cache(r, **kw), np.zeros(1, np.int32)
+    refused(L, attend(L, c, batch(r, q_start=ADDRESS)), 2, "q_start must be null")
+    refused(L, L.rnb_b200_dev_paged_kv_append(C.byref(c), C.byref(batch(r, n_seq=-1)), 0, ADDRESS, ADDRESS, 256, None), 2, "negative")
+    refused(L, L.rnb_b200_dev_paged_kv_copy(C.byref(c), 1, 0, one.ctypes.data, one.ctypes.data, None, 1, None), 2, "read and written")
 
 
 @pytest.mark.parametrize("kw,status,what", BAD_BATCH)
