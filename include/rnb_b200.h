@@ -782,7 +782,7 @@ typedef struct {
     /* elements from one page, position and head to the next: multiples of 8, at least head_dim (of one page or one
      * head only: anything).  Rows of head_dim elements are contiguous and must not overlap; any order of the three is taken */
     uint64_t page_stride, pos_stride, head_stride;
-    void *k, *v;        /* 16-byte aligned */
+    void *k, *v;        /* 16-byte aligned; calls that write refuse pools that share elements */
 } rnb_b200_paged_cache;
 typedef struct {
     const int32_t *table;   /* [n_seq] rows of max_pages entries, table_stride entries apart */
@@ -803,7 +803,7 @@ int rnb_b200_dev_paged_kv_append(const rnb_b200_paged_cache *cache, const rnb_b2
                                  const void *k_new, const void *v_new, size_t src_stride, void *stream);
 /* Copies pages within the pool: for every i the first rows[i] positions (null: all) of all heads of page
  * src[i] to page dst[i], keys and values, in n_layers layers that lie layer_stride elements (a multiple of
- * 8) apart.  The lists are host memory, read before the call returns.  Copies happen as if at the same time:
+ * 8; behind each other, or between the pages, positions or heads of one another) apart.  The lists are host memory, read before the call returns.  Copies happen as if at the same time:
  * a page may be copied to several places, but be written once only, and a page that is written must not be
  * read (RNB_B200_VALIDATION_FAILED). */
 int rnb_b200_dev_paged_kv_copy(const rnb_b200_paged_cache *cache, size_t n_layers, uint64_t layer_stride, const int32_t *src,

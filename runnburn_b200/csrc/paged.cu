@@ -29,6 +29,41 @@ struct PkCall {
 
 static int pk_bad(const char *what) { return fail(RNB_B200_VALIDATION_FAILED, "paged cache: %s", what); }
 
+struct PkStep {
+    uint64_t stride, n;
+};
+// Steps from the smallest to the largest: each at least what the ones below it span, so that no two rows of `dim` elements overlap.  A stride that is
+// never stepped (one head) may be anything.
+static bool pk_steps_apart(PkStep *steps, int n, uint64_t dim) {
+    std::sort(steps, steps + n, [](const PkStep &a, const PkStep &b) { return a.stride < b.stride; });
+    unsigned __int128 span = dim;
+    for (int i = 0; i < n; i++) {
+        if (steps[i].n == 1) continue;
+        if (steps[i].stride < span) return false;
+        span += (unsigned __int128)steps[i].stride * (steps[i].n - 1);
+    }
+    return true;
+}
+// Whether two pools of such steps, in ascending order, share elements when they begin d elements apart: some difference of two rows is d to within a row.
+// From the largest step down, what is left of d has to be below one step: the ones below do not span more.
+static bool pk_pools_meet(const PkStep *steps, int n, uint64_t dim, int64_t d) {
+    if (n == 0) return d < (int64_t)dim && -d < (int64_t)dim;
+    const PkStep &s = steps[n - 1];
+    if (s.n == 1) return pk_pools_meet(steps, n - 1, dim, d);
+    const int64_t stride = (int64_t)s.stride, most = (int64_t)s.n - 1, low = d / stride - (d % stride < 0 ? 1 : 0);
+    for (int64_t i = low; i <= low + 1; i++)
+        if (i >= -most && i <= most && pk_pools_meet(steps, n - 1, dim, d - i * stride)) return true;
+    return false;
+}
+// For calls that write: layers of a pool, and keys and values, must not share elements.
+static int pk_check_written(const rnb_b200_paged_cache *c, size_t n_layers, uint64_t layer_stride) {
+    const uint64_t dim = (uint64_t)c->head_dim;
+    PkStep steps[4] = {{c->page_stride, (uint64_t)c->n_pages}, {c->pos_stride, (uint64_t)c->page_size}, {c->head_stride, (uint64_t)c->kv_heads}, {layer_stride, (uint64_t)n_layers}};
+    if (!pk_steps_apart(steps, 4, dim)) return pk_bad("layers overlap: a stride is smaller than what lies below it");
+    if (pk_pools_meet(steps, 4, dim, ((int64_t)(uintptr_t)c->v - (int64_t)(uintptr_t)c->k) / 2)) return pk_bad("keys and values overlap");
+    return RNB_B200_OK;
+}
+
 static int pk_check_cache(const rnb_b200_paged_cache *c, PkCache *out) {
     if (!c || !c->k || !c->v) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
     if (c->type != RNB_B200_TYPE_F16 && c->type != RNB_B200_TYPE_BF16) return fail(RNB_B200_UNSUPPORTED, "paged cache: type must be F16 or BF16, got %u", c->type);
@@ -37,20 +72,10 @@ static int pk_check_cache(const rnb_b200_paged_cache *c, PkCache *out) {
     if (c->page_size < 8 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
         return fail(RNB_B200_VALIDATION_FAILED, "paged cache: page_size must be a power of two from 8 to 256, got %d", c->page_size);
     if (c->n_pages < 1) return fail(RNB_B200_VALIDATION_FAILED, "paged cache: n_pages must be at least 1, got %d", c->n_pages);
-    // Strides from the smallest to the largest: each at least what the ones below it span, so that no two rows overlap.  A stride that is
-    // never stepped (one head) may be anything.
-    const uint64_t dim = (uint64_t)c->head_dim;
-    struct Step {
-        uint64_t stride, n;
-    } steps[3] = {{c->page_stride, (uint64_t)c->n_pages}, {c->pos_stride, (uint64_t)c->page_size}, {c->head_stride, (uint64_t)c->kv_heads}};
-    std::sort(steps, steps + 3, [](const Step &a, const Step &b) { return a.stride < b.stride; });
-    uint64_t span = dim;
-    for (const Step &s : steps) {
-        if (s.n == 1) continue;
-        if (s.stride % 8 || s.stride > (uint64_t)1 << 38) return pk_bad("strides must be multiples of 8 elements, at most 2^38");
-        if (s.stride < span) return pk_bad("rows overlap: a stride is smaller than what lies below it");
-        span = s.stride * (s.n - 1) + span;
-    }
+    PkStep steps[3] = {{c->page_stride, (uint64_t)c->n_pages}, {c->pos_stride, (uint64_t)c->page_size}, {c->head_stride, (uint64_t)c->kv_heads}};
+    for (const PkStep &s : steps)
+        if (s.n > 1 && (s.stride % 8 || s.stride > (uint64_t)1 << 38)) return pk_bad("strides must be multiples of 8 elements, at most 2^38");
+    if (!pk_steps_apart(steps, 3, (uint64_t)c->head_dim)) return pk_bad("rows overlap: a stride is smaller than what lies below it");
     if (((uintptr_t)c->k | (uintptr_t)c->v) & 15u) return pk_bad("k and v must be 16-byte aligned");
     int shift = 0;
     while ((1 << shift) < c->page_size) shift++;
@@ -80,6 +105,7 @@ static int pk_append(const rnb_b200_paged_cache *cache, const rnb_b200_paged_bat
     if (!k_new || !v_new) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");
     if (((uintptr_t)k_new | (uintptr_t)v_new) & 15u || src_stride % 8) return pk_bad("rows must be 16-byte aligned and src_stride a multiple of 8");
     if (b.n_tokens > 1 && src_stride < (size_t)c.kv_heads * c.head_dim) return pk_bad("src_stride is smaller than a token's rows");
+    RNB_TRY(pk_check_written(cache, 1, 0));
     PkCall call;
     RNB_TRY(call.rc);
     const dim3 grid((unsigned)b.n_tokens), block((unsigned)std::min(256, (c.kv_heads * c.head_dim / 8 + 31) / 32 * 32));
@@ -129,6 +155,7 @@ static int pk_copy(const rnb_b200_paged_cache *cache, size_t n_layers, uint64_t 
         role[src[i]] = 1;
         role[dst[i]] = 2;
     }
+    RNB_TRY(pk_check_written(cache, n_layers, layer_stride));
     PkCall call;
     RNB_TRY(call.rc);
     for (size_t at = 0; at < n;) {

@@ -468,6 +468,51 @@ def test_the_device_is_the_one_that_would_be_opened(r):
         assert got.stdout.strip() == want, got.stderr
 
 
+def places(strides, counts, dim):
+    """Every element of a pool."""
+    import itertools
+    return {sum(i * s for i, s in zip(at, strides)) + e for at in itertools.product(*map(range, counts)) for e in range(dim)}
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_what_is_written_must_not_overlap(r, seed):
+    """Layers and the pools of keys and values, wherever they lie: side by side, one in the gaps of the other, or on top of each other in part."""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are made up, and a call that is let through would run")
+    rng, L, n_free, n_met = random.Random(seed), r.load(), 0, 0
+    a, b = np.zeros(1, np.int32), np.ones(1, np.int32)
+    for _ in range(400):
+        counts = [rng.choice([1, 2, 3]), rng.choice([2, 3]), 8, rng.choice([1, 2])]   # layers, pages, positions, heads
+        strides, span = [0] * 4, 8
+        for i in rng.sample(range(4), 4):
+            strides[i] = span + rng.choice([0, 0, 8, 24])
+            span = strides[i] * (counts[i] - 1) + span if counts[i] > 1 else span
+        if rng.random() < 0.3:
+            strides[0] = 8 * rng.randint(1, span // 8)   # layers anywhere
+        shift = 8 * rng.choice([0, 1, rng.randint(0, span // 8 + 2), rng.randint(0, 40)]) * rng.choice([-1, 1])
+        c = cache(r, head_dim=8, kv_heads=counts[3], page_size=8, n_pages=counts[1], page_stride=strides[1], pos_stride=strides[2], head_stride=strides[3],
+                  k=ADDRESS + (1 << 20), v=ADDRESS + (1 << 20) + 2 * shift)
+        for layers in {1, counts[0]}:
+            n = [layers] + counts[1:]
+            keys = places(strides, n, 8)
+            met = not keys.isdisjoint(x + shift for x in keys) or len(keys) < 8 * n[0] * n[1] * n[2] * n[3]
+            rc = L.rnb_b200_dev_paged_kv_copy(C.byref(c), layers, strides[0], a.ctypes.data, b.ctypes.data, None, 1, None) if counts[1] > 1 else None
+            said = L.rnb_b200_last_error().decode()
+            if met:
+                assert rc == 2 and "overlap" in said, (n, strides, shift, said)
+                n_met += 1
+            elif "overlap" in said and rc == 2:   # layers that lie between others without a common element, but not one level inside the next
+                assert "layers" in said and strides[0] < span, (n, strides, shift, said)
+            else:
+                assert rc != 2, (n, strides, shift, said)   # without a GPU the call ends behind its checks
+                n_free += 1
+            if layers == 1:
+                rc = L.rnb_b200_dev_paged_kv_append(C.byref(c), C.byref(batch(r)), 0, ADDRESS, ADDRESS, 8 * counts[3], None)
+                assert (rc == 2 and "overlap" in L.rnb_b200_last_error().decode()) == met
+    assert n_free > 100 and n_met > 100
+
+
 def test_nothing_to_do_is_no_call(r):
     """No tokens, no sequences, no copies: fine without a GPU."""
     L = r.load()
