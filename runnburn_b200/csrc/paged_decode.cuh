@@ -25,7 +25,9 @@ constexpr float PD_BIAS = 12.f;
 // where there are CTAs enough.  32 heads on 8 key heads, 128 dims: 300 positions 7.0 us, 600 8.1, 1000 8.7 (with runs of four tiles 10.6, 10.5, 9.9);
 // 32768 positions of one key head 19.8 us (with the shortest that give all CTAs work 35.5).
 constexpr float PD_RUN = 0.25f;
-constexpr int PD_WHOLE = 3;   // tiles of a sequence that is not cut at all (180 positions: 6.4 us, cut 6.9; 250: 7.2, cut 7.0)
+// Where the longest sequence has up to so many tiles, the shortest run is as long as it: sequences of one length are then not cut at all (180 positions: 6.4 us,
+// cut 6.9; 250: 7.2, cut 7.0).  Of unlike ones some still are, at the ends of equal runs.
+constexpr int PD_WHOLE = 3;
 constexpr size_t PD_WS_HEAD = 256;                      // a mark that the workspace has been initialised
 constexpr int PD_MAX_GRID = 1024;                       // runs of a launch
 constexpr size_t PD_WS_RECORDS = PD_WS_HEAD + PD_MAX_GRID * sizeof(unsigned);

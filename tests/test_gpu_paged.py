@@ -114,6 +114,16 @@ def test_decode_split_and_joined(P, ws, kv_len, heads, kv_heads, q, cache, dim):
     assert (c.run(ws) == first).all()   # the sums' order does not depend on who comes first
 
 
+@pytest.mark.parametrize("kv_len", [[128, 192], [192, 128, 64, 1, 130, 64, 192, 65], [64] * 5 + [192], [1, 192] * 40])
+@pytest.mark.parametrize("q,cache,dim,heads", [("f32", "f16", 128, 3), ("bf16", "bf16", 64, 8), ("f16", "f16", 128, 16)])
+def test_decode_of_short_sequences_that_differ(P, ws, kv_len, q, cache, dim, heads):
+    """One key head and sequences of one to three tiles, some of which the equal runs cut."""
+    c = Case(P, kv_len, heads=heads, kv_heads=1, q=q, cache=cache, dim=dim, seed=len(kv_len))
+    first = c.run(ws)
+    c.check(first)
+    assert (c.run(ws) == first).all()
+
+
 # ---- prompts ------------------------------------------------------------------------------------------------------------
 PROMPTS = [
     ([1], [1]), ([5], [5]), ([64], [64]), ([129], [65]), ([300, 0, 77], [33, 0, 77]), ([1000, 130, 7, 64], [1, 130, 2, 63]), ([257], [256]), ([513, 700], [513, 31]),
@@ -451,6 +461,105 @@ def test_a_new_workspace_serves_any_stream(P):
     out = c.run(space, stream=s)
     s.synchronize()
     c.check(out)
+
+
+@pytest.mark.parametrize("q,cache", PAIRS)
+@pytest.mark.parametrize("prompt", [False, True])
+def test_a_captured_step_with_room(P, prompt, q, cache):
+    """Append and attention captured once, with tables as wide as the longest sequence may become, sequences that are not there (of length zero, or
+    without tokens) and rows of padding; replayed with other lengths, starts and pages, two graphs on one workspace in turns."""
+    import torch
+    page, kvh, heads, dim, n_pages, width, i32 = 16, 2, 8, 64, 400, 2000, dict(dtype=torch.int32, device="cuda")
+    g, h = torch.Generator("cuda").manual_seed(3), torch.Generator().manual_seed(3)
+    n_seq, tokens, dt = 6, 90 if prompt else 6, TYPES[q]
+    steps = [([200, 0, 33, 700, 5, 0], [40, 0, 33, 1, 2, 0]), ([64, 128, 0, 0, 0, 1], [64, 20, 0, 0, 0, 1]), ([0] * 6, [0] * 6), ([1500, 1, 1, 1, 1, 1], [85, 1, 1, 1, 1, 1])]
+    if not prompt:
+        steps = [(kv, [int(n > 0) for n in kv]) for kv, _ in steps]
+    stream, space, sides = torch.cuda.Stream(), P.Workspace(), []
+    for window in (0, 50):
+        k, v = (torch.randn(n_pages, page, kvh, dim, device="cuda", generator=g).to(TYPES[cache]) for _ in range(2))
+        s = dict(k=k, v=v, window=window, table=torch.zeros(n_seq, width, **i32), kv=torch.zeros(n_seq, **i32), start=torch.zeros(n_seq + 1, **i32),
+                 q=torch.zeros(tokens, heads, dim, device="cuda", dtype=dt), rows=torch.zeros(2, tokens, kvh, dim, device="cuda", dtype=dt),
+                 out=torch.zeros(tokens, heads, dim, device="cuda", dtype=dt), lse=torch.zeros(tokens, heads, device="cuda"), graph=torch.cuda.CUDAGraph())
+        one, ragged = P.PagedCache(k, v), P.PagedBatch(s["table"], s["kv"], s["start"], tokens)
+        batch = ragged if prompt else P.PagedBatch(s["table"], s["kv"])
+        torch.cuda.synchronize()
+        with torch.cuda.graph(s["graph"], stream=stream):
+            P.paged_kv_append(one, ragged, s["rows"][0], s["rows"][1])   # (a sequence that is not there has no token here)
+            (P.attention_prefill_paged if prompt else P.attention_decode_paged)(one, batch, s["q"], dim ** -0.5, out=s["out"], lse=s["lse"], window=window, sinks=2, workspace=space)
+        sides.append(s)
+    for kv, new in steps * 2:
+        table = pu.tables(kv, page, n_pages, h, width)
+        start = torch.tensor([0] + new).cumsum(0)
+        used = int(start[-1])
+        for s in sides:
+            s["table"].copy_(table), s["kv"].copy_(torch.tensor(kv)), s["start"].copy_(start)
+            s["q"].normal_(generator=g), s["rows"].normal_(generator=g), s["out"].fill_(3), s["lse"].fill_(3)
+        # of a step of single tokens, the rows of append follow each other, those of attention go by sequence
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for _ in range(2):
+                for s in sides:
+                    s["graph"].replay()
+        torch.cuda.synchronize()
+        for s in sides:
+            for i, (n, m) in enumerate(zip(kv, new)):
+                j = torch.arange(n - m, n)
+                at = table[i, j // page].long().cuda(), (j % page).cuda()
+                for t, rows in zip((s["k"], s["v"]), s["rows"]):
+                    assert torch.equal(t[at], rows[start[i]:start[i + 1]].to(t.dtype))
+            rows = list(range(used)) if prompt else [i for i in range(n_seq) if kv[i]]
+            starts = start.tolist() if prompt else list(range(n_seq + 1))
+            out, lse, mass = pu.attention(s["q"], s["k"], s["v"], table, page, kv, starts, dim ** -0.5, s["window"], 2)
+            assert worst(s["out"][rows], out[rows], tolerance(out, mass, dt)[rows]) <= 1 if rows else True
+            assert bool(((s["lse"][rows].double() - lse[rows]).abs() <= LSE_OFF + lse[rows].abs() * 2.0 ** -22).all())
+            rest = [i for i in range(tokens) if i not in rows]
+            assert (s["out"][rest] == (3 if prompt else 0)).all() and (s["lse"][rest] == (3 if prompt else -math.inf)).all()
+
+
+def test_threads_that_call_at_once(P):
+    """Each with a stream and a workspace of its own."""
+    import threading
+
+    import torch
+    kinds = [dict(kv_len=[3000, 5, 700]), dict(kv_len=[300, 0, 77], new=[33, 0, 77], q="bf16", cache="bf16"), dict(kv_len=[900, 40], new=[700, 3], dim=64),
+             dict(kv_len=[64] * 30, q="f16", heads=16, kv_heads=1)]
+    cases = [Case(P, **k, seed=i) for i, k in enumerate(kinds * 2)]
+    torch.cuda.synchronize()
+    outs, failed = [[] for _ in cases], []
+
+    def work(i):
+        try:
+            c, s, space = cases[i], torch.cuda.Stream(), P.Workspace()
+            n, kvh, dim = c.batch.n_tokens, c.k.shape[2], c.k.shape[3]
+            k, v = (torch.zeros(4, 16, kvh, dim, device="cuda", dtype=c.k.dtype) for _ in range(2))
+            mine = P.PagedCache(k, v)
+            s.wait_stream(torch.cuda.current_stream())
+            for turn in range(30):
+                out = torch.empty_like(c.q)
+                s.wait_stream(torch.cuda.current_stream())
+                c.run(space, out=out, stream=s, lse=None)
+                P.paged_kv_copy(mine, [0, 1], [2, 3], stream=s)
+                outs[i].append(out)
+                pages = P.KvPages(20, 16)
+                a = pages.new()
+                pages.extend(a, 50 + turn)
+                pages.free(a)
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001 - told by the main thread
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for c, got in zip(cases, outs):
+        for out in got:
+            assert torch.equal(out, got[0])
+        c.run(P.Workspace(), out=got[1])   # the sums beside it
+        c.check(got[0])
 
 
 def test_a_sequence_in_more_parts_than_a_join_has_weights_for(P, ws):
