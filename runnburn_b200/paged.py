@@ -158,8 +158,9 @@ class PagedBatch:
 
 
 class Workspace:
-    """Scratch of the attention calls, on the library's device, allocated on the given stream and initialised when this returns (unless the stream is being captured).  Calls that may
-    overlap on the GPU (other streams) need one each."""
+    """Scratch of the attention calls, on the library's device, allocated on the given stream and initialised when this returns (unless the
+    stream is being captured).  Calls that may overlap on the GPU (other streams) need one each.  PyTorch's streams that use it are told to the
+    allocator; work on a stream that is given by its handle has to be through before the workspace goes."""
 
     def __init__(self, device=None, stream=None):
         import torch
@@ -174,10 +175,13 @@ class Workspace:
                 torch.cuda.current_stream(self.index).synchronize()   # it may be used on any stream from here on
         self._streams = {on}
 
-    def _used_on(self, handle: int) -> None:
-        """The memory is not given to others before this stream's work is through, either."""
-        self.buffer.record_stream(_stream_object(self.index, handle))
-        self._streams.add(handle)
+    def _used_on(self, handle: int, stream) -> None:
+        """The memory is not given to others before this stream's work is through, either.  (Not of a bare handle: its stream may be gone by the time that
+        the allocator would ask it.)"""
+        import torch
+        if stream is None or (isinstance(stream, torch.cuda.Stream) and not isinstance(stream, torch.cuda.ExternalStream)):
+            self.buffer.record_stream(_stream_object(self.index, handle))
+            self._streams.add(handle)
 
 
 def _rows(t, what: str, tokens: int, heads: int | None, dim: int):
@@ -212,7 +216,7 @@ def _attention(fn, cache, batch, q, scale, out, window, sinks, lse, workspace, s
         lse = lse.data_ptr()
     on = _stream(index, stream)
     if on not in workspace._streams:
-        workspace._used_on(on)
+        workspace._used_on(on, stream)
     check(fn(cache._ref, batch._ref, _type(q), q.data_ptr(), q_stride, heads, scale, _int(window, "window"), _int(sinks, "sinks"), workspace.ptr, workspace.bytes, out.data_ptr(), out_stride, lse, on))
     return out
 

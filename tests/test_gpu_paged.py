@@ -451,6 +451,26 @@ def test_a_workspace_that_goes_while_another_stream_uses_it(P):
     c.check(out)
 
 
+def test_a_workspace_outlives_a_foreign_stream(P):
+    """A stream that PyTorch does not know, given by its handle, may be gone before the workspace."""
+    import ctypes as C
+
+    import torch
+    rt, handle, c, space = C.CDLL("libcudart.so.12"), C.c_void_p(), Case(P, [3000, 5]), P.Workspace()
+    torch.cuda.synchronize()
+    assert rt.cudaStreamCreate(C.byref(handle)) == 0
+    out = c.run(space, stream=handle.value)
+    again = c.run(space, stream=handle)
+    torch.cuda.synchronize()
+    assert rt.cudaStreamDestroy(handle) == 0
+    n = space.bytes
+    del space
+    torch.empty(n, dtype=torch.uint8, device="cuda").zero_()
+    torch.cuda.synchronize()
+    assert torch.equal(out, again)
+    c.check(out)
+
+
 def test_a_new_workspace_serves_any_stream(P):
     """Without a wait of the caller's between its making and its use."""
     import torch
