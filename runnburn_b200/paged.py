@@ -330,5 +330,5 @@ class KvPages:
             max_pages = max(1, -(-int(lens.max(initial=0)) // self.page_size))
         _int(max_pages, "max_pages")
         table = np.empty((seqs.size, max_pages), np.int32)
-        check(load().rnb_b200_kv_pages_tables(self._h, seqs.ctypes.data, seqs.size, table.ctypes.data, max_pages, None))
+        check(load().rnb_b200_kv_pages_tables(self._h, seqs.ctypes.data, seqs.size, table.ctypes.data, max_pages, lens.ctypes.data))   # both of one moment
         return table, lens

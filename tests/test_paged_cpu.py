@@ -410,6 +410,32 @@ def test_numbers_of_more_than_32_bits_are_refused(r):
         r.paged.PagedBatch(table, lens, start, far + 9)
 
 
+def test_tables_and_lengths_are_of_one_moment(r, monkeypatch):
+    """Another thread may shorten a sequence while its table is asked for."""
+    p = r.paged.KvPages(8, 8)
+    s = p.new()
+    p.extend(s, 40)
+    real, calls = r.paged.load(), []
+
+    class Between:
+        """Takes positions back behind the first question for tables."""
+        def __getattr__(self, name):
+            f = getattr(real, name)
+            if name != "rnb_b200_kv_pages_tables":
+                return f
+
+            def asked(*a):
+                rc = f(*a)
+                if not calls:
+                    calls.append(1)
+                    assert real.rnb_b200_kv_pages_truncate(p._h, s, 10) == 0
+                return rc
+            return asked
+    monkeypatch.setattr(r.paged, "load", lambda: Between())
+    table, lens = p.tables([s])
+    assert calls and lens[0] in (10, 40) and (table[0] >= 0).sum() == -(-lens[0] // 8)
+
+
 def test_copies_refuse_bad_layers(r):
     L, z = r.load(), np.array([0, 1], np.int32)
     for layers, stride in ((0, 0), (40000, 1 << 20), (2, 0), (2, 12), (2, 1 << 40), (1, (1 << 64) - 8)):
