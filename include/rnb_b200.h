@@ -808,7 +808,7 @@ int rnb_b200_dev_paged_kv_append(const rnb_b200_paged_cache *cache, const rnb_b2
  * read (RNB_B200_VALIDATION_FAILED). */
 int rnb_b200_dev_paged_kv_copy(const rnb_b200_paged_cache *cache, size_t n_layers, uint64_t layer_stride, const int32_t *src,
                                const int32_t *dst, const int32_t *rows, size_t n_pages, void *stream);
-/* softmax(scale q.K^T) V over the pages.  A query at position p sees positions j <= p with window = 0, else
+/* softmax(scale q.K^T) V over the pages; |scale| up to 2.3e38.  A query at position p sees positions j <= p with window = 0, else
  * those with j > p - window or j < sinks.  A query that sees nothing (kv_len 0) gets zeros.  q_type: F32 with an
  * F16 cache, or the cache's type; `out` has the same type.  Sums, maxima and the softmax are f32.  f32 queries and
  * their probabilities enter the products as two f16 terms: 22 bits are kept of elements down to 2^-17 of their row's

@@ -205,7 +205,8 @@ static int pk_check_attention(const rnb_b200_paged_cache *cache, const rnb_b200_
     if (!(q_type == cache->type || (q_type == RNB_B200_TYPE_F32 && cache->type == RNB_B200_TYPE_F16)))
         return fail(RNB_B200_UNSUPPORTED, "paged attention: queries must be F32 on an F16 cache or of the cache's type, got type %u on %u", q_type, cache->type);
     if (window < 0 || sinks < 0) return fail(RNB_B200_VALIDATION_FAILED, "paged attention: window and sinks must not be negative, got %d and %d", window, sinks);
-    if (!(scale - scale == 0.f)) return fail(RNB_B200_VALIDATION_FAILED, "paged attention: scale must be finite");
+    const float to_log2 = scale * 1.4426950408889634f;
+    if (!(to_log2 - to_log2 == 0.f)) return fail(RNB_B200_VALIDATION_FAILED, "paged attention: scale must be finite, and so must scale * log2(e)");
     if (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < PK_WORKSPACE_BYTES)
         return fail(RNB_B200_VALIDATION_FAILED, "paged attention: the workspace must be 256-byte aligned and hold %zu bytes, got %zu", PK_WORKSPACE_BYTES, workspace_bytes);
     if (a->b.n_tokens > 0 && (!q || !out)) return fail(RNB_B200_VALIDATION_FAILED, "null pointer argument");

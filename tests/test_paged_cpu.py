@@ -331,6 +331,13 @@ def test_attention_refuses(r, kw, status, what):
         refused(L, attend(L, cache(r), batch(r), prefill=prefill, **kw), status, what)
 
 
+@pytest.mark.parametrize("scale,fine", [(3e38, False), (-3e38, False), (2.4e38, False), (2.3e38, True), (-2.3e38, True), (0.0, True), (-float("inf"), False)])
+def test_scales_up_to_the_end_of_f32(r, scale, fine):
+    """Scores are counted in powers of two: the scale times log2 e has to be a number.  What is let through stops at the check behind it."""
+    L = r.load()
+    refused(L, attend(L, cache(r), batch(r), scale=scale, ws=None), 2, "workspace" if fine else "scale")
+
+
 @pytest.mark.parametrize("tokens,q_stride,out_stride,shift,ok", [
     (2, 512, 512, 0, False), (2, 512, 512, 2048, False), (2, 512, 512, 4096, True), (2, 512, 512, -4096, True), (2, 512, 512, -4080, False), (1, 512, 512, 2048, True),
     (1, 512, 512, 2032, False), (5, 1024, 1024, 2048, True), (5, 1024, 1024, -2048, True), (5, 1024, 1024, 2064, False), (5, 1024, 1024, 4096 * 3 + 2048, True),
