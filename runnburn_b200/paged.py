@@ -3,7 +3,7 @@
 The functions take device tensors of PyTorch (anything with its `data_ptr`, `shape`, `stride`, `dtype`, `device` and the like will do)
 on the library's device (`ops.device_index()`), whatever device is current, and run on the given stream (a stream of PyTorch or its
 handle), else on PyTorch's current one; they do not synchronise and allocate nothing but a missing `out`, so calls with `out` can be
-captured into graphs.  A missing `out` is allocated on the stream that writes it.  Tensors that the caller brings are used as they are:
+captured into graphs once the library is open (`ops.open()`, or a `Workspace`).  A missing `out` is allocated on the stream that writes it.  Tensors that the caller brings are used as they are:
 those of another stream than the call's have to be kept until it is through (`record_stream`), as ever in PyTorch.  Tables, lengths and
 starts are read when the work runs.  What they hold is checked on the device: a page outside the pool, a length that the table cannot
 hold or a start out of order sets the device error word (`ops.dev_error_flag()` returns 5) instead of touching memory outside.  The C
@@ -158,29 +158,41 @@ class PagedBatch:
 
 
 class Workspace:
-    """Scratch of the attention calls, on the library's device, allocated on the given stream and initialised when this returns (unless the
-    stream is being captured).  Calls that may overlap on the GPU (other streams) need one each.  PyTorch's streams that use it are told to the
-    allocator; work on a stream that is given by its handle has to be through before the workspace goes."""
+    """Scratch of the attention calls, on the library's device, allocated and initialised on the given stream; other streams wait for that at
+    their first call (one that is being captured does not: begin the capture behind it).  Calls that may overlap on the GPU (other streams)
+    need one each.  PyTorch's streams that use it are told to the allocator; work on a stream that is given by its handle has to be through
+    before the workspace goes."""
 
     def __init__(self, device=None, stream=None):
         import torch
         device = torch.device("cuda", ops.device_index()) if device is None else torch.device(device)
         n = load().rnb_b200_paged_workspace_bytes()
+        self._ready = None
         with torch.cuda.device(device), _allocating(device.index, stream):
             self.buffer = torch.empty(n, dtype=torch.uint8, device=device)
             self.index, self.ptr, self.bytes = _library_index(self.buffer), self.buffer.data_ptr(), n
             on = _stream(self.index, stream)
             check(load().rnb_b200_paged_workspace_init(self.ptr, n, on))
             if not torch.cuda.is_current_stream_capturing():
-                torch.cuda.current_stream(self.index).synchronize()   # it may be used on any stream from here on
-        self._streams = {on}
+                self._ready = torch.cuda.current_stream(self.index).record_event()
+        self._streams, self._handles = {on}, set()   # that have waited: PyTorch's, and bare handles
 
     def _used_on(self, handle: int, stream) -> None:
-        """The memory is not given to others before this stream's work is through, either.  (Not of a bare handle: its stream may be gone by the time that
-        the allocator would ask it.)"""
+        """Another stream's first call."""
         import torch
-        if stream is None or (isinstance(stream, torch.cuda.Stream) and not isinstance(stream, torch.cuda.ExternalStream)):
-            self.buffer.record_stream(_stream_object(self.index, handle))
+        bare = stream is not None and (not isinstance(stream, torch.cuda.Stream) or isinstance(stream, torch.cuda.ExternalStream))
+        if bare and handle in self._handles:
+            return
+        other = _stream_object(self.index, handle)
+        with torch.cuda.stream(other):
+            if torch.cuda.is_current_stream_capturing():
+                return
+        if self._ready is not None:
+            other.wait_event(self._ready)
+        if bare:   # (not told to the allocator: the stream may be gone by the time that it would be asked)
+            self._handles.add(handle)
+        else:
+            self.buffer.record_stream(other)
             self._streams.add(handle)
 
 

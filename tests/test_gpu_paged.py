@@ -471,14 +471,16 @@ def test_a_workspace_outlives_a_foreign_stream(P):
     c.check(out)
 
 
-def test_a_new_workspace_serves_any_stream(P):
+@pytest.mark.parametrize("bare", [False, True])
+def test_a_new_workspace_serves_any_stream(P, bare):
     """Without a wait of the caller's between its making and its use."""
     import torch
     c = Case(P, [9000, 3])
     torch.cuda.synchronize()
     torch.cuda._sleep(50_000_000)
     space, s = P.Workspace(), torch.cuda.Stream()
-    out = c.run(space, stream=s)
+    assert not torch.cuda.current_stream().query()   # it does not wait itself
+    out = c.run(space, stream=s.cuda_stream if bare else s)
     s.synchronize()
     c.check(out)
 
