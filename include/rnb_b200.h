@@ -765,7 +765,8 @@ int rnb_b200_attention_decode_hd128_noalloc_status(int *status_out, void *stream
  *
  * Device-pointer tier: all pointers but the host structs themselves and the lists of
  * rnb_b200_dev_paged_kv_copy are device addresses on the library's device (RNB_CUDA_DEVICE); calls may
- * come with another device current, allocate nothing, do not synchronise and can be captured into graphs.
+ * come with another device current, allocate nothing, do not synchronise and can be captured into graphs once the
+ * library is open (rnb_b200_open, or any earlier call).
  * Tables, lengths and starts are read on the device when the work runs.  What they hold is checked there:
  * a page outside the pool, a length outside the table or a start out of order raises
  * RNB_B200_DEVICE_BAD_PAGE in the device error word (rnb_b200_dev_error_flag) instead of touching memory
@@ -797,7 +798,8 @@ typedef struct {
 } rnb_b200_paged_batch;
 /* K and V rows of the call's tokens to their places in the pages, rounded to the cache's type (to nearest,
  * ties to even).  src_type: F32, or the cache's type.  k_new, v_new [n_tokens][kv_heads][head_dim], 16-byte
- * aligned, src_stride elements from one token to the next (a multiple of 8).  Pages that several sequences
+ * aligned, src_stride elements from one token to the next (a multiple of 8), outside the pools.  A sequence that is not there
+ * (kv_len 0) has no tokens by q_start; without q_start its token has no place, which is flagged.  Pages that several sequences
  * share are the caller's to part first (rnb_b200_kv_pages_extend says which). */
 int rnb_b200_dev_paged_kv_append(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t src_type,
                                  const void *k_new, const void *v_new, size_t src_stride, void *stream);
@@ -814,14 +816,15 @@ int rnb_b200_dev_paged_kv_copy(const rnb_b200_paged_cache *cache, size_t n_layer
  * their probabilities enter the products as two f16 terms: 22 bits are kept of elements down to 2^-17 of their row's
  * largest, 19 bits down to 2^-20, and outputs are some 6e-7 off where f32 throughout gives 4e-7.  q, out
  * [n_tokens][heads][head_dim], 16-byte aligned, q_stride / out_stride elements from one token to the next
- * (multiples of 8), that do not overlap; heads a multiple of kv_heads.  lse (may be null): f32 [n_tokens][heads], the logarithm of
- * the sum of exponentials, -inf for a query that sees nothing.
+ * (multiples of 8), that do not overlap (nor lse); heads a multiple of kv_heads.  lse (may be null): f32 [n_tokens][heads], the
+ * logarithm of the sum of exponentials, -inf for a query that sees nothing.
  * `workspace`: rnb_b200_paged_workspace_bytes() bytes, 256-byte aligned, initialised once by
  * rnb_b200_paged_workspace_init; one workspace serves any number of calls one after another (of any sizes, of both
  * calls, of captured graphs), but calls that may overlap on the GPU need one each.  Decode keeps parts of long
  * sequences there until they are joined; _prefill checks the argument and joins on the chip.
  * _decode: one new token per sequence (q_start null), the work split over the lengths so that few sequences
- * use the whole GPU too.  _prefill: the tokens of every sequence, causal. */
+ * use the whole GPU too.  _prefill: the tokens of every sequence, causal; how its work is shared out goes by max_pages, so
+ * short prompts are faster with a table that is not much wider than they need. */
 size_t rnb_b200_paged_workspace_bytes(void);
 int rnb_b200_paged_workspace_init(void *workspace, size_t workspace_bytes, void *stream);
 int rnb_b200_dev_attention_decode_paged(const rnb_b200_paged_cache *cache, const rnb_b200_paged_batch *batch, uint32_t q_type,

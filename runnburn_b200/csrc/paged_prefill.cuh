@@ -9,14 +9,16 @@
 // 16-bit queries: two blocks, which use a tile while it is in shared memory, two threads a row.  One block's softmax runs under the other's
 // products.  Tensor memory holds two outputs and probabilities, and scores of one block at a time: as soon as they are read it is the other's turn.
 // What sets the pace is this turn: 1650 cycles from one block's reading to the other's (the exponentials take 1024 of a block's tile, its products 1100).
-// (5 prompts of up to 512 tokens behind up to 6000, 32 heads on 8: 92 us; with columns of its own for each block's scores, in which its probabilities come, so
-// that the next scores wait for their product: 117; the same in steps of 64 keys, two of them in flight: 146.)
-// Queries are exact; probabilities are rounded once to the cache's type, half a step of the output's own rounding.
+// (5 prompts of up to 512 tokens behind up to 6000, 32 heads on 8: 93 us.  Of 92, with one meeting a tile of a row's warps less: with columns of its own for each
+// block's scores, in which its probabilities come, so that the next scores wait for their product: 117; the same in steps of 64 keys, two of them in flight: 146.)
+// Queries are exact; probabilities are rounded once to the cache's type, half a step of the output's own rounding (against 64 bits 1.9e-3 with bf16 and 2.7e-4
+// with f16, where rounded outputs alone give 1.6e-3 and 2.0e-4; in two terms every product of theirs would be made twice).  The sum that divides the output is of
+// the probabilities as they were, since the logarithm of the sum keeps f32 accuracy: keys that all score alike are off by their common rounding.
 //
 // f32 queries: one block, four threads a row.  Queries enter as f16 "hi" + remainder "lo" (scaled by a power of two per row into f16's range), and so do the
 // probabilities: every product is made twice and keeps 22 bits, so the products set the pace.  Three tiles' scores are under way, and probabilities take their place.
 // The tensor cores cut sums off at every step, which adds up over long rows: outputs are taken out of tensor memory every FLUSH tiles and summed in f32
-// registers, behind the next probabilities, while the last product is still under way (2048 tokens, 32 heads on 8: 78 us; error against 64 bits 6.3e-7, at
+// registers, behind the next probabilities, while the last product is still under way (2048 tokens, 32 heads on 8: 80.5 us; error against 64 bits 6.2e-7, at
 // 60000 positions 9.4e-7; summed in tensor memory throughout 1.6e-6 and more).
 //
 // Probabilities are scaled by 2^BIAS so that small ones keep their bits, and the output is scaled only when a row's maximum has grown by more than 2^GROWTH.
@@ -33,7 +35,7 @@ constexpr int PP_SOFTMAX_WARPS = 16, PP_THREADS = PP_SOFTMAX_WARPS * 32 + 128;  
 constexpr int PP_SOFTMAX_REGS = 104, PP_OTHER_REGS = 64;
 static_assert(PP_SOFTMAX_WARPS * 32 * PP_SOFTMAX_REGS + 128 * PP_OTHER_REGS <= PP_THREADS * 96, "what the block is launched with");
 constexpr float PP_BIAS = 8.f, PP_GROWTH = 7.f;   // log2; together below f16's 2^16
-constexpr int PP_FLUSH = 2;                       // 3: 76 us for 78 and errors of 7.6e-7 and 1.2e-6, in sums that are too small
+constexpr int PP_FLUSH = 2;                       // 3: 2 us less of 80 and errors of 7.6e-7 and 1.2e-6, in sums that are too small
 constexpr int PP_MAX_CLUSTER = 8;
 constexpr uint32_t PP_PANEL = 128 * 128;          // 128 rows of 64 elements, 128-byte swizzle
 
@@ -380,8 +382,9 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
             for (int j = 0; j < 4; j++) mxs[j] = __uint_as_float(s[j]);
 #pragma unroll
             for (int i = 4; i < KEYS; i++) mxs[i & 3] = fmaxf(mxs[i & 3], __uint_as_float(s[i]));
-            // the row's maximum, once all its threads have read the last tile's (no barrier of the products holds a warp back until then); when all have their scores,
-            // probabilities may take the scores' place
+            // The row's maximum, once all its threads have read the last tile's: no barrier of the products holds a warp back until then.  (f32 2048 tokens 80.6 us, 16-bit
+            // 5 x 512 93.3; with this meeting ahead of the wait for the scores 82.6 and 94.4, with a barrier that the readers arrive at 83.5 and 101.9.)  When all
+            // have their scores, probabilities may take the scores' place.
             meet();
             *say = fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3]));
             pg_fence_before();
@@ -649,7 +652,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                 pg_commit(of_tile(s_full, x, t));
                 if (x == last) pg_commit(&empty[slot]);
             };
-            auto outputs = [&](int x, int t, int mine, int slot) {
+            auto outputs = [&](int x, int t, int slot) {
                 ok = passed(p_full, x, t);
                 if (!ok) return;
                 pg_fence_after();
@@ -677,7 +680,7 @@ paged_prefill_kernel(PkCache c, PkBatch b, PpParams P, const __grid_constant__ P
                     if (S::TURNS && t + AHEAD < mine) scores(x, t + AHEAD);
                     if (ok && t < mine) {
                         if (x == 0 || n_a <= t) ok = mbar_wait_bounded(&cleared[t & 7], (uint32_t)(t >> 3) & 1u) && arrived(2 * t + 1);
-                        if (ok) outputs(x, t, mine, slot);
+                        if (ok) outputs(x, t, slot);
                     }
                     // (behind the product: a flush waits for that one)
                     if (!S::TURNS && ok && t + AHEAD < mine) scores(x, t + AHEAD);
