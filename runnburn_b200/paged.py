@@ -3,11 +3,11 @@
 The functions take device tensors of PyTorch (anything with its `data_ptr`, `shape`, `stride`, `dtype`, `device` and the like will do)
 on the library's device (`ops.device_index()`), whatever device is current, and run on the given stream (a stream of PyTorch or its
 handle), else on PyTorch's current one; they do not synchronise and allocate nothing but a missing `out`, so calls with `out` can be
-captured into graphs once the library is open (`ops.open()`, or a `Workspace`).  A missing `out` is allocated on the stream that writes it.  Tensors that the caller brings are used as they are:
-those of another stream than the call's have to be kept until it is through (`record_stream`), as ever in PyTorch.  Tables, lengths and
-starts are read when the work runs.  What they hold is checked on the device: a page outside the pool, a length that the table cannot
-hold or a start out of order sets the device error word (`ops.dev_error_flag()` returns 5) instead of touching memory outside.  The C
-ABI behind it is declared in include/rnb_b200.h.
+captured into graphs once the library is open (`ops.open()`, or a `Workspace`).  A missing `out` is allocated on the stream that writes
+it.  Tensors that the caller brings are used as they are: those of another stream than the call's have to be kept until it is through
+(`record_stream`), as ever in PyTorch.  Tables, lengths and starts are read when the work runs.  What they hold is checked on the
+device: a page outside the pool, a length that the table cannot hold or a start out of order sets the device error word
+(`ops.dev_error_flag()` returns 5) instead of touching memory outside.  The C ABI behind it is declared in include/rnb_b200.h.
 
     pages = KvPages(n_pages, page_size)                    # host: who holds which page
     cache = PagedCache(k, v)                               # [n_pages, page_size, kv_heads, head_dim] each, any strides
@@ -71,7 +71,7 @@ def _stream(index: int, stream) -> int:
     """The stream's handle; None: the current one of PyTorch (asked for by its number alone where that is offered: an object for it takes 2 us)."""
     global _raw_stream
     if stream is not None:
-        handle = getattr(stream, "cuda_stream", stream)
+        handle = getattr(stream, "cuda_stream", getattr(stream, "_as_parameter_", stream))
         return getattr(handle, "value", handle) or 0
     if _raw_stream is None:
         import torch

@@ -490,6 +490,16 @@ def test_calls_of_one_layer_refuse_a_cache_of_several(r):
             call()
 
 
+def test_a_stream_is_any_object_that_stands_for_one(r):
+    class Torch:
+        cuda_stream = 77
+
+    class Foreign:
+        _as_parameter_ = C.c_void_p(78)
+    for stream, handle in ((Torch(), 77), (Foreign(), 78), (79, 79), (C.c_void_p(80), 80), (C.c_void_p(), 0), (0, 0)):
+        assert r.paged._stream(0, stream) == handle
+
+
 def test_the_device_is_the_one_that_would_be_opened(r):
     """Asked for in a process of its own, where nothing is open."""
     import os
