@@ -31,6 +31,7 @@ from ._lib import TYPE_BF16, TYPE_F16, TYPE_F32, check, load
 DEVICE_BAD_PAGE, DEVICE_BAD_WORKSPACE = 5, 6   # what ops.dev_error_flag() tells of a call
 
 _types: dict = {}
+_I32 = np.dtype(np.int32)
 
 
 def _type(t) -> int:
@@ -261,7 +262,9 @@ def paged_kv_append(cache: PagedCache, batch: PagedBatch, k_new, v_new, *, strea
 def _host(a, what: str) -> np.ndarray:
     """A list of whole numbers as int32; what would be cut on the way is refused."""
     a = np.asarray(a)
-    if a.dtype != np.int32 and a.size:
+    if a.dtype is _I32:
+        return a if a.ndim == 1 and a.flags.c_contiguous else np.ascontiguousarray(a).ravel()
+    if a.size:
         if a.dtype.kind not in "iu":
             raise TypeError(f"{what} has to hold whole numbers, got {a.dtype}")
         _int(a.min(), what), _int(a.max(), what)
